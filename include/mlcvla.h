@@ -39,6 +39,8 @@ extern "C" {
  * reference runs in float32; the other entry points and options of the step forms report that
  * they are not built for them. */
 #define MLCV_DTYPE_F32 2
+/* bfloat16: the tensors of the request entry points (mlcv_kv_*, mlcv_prompt_attention) only */
+#define MLCV_DTYPE_BF16 3
 #define MLCV_QUANT_NONE 0
 #define MLCV_QUANT_Q4F16_1 1
 
@@ -293,6 +295,91 @@ int mlcv_linear_noalloc(const void* x, int32_t M, int32_t K, const void* w, cons
 #define MLCV_TILE_GEGLU 2
 int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t N, void* y, int32_t epi,
                      int32_t small_tiles, int32_t meet_polls, void* stream);
+
+/* ---- several requests: a paged 8-bit key/value cache and packed prompts ----------------------
+ *
+ * No counterpart in the reference, which serves one request over a dense cache.  Tokens of B
+ * requests are packed one after another: request b owns tokens [cu_seqlens[b], cu_seqlens[b+1])
+ * of a call, B + 1 int32 on the device, ascending from 0.  Every length stays on the device; the
+ * entry points do not synchronize, allocate or keep anything between calls, and can be captured.
+ * Sizes, types, strides and alignment are checked on the host (-2).  Lengths and indices are
+ * device data: they are brought into range in the kernels, which neither read nor write outside
+ * the given arrays whatever they hold.  Rows of tokens behind cu_seqlens[B] are left as they were.
+ *
+ * The cache: pages of `page` tokens (16, 32, 64 or 128), hd 64, 128 or 256, in e4m3 codes:
+ *   k_cache [num_pages][KV][page][hd]   v_cache [num_pages][KV][hd][page]  (token innermost)
+ *   k_scale, v_scale [num_pages][KV] f32: x = code * scale
+ * both caches 16-byte aligned; at most 2^31 - 1 slots (num_pages * page).  Slot s is token
+ * s % page of page s / page. */
+
+/* Attention over whole prompts: row i of a prompt of n tokens sees the keys [0, n) of its own prompt
+ * (causal = 0), or [0, max(i + 1, min(bidir[b], n))) (causal = 1; bidir [B] or NULL for all 0): the
+ * first bidir tokens -- images and instruction -- see one another, what follows is causal.
+ *   q, out element (t, h, d) at t * tok + h * head + d, k, v of KV heads likewise; MLCV_DTYPE_F16 or
+ *   _BF16; query head h reads kv head h / (H / KV); hd 64, 128 or 256; q, k and v rows 16-byte
+ *   aligned, out rows 8-byte; k and v tokens hd to 2^24 elements apart
+ *   out = sum_j softmax_j(scale * q . k_j) v_j      float32 logits, statistics and sums; the weights
+ *   are rounded to the tensors' type for the matrix cores
+ * What a row does not see does not reach it, whatever it holds. */
+int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                          const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int32_t tokens,
+                          const int32_t* cu_seqlens, int32_t B, int32_t H, int32_t KV, int32_t hd, float scale,
+                          int32_t causal, const int32_t* bidir, void* out, int64_t o_tok, int64_t o_head,
+                          void* stream);
+
+/* Block tables and slot maps: request b has past_lens[b] tokens in the cache, on the pages of its
+ * row block_table[b] [max_pages], and brings new_lens[b] more.  Pages are taken from free_pages
+ * [n_free] in order, request by request, and written behind the row's ceil(past / page) entries
+ * (the other entries stay as they were).
+ *   cu_seqlens [B+1], kv_lens [B] (past + new), slot_map [tokens] (where each new token goes)
+ *   status [2]: pages taken from the front of free_pages; requests that were refused
+ * A request is refused as a whole where a length is negative, its row has too few entries, its
+ * tokens do not fit into `tokens`, or the free pages do not last (every later one that needs a
+ * page is then refused too): it takes no page, its kv_lens is 0 and its slots are -1.  So are the
+ * slots behind the last request and those on a page outside [0, num_pages).  At most 4096
+ * requests.  The outputs must not overlap the inputs. */
+int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
+                 int32_t n_free, int32_t num_pages, int32_t page, int32_t* block_table, int32_t max_pages,
+                 int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,
+                 void* stream);
+
+/* Write the new tokens' keys and values into their slots.  k, v: element (t, h, d) at
+ * t * k_tok + h * k_head + d elements (any strides; rows of 16-byte alignment are read faster),
+ * each of MLCV_DTYPE_F16, _BF16 or _F32 -- mlcv_prefill's float32 keys and float16 values
+ * [KV][P][hd] are k_tok = hd, k_head = P * hd.
+ * The scale of a page, kv head and side is 2^e with the smallest e >= -64 such that
+ * max|x| <= 448 * 2^e over the finite values written to it.  Writing from the middle of a page on
+ * keeps the tokens before the first new one: the scale then only grows, and their codes follow it
+ * (rounded to nearest even, which a power of two leaves exact but for subnormal codes).  Positions
+ * behind the last new one keep their codes.  Values past 448 * scale and infinities saturate, NaN
+ * stays NaN.  A request's slots follow one another within a page, as the plan makes them: the
+ * tokens of a page from the first on whose slot does not are not written, nor are those of a
+ * negative slot.  Requests that write must not share the pages they write to (their contents are
+ * then undefined). */
+int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head, const void* v, int32_t v_dtype,
+                  int64_t v_tok, int64_t v_head, int32_t tokens, const int32_t* cu_seqlens, int32_t B,
+                  const int32_t* slot_map, void* k_cache, float* k_scale, void* v_cache, float* v_scale,
+                  int32_t num_pages, int32_t page, int32_t KV, int32_t hd, void* stream);
+
+/* Attention of the new tokens over the cache: request b's n = cu[b+1] - cu[b] queries are its last n
+ * of kv_lens[b] cached tokens; query t sees the keys [0, kv_lens[b] - n + t + 1) (causal = 1) or all
+ * kv_lens[b] of them (0, the action suffix).  q, out: element (t, h, d) at t * tok + h * head + d,
+ * MLCV_DTYPE_F16 or _BF16; query head h reads kv head h / (H / KV).
+ *   out = sum_j softmax_j(scale * q . k_j) v_j     float32 sums and statistics; the weights are
+ *   rounded to fp16 (2^-11 of each, below the output's rounding) for the matrix cores
+ * A query that sees nothing gives zeros; so does one whose request was refused (kv_lens 0).  Pages
+ * outside [0, num_pages) count as not seen.  max_kv: a bound on kv_lens for the plan of the work
+ * (larger lengths are still right, only slower).  workspace: mlcv_kv_attention_workspace bytes of
+ * device memory, 16-byte aligned, for this call alone while it runs (calls, captured ones among
+ * them, that may overlap need their own). */
+int mlcv_kv_attention_workspace(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv,
+                                size_t* bytes);
+int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_head, int32_t tokens,
+                      const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens, const int32_t* block_table,
+                      int32_t max_pages, const void* k_cache, const float* k_scale, const void* v_cache,
+                      const float* v_scale, int32_t num_pages, int32_t page, int32_t H, int32_t KV, int32_t hd,
+                      float scale, int32_t causal, int32_t max_kv, void* out, int64_t o_tok, int64_t o_head,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* Enqueue `iters` launches of one operation of denoise_step_kv on `stream`, on the
  * context's current buffers (benchmarking / profiling only; no counterpart in the

@@ -1,0 +1,950 @@
+// The paged 8-bit key/value cache of several requests: block tables and slot maps from request lengths
+// (mlcv_kv_plan), the cache's writer (mlcv_kv_write) and the attention over it (mlcv_kv_attention).
+//
+// A page holds `page` tokens (16, 32, 64 or 128) of every kv head in e4m3 with one float32 scale per page, kv
+// head and side:
+//   keys   [pages][KV][page][hd]      values [pages][KV][hd][page] (token innermost)
+// x is held as code * scale with scale = 2^e, the smallest e >= -64 with max|x| <= 448 * 2^e over the page's
+// tokens.  A power of two loses nothing against any other scale (a floating-point code has the same relative
+// step at every exponent), and it makes every rescaling exact but for the codes that fall below 2^-6: a page
+// that grows token by token holds what one write of all its tokens would hold, to the subnormals' step.
+// Values are held token-innermost because the attention's second product contracts over tokens: its matrix
+// operand is then 16 contiguous bytes per lane, as is the first product's over the head dim.
+#include "kernels.h"
+#include "mlcvla.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mlcv {
+
+namespace {
+
+constexpr int KV_NT = 256;         // threads per workgroup of every kernel here
+constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
+
+// ---- plan ------------------------------------------------------------------------------------------
+
+// Inclusive prefix sums of one value per thread over the workgroup (KV_NT threads); `part` holds a sum per wave.
+__device__ __forceinline__ long long block_scan(long long v, long long* part) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 63) part[w] = v;
+  __syncthreads();
+  long long before = 0;
+#pragma unroll
+  for (int i = 0; i < KV_NT / 64 - 1; ++i) before += i < w ? part[i] : 0;
+  __syncthreads();
+  return v + before;
+}
+
+// The last index b in [0, n) with a[b] <= v (a ascending, a[0] <= v).
+__device__ __forceinline__ int last_le(const int* a, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct PlanArgs {
+  const int32_t *past, *fresh, *free_pages;
+  int32_t *table, *cu, *kv_lens, *slots, *status;
+  int32_t B, n_free, num_pages, psh, max_pages, tokens, slot_blocks;
+};
+
+// Every workgroup runs the same scan over the requests (two loads and a prefix sum per 256 of them, which costs
+// less than a second launch that waits for the first), then fills its own part of the slot map or of the table.
+// Bound by launch and load latency.
+__global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
+  extern __shared__ int sm[];
+  __shared__ long long part[KV_NT / 64];
+  __shared__ int sbad, sused;
+  int* scu = sm;                // [B + 1] first token of each request
+  int* sbase = sm + a.B + 1;    // [B + 1] first page it takes from the free list; ~base where it is refused
+  const int tid = threadIdx.x, page = 1 << a.psh;
+  if (tid == 0) sbad = sused = 0;
+  __syncthreads();
+  long long tok0 = 0, pg0 = 0;
+  int bad = 0, used = 0;
+  for (int b0 = 0; b0 < a.B; b0 += KV_NT) {
+    const int b = b0 + tid;
+    const bool in = b < a.B;
+    const long long p = in ? a.past[b] : 0, q = in ? a.fresh[b] : 0;
+    const long long qn = q > 0 ? q : 0;
+    const long long end = block_scan(qn, part) + tok0;
+    const long long had = (p + page - 1) >> a.psh, has = (p + qn + page - 1) >> a.psh;
+    const bool fits = in && p >= 0 && q >= 0 && has <= a.max_pages && end <= a.tokens;
+    const long long need = fits ? has - had : 0;
+    const long long pend = block_scan(need, part) + pg0;
+    const bool ok = fits && (need == 0 || pend <= a.n_free);
+    if (in) {
+      const long long first = end - qn;
+      scu[b] = (int)(first < a.tokens ? first : a.tokens);
+      // pages past the free list are never indexed: a refused request has no slots and no table entries
+      const long long base = pend - need < a.n_free ? pend - need : a.n_free;
+      sbase[b] = ok ? (int)base : ~(int)base;
+      bad += !ok;
+      if (ok && need > 0) used = (int)pend;  // granted: at most n_free; ascending over b
+      if (blockIdx.x == 0) {
+        a.cu[b] = scu[b];
+        a.kv_lens[b] = ok ? (int)(p + q) : 0;
+      }
+    }
+    // the last thread's sums carry over
+    __shared__ long long carry[2];
+    if (tid == KV_NT - 1) {
+      carry[0] = end;
+      carry[1] = pend;
+    }
+    __syncthreads();
+    tok0 = carry[0];
+    pg0 = carry[1];
+    __syncthreads();
+  }
+  if (bad) atomicAdd(&sbad, bad);
+  if (used) atomicMax(&sused, used);
+  if (tid == 0) {
+    scu[a.B] = (int)(tok0 < a.tokens ? tok0 : a.tokens);
+    sbase[a.B] = (int)(pg0 < a.n_free ? pg0 : a.n_free);
+  }
+  __syncthreads();
+  if ((int)blockIdx.x < a.slot_blocks) {  // slots
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long t = (long long)blockIdx.x * 4 * KV_NT + i * KV_NT + tid;
+      if (t >= a.tokens) break;
+      int slot = -1;
+      if (t < scu[a.B]) {
+        const int b = last_le(scu, a.B, (int)t), base = sbase[b];
+        if (base >= 0) {
+          const int p = a.past[b], had = (int)(((long long)p + page - 1) >> a.psh);
+          const int pos = p + ((int)t - scu[b]), pg = pos >> a.psh;
+          const int id = pg < had ? a.table[(size_t)b * a.max_pages + pg] : a.free_pages[base + pg - had];
+          if (id >= 0 && id < a.num_pages) slot = (id << a.psh) + (pos & (page - 1));
+        }
+      }
+      a.slots[t] = slot;
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+      a.cu[a.B] = scu[a.B];
+      a.status[0] = sused;
+      a.status[1] = sbad;
+    }
+  } else {  // table entries, one thread for each page taken
+    const int f = ((int)blockIdx.x - a.slot_blocks) * KV_NT + tid;
+    if (f >= sbase[a.B]) return;
+    // the request that takes page f: the last whose base (refused or not) is <= f
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, v = sbase[mid];
+      if ((v >= 0 ? v : ~v) <= f) lo = mid;
+      else hi = mid;
+    }
+    if (sbase[lo] < 0) return;
+    const int had = (int)(((long long)a.past[lo] + page - 1) >> a.psh);
+    a.table[(size_t)lo * a.max_pages + had + f - sbase[lo]] = a.free_pages[f];
+  }
+}
+
+// ---- the page a workgroup works on ------------------------------------------------------------------
+
+// Work items of a packed batch, without knowing its lengths on the host: request b takes the item numbers
+// [f(b), f(b + 1)) with f(b) = floor(cu[b] * mul / div) + extra * b.  f grows by at least the request's
+// ceil(n * mul / div) items (extra = 1), or one more for a first page that is not empty (extra = 2), so that
+// floor(tokens * mul / div) + extra * B items always do; the few that are left over end at once.
+// Every thread tests its own b: one round of loads instead of a chain of dependent ones.
+__device__ __forceinline__ int clamp_i(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+struct Item {
+  int b, c0, n;  // request, its first token and number of tokens; b = -1: none
+  int i;         // the item's number within its request
+};
+__device__ __forceinline__ Item find_item(const int32_t* cu, int B, int tokens, long long item, int mul, int div,
+                                          int extra, int* sh) {
+  if (threadIdx.x == 0) sh[0] = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < B; b += KV_NT) {
+    const int c0 = clamp_i(cu[b], 0, tokens), c1 = clamp_i(cu[b + 1], 0, tokens);
+    const long long f0 = (long long)c0 * mul / div + (long long)extra * b;
+    const long long f1 = (long long)c1 * mul / div + (long long)extra * (b + 1);
+    if (f0 <= item && item < f1 && c1 > c0) {
+      sh[0] = b;
+      sh[1] = c0;
+      sh[2] = c1 - c0;
+      sh[3] = (int)(item - f0);
+    }
+  }
+  __syncthreads();
+  Item r;
+  r.b = __builtin_amdgcn_readfirstlane(sh[0]);
+  r.c0 = __builtin_amdgcn_readfirstlane(sh[1]);
+  r.n = __builtin_amdgcn_readfirstlane(sh[2]);
+  r.i = __builtin_amdgcn_readfirstlane(sh[3]);
+  return r;
+}
+
+// ---- write -----------------------------------------------------------------------------------------
+
+struct WriteArgs {
+  const void* x[2];       // keys, values
+  int64_t tok[2], head[2];  // element strides
+  uint8_t* cache[2];
+  float* scale[2];
+  const int32_t *cu, *slots;
+  int32_t type[2], vec[2];  // vec: rows are 16-byte aligned
+  int32_t tokens, B, num_pages, psh, KV;
+};
+
+// 8 consecutive elements as float32
+template <int HD>
+__device__ __forceinline__ void load8(const void* p, int type, int vec, int64_t at, float* out) {
+  if (type == MLCV_DTYPE_F32) {
+    const float* x = reinterpret_cast<const float*>(p) + at;
+    if (vec) {
+      const f4 a = load_global(reinterpret_cast<const f4*>(x)), b = load_global(reinterpret_cast<const f4*>(x) + 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        out[i] = a[i];
+        out[4 + i] = b[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = load_global(x + i);
+    }
+    return;
+  }
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(p) + at;
+  uint32_t w[4];
+  if (vec) {
+    const u4 v = load_global(reinterpret_cast<const u4*>(x));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = load_global(x + 2 * i) | (uint32_t)load_global(x + 2 * i + 1) << 16;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == MLCV_DTYPE_F16) {
+      const h2 v = __builtin_bit_cast(h2, w[i]);
+      out[2 * i] = (float)v[0];
+      out[2 * i + 1] = (float)v[1];
+    } else {
+      out[2 * i] = __uint_as_float(w[i] << 16);
+      out[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// four values as e4m3, rounded to nearest even; past the largest finite value (infinities among them) they
+// saturate, NaN stays NaN
+__device__ __forceinline__ float sat448(float x) { return x > 448.f ? 448.f : x < -448.f ? -448.f : x; }
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(sat448(a), sat448(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(sat448(c), sat448(d), r, true);
+}
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return pack4(a[0] * ratio, a[1] * ratio, b[0] * ratio, b[1] * ratio);
+}
+// bytes [lo, hi) of a 4-byte word
+__device__ __forceinline__ uint32_t byte_mask(int lo, int hi) {
+  lo = clamp_i(lo, 0, 4);
+  hi = clamp_i(hi, 0, 4);
+  if (lo >= hi) return 0u;
+  const uint32_t up = hi == 4 ? 0xffffffffu : (1u << (8 * hi)) - 1u;
+  return up & ~((1u << (8 * lo)) - 1u);
+}
+
+// One workgroup: one page of one request, one kv head, keys or values (blockIdx.z).  A unit of work is 4
+// positions of the page x 8 dims, UNITS of them per thread, held in registers from the maximum to the codes, so
+// that the input is read once.  Keys leave as 8 bytes per position; values go through LDS to be turned to
+// [hd][page] and leave as 16-byte pieces.  A piece that is not wholly new is merged with what the page held.
+template <int HD, int UNITS>
+__global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
+  constexpr int CH = HD / 8;               // 8-dim pieces of a row
+  __shared__ int sh[4];
+  __shared__ float smax[KV_NT / 64];
+  __shared__ __attribute__((aligned(16))) char turn[HD * (UNITS * KV_NT / CH * 4 + 16)];
+  const int tid = threadIdx.x, page = 1 << a.psh, h = blockIdx.y, z = blockIdx.z;
+  const Item it = find_item(a.cu, a.B, a.tokens, blockIdx.x, 1, page, 2, sh);
+  if (it.b < 0) return;
+  const int o0 = a.slots[it.c0] & (page - 1);  // of a negative slot: any value, the tokens are dropped below
+  const int start = it.i == 0 ? it.c0 : it.c0 + it.i * page - o0;
+  const int stop = min(it.c0 + it.n, it.i == 0 ? it.c0 + page - o0 : start + page);
+  if (start >= stop) return;
+  const int slot = a.slots[start];
+  const int id = slot >> a.psh, o = slot & (page - 1);
+  if (slot < 0 || id >= a.num_pages) return;
+  // positions [o, o + count) of the page are new: the group's tokens up to the first whose slot does not follow
+  // its neighbour's
+  __syncthreads();
+  if (tid == 0) sh[0] = min(stop - start, page - o);
+  __syncthreads();
+  if (tid < min(stop - start, page - o) && a.slots[start + tid] != slot + tid) atomicMin(sh, tid);
+  __syncthreads();
+  const int count = sh[0];
+
+  const void* x = a.x[z];
+  const int64_t xt = a.tok[z], base = (int64_t)h * a.head[z];
+  float v[UNITS][4][8];
+  float big = 0.f;
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int unit = tid + u * KV_NT, quad = unit / CH, ch = unit % CH;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = 4 * quad + i - o;  // token within the group
+      if (j >= 0 && j < count) {
+        load8<HD>(x, a.type[z], a.vec[z], (int64_t)(start + j) * xt + base + 8 * ch, v[u][i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float m = fabsf(v[u][i][e]);
+          big = m < INFINITY ? fmaxf(big, m) : big;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[u][i][e] = 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor(big, s));
+  if ((tid & 63) == 0) smax[tid >> 6] = big;
+  float* scale = a.scale[z] + (size_t)id * a.KV + h;
+  const float old = o > 0 ? load_global(scale) : 0.f;
+  __syncthreads();
+  big = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+  // big = m * 2^E, 1 <= m < 2: 448 = 1.75 * 2^8, so e = E - 8, one more where m > 1.75
+  const uint32_t bits = __float_as_uint(big);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < -64 ? -64 : e;
+  const float need = __uint_as_float((uint32_t)(e + 127) << 23);
+  const float now = fmaxf(need, old);  // a NaN that the page held counts as nothing
+  const bool grown = o > 0 && now != old;
+  const float inv = 1.0f / now;        // exact where the scale is a power of two, as this kernel's are
+  const float ratio = old * inv;
+
+  uint8_t* dst = a.cache[z] + ((size_t)id * a.KV + h) * (size_t)page * HD;
+  if (z == 0) {  // keys [page][HD]
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int unit = tid + u * KV_NT, quad = unit / CH, ch = unit % CH;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int pos = 4 * quad + i, j = pos - o;
+        if (j >= 0 && j < count) {
+          u2v w;
+          w[0] = pack4(v[u][i][0] * inv, v[u][i][1] * inv, v[u][i][2] * inv, v[u][i][3] * inv);
+          w[1] = pack4(v[u][i][4] * inv, v[u][i][5] * inv, v[u][i][6] * inv, v[u][i][7] * inv);
+          *reinterpret_cast<u2v*>(dst + (size_t)pos * HD + 8 * ch) = w;
+        }
+      }
+    }
+    if (grown)
+      for (int i = tid; i < o * (HD / 4); i += KV_NT) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(dst) + i;
+        *w = rescale4(*w, ratio);
+      }
+  } else {  // values [HD][page]
+    const int row = page + 16;  // bytes of a row in LDS
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int unit = tid + u * KV_NT, quad = unit / CH, ch = unit % CH;
+      if (4 * quad < page && 4 * quad + 4 > o && 4 * quad < o + count) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          *reinterpret_cast<uint32_t*>(turn + (8 * ch + d) * row + 4 * quad) =
+              pack4(v[u][0][d] * inv, v[u][1][d] * inv, v[u][2][d] * inv, v[u][3][d] * inv);
+      }
+    }
+    __syncthreads();
+    const int segs = page >> 4;
+    for (int i = tid; i < HD * segs; i += KV_NT) {
+      const int d = i / segs, s = i % segs;
+      const int lo = o - 16 * s, hi = o + count - 16 * s;  // new bytes of this piece: [lo, hi)
+      const bool fresh = lo < 16 && hi > 0;
+      if (!fresh && !(grown && lo > 0)) continue;
+      u4* g = reinterpret_cast<u4*>(dst + (size_t)d * page + 16 * s);
+      u4 w = fresh ? *reinterpret_cast<const u4*>(turn + d * row + 16 * s) : (u4){0, 0, 0, 0};
+      if (lo > 0 || hi < 16) {
+        const u4 was = *g;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t fm = byte_mask(lo - 4 * q, hi - 4 * q), km = byte_mask(0, lo - 4 * q);
+          const uint32_t kept = grown ? rescale4(was[q], ratio) : was[q];
+          w[q] = (w[q] & fm) | (kept & km) | (was[q] & ~(fm | km));
+        }
+      }
+      *g = w;
+    }
+  }
+  if (tid == 0 && now != old) *scale = now;
+}
+
+// ---- attention -------------------------------------------------------------------------------------
+
+struct KvAttnArgs {
+  const void* q;
+  int64_t q_tok, q_head, o_tok, o_head;  // element strides
+  const int32_t *cu, *kv_lens, *table;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  void* out;
+  float *part_o, *part_ml;  // of the splits: O [items][KV][S][RT][HD], (m, l) [items][KV][S][RT]
+  int32_t tokens, B, H, KV, grp, max_pages, num_pages, psh, causal, q_vec;
+  int32_t S, span;   // splits, tiles of 64 keys per split
+  float c;           // scale * log2(e)
+};
+
+template <bool BF>
+struct El {
+  typedef _Float16 T;
+  typedef h8 V8;
+};
+template <>
+struct El<true> {
+  typedef __bf16 T;
+  typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+};
+__device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return mfma16x16x32(a, b, c); }
+__device__ __forceinline__ f4 mfma16(El<true>::V8 a, El<true>::V8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// 8 codes as values of either type, exactly (both types hold every e4m3 value)
+template <bool BF>
+__device__ __forceinline__ typename El<BF>::V8 widen8(uint32_t lo, uint32_t hi) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  u4 w;
+  if constexpr (BF) {
+    w[0] = __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    w[1] = __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    w[2] = __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    w[3] = __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else {
+    w[0] = __builtin_bit_cast(uint32_t, (h2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    w[1] = __builtin_bit_cast(uint32_t, (h2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    w[2] = __builtin_bit_cast(uint32_t, (h2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    w[3] = __builtin_bit_cast(uint32_t, (h2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+  }
+  return __builtin_bit_cast(typename El<BF>::V8, w);
+}
+__device__ __forceinline__ bool has_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// keys that any row of [row0, row0 + rows) of a request sees
+__device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, int kv_len, int row0, int rt) {
+  const int rows = it.n * a.grp, last = min(row0 + rt, rows) - 1;
+  return a.causal ? kv_len - it.n + last / a.grp + 1 : kv_len;
+}
+
+// Row r of a request is token r / grp of its n new tokens and head h * grp + r % grp: the query heads of a kv
+// head share its keys.  A workgroup (4 waves) takes RT = 16 R such rows and one split of the keys; its waves
+// take tiles of 64 keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
+//
+// A wave's tile has no LDS and no shuffle of data in it.  S^T = K . Q^T and O^T = V^T . P^T on
+// v_mfma_f32_16x16x32: with lane = 16 g + r, S^T puts keys 4 g .. 4 g + 3 of each 16-key sub-tile and query row
+// r into a lane, and the second product wants 8 keys of row r in it.  Both contractions may run in any order,
+// so the order is chosen by the loads: sub-tile t's row 4 g + i is key 16 g + 4 t + i of the tile, a lane then
+// owns keys 16 g .. 16 g + 15, which are 16 contiguous bytes of the value page, lie in one page and have one
+// scale of each side.  Dims likewise: a lane's 16 key bytes are two steps of the first contraction.
+//
+// The value scale is folded into the weights before they are rounded to fp16: with x = logit * log2(e) the
+// running maximum is that of x + log2(scale_v), so that w = 2^(x - m) * scale_v stays within [0, 2^12] whatever
+// the pages' scales are; the sum of 2^(x - m) is kept in float32.  Weights and values are fp16 for either type
+// of query (an e4m3 value is exact in it).  2^12 of headroom keeps weights down to 2^-26 of the largest above
+// fp16's subnormals.
+//
+// A key or page that a row does not see has weight 0, which a NaN code behind it would turn into NaN: codes
+// behind the request's last token are cleared, and a tile of which some rows see a NaN and others do not is
+// taken key by key (visible_only).
+template <bool BF, int HD, int R>
+__global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
+  typedef typename El<BF>::T T;
+  typedef typename El<BF>::V8 V8;
+  constexpr int RT = 16 * R, NJ = HD / 64, ND = HD / 16;
+  __shared__ int sh[4];
+  __shared__ float sm[4][RT], sl[4][RT];
+  __shared__ __attribute__((aligned(16))) float so[4][RT][64 + 4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int item = blockIdx.x / (a.KV * a.S), rest = blockIdx.x % (a.KV * a.S);
+  const int h = rest % a.KV, split = rest / a.KV;
+  const Item it = find_item(a.cu, a.B, a.tokens, item, a.grp, RT, 1, sh);
+  if (it.b < 0) return;
+  const int rows = it.n * a.grp, row0 = it.i * RT, page = 1 << a.psh;
+  if (row0 >= rows) return;
+  const int kv_len = clamp_i(load_global(a.kv_lens + it.b), 0, a.max_pages << a.psh);
+  const int most = last_limit(a, it, kv_len, row0, RT);
+  const int first = a.causal ? kv_len - it.n + row0 / a.grp + 1 : kv_len;  // keys that every row sees
+  const int tiles = (most + 63) >> 6;
+  const int t_begin = split * a.span, t_end = split == a.S - 1 ? tiles : min(tiles, t_begin + a.span);
+  if (split > 0 && t_begin >= tiles) return;
+
+  // the query operand: row r16 of each 16, dims 64 j + 16 g + 8 s .. + 7 for step 2 j + s
+  V8 q[R][2 * NJ];
+  int lim[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = min(row0 + 16 * r + r16, rows - 1), t = row / a.grp;
+    lim[r] = a.causal ? kv_len - it.n + t + 1 : kv_len;
+    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(it.c0 + t) * a.q_tok +
+                 (int64_t)(h * a.grp + row - t * a.grp) * a.q_head + 16 * g;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (a.q_vec) {
+          q[r][2 * j + s] = load_global(reinterpret_cast<const V8*>(p + 64 * j + 8 * s));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[r][2 * j + s][e] = load_global(p + 64 * j + 8 * s + e);
+        }
+      }
+  }
+  f4 o[R][ND];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[r][d] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  const int32_t* table = a.table + (size_t)it.b * a.max_pages;
+  // page of the 16 keys at `pos`; -1: none that can be read
+  auto page_at = [&](int pos) {
+    const int pg = pos >> a.psh;
+    const int id = pg < a.max_pages ? load_global(table + pg) : -1;
+    return id >= 0 && id < a.num_pages ? id : -1;
+  };
+  for (int t = t_begin + w; t < t_end; t += 4) {
+    const int pk = 64 * t + 16 * (r16 >> 2) + (r16 & 3), pv = 64 * t + 16 * g;
+    const int idk = page_at(64 * t + 16 * (r16 >> 2)), idv = page_at(pv);
+    const uint8_t* kp = a.kc + (((size_t)max(idk, 0) * a.KV + h) * page + (pk & (page - 1))) * HD + 16 * g;
+    const uint8_t* vp = a.vc + (((size_t)max(idv, 0) * a.KV + h) * HD + r16) * page + (pv & (page - 1));
+    u4 kr[4][NJ], vr[ND];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) kr[s][j] = load_global(reinterpret_cast<const u4*>(kp + 4 * s * HD + 64 * j));
+    const size_t si = (size_t)max(idv, 0) * a.KV + h;
+    const float skc = load_global(a.ks + si) * a.c, sv = load_global(a.vs + si);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const u4*>(vp + (size_t)16 * d * page));
+
+    f4 x[R][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r][s] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const V8 k0 = widen8<BF>(kr[s][j][0], kr[s][j][1]), k1 = widen8<BF>(kr[s][j][2], kr[s][j][3]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          x[r][s] = mfma16(k0, q[r][2 * j], x[r][s]);
+          x[r][s] = mfma16(k1, q[r][2 * j + 1], x[r][s]);
+        }
+      }
+    }
+    const int own = idv < 0 ? 0 : clamp_i(kv_len - pv, 0, 16);  // the lane's keys that are the request's
+    const bool edge = 64 * t + 64 > first || __any(idv < 0);
+    bool apart = false;  // some rows see a NaN that others do not
+    if (edge) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t keep = byte_mask(0, own - 4 * i);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          vr[d][i] &= keep;
+          nan = nan || has_nan(vr[d][i]);
+        }
+      }
+      apart = a.causal && __any(nan);
+    }
+    const float lsv = __builtin_amdgcn_logf(fmaxf(sv, 0x1p-64f)) - 12.0f;
+    h8 p[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
+      const int see = min(lim[r] - pv, own);  // keys pv .. pv + see - 1 are visible
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = x[r][s][i] * skc;
+          if (edge && 4 * s + i >= see) v = -INFINITY;
+          x[r][s][i] = v;
+          top = fmaxf(top, v);
+        }
+      top = xor_max_16_32(top + lsv);
+      const float mn = fmaxf(m[r], top), mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m[r] - mu);
+      m[r] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(x[r][s][i] - mu);
+          sum += e;
+          p[r][s >> 1][4 * (s & 1) + i] = (_Float16)(e * sv);
+        }
+      l[r] = l[r] * alpha + sum;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
+    }
+    if (!apart) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const h8 v0 = widen8<false>(vr[d][0], vr[d][1]), v1 = widen8<false>(vr[d][2], vr[d][3]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          o[r][d] = mfma16(v0, p[r][0], o[r][d]);
+          o[r][d] = mfma16(v1, p[r][1], o[r][d]);
+        }
+      }
+    } else {
+      // key by key: a product with that key alone, added to the rows that see it
+      for (int key = 0; key < 64; ++key) {
+        const int e = key & 7, s = (key >> 3) & 1;
+        const uint32_t mine = g == (key >> 4) ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          u4 v = __builtin_bit_cast(u4, s ? widen8<false>(vr[d][2], vr[d][3]) : widen8<false>(vr[d][0], vr[d][1]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] &= (e >> 1) == i ? mine : 0u;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const f4 add = mfma16(__builtin_bit_cast(h8, v), s ? p[r][1] : p[r][0], (f4){0.f, 0.f, 0.f, 0.f});
+            if (64 * t + key < lim[r]) o[r][d] += add;
+          }
+        }
+      }
+    }
+  }
+
+  // ---- the waves meet ------------------------------------------------------------------------------
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    l[r] = xor_sum_16_32(l[r]);
+    if (g == 0) {
+      sm[w][16 * r + r16] = m[r];
+      sl[w][16 * r + r16] = l[r];
+    }
+  }
+  __syncthreads();
+  float f[R];  // this wave's share of the workgroup's sum
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = 16 * r + r16;
+    const float mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    f[r] = __builtin_amdgcn_exp2f(m[r] - mu);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += sl[i][row] * __builtin_amdgcn_exp2f(sm[i][row] - mu);
+    if (a.S > 1) {
+      if (w == 0 && g == 0 && row0 + row < rows) {
+        f2* ml = reinterpret_cast<f2*>(a.part_ml) +
+                 (((size_t)item * a.KV + h) * a.S + split) * RT + row;
+        *ml = (f2){mx, sum};
+      }
+    } else {
+      f[r] = sum > 0.f ? f[r] / sum : sum == 0.f ? 0.f : sum;  // nothing visible: zeros; NaN stays
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NJ; ++c) {  // 64 dims at a time
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        f4 v = o[r][4 * c + d];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f[r] == 0.f ? 0.f : v[i] * f[r];
+        *reinterpret_cast<f4*>(&so[w][16 * r + r16][16 * d + 4 * g]) = v;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < RT * 16; i += KV_NT) {
+      const int row = i >> 4, d = 4 * (i & 15);
+      if (row0 + row >= rows) continue;
+      f4 v = *reinterpret_cast<const f4*>(&so[0][row][d]);
+#pragma unroll
+      for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const f4*>(&so[k][row][d]);
+      if (a.S > 1) {
+        float* dst = a.part_o + ((((size_t)item * a.KV + h) * a.S + split) * RT + row) * HD + 64 * c + d;
+        *reinterpret_cast<f4*>(dst) = v;
+      } else {
+        const int rr = row0 + row, t = rr / a.grp;
+        T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + t) * a.o_tok +
+                 (int64_t)(h * a.grp + rr - t * a.grp) * a.o_head + 64 * c + d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[k] = (T)v[k];
+      }
+    }
+  }
+}
+
+// The splits of one row: sums of the partial results under their common maximum.  One workgroup per row, so
+// that the reads of a long request's many splits spread over the GPU; HD / 4 threads for one split's row.
+template <bool BF, int HD>
+__global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int rt) {
+  typedef typename El<BF>::T T;
+  constexpr int NQ = HD / 4, NG = KV_NT / NQ;
+  __shared__ int sh[4];
+  __shared__ __attribute__((aligned(16))) float so[NG][HD];
+  __shared__ float sl[NG];
+  const int tid = threadIdx.x, row = blockIdx.x % rt, h = blockIdx.x / rt % a.KV;
+  const int item = blockIdx.x / (rt * a.KV);
+  const Item it = find_item(a.cu, a.B, a.tokens, item, a.grp, rt, 1, sh);
+  if (it.b < 0) return;
+  const int rr = it.i * rt + row;
+  if (rr >= it.n * a.grp) return;
+  const int kv_len = clamp_i(load_global(a.kv_lens + it.b), 0, a.max_pages << a.psh);
+  const int tiles = (last_limit(a, it, kv_len, it.i * rt, rt) + 63) >> 6;
+  const int n = clamp_i((tiles + a.span - 1) / a.span, 1, a.S);  // splits that there are
+  const size_t p0 = ((size_t)item * a.KV + h) * a.S * rt + row;
+  const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + p0;
+  float mx = -INFINITY;
+  for (int s = 0; s < n; ++s) mx = fmaxf(mx, load_global(ml + (size_t)s * rt)[0]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  const int gq = tid / NQ, d = 4 * (tid % NQ);
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int s = gq; s < n; s += NG) {
+    const f2 e = load_global(ml + (size_t)s * rt);
+    const float f = __builtin_amdgcn_exp2f(e[0] - mu);
+    const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * rt) * HD + d));
+    if (f != 0.f) v += u * f;
+    sum += e[1] * f;
+  }
+  *reinterpret_cast<f4*>(&so[gq][d]) = v;
+  if (d == 0) sl[gq] = sum;
+  __syncthreads();
+  if (gq > 0) return;
+#pragma unroll
+  for (int k = 1; k < NG; ++k) {
+    v += *reinterpret_cast<const f4*>(&so[k][d]);
+    sum += sl[k];
+  }
+  const float f = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
+  const int t = rr / a.grp;
+  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + t) * a.o_tok +
+           (int64_t)(h * a.grp + rr - t * a.grp) * a.o_head + d;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) dst[k] = (T)(v[k] * f);
+}
+
+// How an attention call is cut: rows per workgroup and splits of the keys, from what the host knows.
+struct KvAttnPlan {
+  int R, S, span;
+  long long items;
+  size_t o_floats, bytes;
+};
+KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
+  KvAttnPlan p;
+  const long long grp = H / KV, rows = tokens * grp;
+  p.R = rows <= 16ll * B ? 1 : 2;
+  const int rt = 16 * p.R;
+  p.items = rows / rt + B;
+  const long long busy = std::max((rows + rt - 1) / rt, (long long)std::min(B, tokens)) * KV;
+  const int tiles = std::max(1, (max_kv + 63) / 64);
+  const long long want = std::max(1ll, std::min((1024 + busy - 1) / busy, (long long)(tiles + 3) / 4));
+  p.span = (int)((tiles + want - 1) / want);
+  p.S = (tiles + p.span - 1) / p.span;
+  const size_t parts = (size_t)p.items * KV * p.S * rt;
+  p.o_floats = p.S > 1 ? parts * hd : 0;
+  p.bytes = p.S > 1 ? (p.o_floats + parts * 2) * sizeof(float) : 0;
+  return p;
+}
+
+bool kv_page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
+bool kv_hd_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int log2_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+template <int HD>
+int kv_write_launch(const WriteArgs& a, hipStream_t st) {
+  const int page = 1 << a.psh;
+  const dim3 grid(a.tokens / page + 2 * a.B, a.KV, 2);
+  constexpr int PER = 4 * KV_NT / (HD / 8);  // positions that one unit per thread covers
+  if (page <= PER) kv_write_kernel<HD, 1><<<grid, KV_NT, 0, st>>>(a);
+  else if (page <= 2 * PER) kv_write_kernel<HD, (PER >= 128 ? 1 : 2)><<<grid, KV_NT, 0, st>>>(a);
+  else kv_write_kernel<HD, (PER >= 64 ? 1 : 4)><<<grid, KV_NT, 0, st>>>(a);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+template <bool BF, int HD>
+int kv_attn_launch(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_t st) {
+  const unsigned grid = (unsigned)(p.items * a.KV * p.S);
+  if (p.R == 1) kv_attn_kernel<BF, HD, 1><<<grid, KV_NT, 0, st>>>(a);
+  else kv_attn_kernel<BF, HD, 2><<<grid, KV_NT, 0, st>>>(a);
+  MLCV_HIP(hipGetLastError());
+  if (p.S > 1) {
+    kv_join_kernel<BF, HD><<<(unsigned)(p.items * a.KV * 16 * p.R), KV_NT, 0, st>>>(a, 16 * p.R);
+    MLCV_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace mlcv
+
+using namespace mlcv;
+
+extern "C" {
+
+int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
+                 int32_t n_free, int32_t num_pages, int32_t page, int32_t* block_table, int32_t max_pages,
+                 int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,
+                 void* stream) {
+  MLCV_REQUIRE(B >= 0 && n_free >= 0 && num_pages >= 0 && max_pages >= 0 && tokens >= 0, "negative size");
+  MLCV_REQUIRE(cu_seqlens && status, "null output");
+  MLCV_REQUIRE(B == 0 || (past_lens && new_lens && kv_lens && (block_table || max_pages == 0)), "null request array");
+  MLCV_REQUIRE(n_free == 0 || free_pages, "null free_pages");
+  MLCV_REQUIRE(tokens == 0 || slot_map, "null slot_map");
+  MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
+  MLCV_REQUIRE(B <= KV_MAX_REQ, "more than 4096 requests");
+  MLCV_REQUIRE((int64_t)num_pages * page <= INT32_MAX && (int64_t)max_pages * page <= INT32_MAX,
+               "more than 2^31 - 1 slots");
+  PlanArgs a{past_lens, new_lens, free_pages, block_table, cu_seqlens, kv_lens, slot_map, status, B, n_free,
+             num_pages, log2_of(page), max_pages, tokens, 0};
+  a.slot_blocks = std::max(1, (int)(((int64_t)tokens + 4 * KV_NT - 1) / (4 * KV_NT)));
+  // a request takes at most new / page + 1 pages
+  const int64_t pages = std::min<int64_t>(n_free, (int64_t)tokens / page + B);
+  const unsigned grid = (unsigned)(a.slot_blocks + (pages + KV_NT - 1) / KV_NT);
+  kv_plan_kernel<<<grid, KV_NT, (size_t)2 * (B + 1) * sizeof(int), reinterpret_cast<hipStream_t>(stream)>>>(a);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head, const void* v, int32_t v_dtype,
+                  int64_t v_tok, int64_t v_head, int32_t tokens, const int32_t* cu_seqlens, int32_t B,
+                  const int32_t* slot_map, void* k_cache, float* k_scale, void* v_cache, float* v_scale,
+                  int32_t num_pages, int32_t page, int32_t KV, int32_t hd, void* stream) {
+  MLCV_REQUIRE(tokens >= 0 && B >= 0 && num_pages >= 0 && KV > 0, "bad size");
+  if (tokens == 0 || B == 0 || num_pages == 0) return 0;
+  MLCV_REQUIRE(k && v && cu_seqlens && slot_map && k_cache && k_scale && v_cache && v_scale, "null pointer");
+  auto type_ok = [](int t) { return t == MLCV_DTYPE_F16 || t == MLCV_DTYPE_F32 || t == MLCV_DTYPE_BF16; };
+  MLCV_REQUIRE(type_ok(k_dtype) && type_ok(v_dtype), "keys and values are float16, bfloat16 or float32");
+  MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
+  MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
+  MLCV_REQUIRE(KV <= 65535, "more than 65535 kv heads");
+  MLCV_REQUIRE((int64_t)num_pages * page <= INT32_MAX, "more than 2^31 - 1 slots");
+  MLCV_REQUIRE((int64_t)tokens / page + 2 * (int64_t)B <= INT32_MAX, "too many requests");
+  MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
+  WriteArgs a{};
+  a.x[0] = k;
+  a.x[1] = v;
+  a.tok[0] = k_tok;
+  a.tok[1] = v_tok;
+  a.head[0] = k_head;
+  a.head[1] = v_head;
+  a.cache[0] = static_cast<uint8_t*>(k_cache);
+  a.cache[1] = static_cast<uint8_t*>(v_cache);
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.cu = cu_seqlens;
+  a.slots = slot_map;
+  a.type[0] = k_dtype;
+  a.type[1] = v_dtype;
+  for (int z = 0; z < 2; ++z) {
+    const int per = a.type[z] == MLCV_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+    a.vec[z] = aligned16(a.x[z]) && a.tok[z] % per == 0 && a.head[z] % per == 0;
+  }
+  a.tokens = tokens;
+  a.B = B;
+  a.num_pages = num_pages;
+  a.psh = log2_of(page);
+  a.KV = KV;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return hd == 64 ? kv_write_launch<64>(a, st) : hd == 128 ? kv_write_launch<128>(a, st) : kv_write_launch<256>(a, st);
+}
+
+static int kv_attn_sizes_ok(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv) {
+  MLCV_REQUIRE(tokens >= 0 && B >= 0 && max_kv >= 0, "negative size");
+  MLCV_REQUIRE(H > 0 && KV > 0 && H % KV == 0, "query heads must be a multiple of the kv heads");
+  MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
+  MLCV_REQUIRE((int64_t)tokens * (H / KV) <= INT32_MAX, "more than 2^31 - 1 query rows of a kv head");
+  const KvAttnPlan p = kv_attn_plan(tokens, std::max(B, 1), H, KV, hd, max_kv);
+  MLCV_REQUIRE(p.items * KV * std::max(p.S, 16 * p.R) <= INT32_MAX, "too many workgroups");
+  return 0;
+}
+
+int mlcv_kv_attention_workspace(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv,
+                                size_t* bytes) {
+  MLCV_REQUIRE(bytes, "null pointer");
+  MLCV_TRY(kv_attn_sizes_ok(tokens, B, H, KV, hd, max_kv));
+  *bytes = tokens == 0 || B == 0 ? 0 : kv_attn_plan(tokens, B, H, KV, hd, max_kv).bytes;
+  return 0;
+}
+
+int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_head, int32_t tokens,
+                      const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens, const int32_t* block_table,
+                      int32_t max_pages, const void* k_cache, const float* k_scale, const void* v_cache,
+                      const float* v_scale, int32_t num_pages, int32_t page, int32_t H, int32_t KV, int32_t hd,
+                      float scale, int32_t causal, int32_t max_kv, void* out, int64_t o_tok, int64_t o_head,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  MLCV_REQUIRE(dtype == MLCV_DTYPE_F16 || dtype == MLCV_DTYPE_BF16, "queries are float16 or bfloat16");
+  MLCV_TRY(kv_attn_sizes_ok(tokens, B, H, KV, hd, max_kv));
+  MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
+  MLCV_REQUIRE(num_pages >= 0 && max_pages >= 0 && (int64_t)num_pages * page <= INT32_MAX &&
+                   (int64_t)max_pages * page <= INT32_MAX, "more than 2^31 - 1 slots");
+  MLCV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
+  if (tokens == 0 || B == 0) return 0;
+  MLCV_REQUIRE(q && cu_seqlens && kv_lens && out, "null pointer");
+  MLCV_REQUIRE(max_pages == 0 || num_pages == 0 || (block_table && k_cache && k_scale && v_cache && v_scale),
+               "null cache");
+  MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
+  const KvAttnPlan p = kv_attn_plan(tokens, B, H, KV, hd, max_kv);
+  MLCV_REQUIRE(p.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes),
+               "workspace missing, not 16-byte aligned or too small");
+  KvAttnArgs a{};
+  a.q = q;
+  a.q_tok = q_tok;
+  a.q_head = q_head;
+  a.o_tok = o_tok;
+  a.o_head = o_head;
+  a.cu = cu_seqlens;
+  a.kv_lens = kv_lens;
+  a.table = block_table;
+  a.kc = static_cast<const uint8_t*>(k_cache);
+  a.vc = static_cast<const uint8_t*>(v_cache);
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.out = out;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o ? a.part_o + p.o_floats : nullptr;
+  a.tokens = tokens;
+  a.B = B;
+  a.H = H;
+  a.KV = KV;
+  a.grp = H / KV;
+  a.max_pages = num_pages > 0 ? max_pages : 0;  // a cache without pages holds nothing that could be read
+  a.num_pages = num_pages;
+  a.psh = log2_of(page);
+  a.causal = causal != 0;
+  a.q_vec = aligned16(q) && q_tok % 8 == 0 && q_head % 8 == 0;
+  a.S = p.S;
+  a.span = p.span;
+  a.c = scale * 1.4426950408889634f;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool bf = dtype == MLCV_DTYPE_BF16;
+  if (hd == 64) return bf ? kv_attn_launch<true, 64>(a, p, st) : kv_attn_launch<false, 64>(a, p, st);
+  if (hd == 128) return bf ? kv_attn_launch<true, 128>(a, p, st) : kv_attn_launch<false, 128>(a, p, st);
+  return bf ? kv_attn_launch<true, 256>(a, p, st) : kv_attn_launch<false, 256>(a, p, st);
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("MLCV_LIB") or os.path.join(os.path.dirname(os.path.ab
 
 MLCV_DTYPE_F16 = 1
 MLCV_DTYPE_F32 = 2
+MLCV_DTYPE_BF16 = 3
 MLCV_QUANT_NONE = 0
 MLCV_QUANT_Q4F16_1 = 1
 MLCV_OPT_USE_GRAPH = 1
@@ -31,6 +32,7 @@ PROBES = {"x": 0, "q": 1, "k": 2, "v": 3, "attn": 4, "x_mid": 5, "h": 6, "mod": 
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 
 
 class MlcvError(RuntimeError):
@@ -83,6 +85,15 @@ SIGNATURES = {
     "mlcv_linear": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
     "mlcv_linear_noalloc": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
     "mlcv_tile_linear": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
+    "mlcv_kv_plan": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "mlcv_kv_write": (ctypes.c_int, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
+                                     _vp, _i32, _i32, _i32, _i32, _vp]),
+    "mlcv_kv_attention_workspace": (ctypes.c_int, [_i32] * 6 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlcv_kv_attention": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp,
+                                         _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _i32, _i32, _vp, _i64, _i64,
+                                         _vp, ctypes.c_size_t, _vp]),
+    "mlcv_prompt_attention": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32,
+                                             _i32, _i32, _i32, ctypes.c_float, _i32, _vp, _vp, _i64, _i64, _vp]),
     "mlcv_bench_op": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
 }
 
