@@ -281,7 +281,8 @@ __global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
   if (start >= stop) return;
   const int slot = a.slots[start];
   const int id = slot >> a.psh, o = slot & (page - 1);
-  if (slot < 0 || id >= a.num_pages) return;
+  // a page after the request's first is written from its beginning
+  if (slot < 0 || id >= a.num_pages || (it.i > 0 && o > 0)) return;
   // positions [o, o + count) of the page are new: the group's tokens up to the first whose slot does not follow
   // its neighbour's
   __syncthreads();
@@ -758,7 +759,7 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   p.R = rows <= 16ll * B ? 1 : 2;
   const int rt = 16 * p.R;
   p.items = rows / rt + B;
-  const long long busy = std::max((rows + rt - 1) / rt, (long long)std::min(B, tokens)) * KV;
+  const long long busy = std::max({1ll, (rows + rt - 1) / rt, (long long)std::min(B, tokens)}) * KV;
   const int tiles = std::max(1, (max_kv + 63) / 64);
   const long long want = std::max(1ll, std::min((1024 + busy - 1) / busy, (long long)(tiles + 3) / 4));
   p.span = (int)((tiles + want - 1) / want);
