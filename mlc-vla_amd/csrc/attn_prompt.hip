@@ -58,11 +58,13 @@ __device__ __forceinline__ f16v mfma32(Elem<true>::V8 a, Elem<true>::V8 b, f16v 
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// 16 bytes per lane from the buffer into LDS at lds + 16 lane (device pass only: in the host pass the builtin
-// drops the kernel's launch stub)
-__device__ __forceinline__ void pr_dma16(__amdgpu_buffer_rsrc_t r, char* lds, int voff) {
+// 16 bytes per lane from the buffer into LDS at lds + 16 lane.  In assembly, because the compiler waits for every
+// DMA in flight before a transposing LDS read, whose memory it does not know; it returns nothing into registers,
+// and the loop waits for it before the barrier after which the tile is read.
+__device__ __forceinline__ void pr_dma16(u4 r, char* lds, int voff) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(r));
 #endif
 }
 // four 16-bit elements of one column: per 16 lanes a 4 x 16 block, lane i giving the address of row i / 4,
@@ -90,14 +92,18 @@ __device__ __forceinline__ int v_slot(int r, int p) {
 }
 
 // DMA of rows [row, row + NK) of one head of K or V into LDS; rows past the prompt's end become zeros (the
-// buffer ends there)
+// buffer ends there; a tile that lies behind it reads nothing)
 template <int HD, int NK, bool V>
 __device__ __forceinline__ void load_tile(const char* base, int64_t tok_bytes, int row, int n, char* lds, int w,
                                           int lane) {
   constexpr int PP = HD / 8, PER = NK * PP / PR_NT;  // 16-byte pieces per row, DMA instructions per wave
-  const int have = min(n - row, NK);                 // >= 1
-  const __amdgpu_buffer_rsrc_t r =
-      dev_rsrc(base + (int64_t)row * tok_bytes, (uint32_t)((have - 1) * tok_bytes + HD * 2));
+  const int have = min(n - row, NK);
+  const uint64_t at = reinterpret_cast<uint64_t>(base) + (int64_t)row * tok_bytes;
+  u4 r;  // a raw buffer
+  r[0] = (uint32_t)at;
+  r[1] = (uint32_t)(at >> 32) & 0xffffu;
+  r[2] = have > 0 ? (uint32_t)((have - 1) * tok_bytes + HD * 2) : 0u;
+  r[3] = 0x00020000u;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int blk = 4 * i + w, slot = blk * 64 + lane, key = slot / PP, s = slot % PP;
@@ -111,15 +117,20 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
   typedef typename Elem<BF>::T T;
   typedef typename Elem<BF>::V8 V8;
   constexpr int TILE = NK * HD * 2, KS = HD / 16, ND = HD / 32, NS = NK / 32;
-  // one LDS object, so that the compiler sees one thing that the DMA and the reads touch
+  // one LDS object: with several, the compiler tags each access with its object and waits for every DMA in flight
+  // before a read of the object that the DMA fills
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lh = lane >> 5;
 
-  // request b has the work items [f(b), f(b + 1)), f(b) = floor(cu[b] / 128) + b, at least ceil(n / 128) of them
+  // request b has the work items [f(b), f(b + 1)), f(b) = floor(cu[b] / 128) + b, at least ceil(n / 128) of them;
+  // the long rows of a causal prompt first
   const int h = blockIdx.x % a.H, item = a.items - 1 - blockIdx.x / a.H;
   int* sh = reinterpret_cast<int*>(lds + 4 * TILE);
-  if (tid == 0) sh[0] = -1;
+  if (tid == 0) {
+    sh[0] = -1;
+    sh[4] = 0;
+  }
   __syncthreads();
   for (int b = tid; b < a.B; b += PR_NT) {
     const int c0 = min(max(a.cu[b], 0), a.tokens), c1 = min(max(a.cu[b + 1], 0), a.tokens);
@@ -145,10 +156,12 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
 
   const char* kb = reinterpret_cast<const char*>(a.k) + 2 * ((int64_t)c0 * a.k_tok + (int64_t)(h / a.grp) * a.k_head);
   const char* vb = reinterpret_cast<const char*>(a.v) + 2 * ((int64_t)c0 * a.v_tok + (int64_t)(h / a.grp) * a.v_head);
+  // K tiles in buffers 0 and 1, V tiles in 2 and 3
   load_tile<HD, NK, false>(kb, 2 * a.k_tok, 0, n, lds, w, lane);
-  load_tile<HD, NK, true>(vb, 2 * a.v_tok, 0, n, lds + TILE, w, lane);
+  load_tile<HD, NK, true>(vb, 2 * a.v_tok, 0, n, lds + 2 * TILE, w, lane);
+  load_tile<HD, NK, false>(kb, 2 * a.k_tok, NK, n, lds + TILE, w, lane);
 
-  V8 q[KS];  // row r, dims 16 ks + 8 lh .. + 7
+  V8 q[KS];  // row l32, dims 16 ks + 8 lh .. + 7
   {
     const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(c0 + min(row, n - 1)) * a.q_tok + (int64_t)h * a.q_head +
                  8 * lh;
@@ -162,139 +175,224 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  for (int t = 0; t < tiles; ++t) {
-    char* cur = lds + (t & 1) * 2 * TILE;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is in LDS
-    __syncthreads();
-    if (t + 1 < tiles) {
-      char* nxt = lds + ((t + 1) & 1) * 2 * TILE;
-      load_tile<HD, NK, false>(kb, 2 * a.k_tok, (t + 1) * NK, n, nxt, w, lane);
-      load_tile<HD, NK, true>(vb, 2 * a.v_tok, (t + 1) * NK, n, nxt + TILE, w, lane);
-    }
-    const int key0 = t * NK;
-    const bool edge = key0 + NK > every;  // some row of the wave does not see all of the tile
-    // a tile that every row sees in part: a non-finite value behind a weight of 0 would reach rows that do not
-    // see its key, so such a tile is looked through, by the whole workgroup
-    bool apart = false;
-    if (key0 + NK > max(row0 + 1, pre)) {
-      int bad = 0;
-      for (int i = tid; i < TILE / 16; i += PR_NT) {
-        const u4 x = *reinterpret_cast<const u4*>(cur + TILE + 16 * i);
-        const uint32_t ones = BF ? 0x7f80u : 0x7c00u;
+  // The operands of a tile's products in their order.  The next logits': K's row 32 u + l32, piece 2 ks + lh.  The
+  // output's: of k step kk and dims 32 d + l32, V's rows 16 kk + 4 lh + (0..3) and 8 more.
+  constexpr int NKF = NS * KS, NVF = 2 * NS * ND;
+  const int vr = 4 * lh + ((lane & 15) >> 2);                // row of the 4 x 16 block this lane addresses
+  const int vc = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);  // its 16-byte piece among the tile's 32 dims
+  auto k_frag = [&](const char* kt, int u, int ks) {
+    return *reinterpret_cast<const V8*>(kt + (32 * u + l32) * HD * 2 + k_slot<HD>(32 * u + l32, 2 * ks + lh) * 16);
+  };
+  auto frag = [&](const char* kt, const char* vt, int i) {
+    if (i < NKF) return k_frag(kt, i % NS, i / NS);
+    const int d = (i - NKF) % ND, kk = (i - NKF) / ND;
+    u4 x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          bad |= (x[j] & ones) == ones || ((x[j] >> 16) & ones) == ones;
-      }
-      apart = __syncthreads_or(bad);
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * kk + 8 * j + vr;
+      const u2v y = pr_read_tr(vt + r * HD * 2 + v_slot<HD>(r, 4 * d + vc) * 16 + 8 * (lane & 1));
+      x[2 * j] = y[0];
+      x[2 * j + 1] = y[1];
     }
-    if (key0 >= some) continue;  // nothing that this wave's rows see
+    return __builtin_bit_cast(V8, x);
+  };
+  // the larger of a row's two lanes, times c
+  auto row_top = [&](float x) {
+    const unsigned bits = __float_as_uint(x);
+    const auto sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.c;
+  };
 
-    f16v s[NS];
+  bool poison = false;  // a non-finite value was taken out of a tile that not every row sees
+  int poison0 = 0;      // the first key of such a tile
+  float top;            // the tile's largest logit of the row, times c
+  V8 ring[2];           // operands: the one in use and the next
+  // Tile t, s its logits; P = t mod 2 (its buffers).  False: no row of this wave sees any of it.
+  auto begin = [&](int t, int P, f16v (&s)[NS]) {
+    const char *kt = lds + (P ^ 1) * TILE, *vt = lds + (2 + P) * TILE;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tiles is in LDS
+    __syncthreads();
+    ring[0] = frag(kt, vt, 0);
+    load_tile<HD, NK, false>(kb, 2 * a.k_tok, (t + 2) * NK, n, lds + P * TILE, w, lane);
+    load_tile<HD, NK, true>(vb, 2 * a.v_tok, (t + 1) * NK, n, lds + (2 + (P ^ 1)) * TILE, w, lane);
+    const int key0 = t * NK;
+    // In a tile that not every row sees whole, a non-finite value behind a weight of 0 would reach rows that do
+    // not see its key.  Such values are cleared here, and added at the end to the rows that see them.
+    if (key0 + NK > max(row0 + 1, pre)) {
+      for (int i = tid; i < TILE / 16; i += PR_NT) {
+        u4* at = reinterpret_cast<u4*>(lds + (2 + P) * TILE + 16 * i);
+        u4 x = *at;
+        const uint32_t ones = BF ? 0x7f80u : 0x7c00u;
+        bool hit = false;
 #pragma unroll
-    for (int u = 0; u < NS; ++u) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-      const char* krow = cur + (32 * u + l32) * HD * 2;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const V8 kf = *reinterpret_cast<const V8*>(krow + k_slot<HD>(32 * u + l32, 2 * ks + lh) * 16);
-        s[u] = mfma32(kf, q[ks], s[u]);
+        for (int j = 0; j < 4; ++j) {
+          const bool lo = (x[j] & ones) == ones, hi = ((x[j] >> 16) & ones) == ones;
+          x[j] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          hit = hit || lo || hi;
+        }
+        if (hit) {
+          *at = x;
+          sh[4] = 1;
+        }
+      }
+      __syncthreads();
+      if (!poison && sh[4]) {
+        poison0 = key0;
+        poison = true;
       }
     }
-    if (edge) {
+    if (key0 >= some) return false;
+    if (key0 + NK > every) {  // some row of the wave does not see all of the tile
+      float x = -INFINITY;
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int e = 0; e < 16; ++e) {
           if (key0 + 32 * u + 8 * (e >> 2) + 4 * lh + (e & 3) >= lim) s[u][e] = -INFINITY;
+          x = fmaxf(x, s[u][e]);
+        }
+      top = row_top(x);
     }
-    float top = -INFINITY;
+    return true;
+  };
+  auto outgrown = [&] { return __any(top > m + 8.0f); };  // also where m is still -inf
+  auto raise = [&] {
+    const float mn = fmaxf(m, top);
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= alpha;
 #pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-    {
-      const unsigned bits = __float_as_uint(top);
-      const auto sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
-      top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.c;
-    }
-    if (__any(top > m + 8.0f)) {  // also where m is still -inf
-      const float mn = fmaxf(m, top);
-      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= alpha;
-    }
+    for (int d = 0; d < ND; ++d) o[d] *= alpha;
+  };
+  // The rest of the tile; nx becomes the next tile's logits (of the last tile: not used).  The matrix products are
+  // issued one by one, each behind the LDS read of the next one's operand and before a share of the softmax: the
+  // next logits' between the exponentials, the output's between the comparisons of the next logits.
+  auto finish = [&](int P, const f16v (&s)[NS], f16v (&nx)[NS]) {
+    const char *kt = lds + (P ^ 1) * TILE, *vt = lds + (2 + P) * TILE;
     const float mu = m == -INFINITY ? 0.f : m;
     V8 p[2 * NS];
+    float big = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], a.c, -mu));
-        l += x;
-        p[2 * u + (e >> 3)][e & 7] = (T)x;
+    for (int i = 0; i < NKF + NVF; ++i) {
+      if (i + 1 < NKF + NVF) {
+        ring[(i + 1) & 1] = frag(kt, vt, i + 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    // V's operand of k step kk, dims 32 d + l32: rows 16 kk + 4 lh + (0..3) and 8 more
-    const int vr = 4 * lh + ((lane & 15) >> 2);  // row of the 4 x 16 block this lane addresses
-    const int vc = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);  // its 16-byte piece among the tile's 32 dims
-    auto v_frag = [&](int d, int kk) {
-      u4 x;
+      const V8 f = ring[i & 1];
+      if (i < NKF) {
+        const int u = i % NS, ks = i / NS;
+        if (ks == 0) {
+          f16v z;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 16 * kk + 8 * j + vr;
-        const u2v y = pr_read_tr(cur + TILE + r * HD * 2 + v_slot<HD>(r, 4 * d + vc) * 16 + 8 * (lane & 1));
-        x[2 * j] = y[0];
-        x[2 * j + 1] = y[1];
-      }
-      return x;
-    };
-    if (!apart) {
-#pragma unroll
-      for (int kk = 0; kk < 2 * NS; ++kk)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = mfma32(__builtin_bit_cast(V8, v_frag(d, kk)), p[kk], o[d]);
-    } else {
-      // key by key: a product with that key alone, added to the rows that see it
-#pragma unroll
-      for (int kk = 0; kk < 2 * NS; ++kk)
-        for (int i = 0; i < 16; ++i) {
-          const int e = i & 7, half = i >> 3, key = key0 + 16 * kk + 8 * (e >> 2) + 4 * half + (e & 3);
-          const uint32_t mine = lh == half ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            u4 x = v_frag(d, kk);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] &= (e >> 1) == j ? mine : 0u;
-            f16v z;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) z[j] = 0.f;
-            z = mfma32(__builtin_bit_cast(V8, x), p[kk], z);
-            if (key < lim) o[d] += z;
-          }
+          for (int e = 0; e < 16; ++e) z[e] = 0.f;
+          nx[u] = mfma32(f, q[0], z);
+        } else {
+          nx[u] = mfma32(f, q[ks], nx[u]);
         }
+        constexpr int EX = 16 / KS;  // exponentials per product
+#pragma unroll
+        for (int j = i * EX; j < (i + 1) * EX; ++j) {
+          const int uu = j / 16, e = j & 15;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[uu][e], a.c, -mu));
+          l += x;
+          p[2 * uu + (e >> 3)][e & 7] = (T)x;
+        }
+      } else {
+        const int d = (i - NKF) % ND, kk = (i - NKF) / ND;
+        o[d] = mfma32(f, p[kk], o[d]);
+        constexpr int MX = 8 / ND;  // comparisons per product
+#pragma unroll
+        for (int j = (i - NKF) * MX; j < (i - NKF + 1) * MX; ++j) big = fmaxf(big, nx[j / 16][j & 15]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    top = row_top(big);
+  };
+
+  f16v s0[NS];
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  __syncthreads();
+  {
+    float x = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s0[u][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s0[u] = mfma32(k_frag(lds, u, ks), q[ks], s0[u]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = fmaxf(x, s0[u][e]);
+    }
+    top = row_top(x);
+  }
+  if constexpr (HD < 256) {
+    f16v s1[NS];
+    auto step = [&](int t, int P, f16v (&s)[NS], f16v (&nx)[NS]) {
+      if (!begin(t, P, s)) return;
+      if (outgrown()) raise();
+      finish(P, s, nx);
+    };
+    for (int t = 0; t < tiles; t += 2) {
+      step(t, 0, s0, s1);
+      if (t + 1 < tiles) step(t + 1, 1, s1, s0);
+    }
+  } else {
+    // The output is rescaled outside the loop that the tiles usually stay in: with a multiply of it inside, the
+    // compiler moves its 128 registers between the two kinds of them in every tile (816 instead of 924 TFLOP/s
+    // over 2 x 4096 tokens of 16 heads; at the smaller head dims, where there is one kind, this form loses 4%).
+    auto advance = [&](int t) {
+      f16v s1[NS];
+      finish(t & 1, s0, s1);
+#pragma unroll
+      for (int u = 0; u < NS; ++u) s0[u] = s1[u];
+    };
+    auto look = [&](int t) { return begin(t, t & 1, s0) ? 1 + outgrown() : 0; };
+    for (int t = 0;;) {
+      bool moved = false;
+      for (; t < tiles; ++t) {
+        const int how = look(t);
+        if (how == 2) {
+          moved = true;
+          break;
+        }
+        if (how == 1) advance(t);
+      }
+      if (!moved) break;
+      raise();
+      advance(t);
+      ++t;
     }
   }
 
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA outlives the loop
   {
     const unsigned bits = __float_as_uint(l);
     const auto sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
-  if (row < n) {
-    const float f = 1.0f / l;  // every row sees its own key at least
-    T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(c0 + row) * a.o_tok + (int64_t)h * a.o_head;
+  if (row >= n) return;
+  if (poison)
+    for (int key = poison0; key < lim; ++key) {
+      const T* x = reinterpret_cast<const T*>(vb + (int64_t)key * 2 * a.v_tok) + 4 * lh;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        typename Elem<BF>::V4 x;
+        for (int i = 0; i < 16; ++i) {
+          const float y = (float)load_global(x + 32 * d + 8 * (i >> 2) + (i & 3));
+          if (!(fabsf(y) < INFINITY)) o[d][i] += y;
+        }
+    }
+  const float f = 1.0f / l;  // every row sees its own key at least
+  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(c0 + row) * a.o_tok + (int64_t)h * a.o_head;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (T)(o[d][4 * i + e] * f);
-        *reinterpret_cast<typename Elem<BF>::V4*>(dst + 32 * d + 8 * i + 4 * lh) = x;
-      }
-  }
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      typename Elem<BF>::V4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (T)(o[d][4 * i + e] * f);
+      *reinterpret_cast<typename Elem<BF>::V4*>(dst + 32 * d + 8 * i + 4 * lh) = x;
+    }
 }
 
 template <bool BF>
