@@ -6,7 +6,8 @@
 //
 // Bound by the matrix cores (4 hd flops per query head and visible pair, against 2 bytes per element read).
 //
-// A workgroup (4 waves) takes 128 rows of one query head of one prompt, 32 per wave, and streams the keys and
+// A workgroup (4 waves) takes 128 rows of one query head of one prompt, 32 per wave (SP = 2: 64 rows, two waves of
+// the same 32 rows each with half of a tile's keys, joined at the end), and streams the keys and
 // values in tiles through two LDS buffers that global -> LDS DMA fills one tile ahead.  A wave computes
 // S^T = K . Q^T and O^T = V^T . P^T on v_mfma_f32_32x32x16: with lane = 32 lh + r, S^T leaves keys
 // 8 i + 4 lh + (0..3) of row r in a lane, and the second product contracts over keys in any order as long as
@@ -112,16 +113,17 @@ __device__ __forceinline__ void load_tile(const char* base, int64_t tok_bytes, i
   }
 }
 
-template <bool BF, int HD, int NK>
+template <bool BF, int HD, int NK, int SP>
 __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(const PromptArgs a) {
   typedef typename Elem<BF>::T T;
   typedef typename Elem<BF>::V8 V8;
-  constexpr int TILE = NK * HD * 2, KS = HD / 16, ND = HD / 32, NS = NK / 32;
+  constexpr int TILE = NK * HD * 2, KS = HD / 16, ND = HD / 32, NS = NK / 32 / SP, ROWS = PR_ROWS / SP;
   // one LDS object: with several, the compiler tags each access with its object and waits for every DMA in flight
   // before a read of the object that the DMA fills
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lh = lane >> 5;
+  const int part = SP == 1 ? 0 : w >> 1, rw = SP == 1 ? w : w & 1;  // this wave's keys of a tile, its rows
 
   // request b has the work items [f(b), f(b + 1)), f(b) = floor(cu[b] / 128) + b, at least ceil(n / 128) of them;
   // the long rows of a causal prompt first
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
   __syncthreads();
   for (int b = tid; b < a.B; b += PR_NT) {
     const int c0 = min(max(a.cu[b], 0), a.tokens), c1 = min(max(a.cu[b + 1], 0), a.tokens);
-    const int f0 = c0 / PR_ROWS + b, f1 = c1 / PR_ROWS + b + 1;
+    const int f0 = c0 / ROWS + b, f1 = c1 / ROWS + b + 1;
     if (f0 <= item && item < f1 && c1 > c0) {
       sh[0] = b;
       sh[1] = c0;
@@ -145,12 +147,12 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
   __syncthreads();
   const int b = __builtin_amdgcn_readfirstlane(sh[0]), c0 = __builtin_amdgcn_readfirstlane(sh[1]);
   const int n = __builtin_amdgcn_readfirstlane(sh[2]);
-  const int row0 = __builtin_amdgcn_readfirstlane(sh[3]) * PR_ROWS;
+  const int row0 = __builtin_amdgcn_readfirstlane(sh[3]) * ROWS;
   if (b < 0 || row0 >= n) return;
   const int pre = a.causal ? (a.bidir ? min(max(load_global(a.bidir + b), 0), n) : 0) : n;
-  const int most = max(min(row0 + PR_ROWS, n), pre);  // keys that some row sees
+  const int most = max(min(row0 + ROWS, n), pre);  // keys that some row sees
   const int tiles = (most + NK - 1) / NK;
-  const int wrow = row0 + 32 * w, row = wrow + l32;
+  const int wrow = row0 + 32 * rw, row = wrow + l32;
   const int lim = min(max(row + 1, pre), n);
   const int every = max(wrow + 1, pre), some = min(max(wrow + 32, pre), n);  // of this wave's rows
 
@@ -178,10 +180,12 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
   // The operands of a tile's products in their order.  The next logits': K's row 32 u + l32, piece 2 ks + lh.  The
   // output's: of k step kk and dims 32 d + l32, V's rows 16 kk + 4 lh + (0..3) and 8 more.
   constexpr int NKF = NS * KS, NVF = 2 * NS * ND;
+  const int kr = 32 * NS * part;                             // the wave's first key of a tile
   const int vr = 4 * lh + ((lane & 15) >> 2);                // row of the 4 x 16 block this lane addresses
   const int vc = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);  // its 16-byte piece among the tile's 32 dims
   auto k_frag = [&](const char* kt, int u, int ks) {
-    return *reinterpret_cast<const V8*>(kt + (32 * u + l32) * HD * 2 + k_slot<HD>(32 * u + l32, 2 * ks + lh) * 16);
+    return *reinterpret_cast<const V8*>(kt + (kr + 32 * u + l32) * HD * 2 +
+                                        k_slot<HD>(kr + 32 * u + l32, 2 * ks + lh) * 16);
   };
   auto frag = [&](const char* kt, const char* vt, int i) {
     if (i < NKF) return k_frag(kt, i % NS, i / NS);
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
     u4 x;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int r = 16 * kk + 8 * j + vr;
+      const int r = kr + 16 * kk + 8 * j + vr;
       const u2v y = pr_read_tr(vt + r * HD * 2 + v_slot<HD>(r, 4 * d + vc) * 16 + 8 * (lane & 1));
       x[2 * j] = y[0];
       x[2 * j + 1] = y[1];
@@ -241,14 +245,14 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
         poison = true;
       }
     }
-    if (key0 >= some) return false;
-    if (key0 + NK > every) {  // some row of the wave does not see all of the tile
+    if (key0 + kr >= some) return false;
+    if (key0 + kr + 32 * NS > every) {  // some row of the wave does not see all of the tile
       float x = -INFINITY;
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          if (key0 + 32 * u + 8 * (e >> 2) + 4 * lh + (e & 3) >= lim) s[u][e] = -INFINITY;
+          if (key0 + kr + 32 * u + 8 * (e >> 2) + 4 * lh + (e & 3) >= lim) s[u][e] = -INFINITY;
           x = fmaxf(x, s[u][e]);
         }
       top = row_top(x);
@@ -370,6 +374,35 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
     const auto sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
+  if constexpr (SP == 2) {
+    // the two waves of the same rows meet: the second hands over its output (16 bytes per lane and instruction),
+    // maximum and sum
+    __syncthreads();
+    f4* po = reinterpret_cast<f4*>(lds) + rw * (ND * 4 * 64 + 32) + lane;
+    f2* pm = reinterpret_cast<f2*>(lds) + (rw * (ND * 4 * 64 + 32) + ND * 4 * 64) * 2 + l32;
+    if (part == 1) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          po[(4 * d + i) * 64] = (f4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+      if (lh == 0) *pm = (f2){m, l};
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const f2 ml = *pm;
+    const float mn = fmaxf(m, ml[0]);  // finite: every row sees a key of its first tile
+    const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[0] - mn);
+    l = l * f0 + ml[1] * f1;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 x = po[(4 * d + i) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][4 * i + e] = o[d][4 * i + e] * f0 + x[e] * f1;
+      }
+  }
   if (row >= n) return;
   if (poison)
     for (int key = poison0; key < lim; ++key) {
@@ -396,11 +429,17 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
 }
 
 template <bool BF>
-int prompt_launch(const PromptArgs& a, int hd, hipStream_t st) {
+int prompt_launch(const PromptArgs& a, int hd, bool split, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)a.items * a.H);
-  if (hd == 64) prompt_attn_kernel<BF, 64, 64><<<grid, PR_NT, 0, st>>>(a);
-  else if (hd == 128) prompt_attn_kernel<BF, 128, 64><<<grid, PR_NT, 0, st>>>(a);
-  else prompt_attn_kernel<BF, 256, 32><<<grid, PR_NT, 0, st>>>(a);
+  if (split) {
+    if (hd == 64) prompt_attn_kernel<BF, 64, 64, 2><<<grid, PR_NT, 0, st>>>(a);
+    else if (hd == 128) prompt_attn_kernel<BF, 128, 64, 2><<<grid, PR_NT, 0, st>>>(a);
+    else prompt_attn_kernel<BF, 256, 64, 2><<<grid, PR_NT, 0, st>>>(a);
+  } else {
+    if (hd == 64) prompt_attn_kernel<BF, 64, 64, 1><<<grid, PR_NT, 0, st>>>(a);
+    else if (hd == 128) prompt_attn_kernel<BF, 128, 64, 1><<<grid, PR_NT, 0, st>>>(a);
+    else prompt_attn_kernel<BF, 256, 32, 1><<<grid, PR_NT, 0, st>>>(a);
+  }
   MLCV_HIP(hipGetLastError());
   return 0;
 }
@@ -421,7 +460,11 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
   MLCV_REQUIRE(hd == 64 || hd == 128 || hd == 256, "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   MLCV_REQUIRE(causal || !bidir, "bidir goes with causal attention");
-  const int64_t items = (int64_t)tokens / PR_ROWS + B;
+  // Few rows: workgroups of 64 rows, whose waves share them by keys, while even those leave no CU two of them
+  // (up to 128 workgroups of 128 rows).  One prompt of 968 tokens, 8 heads of 256: 43.9 -> 32.2 us; 16 heads of 128:
+  // 24.5 -> 19.4, of 64: 17.6 -> 13.7.  At 256 workgroups it is level (heads of 64 and 128) or 1.28 times slower.
+  const bool split = ((int64_t)tokens + PR_ROWS - 1) / PR_ROWS * H <= 128;
+  const int64_t items = (int64_t)tokens / (split ? PR_ROWS / 2 : PR_ROWS) + B;
   MLCV_REQUIRE(items * H <= INT32_MAX, "too many workgroups");
   if (tokens == 0 || B == 0) return 0;
   MLCV_REQUIRE(q && k && v && cu_seqlens && out, "null pointer");
@@ -438,5 +481,5 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
   PromptArgs a{q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_seqlens, bidir, tokens, B,
                H, H / KV, causal != 0, (int32_t)items, scale * 1.4426950408889634f};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return dtype == MLCV_DTYPE_BF16 ? prompt_launch<true>(a, hd, st) : prompt_launch<false>(a, hd, st);
+  return dtype == MLCV_DTYPE_BF16 ? prompt_launch<true>(a, hd, split, st) : prompt_launch<false>(a, hd, split, st);
 }
