@@ -164,12 +164,14 @@ __device__ __forceinline__ int clamp_i(int v, int lo, int hi) { return v < lo ? 
 struct Item {
   int b, c0, n;  // request, its first token and number of tokens; b = -1: none
   int i;         // the item's number within its request
+  int len;       // its kv_lens entry, where the caller gives them
 };
-__device__ __forceinline__ Item find_item(const int32_t* cu, int B, int tokens, long long item, int mul, int div,
-                                          int extra, int* sh) {
+__device__ __forceinline__ Item find_item(const int32_t* cu, const int32_t* lens, int B, int tokens, long long item,
+                                          int mul, int div, int extra, int* sh) {
   if (threadIdx.x == 0) sh[0] = -1;
   __syncthreads();
   for (int b = threadIdx.x; b < B; b += KV_NT) {
+    const int len = lens ? lens[b] : 0;
     const int c0 = clamp_i(cu[b], 0, tokens), c1 = clamp_i(cu[b + 1], 0, tokens);
     const long long f0 = (long long)c0 * mul / div + (long long)extra * b;
     const long long f1 = (long long)c1 * mul / div + (long long)extra * (b + 1);
@@ -178,6 +180,7 @@ __device__ __forceinline__ Item find_item(const int32_t* cu, int B, int tokens, 
       sh[1] = c0;
       sh[2] = c1 - c0;
       sh[3] = (int)(item - f0);
+      sh[4] = len;
     }
   }
   __syncthreads();
@@ -186,6 +189,7 @@ __device__ __forceinline__ Item find_item(const int32_t* cu, int B, int tokens, 
   r.c0 = __builtin_amdgcn_readfirstlane(sh[1]);
   r.n = __builtin_amdgcn_readfirstlane(sh[2]);
   r.i = __builtin_amdgcn_readfirstlane(sh[3]);
+  r.len = __builtin_amdgcn_readfirstlane(sh[4]);
   return r;
 }
 
@@ -269,11 +273,11 @@ __device__ __forceinline__ uint32_t byte_mask(int lo, int hi) {
 template <int HD, int UNITS>
 __global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
   constexpr int CH = HD / 8;               // 8-dim pieces of a row
-  __shared__ int sh[4];
+  __shared__ int sh[5];
   __shared__ float smax[KV_NT / 64];
   __shared__ __attribute__((aligned(16))) char turn[HD * (UNITS * KV_NT / CH * 4 + 16)];
   const int tid = threadIdx.x, page = 1 << a.psh, h = blockIdx.y, z = blockIdx.z;
-  const Item it = find_item(a.cu, a.B, a.tokens, blockIdx.x, 1, page, 2, sh);
+  const Item it = find_item(a.cu, nullptr, a.B, a.tokens, blockIdx.x, 1, page, 2, sh);
   if (it.b < 0) return;
   const int o0 = a.slots[it.c0] & (page - 1);  // of a negative slot: any value, the tokens are dropped below
   const int start = it.i == 0 ? it.c0 : it.c0 + it.i * page - o0;
@@ -437,7 +441,6 @@ __device__ __forceinline__ typename El<BF>::V8 widen8(uint32_t lo, uint32_t hi) 
   }
   return __builtin_bit_cast(typename El<BF>::V8, w);
 }
-__device__ __forceinline__ bool has_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // keys that any row of [row0, row0 + rows) of a request sees
 __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, int kv_len, int row0, int rt) {
@@ -447,14 +450,16 @@ __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, i
 
 // Row r of a request is token r / grp of its n new tokens and head h * grp + r % grp: the query heads of a kv
 // head share its keys.  A workgroup (4 waves) takes RT = 16 R such rows and one split of the keys; its waves
-// take tiles of 64 keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
+// take tiles of TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
 //
 // A wave's tile has no LDS and no shuffle of data in it.  S^T = K . Q^T and O^T = V^T . P^T on
 // v_mfma_f32_16x16x32: with lane = 16 g + r, S^T puts keys 4 g .. 4 g + 3 of each 16-key sub-tile and query row
 // r into a lane, and the second product wants 8 keys of row r in it.  Both contractions may run in any order,
-// so the order is chosen by the loads: sub-tile t's row 4 g + i is key 16 g + 4 t + i of the tile, a lane then
-// owns keys 16 g .. 16 g + 15, which are 16 contiguous bytes of the value page, lie in one page and have one
-// scale of each side.  Dims likewise: a lane's 16 key bytes are two steps of the first contraction.
+// so the order is chosen by the loads: with PL = TK / 4, sub-tile s's row 4 g + i is key PL g + 4 s + i of the
+// tile; a lane then owns PL consecutive keys, which are PL contiguous bytes of the value page, lie in one page
+// and have one scale of each side.  Dims likewise: a lane's 16 key bytes are two steps of the first contraction.
+// The loads of a wave's next tile are issued as soon as their registers are free: the keys' behind the first
+// product, the values' behind the second, the page numbers a tile earlier.
 //
 // The value scale is folded into the weights before they are rounded to fp16: with x = logit * log2(e) the
 // running maximum is that of x + log2(scale_v), so that w = 2^(x - m) * scale_v stays within [0, 2^12] whatever
@@ -462,41 +467,87 @@ __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, i
 // of query (an e4m3 value is exact in it).  2^12 of headroom keeps weights down to 2^-26 of the largest above
 // fp16's subnormals.
 //
-// A key or page that a row does not see has weight 0, which a NaN code behind it would turn into NaN: codes
-// behind the request's last token are cleared, and a tile of which some rows see a NaN and others do not is
-// taken key by key (visible_only).
-template <bool BF, int HD, int R>
-__global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
+// A key or page that a row does not see has weight 0, which a NaN code behind it would turn into NaN.  In a tile
+// that not every row sees whole such codes are cleared, and at the end the rows that do see one are set to NaN.
+template <bool BF, int HD, int R, int TK, bool ROWS>
+__global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const KvAttnArgs a) {
   typedef typename El<BF>::T T;
   typedef typename El<BF>::V8 V8;
-  constexpr int RT = 16 * R, NJ = HD / 64, ND = HD / 16;
-  __shared__ int sh[4];
-  __shared__ float sm[4][RT], sl[4][RT];
-  __shared__ __attribute__((aligned(16))) float so[4][RT][64 + 4];
+  constexpr int RT = ROWS ? 64 * R : 16 * R, NJ = HD / 64, ND = HD / 16, SUB = TK / 16, PL = TK / 4, VW = PL / 4;
+  constexpr int STEP = ROWS ? 1 : 4;  // tiles from one of a wave's to its next
+  typedef uint32_t VWords __attribute__((ext_vector_type(VW)));
+  __shared__ int sh[5];
+  __shared__ float sm[4][16 * R], sl[4][16 * R];
+  __shared__ __attribute__((aligned(16))) float so[ROWS ? 1 : 4][ROWS ? 1 : 16 * R][HD + 4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / (a.KV * a.S), rest = blockIdx.x % (a.KV * a.S);
   const int h = rest % a.KV, split = rest / a.KV;
-  const Item it = find_item(a.cu, a.B, a.tokens, item, a.grp, RT, 1, sh);
+  const Item it = find_item(a.cu, a.kv_lens, a.B, a.tokens, item, a.grp, RT, 1, sh);
   if (it.b < 0) return;
   const int rows = it.n * a.grp, row0 = it.i * RT, page = 1 << a.psh;
-  if (row0 >= rows) return;
-  const int kv_len = clamp_i(load_global(a.kv_lens + it.b), 0, a.max_pages << a.psh);
+  const int wrow = ROWS ? row0 + 16 * R * w : row0;  // this wave's first row
+  if (ROWS ? wrow >= rows : row0 >= rows) return;
+  const int kv_len = clamp_i(it.len, 0, a.max_pages << a.psh);
   const int most = last_limit(a, it, kv_len, row0, RT);
-  const int first = a.causal ? kv_len - it.n + row0 / a.grp + 1 : kv_len;  // keys that every row sees
-  const int tiles = (most + 63) >> 6;
-  const int t_begin = split * a.span, t_end = split == a.S - 1 ? tiles : min(tiles, t_begin + a.span);
+  const int first = a.causal ? kv_len - it.n + wrow / a.grp + 1 : kv_len;  // keys that every row of the wave sees
+  const int t_begin = split * a.span * (64 / TK), tiles = (most + TK - 1) / TK;
+  const int t_end = split == a.S - 1 ? tiles : min(tiles, t_begin + a.span * (64 / TK));
   if (split > 0 && t_begin >= tiles) return;
+
+  const int32_t* table = a.table + (size_t)it.b * a.max_pages;
+  // pages of this lane's key row and of its own keys in tile t; -1: none that can be read
+  struct Pages {
+    int k, v;
+  };
+  auto pages_at = [&](int t) {
+    auto one = [&](int pos) {
+      const int pg = pos >> a.psh;
+      const int id = pg < a.max_pages ? load_global(table + pg) : -1;
+      return id >= 0 && id < a.num_pages ? id : -1;
+    };
+    return Pages{one(TK * t + PL * (r16 >> 2)), one(TK * t + PL * g)};
+  };
+  u4 kr[SUB][NJ];
+  VWords vr[ND];
+  auto load_keys = [&](int t, int id) {
+    const int pos = TK * t + PL * (r16 >> 2) + (r16 & 3);
+    const uint8_t* p = a.kc + (((size_t)max(id, 0) * a.KV + h) * page + (pos & (page - 1))) * HD + 16 * g;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) kr[s][j] = load_global(reinterpret_cast<const u4*>(p + 4 * s * HD + 64 * j));
+  };
+  auto load_values = [&](int t, int id) {
+    const uint8_t* p = a.vc + (((size_t)max(id, 0) * a.KV + h) * HD + r16) * page + ((TK * t + PL * g) & (page - 1));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const VWords*>(p + (size_t)16 * d * page));
+  };
+  int t = ROWS ? t_begin : t_begin + w;
+  Pages now = {-1, -1}, next = {-1, -1};
+  float sk = 0.f, sv = 0.f;  // scales of the lane's keys
+  auto load_scales = [&](int id) {
+    const size_t i = (size_t)max(id, 0) * a.KV + h;
+    sk = load_global(a.ks + i);
+    sv = load_global(a.vs + i);
+  };
+  if (t < t_end) {
+    now = pages_at(t);
+    if (t + STEP < t_end) next = pages_at(t + STEP);
+    load_scales(now.v);
+    load_keys(t, now.k);
+    load_values(t, now.v);
+  }
 
   // the query operand: row r16 of each 16, dims 64 j + 16 g + 8 s .. + 7 for step 2 j + s
   V8 q[R][2 * NJ];
   int lim[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = min(row0 + 16 * r + r16, rows - 1), t = row / a.grp;
-    lim[r] = a.causal ? kv_len - it.n + t + 1 : kv_len;
-    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(it.c0 + t) * a.q_tok +
-                 (int64_t)(h * a.grp + row - t * a.grp) * a.q_head + 16 * g;
+    const int row = min(wrow + 16 * r + r16, rows - 1), tok = row / a.grp;
+    lim[r] = a.causal ? kv_len - it.n + tok + 1 : kv_len;
+    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(it.c0 + tok) * a.q_tok +
+                 (int64_t)(h * a.grp + row - tok * a.grp) * a.q_head + 16 * g;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -518,31 +569,17 @@ __global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[r][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
-  const int32_t* table = a.table + (size_t)it.b * a.max_pages;
-  // page of the 16 keys at `pos`; -1: none that can be read
-  auto page_at = [&](int pos) {
-    const int pg = pos >> a.psh;
-    const int id = pg < a.max_pages ? load_global(table + pg) : -1;
-    return id >= 0 && id < a.num_pages ? id : -1;
-  };
-  for (int t = t_begin + w; t < t_end; t += 4) {
-    const int pk = 64 * t + 16 * (r16 >> 2) + (r16 & 3), pv = 64 * t + 16 * g;
-    const int idk = page_at(64 * t + 16 * (r16 >> 2)), idv = page_at(pv);
-    const uint8_t* kp = a.kc + (((size_t)max(idk, 0) * a.KV + h) * page + (pk & (page - 1))) * HD + 16 * g;
-    const uint8_t* vp = a.vc + (((size_t)max(idv, 0) * a.KV + h) * HD + r16) * page + (pv & (page - 1));
-    u4 kr[4][NJ], vr[ND];
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) kr[s][j] = load_global(reinterpret_cast<const u4*>(kp + 4 * s * HD + 64 * j));
-    const size_t si = (size_t)max(idv, 0) * a.KV + h;
-    const float skc = load_global(a.ks + si) * a.c, sv = load_global(a.vs + si);
-#pragma unroll
-    for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const u4*>(vp + (size_t)16 * d * page));
+  bool poison = false;  // a NaN code was cleared
+  for (; t < t_end; t += STEP) {
+    const int pv = TK * t + PL * g;
+    const float skc = sk * a.c, svc = sv;
+    const bool more = t + STEP < t_end;
+    Pages after = {-1, -1};
+    if (t + 2 * STEP < t_end) after = pages_at(t + 2 * STEP);
 
-    f4 x[R][4];
+    f4 x[R][SUB];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < SUB; ++s) {
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r][s] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -555,30 +592,36 @@ __global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
         }
       }
     }
-    const int own = idv < 0 ? 0 : clamp_i(kv_len - pv, 0, 16);  // the lane's keys that are the request's
-    const bool edge = 64 * t + 64 > first || __any(idv < 0);
-    bool apart = false;  // some rows see a NaN that others do not
+    if (more) {
+      load_scales(next.v);
+      load_keys(t + STEP, next.k);
+    }
+    const int own = now.v < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
+    const bool edge = TK * t + TK > first || __any(now.v < 0);
     if (edge) {
       bool nan = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < VW; ++i) {
         const uint32_t keep = byte_mask(0, own - 4 * i);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           vr[d][i] &= keep;
-          nan = nan || has_nan(vr[d][i]);
+          // bytes that are NaN codes (0x7f or 0xff) to zero
+          const uint32_t bad = ((((vr[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+          nan = nan || bad;
+          vr[d][i] &= ~bad;
         }
       }
-      apart = a.causal && __any(nan);
+      poison = poison || __any(nan);
     }
-    const float lsv = __builtin_amdgcn_logf(fmaxf(sv, 0x1p-64f)) - 12.0f;
-    h8 p[R][2];
+    const float lsv = __builtin_amdgcn_logf(fmaxf(svc, 0x1p-64f)) - 12.0f;
+    h8 p[R][PL / 8];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float top = -INFINITY;
       const int see = min(lim[r] - pv, own);  // keys pv .. pv + see - 1 are visible
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = x[r][s][i] * skc;
@@ -592,45 +635,75 @@ __global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
       m[r] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float e = __builtin_amdgcn_exp2f(x[r][s][i] - mu);
           sum += e;
-          p[r][s >> 1][4 * (s & 1) + i] = (_Float16)(e * sv);
+          p[r][s >> 1][4 * (s & 1) + i] = (_Float16)(e * svc);
         }
       l[r] = l[r] * alpha + sum;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
     }
-    if (!apart) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int k = 0; k < PL / 8; ++k) {
+        const h8 v = widen8<false>(vr[d][2 * k], vr[d][2 * k + 1]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) o[r][d] = mfma16(v, p[r][k], o[r][d]);
+      }
+    if (more) load_values(t + STEP, next.v);
+    now = next;
+    next = after;
+  }
+  if (poison)  // the tiles of this wave that hold keys from `first` on, or pages that are not there
+    for (t = ROWS ? t_begin : t_begin + w; t < t_end; t += STEP) {
+      const int idv = pages_at(t).v;
+      if (!(TK * t + TK > first || __any(idv < 0))) continue;
+      load_values(t, idv);
+      const int own = idv < 0 ? 0 : clamp_i(kv_len - (TK * t + PL * g), 0, PL);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const h8 v0 = widen8<false>(vr[d][0], vr[d][1]), v1 = widen8<false>(vr[d][2], vr[d][3]);
+        int at = 0x7fffffff;  // the first of the lane's keys whose value at dim 16 d + r16 is NaN
+        for (int i = PL - 1; i >= 0; --i)
+          if (i < own && (vr[d][i >> 2] >> (8 * (i & 3)) & 0x7f) == 0x7f) at = TK * t + PL * g + i;
+        at = min(at, __shfl_xor(at, 16));
+        at = min(at, __shfl_xor(at, 32));
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          o[r][d] = mfma16(v0, p[r][0], o[r][d]);
-          o[r][d] = mfma16(v1, p[r][1], o[r][d]);
-        }
-      }
-    } else {
-      // key by key: a product with that key alone, added to the rows that see it
-      for (int key = 0; key < 64; ++key) {
-        const int e = key & 7, s = (key >> 3) & 1;
-        const uint32_t mine = g == (key >> 4) ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+        for (int i = 0; i < 4; ++i) {
+          const int key = __shfl(at, 4 * g + i);  // of dim 16 d + 4 g + i
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          u4 v = __builtin_bit_cast(u4, s ? widen8<false>(vr[d][2], vr[d][3]) : widen8<false>(vr[d][0], vr[d][1]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] &= (e >> 1) == i ? mine : 0u;
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const f4 add = mfma16(__builtin_bit_cast(h8, v), s ? p[r][1] : p[r][0], (f4){0.f, 0.f, 0.f, 0.f});
-            if (64 * t + key < lim[r]) o[r][d] += add;
-          }
+          for (int r = 0; r < R; ++r)
+            if (key < lim[r]) o[r][d][i] = NAN;
         }
       }
     }
+
+  const size_t part0 = (((size_t)item * a.KV + h) * a.S + split) * RT;  // of the partial results' rows
+  if constexpr (ROWS) {  // every wave has the split's result for its own rows
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = wrow + 16 * r + r16, tok = row / a.grp;
+      l[r] = xor_sum_16_32(l[r]);
+      if (row >= rows) continue;
+      if (a.S > 1) {
+        if (g == 0) reinterpret_cast<f2*>(a.part_ml)[part0 + row - row0] = (f2){m[r], l[r]};
+        float* dst = a.part_o + (part0 + row - row0) * HD + 4 * g;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = o[r][d];
+      } else {
+        const float f = l[r] > 0.f ? 1.0f / l[r] : l[r] == 0.f ? 0.f : l[r];  // nothing visible: zeros; NaN stays
+        T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + tok) * a.o_tok +
+                 (int64_t)(h * a.grp + row - tok * a.grp) * a.o_head + 4 * g;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dst[16 * d + k] = (T)(o[r][d][k] * f);
+      }
+    }
+    return;
   }
 
   // ---- the waves meet ------------------------------------------------------------------------------
@@ -655,94 +728,112 @@ __global__ __launch_bounds__(KV_NT, 1) void kv_attn_kernel(const KvAttnArgs a) {
     for (int i = 0; i < 4; ++i) sum += sl[i][row] * __builtin_amdgcn_exp2f(sm[i][row] - mu);
     if (a.S > 1) {
       if (w == 0 && g == 0 && row0 + row < rows) {
-        f2* ml = reinterpret_cast<f2*>(a.part_ml) +
-                 (((size_t)item * a.KV + h) * a.S + split) * RT + row;
-        *ml = (f2){mx, sum};
+        reinterpret_cast<f2*>(a.part_ml)[part0 + row] = (f2){mx, sum};
       }
     } else {
       f[r] = sum > 0.f ? f[r] / sum : sum == 0.f ? 0.f : sum;  // nothing visible: zeros; NaN stays
     }
   }
 #pragma unroll
-  for (int c = 0; c < NJ; ++c) {  // 64 dims at a time
-    if (c > 0) __syncthreads();
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int d = 0; d < ND; ++d) {
+      f4 v = o[r][d];
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        f4 v = o[r][4 * c + d];
+      for (int i = 0; i < 4; ++i) v[i] = f[r] == 0.f ? 0.f : v[i] * f[r];
+      *reinterpret_cast<f4*>(&so[w][16 * r + r16][16 * d + 4 * g]) = v;
+    }
+  __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = f[r] == 0.f ? 0.f : v[i] * f[r];
-        *reinterpret_cast<f4*>(&so[w][16 * r + r16][16 * d + 4 * g]) = v;
-      }
-    __syncthreads();
+  for (int i = tid; i < RT * HD / 4; i += KV_NT) {
+    const int row = i / (HD / 4), d = 4 * (i % (HD / 4));
+    if (row0 + row >= rows) continue;
+    f4 v = *reinterpret_cast<const f4*>(&so[0][row][d]);
 #pragma unroll
-    for (int i = tid; i < RT * 16; i += KV_NT) {
-      const int row = i >> 4, d = 4 * (i & 15);
-      if (row0 + row >= rows) continue;
-      f4 v = *reinterpret_cast<const f4*>(&so[0][row][d]);
+    for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const f4*>(&so[k][row][d]);
+    if (a.S > 1) {
+      *reinterpret_cast<f4*>(a.part_o + (part0 + row) * HD + d) = v;
+    } else {
+      const int rr = row0 + row, tok = rr / a.grp;
+      T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + tok) * a.o_tok +
+               (int64_t)(h * a.grp + rr - tok * a.grp) * a.o_head + d;
 #pragma unroll
-      for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const f4*>(&so[k][row][d]);
-      if (a.S > 1) {
-        float* dst = a.part_o + ((((size_t)item * a.KV + h) * a.S + split) * RT + row) * HD + 64 * c + d;
-        *reinterpret_cast<f4*>(dst) = v;
-      } else {
-        const int rr = row0 + row, t = rr / a.grp;
-        T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + t) * a.o_tok +
-                 (int64_t)(h * a.grp + rr - t * a.grp) * a.o_head + 64 * c + d;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) dst[k] = (T)v[k];
-      }
+      for (int k = 0; k < 4; ++k) dst[k] = (T)v[k];
     }
   }
 }
 
-// The splits of one row: sums of the partial results under their common maximum.  One workgroup per row, so
-// that the reads of a long request's many splits spread over the GPU; HD / 4 threads for one split's row.
-template <bool BF, int HD>
+// The splits of one row: the partial results under their common maximum.  W waves take DC dims of one row, DC / 4
+// lanes one split of it at a time.  Few splits: a wave takes a whole row.  Many: a workgroup takes 64 dims of one, so
+// that the reads spread over the GPU (two rows of 8 heads and 128 splits: 5.2 us, with whole rows 8.1).
+template <bool BF, int HD, int W, int DC>
 __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int rt) {
   typedef typename El<BF>::T T;
-  constexpr int NQ = HD / 4, NG = KV_NT / NQ;
-  __shared__ int sh[4];
-  __shared__ __attribute__((aligned(16))) float so[NG][HD];
-  __shared__ float sl[NG];
-  const int tid = threadIdx.x, row = blockIdx.x % rt, h = blockIdx.x / rt % a.KV;
-  const int item = blockIdx.x / (rt * a.KV);
-  const Item it = find_item(a.cu, a.B, a.tokens, item, a.grp, rt, 1, sh);
-  if (it.b < 0) return;
-  const int rr = it.i * rt + row;
-  if (rr >= it.n * a.grp) return;
-  const int kv_len = clamp_i(load_global(a.kv_lens + it.b), 0, a.max_pages << a.psh);
-  const int tiles = (last_limit(a, it, kv_len, it.i * rt, rt) + 63) >> 6;
-  const int n = clamp_i((tiles + a.span - 1) / a.span, 1, a.S);  // splits that there are
+  constexpr int LQ = DC / 4, NG = 64 * W / LQ, NC = HD / DC;  // lanes of a split, splits at once, pieces of a row
+  __shared__ __attribute__((aligned(16))) float so[W][DC];
+  __shared__ float sl[W];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const long long at = W == 1 ? (long long)blockIdx.x * 4 + w : blockIdx.x / NC;
+  const int token = (int)(at / a.H), head = (int)(at % a.H), h = head / a.grp;
+  // the token's request
+  int b = -1, c0 = 0, n = 0, kv_len = 0;
+  for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
+    const int i = min(b0 + lane, a.B - 1);
+    const int x = clamp_i(a.cu[i], 0, a.tokens), y = clamp_i(a.cu[i + 1], 0, a.tokens), len = a.kv_lens[i];
+    const unsigned long long hit = __ballot(x <= token && token < y);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      b = min(b0 + src, a.B - 1);
+      c0 = __builtin_amdgcn_readlane(x, src);
+      n = __builtin_amdgcn_readlane(y, src) - c0;
+      kv_len = clamp_i(__builtin_amdgcn_readlane(len, src), 0, a.max_pages << a.psh);
+    }
+  }
+  if (token >= a.tokens || b < 0) return;
+  Item it;
+  it.n = n;
+  const int rr = (token - c0) * a.grp + head - h * a.grp, tile = rr / rt, row = rr - tile * rt;
+  const long long item = (long long)c0 * a.grp / rt + b + tile;
+  const int tiles = (last_limit(a, it, kv_len, tile * rt, rt) + 63) >> 6;
+  const int splits = clamp_i((tiles + a.span - 1) / a.span, 1, a.S);  // splits that there are
   const size_t p0 = ((size_t)item * a.KV + h) * a.S * rt + row;
   const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + p0;
   float mx = -INFINITY;
-  for (int s = 0; s < n; ++s) mx = fmaxf(mx, load_global(ml + (size_t)s * rt)[0]);
+  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, load_global(ml + (size_t)s * rt)[0]);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
   const float mu = mx == -INFINITY ? 0.f : mx;
-  const int gq = tid / NQ, d = 4 * (tid % NQ);
+  const int gq = (W == 1 ? lane : tid) / LQ, d = 4 * (lane % LQ), d0 = W == 1 ? 0 : (int)(blockIdx.x % NC) * DC;
   f4 v = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
-  for (int s = gq; s < n; s += NG) {
+#pragma unroll 4
+  for (int s = gq; s < splits; s += NG) {
     const f2 e = load_global(ml + (size_t)s * rt);
     const float f = __builtin_amdgcn_exp2f(e[0] - mu);
-    const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * rt) * HD + d));
+    const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * rt) * HD + d0 + d));
     if (f != 0.f) v += u * f;
     sum += e[1] * f;
   }
-  *reinterpret_cast<f4*>(&so[gq][d]) = v;
-  if (d == 0) sl[gq] = sum;
-  __syncthreads();
-  if (gq > 0) return;
 #pragma unroll
-  for (int k = 1; k < NG; ++k) {
-    v += *reinterpret_cast<const f4*>(&so[k][d]);
-    sum += sl[k];
+  for (int s = LQ; s < 64; s <<= 1) {  // the splits within a wave
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], s);
+    sum += __shfl_xor(sum, s);
   }
+  if constexpr (W > 1) {
+    if (lane < LQ) *reinterpret_cast<f4*>(&so[w][d]) = v;
+    if (lane == 0) sl[w] = sum;
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      v += *reinterpret_cast<const f4*>(&so[k][d]);
+      sum += sl[k];
+    }
+  }
+  if (lane >= LQ) return;
   const float f = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
-  const int t = rr / a.grp;
-  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + t) * a.o_tok +
-           (int64_t)(h * a.grp + rr - t * a.grp) * a.o_head + d;
+  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)token * a.o_tok + (int64_t)head * a.o_head + d0 + d;
 #pragma unroll
   for (int k = 0; k < 4; ++k) dst[k] = (T)(v[k] * f);
 }
@@ -750,6 +841,8 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int 
 // How an attention call is cut: rows per workgroup and splits of the keys, from what the host knows.
 struct KvAttnPlan {
   int R, S, span;
+  bool rows;  // the waves of a workgroup share its rows instead of its keys
+  int rt() const { return (rows ? 64 : 16) * R; }
   long long items;
   size_t o_floats, bytes;
 };
@@ -757,11 +850,16 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   KvAttnPlan p;
   const long long grp = H / KV, rows = tokens * grp;
   p.R = rows <= 16ll * B ? 1 : 2;
-  const int rt = 16 * p.R;
+  p.rows = rows > 32ll * B;
+  const int rt = p.rt();
   p.items = rows / rt + B;
   const long long busy = std::max({1ll, (rows + rt - 1) / rt, (long long)std::min(B, tokens)}) * KV;
   const int tiles = std::max(1, (max_kv + 63) / 64);
-  const long long want = std::max(1ll, std::min((1024 + busy - 1) / busy, (long long)(tiles + 3) / 4));
+  // Splits while the workgroups still are resident at once (two to a CU with 16 rows, one with more registers): 48
+  // requests of 8 kv heads take 64 us in one split each, 70 in two (768 workgroups); two requests of 131072 tokens
+  // 38 us in 128 or 256, 45 in 512.  At least a tile for every wave (rows: two tiles of 64).
+  const long long fit = (p.R == 1 ? 512 : 256) / busy, least = p.rows || hd == 256 ? 2 : 4;
+  const long long want = std::max(1ll, std::min(fit, (tiles + least - 1) / least));
   p.span = (int)((tiles + want - 1) / want);
   p.S = (tiles + p.span - 1) / p.span;
   const size_t parts = (size_t)p.items * KV * p.S * rt;
@@ -790,11 +888,16 @@ int kv_write_launch(const WriteArgs& a, hipStream_t st) {
 template <bool BF, int HD>
 int kv_attn_launch(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_t st) {
   const unsigned grid = (unsigned)(p.items * a.KV * p.S);
-  if (p.R == 1) kv_attn_kernel<BF, HD, 1><<<grid, KV_NT, 0, st>>>(a);
-  else kv_attn_kernel<BF, HD, 2><<<grid, KV_NT, 0, st>>>(a);
+  constexpr int TK = HD == 256 ? 32 : 64;
+  if (p.rows && p.R == 1) kv_attn_kernel<BF, HD, 1, TK, true><<<grid, KV_NT, 0, st>>>(a);
+  else if (p.rows) kv_attn_kernel<BF, HD, 2, TK, true><<<grid, KV_NT, 0, st>>>(a);
+  else if (p.R == 1) kv_attn_kernel<BF, HD, 1, TK, false><<<grid, KV_NT, 0, st>>>(a);
+  else kv_attn_kernel<BF, HD, 2, TK, false><<<grid, KV_NT, 0, st>>>(a);
   MLCV_HIP(hipGetLastError());
   if (p.S > 1) {
-    kv_join_kernel<BF, HD><<<(unsigned)(p.items * a.KV * 16 * p.R), KV_NT, 0, st>>>(a, 16 * p.R);
+    const long long rows = (long long)a.tokens * a.H;
+    if (p.S <= 16) kv_join_kernel<BF, HD, 1, HD><<<(unsigned)((rows + 3) / 4), KV_NT, 0, st>>>(a, p.rt());
+    else kv_join_kernel<BF, HD, 4, 64><<<(unsigned)(rows * (HD / 64)), KV_NT, 0, st>>>(a, p.rt());
     MLCV_HIP(hipGetLastError());
   }
   return 0;
@@ -880,7 +983,7 @@ static int kv_attn_sizes_ok(int32_t tokens, int32_t B, int32_t H, int32_t KV, in
   MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE((int64_t)tokens * (H / KV) <= INT32_MAX, "more than 2^31 - 1 query rows of a kv head");
   const KvAttnPlan p = kv_attn_plan(tokens, std::max(B, 1), H, KV, hd, max_kv);
-  MLCV_REQUIRE(p.items * KV * std::max(p.S, 16 * p.R) <= INT32_MAX, "too many workgroups");
+  MLCV_REQUIRE(p.items * KV * p.S <= INT32_MAX && (int64_t)tokens * H * (hd / 64) <= INT32_MAX, "too many workgroups");
   return 0;
 }
 
