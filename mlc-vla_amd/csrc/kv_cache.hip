@@ -21,6 +21,7 @@ namespace mlcv {
 namespace {
 
 constexpr int KV_NT = 256;         // threads per workgroup of every kernel here
+constexpr int KV_RT = 16;          // query rows of an attention workgroup
 constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
 
 // ---- plan ------------------------------------------------------------------------------------------
@@ -441,7 +442,7 @@ struct KvAttnArgs {
   const uint8_t *kc, *vc;
   const float *ks, *vs;
   void* out;
-  float *part_o, *part_ml;  // of the splits: O [items][KV][S][RT][HD], (m, l) [items][KV][S][RT]
+  float *part_o, *part_ml;  // of the splits: O [items][KV][S][16][HD], (m, l) [items][KV][S][16]
   int32_t tokens, B, H, KV, grp, max_pages, num_pages, psh, causal, q_vec;
   int32_t S, span;   // splits, tiles of 64 keys per split
   float c;           // scale * log2(e)
@@ -488,8 +489,8 @@ __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, i
 }
 
 // Row r of a request is token r / grp of its n new tokens and head h * grp + r % grp: the query heads of a kv
-// head share its keys.  A workgroup (4 waves) takes RT = 16 R such rows and one split of the keys; its waves
-// take tiles of TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
+// head share its keys.  A workgroup (4 waves) takes 16 such rows and one split of the keys; its waves take tiles of
+// TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
 //
 // A wave's tile has no LDS and no shuffle of data in it.  S^T = K . Q^T and O^T = V^T . P^T on
 // v_mfma_f32_16x16x32: with lane = 16 g + r, S^T puts keys 4 g .. 4 g + 3 of each 16-key sub-tile and query row
@@ -508,28 +509,26 @@ __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, i
 //
 // A key or page that a row does not see has weight 0, which a NaN code behind it would turn into NaN.  In a tile
 // that not every row sees whole such codes are cleared, and at the end the rows that do see one are set to NaN.
-template <bool BF, int HD, int R, int TK, bool ROWS>
-__global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const KvAttnArgs a) {
+template <bool BF, int HD, int TK>
+__global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   typedef typename El<BF>::T T;
   typedef typename El<BF>::V8 V8;
-  constexpr int RT = ROWS ? 64 * R : 16 * R, NJ = HD / 64, ND = HD / 16, SUB = TK / 16, PL = TK / 4, VW = PL / 4;
-  constexpr int STEP = ROWS ? 1 : 4;  // tiles from one of a wave's to its next
+  constexpr int NJ = HD / 64, ND = HD / 16, SUB = TK / 16, PL = TK / 4, VW = PL / 4;
   typedef uint32_t VWords __attribute__((ext_vector_type(VW)));
   __shared__ int sh[5];
-  __shared__ float sm[4][16 * R], sl[4][16 * R];
-  __shared__ __attribute__((aligned(16))) float so[ROWS ? 1 : 4][ROWS ? 1 : 16 * R][HD + 4];
+  __shared__ float sm[4][KV_RT], sl[4][KV_RT];
+  __shared__ __attribute__((aligned(16))) float so[4][KV_RT][HD + 4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / (a.KV * a.S), rest = blockIdx.x % (a.KV * a.S);
   const int h = rest % a.KV, split = rest / a.KV;
-  const Item it = find_item(a.cu, a.kv_lens, a.B, a.tokens, item, a.grp, RT, 1, sh);
+  const Item it = find_item(a.cu, a.kv_lens, a.B, a.tokens, item, a.grp, KV_RT, 1, sh);
   if (it.b < 0) return;
-  const int rows = it.n * a.grp, row0 = it.i * RT, page = 1 << a.psh;
-  const int wrow = ROWS ? row0 + 16 * R * w : row0;  // this wave's first row
-  if (ROWS ? wrow >= rows : row0 >= rows) return;
+  const int rows = it.n * a.grp, row0 = it.i * KV_RT, page = 1 << a.psh;
+  if (row0 >= rows) return;
   const int kv_len = clamp_i(it.len, 0, a.max_pages << a.psh);
-  const int most = last_limit(a, it, kv_len, row0, RT);
-  const int first = a.causal ? kv_len - it.n + wrow / a.grp + 1 : kv_len;  // keys that every row of the wave sees
+  const int most = last_limit(a, it, kv_len, row0, KV_RT);
+  const int first = a.causal ? kv_len - it.n + row0 / a.grp + 1 : kv_len;  // keys that every row sees
   const int t_begin = split * a.span * (64 / TK), tiles = (most + TK - 1) / TK;
   const int t_end = split == a.S - 1 ? tiles : min(tiles, t_begin + a.span * (64 / TK));
   if (split > 0 && t_begin >= tiles) return;
@@ -562,7 +561,7 @@ __global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const Kv
 #pragma unroll
     for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const VWords*>(p + (size_t)16 * d * page));
   };
-  int t = ROWS ? t_begin : t_begin + w;
+  int t = t_begin + w;
   Pages now = {-1, -1}, next = {-1, -1};
   float sk = 0.f, sv = 0.f;  // scales of the lane's keys
   auto load_scales = [&](int id) {
@@ -572,68 +571,56 @@ __global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const Kv
   };
   if (t < t_end) {
     now = pages_at(t);
-    if (t + STEP < t_end) next = pages_at(t + STEP);
+    if (t + 4 < t_end) next = pages_at(t + 4);
     load_scales(now.v);
     load_keys(t, now.k);
     load_values(t, now.v);
   }
 
-  // the query operand: row r16 of each 16, dims 64 j + 16 g + 8 s .. + 7 for step 2 j + s
-  V8 q[R][2 * NJ];
-  int lim[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = min(wrow + 16 * r + r16, rows - 1), tok = row / a.grp;
-    lim[r] = a.causal ? kv_len - it.n + tok + 1 : kv_len;
-    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(it.c0 + tok) * a.q_tok +
-                 (int64_t)(h * a.grp + row - tok * a.grp) * a.q_head + 16 * g;
+  // the query operand: row r16, dims 64 j + 16 g + 8 s .. + 7 for step 2 j + s
+  V8 q[2 * NJ];
+  const int qrow = min(row0 + r16, rows - 1), qtok = qrow / a.grp;
+  const int lim = a.causal ? kv_len - it.n + qtok + 1 : kv_len;  // keys that the row sees
+  {
+    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(it.c0 + qtok) * a.q_tok +
+                 (int64_t)(h * a.grp + qrow - qtok * a.grp) * a.q_head + 16 * g;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (a.q_vec) {
-          q[r][2 * j + s] = load_global(reinterpret_cast<const V8*>(p + 64 * j + 8 * s));
+          q[2 * j + s] = load_global(reinterpret_cast<const V8*>(p + 64 * j + 8 * s));
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q[r][2 * j + s][e] = load_global(p + 64 * j + 8 * s + e);
+          for (int e = 0; e < 8; ++e) q[2 * j + s][e] = load_global(p + 64 * j + 8 * s + e);
         }
       }
   }
-  f4 o[R][ND];
-  float m[R], l[R];
+  f4 o[ND];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[r][d] = (f4){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < ND; ++d) o[d] = (f4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
   bool poison = false;  // a NaN code was cleared
-  for (; t < t_end; t += STEP) {
+  for (; t < t_end; t += 4) {
     const int pv = TK * t + PL * g;
     const float skc = sk * a.c, svc = sv;
-    const bool more = t + STEP < t_end;
+    const bool more = t + 4 < t_end;
     Pages after = {-1, -1};
-    if (t + 2 * STEP < t_end) after = pages_at(t + 2 * STEP);
+    if (t + 8 < t_end) after = pages_at(t + 8);
 
-    f4 x[R][SUB];
+    f4 x[SUB];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) x[r][s] = (f4){0.f, 0.f, 0.f, 0.f};
+      x[s] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const V8 k0 = widen8<BF>(kr[s][j][0], kr[s][j][1]), k1 = widen8<BF>(kr[s][j][2], kr[s][j][3]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          x[r][s] = mfma16(k0, q[r][2 * j], x[r][s]);
-          x[r][s] = mfma16(k1, q[r][2 * j + 1], x[r][s]);
-        }
+        x[s] = mfma16(widen8<BF>(kr[s][j][0], kr[s][j][1]), q[2 * j], x[s]);
+        x[s] = mfma16(widen8<BF>(kr[s][j][2], kr[s][j][3]), q[2 * j + 1], x[s]);
       }
     }
     if (more) {
       load_scales(next.v);
-      load_keys(t + STEP, next.k);
+      load_keys(t + 4, next.k);
     }
     const int own = now.v < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
     const bool edge = TK * t + TK > first || __any(now.v < 0);
@@ -654,51 +641,44 @@ __global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const Kv
       poison = poison || __any(nan);
     }
     const float lsv = __builtin_amdgcn_logf(fmaxf(svc, 0x1p-64f)) - 12.0f;
-    h8 p[R][PL / 8];
+    h8 p[PL / 8];
+    float top = -INFINITY;
+    const int see = min(lim - pv, own);  // keys pv .. pv + see - 1 are visible
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = -INFINITY;
-      const int see = min(lim[r] - pv, own);  // keys pv .. pv + see - 1 are visible
+    for (int s = 0; s < SUB; ++s)
 #pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = x[r][s][i] * skc;
-          if (edge && 4 * s + i >= see) v = -INFINITY;
-          x[r][s][i] = v;
-          top = fmaxf(top, v);
-        }
-      top = xor_max_16_32(top + lsv);
-      const float mn = fmaxf(m[r], top), mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m[r] - mu);
-      m[r] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(x[r][s][i] - mu);
-          sum += e;
-          p[r][s >> 1][4 * (s & 1) + i] = (_Float16)(e * svc);
-        }
-      l[r] = l[r] * alpha + sum;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
-    }
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int k = 0; k < PL / 8; ++k) {
-        const h8 v = widen8<false>(vr[d][2 * k], vr[d][2 * k + 1]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) o[r][d] = mfma16(v, p[r][k], o[r][d]);
+      for (int i = 0; i < 4; ++i) {
+        float v = x[s][i] * skc;
+        if (edge && 4 * s + i >= see) v = -INFINITY;
+        x[s][i] = v;
+        top = fmaxf(top, v);
       }
-    if (more) load_values(t + STEP, next.v);
+    top = xor_max_16_32(top + lsv);
+    const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(x[s][i] - mu);
+        sum += e;
+        p[s >> 1][4 * (s & 1) + i] = (_Float16)(e * svc);
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      o[d] *= alpha;
+#pragma unroll
+      for (int i = 0; i < PL / 8; ++i) o[d] = mfma16(widen8<false>(vr[d][2 * i], vr[d][2 * i + 1]), p[i], o[d]);
+    }
+    if (more) load_values(t + 4, next.v);
     now = next;
     next = after;
   }
   if (poison)  // the tiles of this wave that hold keys from `first` on, or pages that are not there
-    for (t = ROWS ? t_begin : t_begin + w; t < t_end; t += STEP) {
+    for (t = t_begin + w; t < t_end; t += 4) {
       const int idv = pages_at(t).v;
       if (!(TK * t + TK > first || __any(idv < 0))) continue;
       load_values(t, idv);
@@ -713,78 +693,43 @@ __global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const Kv
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = __shfl(at, 4 * g + i);  // of dim 16 d + 4 g + i
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (key < lim[r]) o[r][d][i] = NAN;
+          if (key < lim) o[d][i] = NAN;
         }
       }
     }
 
-  const size_t part0 = (((size_t)item * a.KV + h) * a.S + split) * RT;  // of the partial results' rows
-  if constexpr (ROWS) {  // every wave has the split's result for its own rows
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = wrow + 16 * r + r16, tok = row / a.grp;
-      l[r] = xor_sum_16_32(l[r]);
-      if (row >= rows) continue;
-      if (a.S > 1) {
-        if (g == 0) reinterpret_cast<f2*>(a.part_ml)[part0 + row - row0] = (f2){m[r], l[r]};
-        float* dst = a.part_o + (part0 + row - row0) * HD + 4 * g;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = o[r][d];
-      } else {
-        const float f = l[r] > 0.f ? 1.0f / l[r] : l[r] == 0.f ? 0.f : l[r];  // nothing visible: zeros; NaN stays
-        T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(it.c0 + tok) * a.o_tok +
-                 (int64_t)(h * a.grp + row - tok * a.grp) * a.o_head + 4 * g;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) dst[16 * d + k] = (T)(o[r][d][k] * f);
-      }
-    }
-    return;
-  }
-
+  const size_t part0 = (((size_t)item * a.KV + h) * a.S + split) * KV_RT;  // of the partial results' rows
   // ---- the waves meet ------------------------------------------------------------------------------
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    l[r] = xor_sum_16_32(l[r]);
-    if (g == 0) {
-      sm[w][16 * r + r16] = m[r];
-      sl[w][16 * r + r16] = l[r];
-    }
+  l = xor_sum_16_32(l);
+  if (g == 0) {
+    sm[w][r16] = m;
+    sl[w][r16] = l;
   }
   __syncthreads();
-  float f[R];  // this wave's share of the workgroup's sum
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = 16 * r + r16;
-    const float mx = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+  float f;  // this wave's share of the workgroup's sum
+  {
+    const float mx = fmaxf(fmaxf(sm[0][r16], sm[1][r16]), fmaxf(sm[2][r16], sm[3][r16]));
     const float mu = mx == -INFINITY ? 0.f : mx;
-    f[r] = __builtin_amdgcn_exp2f(m[r] - mu);
+    f = __builtin_amdgcn_exp2f(m - mu);
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += sl[i][row] * __builtin_amdgcn_exp2f(sm[i][row] - mu);
+    for (int i = 0; i < 4; ++i) sum += sl[i][r16] * __builtin_amdgcn_exp2f(sm[i][r16] - mu);
     if (a.S > 1) {
-      if (w == 0 && g == 0 && row0 + row < rows) {
-        reinterpret_cast<f2*>(a.part_ml)[part0 + row] = (f2){mx, sum};
-      }
+      if (w == 0 && g == 0 && row0 + r16 < rows) reinterpret_cast<f2*>(a.part_ml)[part0 + r16] = (f2){mx, sum};
     } else {
-      f[r] = sum > 0.f ? f[r] / sum : sum == 0.f ? 0.f : sum;  // nothing visible: zeros; NaN stays
+      f = sum > 0.f ? f / sum : sum == 0.f ? 0.f : sum;  // nothing visible: zeros; NaN stays
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int d = 0; d < ND; ++d) {
+    f4 v = o[d];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      f4 v = o[r][d];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = f[r] == 0.f ? 0.f : v[i] * f[r];
-      *reinterpret_cast<f4*>(&so[w][16 * r + r16][16 * d + 4 * g]) = v;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = f == 0.f ? 0.f : v[i] * f;
+    *reinterpret_cast<f4*>(&so[w][r16][16 * d + 4 * g]) = v;
+  }
   __syncthreads();
 #pragma unroll
-  for (int i = tid; i < RT * HD / 4; i += KV_NT) {
+  for (int i = tid; i < KV_RT * HD / 4; i += KV_NT) {
     const int row = i / (HD / 4), d = 4 * (i % (HD / 4));
     if (row0 + row >= rows) continue;
     f4 v = *reinterpret_cast<const f4*>(&so[0][row][d]);
@@ -806,7 +751,7 @@ __global__ __launch_bounds__(KV_NT, R == 1 ? 2 : 1) void kv_attn_kernel(const Kv
 // lanes one split of it at a time.  Few splits: a wave takes a whole row.  Many: a workgroup takes 64 dims of one, so
 // that the reads spread over the GPU (two rows of 8 heads and 128 splits: 5.2 us, with whole rows 8.1).
 template <bool BF, int HD, int W, int DC>
-__global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int rt) {
+__global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a) {
   typedef typename El<BF>::T T;
   constexpr int LQ = DC / 4, NG = 64 * W / LQ, NC = HD / DC;  // lanes of a split, splits at once, pieces of a row
   __shared__ __attribute__((aligned(16))) float so[W][DC];
@@ -831,14 +776,14 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int 
   if (token >= a.tokens || b < 0) return;
   Item it;
   it.n = n;
-  const int rr = (token - c0) * a.grp + head - h * a.grp, tile = rr / rt, row = rr - tile * rt;
-  const long long item = (long long)c0 * a.grp / rt + b + tile;
-  const int tiles = (last_limit(a, it, kv_len, tile * rt, rt) + 63) >> 6;
+  const int rr = (token - c0) * a.grp + head - h * a.grp, tile = rr / KV_RT, row = rr % KV_RT;
+  const long long item = (long long)c0 * a.grp / KV_RT + b + tile;
+  const int tiles = (last_limit(a, it, kv_len, tile * KV_RT, KV_RT) + 63) >> 6;
   const int splits = clamp_i((tiles + a.span - 1) / a.span, 1, a.S);  // splits that there are
-  const size_t p0 = ((size_t)item * a.KV + h) * a.S * rt + row;
+  const size_t p0 = ((size_t)item * a.KV + h) * a.S * KV_RT + row;
   const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + p0;
   float mx = -INFINITY;
-  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, load_global(ml + (size_t)s * rt)[0]);
+  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, load_global(ml + (size_t)s * KV_RT)[0]);
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
   const float mu = mx == -INFINITY ? 0.f : mx;
@@ -847,9 +792,9 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int 
   float sum = 0.f;
 #pragma unroll 4
   for (int s = gq; s < splits; s += NG) {
-    const f2 e = load_global(ml + (size_t)s * rt);
+    const f2 e = load_global(ml + (size_t)s * KV_RT);
     const float f = __builtin_amdgcn_exp2f(e[0] - mu);
-    const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * rt) * HD + d0 + d));
+    const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * KV_RT) * HD + d0 + d));
     if (f != 0.f) v += u * f;
     sum += e[1] * f;
   }
@@ -877,31 +822,27 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a, int 
   for (int k = 0; k < 4; ++k) dst[k] = (T)(v[k] * f);
 }
 
-// How an attention call is cut: rows per workgroup and splits of the keys, from what the host knows.
+// How an attention call is cut: splits of the keys, from what the host knows.
 struct KvAttnPlan {
-  int R, S, span;
-  bool rows;  // the waves of a workgroup share its rows instead of its keys
-  int rt() const { return (rows ? 64 : 16) * R; }
-  long long items;
+  int S, span;
+  long long items;  // tiles of 16 rows, at most
   size_t o_floats, bytes;
 };
 KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   KvAttnPlan p;
-  const long long grp = H / KV, rows = tokens * grp;
-  p.R = rows <= 16ll * B ? 1 : 2;
-  p.rows = rows > 32ll * B;
-  const int rt = p.rt();
-  p.items = rows / rt + B;
-  const long long busy = std::max({1ll, (rows + rt - 1) / rt, (long long)std::min(B, tokens)}) * KV;
+  const long long rows = (long long)tokens * (H / KV);
+  p.items = rows / KV_RT + B;
+  const long long busy = std::max({1ll, (rows + KV_RT - 1) / KV_RT, (long long)std::min(B, tokens)}) * KV;
   const int tiles = std::max(1, (max_kv + 63) / 64);
-  // Splits while the workgroups still are resident at once (two to a CU with 16 rows, one with more registers): 48
-  // requests of 8 kv heads take 64 us in one split each, 70 in two (768 workgroups); two requests of 131072 tokens
-  // 38 us in 128 or 256, 45 in 512.  At least a tile for every wave (rows: two tiles of 64).
-  const long long fit = (p.R == 1 ? 512 : 256) / busy, least = p.rows || hd == 256 ? 2 : 4;
-  const long long want = std::max(1ll, std::min(fit, (tiles + least - 1) / least));
+  // Splits while the workgroups are resident at once, two to a CU: two requests of 131072 tokens take 38 us in 128 or
+  // 256 splits each, 45 in 512.  From 171 workgroups on none: two splits of 200 (eight suffixes of 50 tokens, 8 heads)
+  // take 28 us and their join among them, one 25.5; of 384 (48 requests of 8 kv heads) 70, one 64.  At least a tile
+  // for every wave.
+  const long long fit = 512 / busy, least = hd == 256 ? 2 : 4;
+  const long long want = fit < 3 ? 1 : std::min(fit, (tiles + least - 1) / least);
   p.span = (int)((tiles + want - 1) / want);
   p.S = (tiles + p.span - 1) / p.span;
-  const size_t parts = (size_t)p.items * KV * p.S * rt;
+  const size_t parts = (size_t)p.items * KV * p.S * KV_RT;
   p.o_floats = p.S > 1 ? parts * hd : 0;
   p.bytes = p.S > 1 ? (p.o_floats + parts * 2) * sizeof(float) : 0;
   return p;
@@ -931,16 +872,13 @@ int kv_write_launch(const WriteArgs& a, hipStream_t st) {
 template <bool BF, int HD>
 int kv_attn_launch(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_t st) {
   const unsigned grid = (unsigned)(p.items * a.KV * p.S);
-  constexpr int TK = HD == 256 ? 32 : 64;
-  if (p.rows && p.R == 1) kv_attn_kernel<BF, HD, 1, TK, true><<<grid, KV_NT, 0, st>>>(a);
-  else if (p.rows) kv_attn_kernel<BF, HD, 2, TK, true><<<grid, KV_NT, 0, st>>>(a);
-  else if (p.R == 1) kv_attn_kernel<BF, HD, 1, TK, false><<<grid, KV_NT, 0, st>>>(a);
-  else kv_attn_kernel<BF, HD, 2, TK, false><<<grid, KV_NT, 0, st>>>(a);
+  // tiles of 32 keys at head_dim 256: two waves fit a SIMD (131072 tokens 52 -> 38 us)
+  kv_attn_kernel<BF, HD, (HD == 256 ? 32 : 64)><<<grid, KV_NT, 0, st>>>(a);
   MLCV_HIP(hipGetLastError());
   if (p.S > 1) {
     const long long rows = (long long)a.tokens * a.H;
-    if (p.S <= 16) kv_join_kernel<BF, HD, 1, HD><<<(unsigned)((rows + 3) / 4), KV_NT, 0, st>>>(a, p.rt());
-    else kv_join_kernel<BF, HD, 4, 64><<<(unsigned)(rows * (HD / 64)), KV_NT, 0, st>>>(a, p.rt());
+    if (p.S <= 16) kv_join_kernel<BF, HD, 1, HD><<<(unsigned)((rows + 3) / 4), KV_NT, 0, st>>>(a);
+    else kv_join_kernel<BF, HD, 4, 64><<<(unsigned)(rows * (HD / 64)), KV_NT, 0, st>>>(a);
     MLCV_HIP(hipGetLastError());
   }
   return 0;

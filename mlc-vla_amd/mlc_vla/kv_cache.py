@@ -40,8 +40,8 @@ class KVPlan(NamedTuple):
     status: Tensor      # [2] pages taken from the front of the free list; requests refused
 
 
-# The checks below run on every call of a serving loop, whose kernels take a few microseconds: they read the
-# tensors' attributes once and build nothing.
+# A call's checks take longer than the kernels of its smallest sizes: each function first looks at everything it
+# needs in one expression, and only where that fails are the arguments gone through one by one for the message.
 def _t(x) -> torch.Tensor:
     if type(x) is Tensor:
         return x.torch
@@ -54,47 +54,21 @@ def _bad(fn: str, name: str, what: str):
     raise ValueError(f"{fn}: argument {name} {what}")
 
 
-def _dense(fn: str, name: str, x, dtype, shape, dev: int) -> torch.Tensor:
-    """The torch tensor of argument ``name``, which has to be contiguous, of ``dtype`` and ``shape``, on HIP device
-    ``dev`` (None: any)."""
-    t = _t(x)
-    if t.dtype is not dtype:
-        _bad(fn, name, f"has dtype {t.dtype}, not {dtype}")
-    if t.shape != shape:
-        _bad(fn, name, f"expects shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.get_device() != dev:
-        _bad(fn, name, "is not on the HIP device of the other tensors")
-    if not t.is_contiguous():
-        _bad(fn, name, "must be contiguous")
-    return t
-
-
-def _rows(fn: str, name: str, x, dtypes, dev: Optional[int] = None) -> torch.Tensor:
-    """The torch tensor of argument ``name``: [tokens, heads, hd] of one of ``dtypes`` with contiguous rows, on HIP
-    device ``dev`` (None: any)."""
-    t = _t(x)
-    if t.dtype not in dtypes:
-        _bad(fn, name, f"has dtype {t.dtype}")
-    if t.dim() != 3:
-        _bad(fn, name, f"expects shape [tokens, heads, head_dim], got {tuple(t.shape)}")
-    i = t.get_device()
-    if i < 0 or (dev is not None and i != dev):
-        _bad(fn, name, "is not on the HIP device of the other tensors")
-    if t.stride(2) != 1 and t.numel() > 0:
-        _bad(fn, name, "must have contiguous rows")
-    return t
-
-
-def _ids(fn: str, name: str, x) -> torch.Tensor:
-    """A contiguous int32 vector on a HIP device."""
-    t = _t(x)
-    if t.dtype is not _I32:
-        _bad(fn, name, f"has dtype {t.dtype}, not {_I32}")
-    if t.dim() != 1 or not t.is_contiguous():
-        _bad(fn, name, "must be a contiguous vector")
-    if t.get_device() < 0:
-        _bad(fn, name, "is not on a HIP device")
-    return t
+def _refuse(fn: str, dev: int, wanted) -> None:
+    """Raises for the first of ``wanted`` (name, tensor, dtypes, shape with None for any size, contiguous) that is not
+    as said or not on HIP device ``dev``."""
+    for name, t, dtypes, shape, dense in wanted:
+        if t.dtype not in dtypes:
+            _bad(fn, name, f"has dtype {t.dtype}")
+        if t.dim() != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
+            _bad(fn, name, f"expects shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.get_device() < 0 or t.get_device() != dev:
+            _bad(fn, name, "is not on the HIP device of the other tensors")
+        if dense and not t.is_contiguous():
+            _bad(fn, name, "must be contiguous")
+        if not dense and t.stride(-1) != 1 and t.numel() > 0:
+            _bad(fn, name, "must have contiguous rows")
+    _bad(fn, wanted[0][0], "and the others do not go together")
 
 
 _lib = None
@@ -123,12 +97,15 @@ def _aligned(t: torch.Tensor, low: int) -> torch.Tensor:
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-def _out(fn: str, out, q: torch.Tensor, dev: int) -> torch.Tensor:
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    o = _rows(fn, "out", out, (q.dtype,), dev)
-    if o.shape != q.shape:
-        _bad(fn, "out", f"expects shape {tuple(q.shape)}, got {tuple(o.shape)}")
+def _like(q: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def _given(fn: str, out, q: torch.Tensor, dev: int) -> torch.Tensor:
+    o = _t(out)
+    if not (o.shape == q.shape and o.dtype is q.dtype and o.get_device() == dev
+            and (o.stride(2) == 1 or not o.numel())):
+        _refuse(fn, dev, (("out", o, (q.dtype,), q.shape, False),))
     return o
 
 
@@ -138,60 +115,70 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
 
     past_lens, new_lens [B], block_table [B, max_pages] (its new entries are written), free_pages [F], all int32;
     ``tokens``: the packed tokens of the call.  ``out``: a plan of the same sizes to write into."""
-    past, free = _ids("kv_plan", "past_lens", past_lens), _ids("kv_plan", "free_pages", free_pages)
-    table = _t(block_table)
-    n, dev, tokens = past.shape[0], past.get_device(), int(tokens)
-    new = _dense("kv_plan", "new_lens", new_lens, _I32, (n,), dev)
-    if table.dim() != 2:
-        _bad("kv_plan", "block_table", f"expects shape [requests, max_pages], got {tuple(table.shape)}")
-    wide = table.shape[1]
-    _dense("kv_plan", "block_table", table, _I32, (n, wide), dev)
-    if free.get_device() != dev:
-        _bad("kv_plan", "free_pages", "is not on the HIP device of the other tensors")
-    if tokens < 0:
-        _bad("kv_plan", "tokens", "is negative")
+    past, new, table, free = _t(past_lens), _t(new_lens), _t(block_table), _t(free_pages)
+    dev = past.get_device()
+    shape = table.shape
+    n, wide = shape if len(shape) == 2 else (-1, 0)
+    if not (past.dtype is _I32 and new.dtype is _I32 and table.dtype is _I32 and free.dtype is _I32
+            and past.shape == (n,) and new.shape == (n,) and free.dim() == 1 and past.is_contiguous()
+            and new.is_contiguous() and table.is_contiguous() and free.is_contiguous()
+            and dev >= 0 and new.get_device() == table.get_device() == free.get_device() == dev and tokens >= 0):
+        if tokens < 0:
+            _bad("kv_plan", "tokens", "is negative")
+        i32, b = (_I32,), past.shape[0] if past.dim() == 1 else None
+        _refuse("kv_plan", dev, (("past_lens", past, i32, (None,), True), ("new_lens", new, i32, (b,), True),
+                                 ("block_table", table, i32, (b, None), True),
+                                 ("free_pages", free, i32, (None,), True)))
     if out is None:
         cu, lens, slots, status = torch.empty(tokens + 2 * n + 3, dtype=_I32, device=past.device).split(
             (n + 1, n, tokens, 2))
         out = KVPlan(Tensor(cu, "int32"), Tensor(lens, "int32"), Tensor(slots, "int32"), Tensor(status, "int32"))
     else:
-        cu, lens, slots, status = (_dense("kv_plan", "out", x, _I32, (s,), dev)
-                                   for x, s in zip(out, (n + 1, n, tokens, 2)))
+        cu, lens, slots, status = (_t(x) for x in out)
+        if not (cu.shape == (n + 1,) and lens.shape == (n,) and slots.shape == (tokens,) and status.shape == (2,)
+                and all(t.dtype is _I32 and t.is_contiguous() and t.get_device() == dev
+                        for t in (cu, lens, slots, status))):
+            _refuse("kv_plan", dev, tuple(("out." + f, t, (_I32,), (k,), True) for f, t, k in
+                                          zip(KVPlan._fields, (cu, lens, slots, status), (n + 1, n, tokens, 2))))
     _call("mlcv_kv_plan", dev, past.data_ptr(), new.data_ptr(), n, free.data_ptr(), free.shape[0], num_pages,
           page_size, table.data_ptr(), wide, cu.data_ptr(), lens.data_ptr(), slots.data_ptr(), tokens,
           status.data_ptr())
     return out
 
 
-def _cache(fn: str, k_cache, k_scale, v_cache, v_scale, dev: int):
-    kc = _t(k_cache)
-    if kc.dim() != 4:
-        _bad(fn, "k_cache", f"expects shape [pages, heads, page, head_dim], got {tuple(kc.shape)}")
-    pages, kv, page, hd = shape = kc.shape
-    _dense(fn, "k_cache", kc, _F8, shape, dev)
-    return (kc.data_ptr(), _dense(fn, "k_scale", k_scale, _F32, (pages, kv), dev).data_ptr(),
-            _dense(fn, "v_cache", v_cache, _F8, (pages, kv, hd, page), dev).data_ptr(),
-            _dense(fn, "v_scale", v_scale, _F32, (pages, kv), dev).data_ptr(), pages, page), kv, hd
+def _cache_wanted(kc, ks, vc, vs):
+    pages, kv, page, hd = kc.shape if kc.dim() == 4 else (None,) * 4
+    return (("k_cache", kc, (_F8,), (None,) * 4, True), ("k_scale", ks, (_F32,), (pages, kv), True),
+            ("v_cache", vc, (_F8,), (pages, kv, hd, page), True), ("v_scale", vs, (_F32,), (pages, kv), True))
 
 
 def kv_write(k, v, cu_seqlens, slot_map, k_cache, k_scale, v_cache, v_scale) -> None:
     """Write new keys and values [tokens, KV, hd] (float16, bfloat16 or float32, any strides with contiguous rows)
     into their slots of the cache (mlcv_kv_write): k_cache [pages, KV, page, hd] and v_cache [pages, KV, hd, page]
     float8_e4m3fn, their scales [pages, KV] float32."""
-    k = _rows("kv_write", "k", k, _CODE)
-    dev, tokens = k.get_device(), k.shape[0]
-    v = _rows("kv_write", "v", v, _CODE, dev)
-    cache, kv, hd = _cache("kv_write", k_cache, k_scale, v_cache, v_scale, dev)
-    if k.shape != (tokens, kv, hd) or v.shape != k.shape:
-        _bad("kv_write", "k or v", f"expects shape {(tokens, kv, hd)}, got {tuple(k.shape)}, {tuple(v.shape)}")
-    cu = _ids("kv_write", "cu_seqlens", cu_seqlens)
-    if cu.get_device() != dev or cu.shape[0] < 1:
-        _bad("kv_write", "cu_seqlens", "expects requests + 1 offsets on the HIP device of the other tensors")
-    slots = _dense("kv_write", "slot_map", slot_map, _I32, (tokens,), dev)
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
-    _call("mlcv_kv_write", dev, k.data_ptr(), _CODE[k.dtype], kt, kh, v.data_ptr(), _CODE[v.dtype], vt, vh, tokens,
-          cu.data_ptr(), cu.shape[0] - 1, slots.data_ptr(), *cache, kv, hd)
+    k, v, cu, slots = _t(k), _t(v), _t(cu_seqlens), _t(slot_map)
+    kc, ks, vc, vs = _t(k_cache), _t(k_scale), _t(v_cache), _t(v_scale)
+    dev, shape = k.get_device(), kc.shape
+    pages, kv, page, hd = shape if len(shape) == 4 else (-1,) * 4
+    tokens = k.shape[0] if k.dim() == 3 else -1
+    kt, vt = _CODE.get(k.dtype), _CODE.get(v.dtype)
+    if not (kt and vt and kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32
+            and cu.dtype is _I32 and slots.dtype is _I32 and k.shape == (tokens, kv, hd) and v.shape == k.shape
+            and vc.shape == (pages, kv, hd, page) and ks.shape == (pages, kv) and vs.shape == (pages, kv)
+            and slots.shape == (tokens,) and cu.dim() == 1 and cu.shape[0] > 0
+            and (k.stride(2) == v.stride(2) == 1 or not tokens * kv * hd) and kc.is_contiguous() and vc.is_contiguous()
+            and ks.is_contiguous() and vs.is_contiguous() and cu.is_contiguous() and slots.is_contiguous()
+            and dev >= 0 and v.get_device() == kc.get_device() == ks.get_device() == vc.get_device()
+            == vs.get_device() == cu.get_device() == slots.get_device() == dev):
+        rows, i32 = (tokens, kv, hd) if len(shape) == 4 else (None,) * 3, (_I32,)
+        _refuse("kv_write", dev, _cache_wanted(kc, ks, vc, vs)
+                + (("k", k, _CODE, (None,) + rows[1:], False), ("v", v, _CODE, rows, False),
+                   ("slot_map", slots, i32, (tokens,), True), ("cu_seqlens", cu, i32, (None,), True)))
+    ks0, ks1, _ = k.stride()
+    vs0, vs1, _ = v.stride()
+    _call("mlcv_kv_write", dev, k.data_ptr(), kt, ks0, ks1, v.data_ptr(), vt, vs0, vs1, tokens, cu.data_ptr(),
+          cu.shape[0] - 1, slots.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), pages, page,
+          kv, hd)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -207,21 +194,27 @@ def kv_attention(q, cu_seqlens, kv_lens, block_table, k_cache, k_scale, v_cache,
     """Attention of the last tokens of each request, q [tokens, H, hd], over its cached keys and values
     (mlcv_kv_attention).  ``scale``: 1 / sqrt(hd) if not given; ``max_kv``: a bound on kv_lens (default: the
     block table's width); ``workspace``: uint8 tensor of ``kv_attention_workspace`` bytes (default: allocated here)."""
-    q = _rows("kv_attention", "q", q, _NAME)
-    dev = q.get_device()
-    cache, kv, hd = _cache("kv_attention", k_cache, k_scale, v_cache, v_scale, dev)
-    tokens, heads, d = q.shape
-    if d != hd:
-        _bad("kv_attention", "q", f"expects head_dim {hd}, got {d}")
-    table = _t(block_table)
-    if table.dim() != 2:
-        _bad("kv_attention", "block_table", f"expects shape [requests, max_pages], got {tuple(table.shape)}")
-    n, wide = table.shape
-    _dense("kv_attention", "block_table", table, _I32, (n, wide), dev)
-    lens = _dense("kv_attention", "kv_lens", kv_lens, _I32, (n,), dev)
-    cu = _dense("kv_attention", "cu_seqlens", cu_seqlens, _I32, (n + 1,), dev)
-    o = _out("kv_attention", out, q, dev)
-    most = wide * cache[5] if max_kv is None else max_kv
+    q, cu, lens, table = _t(q), _t(cu_seqlens), _t(kv_lens), _t(block_table)
+    kc, ks, vc, vs = _t(k_cache), _t(k_scale), _t(v_cache), _t(v_scale)
+    dev, shape, name = q.get_device(), kc.shape, _NAME.get(q.dtype)
+    pages, kv, page, hd = shape if len(shape) == 4 else (-1,) * 4
+    tokens, heads, d = q.shape if q.dim() == 3 else (-1,) * 3
+    n, wide = table.shape if table.dim() == 2 else (-1, 0)
+    if not (name and d == hd and kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32
+            and cu.dtype is _I32 and lens.dtype is _I32 and table.dtype is _I32
+            and vc.shape == (pages, kv, hd, page) and ks.shape == (pages, kv) and vs.shape == (pages, kv)
+            and cu.shape == (n + 1,) and lens.shape == (n,) and (q.stride(2) == 1 or not tokens * heads)
+            and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and cu.is_contiguous() and lens.is_contiguous() and table.is_contiguous()
+            and dev >= 0 and kc.get_device() == ks.get_device() == vc.get_device() == vs.get_device()
+            == cu.get_device() == lens.get_device() == table.get_device() == dev):
+        i32, b = (_I32,), table.shape[0] if table.dim() else None
+        _refuse("kv_attention", dev, (("q", q, _NAME, (None, None, hd if len(shape) == 4 else None), False),)
+                + _cache_wanted(kc, ks, vc, vs)
+                + (("block_table", table, i32, (None, None), True), ("kv_lens", lens, i32, (b,), True),
+                   ("cu_seqlens", cu, i32, (b + 1 if b is not None else None,), True)))
+    o = _like(q) if out is None else _given("kv_attention", out, q, dev)
+    most = wide * page if max_kv is None else max_kv
     size = kv_attention_workspace(tokens, n, heads, kv, hd, most)
     at = None
     if size:
@@ -230,43 +223,51 @@ def kv_attention(q, cu_seqlens, kv_lens, block_table, k_cache, k_scale, v_cache,
         else:
             workspace = _t(workspace)
             size = workspace.numel()
-            _dense("kv_attention", "workspace", workspace, _U8, (size,), dev)
+            if not (workspace.dtype is _U8 and workspace.is_contiguous() and workspace.get_device() == dev):
+                _refuse("kv_attention", dev, (("workspace", workspace, (_U8,), (None,), True),))
         at = workspace.data_ptr()
     qt, qh, _ = q.stride()
     ot, oh, _ = o.stride()
     _call("mlcv_kv_attention", dev, q.data_ptr(), _CODE[q.dtype], qt, qh, tokens, cu.data_ptr(), n, lens.data_ptr(),
-          table.data_ptr(), wide, *cache, heads, kv, hd, hd ** -0.5 if scale is None else scale, causal, most,
-          o.data_ptr(), ot, oh, at, size)
-    return Tensor(o, _NAME[q.dtype])
+          table.data_ptr(), wide, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), pages, page, heads, kv,
+          hd, hd ** -0.5 if scale is None else scale, causal, most, o.data_ptr(), ot, oh, at, size)
+    return Tensor(o, name)
 
 
 def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, bidir=None, scale: Optional[float] = None,
                      out=None) -> Tensor:
     """Attention of packed prompts, q [tokens, H, hd], k and v [tokens, KV, hd] in float16 or bfloat16
-    (mlcv_prompt_attention).  ``bidir`` [B] int32: the first tokens of each prompt that all see one another."""
-    q = _rows("prompt_attention", "q", q, _NAME)
-    dev, dt = q.get_device(), (q.dtype,)
-    tokens, heads, hd = q.shape
-    k = _rows("prompt_attention", "k", k, dt, dev)
-    kv = k.shape[1]
-    v = _rows("prompt_attention", "v", v, dt, dev)
-    if k.shape != (tokens, kv, hd) or v.shape != k.shape:
-        _bad("prompt_attention", "k or v", f"expects shape [{tokens}, KV, {hd}], got {(*k.shape,)}, {(*v.shape,)}")
-    cu = _ids("prompt_attention", "cu_seqlens", cu_seqlens)
-    n = cu.shape[0] - 1
-    if cu.get_device() != dev or n < 0:
-        _bad("prompt_attention", "cu_seqlens", "expects requests + 1 offsets on the HIP device of the other tensors")
-    pre = None if bidir is None else _dense("prompt_attention", "bidir", bidir, _I32, (n,), dev).data_ptr()
-    o = _out("prompt_attention", out, q, dev)
+    (mlcv_prompt_attention).  ``bidir`` [B] int32: the first tokens of each prompt that all see one another.  Rows
+    that are not 16-byte aligned, and tokens that share keys or values, are copied first."""
+    q, k, v, cu = _t(q), _t(k), _t(v), _t(cu_seqlens)
+    dev, dt, name = q.get_device(), q.dtype, _NAME.get(q.dtype)
+    tokens, heads, hd = q.shape if q.dim() == 3 else (-1,) * 3
+    kv = k.shape[1] if k.dim() == 3 else -1
+    n = cu.shape[0] - 1 if cu.dim() == 1 else -1
+    if not (name and k.dtype is dt and v.dtype is dt and cu.dtype is _I32 and k.shape == (tokens, kv, hd)
+            and v.shape == k.shape and n >= 0 and cu.is_contiguous()
+            and (q.stride(2) == k.stride(2) == v.stride(2) == 1 or not tokens * hd)
+            and dev >= 0 and k.get_device() == v.get_device() == cu.get_device() == dev):
+        t, d = (tokens, hd) if q.dim() == 3 else (None, None)
+        _refuse("prompt_attention", dev, (("q", q, _NAME, (None,) * 3, False), ("k", k, (dt,), (t, None, d), False),
+                                          ("v", v, (dt,), tuple(k.shape), False),
+                                          ("cu_seqlens", cu, (_I32,), (None,), True)))
+    pre = None
+    if bidir is not None:
+        bidir = _t(bidir)
+        if not (bidir.dtype is _I32 and bidir.shape == (n,) and bidir.is_contiguous() and bidir.get_device() == dev):
+            _refuse("prompt_attention", dev, (("bidir", bidir, (_I32,), (n,), True),))
+        pre = bidir.data_ptr()
+    o = _like(q) if out is None else _given("prompt_attention", out, q, dev)
     q, k, v = _aligned(q, 0), _aligned(k, hd), _aligned(v, hd)
     qt, qh, _ = q.stride()
     kt, kh, _ = k.stride()
     vt, vh, _ = v.stride()
     ot, oh, _ = o.stride()
-    _call("mlcv_prompt_attention", dev, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-          _CODE[q.dtype], tokens, cu.data_ptr(), n, heads, kv, hd, hd ** -0.5 if scale is None else scale, causal, pre,
-          o.data_ptr(), ot, oh)
-    return Tensor(o, _NAME[q.dtype])
+    _call("mlcv_prompt_attention", dev, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _CODE[dt],
+          tokens, cu.data_ptr(), n, heads, kv, hd, hd ** -0.5 if scale is None else scale, causal, pre, o.data_ptr(),
+          ot, oh)
+    return Tensor(o, name)
 
 
 class PagedKVCache:

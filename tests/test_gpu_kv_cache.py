@@ -747,8 +747,8 @@ def test_arguments_are_checked():
     for args, kw, what in (
             ((q.float(), cu, lens, t, *cache), {}, "dtype"),
             ((q[0], cu, lens, t, *cache), {}, "shape"),
-            ((q[:, :, :32], cu, lens, t, *cache), {}, "head_dim"),
-            ((q.transpose(1, 2), cu, lens, t, *cache), {}, "head_dim|rows"),
+            ((q[:, :, :32], cu, lens, t, *cache), {}, "argument q expects shape"),
+            ((q.transpose(1, 2), cu, lens, t, *cache), {}, "argument q expects shape"),
             ((q, cu.long(), lens, t, *cache), {}, "cu_seqlens"),
             ((q, cu, lens, t[:, ::2], *cache), {}, "contiguous"),
             ((q, cu, lens, t, kc, ks, kc, vs), {}, "v_cache"),
@@ -768,7 +768,7 @@ def test_arguments_are_checked():
         C.prompt_attention(q, x.bfloat16(), x, cu)
     with pytest.raises(ValueError, match="slot_map"):
         C.kv_write(x, x, cu, _ints([0, 1]), *cache)
-    with pytest.raises(ValueError, match="k or v"):
+    with pytest.raises(ValueError, match="argument k expects shape"):
         C.kv_write(x[:, :1], x, cu, _ints([0]), *cache)
     with pytest.raises(ValueError, match="new_lens"):
         C.kv_plan(_ints([0]), _ints([1, 2]), t, _ints([1]), num_pages=4, page_size=16, tokens=3)
