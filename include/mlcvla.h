@@ -309,7 +309,8 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  * The cache: pages of `page` tokens (16, 32, 64 or 128), hd 64, 128 or 256, in e4m3 codes:
  *   k_cache [num_pages][KV][page][hd]   v_cache [num_pages][KV][hd][page]  (token innermost)
  *   k_scale, v_scale [num_pages][KV] f32: x = code * scale
- * both caches 16-byte aligned; at most 2^31 - 1 slots (num_pages * page).  Slot s is token
+ * both caches 16-byte aligned; at most 2^31 - 256 slots (num_pages * page), and as many positions of a
+ * block table's row.  Slot s is token
  * s % page of page s / page. */
 
 /* Attention over whole prompts: row i of a prompt of n tokens sees the keys [0, n) of its own prompt

@@ -134,15 +134,24 @@ __global__ __launch_bounds__(PR_NT, HD == 256 ? 1 : 2) void prompt_attn_kernel(c
     sh[4] = 0;
   }
   __syncthreads();
+  int mine = -1, mc0 = 0, mn = 0, mi = 0;
   for (int b = tid; b < a.B; b += PR_NT) {
     const int c0 = min(max(a.cu[b], 0), a.tokens), c1 = min(max(a.cu[b + 1], 0), a.tokens);
     const int f0 = c0 / ROWS + b, f1 = c1 / ROWS + b + 1;
     if (f0 <= item && item < f1 && c1 > c0) {
-      sh[0] = b;
-      sh[1] = c0;
-      sh[2] = c1 - c0;
-      sh[3] = item - f0;
+      mine = b;
+      mc0 = c0;
+      mn = c1 - c0;
+      mi = item - f0;
     }
+  }
+  // offsets that do not ascend can put an item into several requests: one of them, whole
+  if (mine >= 0) atomicMax(sh, mine);
+  __syncthreads();
+  if (mine >= 0 && mine == sh[0]) {
+    sh[1] = mc0;
+    sh[2] = mn;
+    sh[3] = mi;
   }
   __syncthreads();
   const int b = __builtin_amdgcn_readfirstlane(sh[0]), c0 = __builtin_amdgcn_readfirstlane(sh[1]);

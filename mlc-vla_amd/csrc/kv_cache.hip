@@ -22,6 +22,7 @@ namespace {
 
 constexpr int KV_NT = 256;         // threads per workgroup of every kernel here
 constexpr int KV_RT = 16;          // query rows of an attention workgroup
+constexpr int64_t KV_MOST = INT32_MAX - 255;  // slots of a cache, positions of a row: the last tile's still are ints
 constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
 
 // ---- plan ------------------------------------------------------------------------------------------
@@ -171,18 +172,28 @@ __device__ __forceinline__ Item find_item(const int32_t* cu, const int32_t* lens
                                           int mul, int div, int extra, int* sh) {
   if (threadIdx.x == 0) sh[0] = -1;
   __syncthreads();
+  int mine = -1, mc0 = 0, mn = 0, mi = 0, ml = 0;
   for (int b = threadIdx.x; b < B; b += KV_NT) {
     const int len = lens ? lens[b] : 0;
     const int c0 = clamp_i(cu[b], 0, tokens), c1 = clamp_i(cu[b + 1], 0, tokens);
     const long long f0 = (long long)c0 * mul / div + (long long)extra * b;
     const long long f1 = (long long)c1 * mul / div + (long long)extra * (b + 1);
     if (f0 <= item && item < f1 && c1 > c0) {
-      sh[0] = b;
-      sh[1] = c0;
-      sh[2] = c1 - c0;
-      sh[3] = (int)(item - f0);
-      sh[4] = len;
+      mine = b;
+      mc0 = c0;
+      mn = c1 - c0;
+      mi = (int)(item - f0);
+      ml = len;
     }
+  }
+  // offsets that do not ascend can put an item into several requests: one of them, whole
+  if (mine >= 0) atomicMax(sh, mine);
+  __syncthreads();
+  if (mine >= 0 && mine == sh[0]) {
+    sh[1] = mc0;
+    sh[2] = mn;
+    sh[3] = mi;
+    sh[4] = ml;
   }
   __syncthreads();
   Item r;
@@ -833,7 +844,7 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   const long long rows = (long long)tokens * (H / KV);
   p.items = rows / KV_RT + B;
   const long long busy = std::max({1ll, (rows + KV_RT - 1) / KV_RT, (long long)std::min(B, tokens)}) * KV;
-  const int tiles = std::max(1, (max_kv + 63) / 64);
+  const int tiles = std::max(1, max_kv / 64 + (max_kv % 64 != 0));
   // Splits while the workgroups are resident at once, two to a CU: two requests of 131072 tokens take 38 us in 128 or
   // 256 splits each, 45 in 512.  From 171 workgroups on none: two splits of 200 (eight suffixes of 50 tokens, 8 heads)
   // take 28 us and their join among them, one 25.5; of 384 (48 requests of 8 kv heads) 70, one 64.  At least a tile
@@ -902,8 +913,8 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
   MLCV_REQUIRE(tokens == 0 || slot_map, "null slot_map");
   MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
   MLCV_REQUIRE(B <= KV_MAX_REQ, "more than 4096 requests");
-  MLCV_REQUIRE((int64_t)num_pages * page <= INT32_MAX && (int64_t)max_pages * page <= INT32_MAX,
-               "more than 2^31 - 1 slots");
+  MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST && (int64_t)max_pages * page <= KV_MOST,
+               "more than 2^31 - 256 slots");
   PlanArgs a{past_lens, new_lens, free_pages, block_table, cu_seqlens, kv_lens, slot_map, status, B, n_free,
              num_pages, log2_of(page), max_pages, tokens, 0};
   a.slot_blocks = std::max(1, (int)(((int64_t)tokens + 4 * KV_NT - 1) / (4 * KV_NT)));
@@ -927,7 +938,7 @@ int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head,
   MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
   MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE(KV <= 65535, "more than 65535 kv heads");
-  MLCV_REQUIRE((int64_t)num_pages * page <= INT32_MAX, "more than 2^31 - 1 slots");
+  MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST, "more than 2^31 - 256 slots");
   MLCV_REQUIRE((int64_t)tokens / page + 2 * (int64_t)B <= INT32_MAX, "too many requests");
   MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
   WriteArgs a{};
@@ -985,8 +996,8 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
   MLCV_REQUIRE(dtype == MLCV_DTYPE_F16 || dtype == MLCV_DTYPE_BF16, "queries are float16 or bfloat16");
   MLCV_TRY(kv_attn_sizes_ok(tokens, B, H, KV, hd, max_kv));
   MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
-  MLCV_REQUIRE(num_pages >= 0 && max_pages >= 0 && (int64_t)num_pages * page <= INT32_MAX &&
-                   (int64_t)max_pages * page <= INT32_MAX, "more than 2^31 - 1 slots");
+  MLCV_REQUIRE(num_pages >= 0 && max_pages >= 0 && (int64_t)num_pages * page <= KV_MOST &&
+                   (int64_t)max_pages * page <= KV_MOST, "more than 2^31 - 256 slots");
   MLCV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   if (tokens == 0 || B == 0) return 0;
   MLCV_REQUIRE(q && cu_seqlens && kv_lens && out, "null pointer");

@@ -122,9 +122,10 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
     if not (past.dtype is _I32 and new.dtype is _I32 and table.dtype is _I32 and free.dtype is _I32
             and past.shape == (n,) and new.shape == (n,) and free.dim() == 1 and past.is_contiguous()
             and new.is_contiguous() and table.is_contiguous() and free.is_contiguous()
-            and dev >= 0 and new.get_device() == table.get_device() == free.get_device() == dev and tokens >= 0):
-        if tokens < 0:
-            _bad("kv_plan", "tokens", "is negative")
+            and dev >= 0 and new.get_device() == table.get_device() == free.get_device() == dev
+            and 0 <= tokens < 1 << 31 and 0 <= num_pages < 1 << 31):
+        if not (0 <= tokens < 1 << 31 and 0 <= num_pages < 1 << 31):
+            _bad("kv_plan", "tokens or num_pages", "is negative or past 2^31 - 1")
         i32, b = (_I32,), past.shape[0] if past.dim() == 1 else None
         _refuse("kv_plan", dev, (("past_lens", past, i32, (None,), True), ("new_lens", new, i32, (b,), True),
                                  ("block_table", table, i32, (b, None), True),
@@ -214,7 +215,7 @@ def kv_attention(q, cu_seqlens, kv_lens, block_table, k_cache, k_scale, v_cache,
                 + (("block_table", table, i32, (None, None), True), ("kv_lens", lens, i32, (b,), True),
                    ("cu_seqlens", cu, i32, (b + 1 if b is not None else None,), True)))
     o = _like(q) if out is None else _given("kv_attention", out, q, dev)
-    most = wide * page if max_kv is None else max_kv
+    most = min(wide * page if max_kv is None else max_kv, 0x7fffffff)
     size = kv_attention_workspace(tokens, n, heads, kv, hd, most)
     at = None
     if size:
@@ -277,8 +278,8 @@ class PagedKVCache:
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, layers: int = 1, dev=None):
         if page_size not in (16, 32, 64, 128) or head_dim not in (64, 128, 256):
             raise ValueError("page_size must be 16, 32, 64 or 128 and head_dim 64, 128 or 256")
-        if num_pages * page_size > 2 ** 31 - 1:
-            raise ValueError("more than 2^31 - 1 slots")
+        if not 0 <= num_pages * page_size <= 2 ** 31 - 256:
+            raise ValueError("more than 2^31 - 256 slots")
         d = (dev or device()).torch
         shape = (layers, num_pages, num_kv_heads)
         self.page_size, self.num_pages, self.layers = page_size, num_pages, layers

@@ -70,7 +70,8 @@ class Tensor:
     def numpy(self) -> np.ndarray:
         if self._check is not None:
             self._check()
-        a = self.torch.detach().cpu().numpy()
+        t = self.torch.detach()
+        a = (t.float() if self.dtype == "bfloat16" else t).cpu().numpy()  # numpy has no bfloat16
         return a.view(np.uint32) if self.dtype == "uint32" else a
 
     def data_ptr(self) -> int:

@@ -188,6 +188,26 @@ def test_write_strides_and_alignment(hd, kv, kt):
         _check_write(k, v, cu, slots, _cache(rng, pages, kv, hd, 32))
 
 
+@pytest.mark.parametrize("hd,kv,page", [(64, 5, 16), (128, 8, 32), (256, 3, 128)])
+def test_write_of_many_pages(hd, kv, page):
+    """Enough pages that a workgroup takes several heads in turn: what a call for each request writes."""
+    rng = np.random.default_rng(page)
+    new = rng.integers(1, 90 * page, 24).tolist()
+    past = rng.integers(0, 3 * page, 24).tolist()
+    slots, pages = _slots(past, new, page, rng)
+    cu = np.concatenate([[0], np.cumsum(new)]).tolist()
+    g = torch.Generator(device="cuda").manual_seed(page)
+    k, v = (torch.randn((cu[-1], kv, hd), generator=g, device="cuda").half() for _ in range(2))
+    one = _cache(rng, pages, kv, hd, page)
+    two = [t.clone() for t in one]
+    s = _ints(slots)
+    C.kv_write(k, v, _ints(cu), s, *one)
+    for a, z in zip(cu, cu[1:]):
+        C.kv_write(k[a:z], v[a:z], _ints([0, z - a]), s[a:z], *two)
+    for a, b in zip(one, two):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_write_values_of_every_size():
     """Zeros, subnormals, the largest values, infinities and NaN; pages that grow past codes that fall below 2^-6."""
     rng = np.random.default_rng(0)
@@ -470,14 +490,27 @@ def test_prompt_attention(dt, heads, kv, hd, lens):
     _check_prompts(q, k, v, cu, True, bidir=[10 ** 6 * (i % 2) + 50 for i in range(len(lens))], scale=0.3)
 
 
+@pytest.mark.parametrize("hd,kv", [(64, 8), (128, 1), (256, 2)])
+def test_prompt_attention_of_many_heads(hd, kv):
+    """More than 128 workgroups of 128 rows: no sharing of rows between waves."""
+    rng = np.random.default_rng(hd)
+    lens = [140, 1, 233]
+    cu = [0] + np.cumsum(lens).tolist()
+    q, k, v = (_rows(rng, (cu[-1], h, hd), torch.bfloat16 if hd == 64 else torch.float16, 0.5) for h in (48, kv, kv))
+    _check_prompts(q, k, v, cu, True, bidir=[0, 1, 150])
+    _check_prompts(q[:, :40], k, v, cu, False, scale=0.2)
+    ramp = torch.linspace(0, 6, cu[-1], device="cuda").to(k.dtype)[:, None, None]  # maxima that come late
+    _check_prompts(q, k * (1 + ramp), v, cu, True)
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
-@pytest.mark.parametrize("hd", [64, 128, 256])
-def test_prompt_attention_non_finite_behind_the_mask(dt, hd):
+@pytest.mark.parametrize("hd,heads", [(64, 2), (128, 2), (256, 2), (64, 64), (128, 64), (256, 64)])
+def test_prompt_attention_non_finite_behind_the_mask(dt, hd, heads):
     """NaN and infinities in tokens that a row does not see, of its own prompt and of its neighbours, do not reach it."""
     rng = np.random.default_rng(12)
     lens = [150, 70, 40]
     cu = [0] + np.cumsum(lens).tolist()
-    q, k, v = (_rows(rng, (cu[-1], h, hd), TYPES[dt], 0.5) for h in (2, 1, 1))
+    q, k, v = (_rows(rng, (cu[-1], h, hd), TYPES[dt], 0.5) for h in (heads, 1, 1))
     v[100, 0, 5] = float("inf")
     v[101, 0, 6] = float("nan")
     v[120, 0, 5] = float("-inf")
@@ -514,6 +547,27 @@ def test_prompt_attention_strides_and_rows_behind():
     a = C.prompt_attention(q, k, v, _ints([0, 45, 10 ** 6])).torch
     b = C.prompt_attention(q, k, v, _ints([0, 45, n])).torch
     assert torch.equal(a, b)
+
+
+def test_offsets_that_do_not_ascend():
+    """cu_seqlens that overlap, descend or lie outside: nothing outside the tensors is touched, and a request whose
+    offsets are sound and meet no other's is right."""
+    rng = np.random.default_rng(17)
+    n, hd = 300, 64
+    q, k, v = (_rows(rng, (n, h, hd), torch.float16, 0.5) for h in (2, 1, 1))
+    store = torch.full((n + 64, 2, hd), 9.0, dtype=torch.float16, device="cuda")
+    out = store[32:32 + n]
+    table, cache = _paged(rng, [500, 500, 500], [1, 1, 1], 1, hd, 16)
+    t = torch.from_numpy(table).cuda()
+    for cu in ([0, 290, 20, 300], [0, 300, 0, 300], [250, 100, 299, 10 ** 6], [-50, -1, 300, 2 ** 31 - 1],
+               [2 ** 31 - 1, -2 ** 31, 300, 0]):
+        out.fill_(9.0)
+        C.prompt_attention(q, k, v, _ints(cu), out=out)
+        C.kv_attention(q, _ints(cu), _ints([400, 2 ** 31 - 1, -5]), t, *cache, out=out)
+        C.kv_attention(q, _ints(cu), _ints([400, 2 ** 31 - 1, -5]), t, *cache, max_kv=1, causal=False, out=out)
+        C.kv_write(k, v, _ints(cu), _ints(range(n)), *cache)
+        torch.cuda.synchronize()
+        assert (store[:32] == 9).all() and (store[32 + n:] == 9).all()
 
 
 def test_prompt_attention_large_logits():

@@ -47,7 +47,7 @@ def _prompt(**kw):
 @pytest.mark.parametrize("fn,bad,what", [
     (_plan, dict(B=-1), "negative"), (_plan, dict(page=48), "page"), (_plan, dict(B=4097), "4096"),
     (_plan, dict(cu=None), "null"), (_plan, dict(past=None), "null"), (_plan, dict(free=None), "free_pages"),
-    (_plan, dict(slots=None), "slot_map"), (_plan, dict(num_pages=2 ** 28), "slots"),
+    (_plan, dict(slots=None), "slot_map"), (_plan, dict(num_pages=2 ** 28), "slots"), (_plan, dict(num_pages=2 ** 27 - 1), "slots"),
     (_plan, dict(max_pages=2 ** 28), "slots"), (_plan, dict(status=None), "null"),
     (_write, dict(hd=96), "head_dim"), (_write, dict(page=8), "page"), (_write, dict(k_dtype=0), "float"),
     (_write, dict(v_dtype=4), "float"), (_write, dict(kc=P + 8), "aligned"), (_write, dict(v=None), "null"),
