@@ -308,7 +308,7 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *
  * The cache: pages of `page` tokens (16, 32, 64 or 128), hd 64, 128 or 256, in e4m3 codes:
  *   k_cache [num_pages][KV][page][hd]   v_cache [num_pages][KV][hd][page]  (token innermost)
- *   k_scale, v_scale [num_pages][KV] f32: x = code * scale
+ *   k_scale, v_scale [num_pages][KV] f32: x = code * scale, finite and positive on every page in use
  * both caches 16-byte aligned; at most 2^31 - 256 slots (num_pages * page), and as many positions of a
  * block table's row.  Slot s is token
  * s % page of page s / page. */
@@ -321,7 +321,9 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *   aligned, out rows 8-byte; k and v tokens hd to 2^24 elements apart
  *   out = sum_j softmax_j(scale * q . k_j) v_j      float32 logits, statistics and sums; the weights
  *   are rounded to the tensors' type for the matrix cores
- * What a row does not see does not reach it, whatever it holds. */
+ * out may be q itself, but must not overlap k or v (nor, below, the cache).
+ * What a row does not see does not reach it, whatever it holds; a logit that it does see and that is
+ * infinite can make it infinite or NaN. */
 int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                           const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int32_t tokens,
                           const int32_t* cu_seqlens, int32_t B, int32_t H, int32_t KV, int32_t hd, float scale,
