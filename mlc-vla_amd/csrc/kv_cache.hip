@@ -502,23 +502,82 @@ __device__ __forceinline__ int last_limit(const KvAttnArgs& a, const Item& it, i
   return a.causal ? kv_len - it.n + last / a.grp + 1 : kv_len;
 }
 
+// Global -> LDS DMA, one address per lane, to lds + 16 (4) lane.  In assembly: the compiler would wait for every DMA in
+// flight before each read of LDS.  It returns nothing into registers; the loop waits for it.
+__device__ __forceinline__ uint32_t lds_at(const char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
+#else
+  return 0;
+#endif
+}
+__device__ __forceinline__ void dma16(const void* base, int off, const char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_at(lds)), "v"(off), "s"(base)
+               : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void dma16(const void* p, const char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_at(lds)), "v"(p)
+               : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void dma4(const void* p, const char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_at(lds)), "v"(p)
+               : "memory", "m0");
+#endif
+}
+// all but the last N DMA instructions have arrived
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+#endif
+}
+// LDS reads have arrived: their memory can be written again
+__device__ __forceinline__ void wait_lds() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+// a value that was loaded is there
+template <class T>
+__device__ __forceinline__ void wait_value(T& v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(v));
+#endif
+}
+
+// Piece p (16 bytes) of key row r lies at piece p ^ k_turn(r): the 16 rows that 16 lanes read at once fall into
+// distinct pieces of a 256-byte bank line.  A field of r's bits, so that k_turn(a | b) = k_turn(a) ^ k_turn(b) for
+// a & b = 0.
+template <int HD>
+__device__ constexpr int k_turn(int r) {
+  return HD == 256 ? (r & 3) | (r >> 3 & 3) << 2 : HD == 128 ? (r >> 1 & 1) | (r >> 4 & 3) << 1 : r >> 4 & 3;
+}
+
 // Row r of a request is token r / grp of its n new tokens and head h * grp + r % grp: the query heads of a kv
 // head share its keys.  A workgroup (4 waves) takes 16 such rows and one split of the keys; its waves take tiles of
 // TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
 //
-// A wave's tile has no LDS and no shuffle of data in it.  S^T = K . Q^T and O^T = V^T . P^T on
+// No data is shuffled between lanes.  S^T = K . Q^T and O^T = V^T . P^T on
 // v_mfma_f32_16x16x32: with lane = 16 g + r, S^T puts keys 4 g .. 4 g + 3 of each 16-key sub-tile and query row
 // r into a lane, and the second product wants 8 keys of row r in it.  Both contractions may run in any order,
 // so the order is chosen by the loads: with PL = TK / 4, sub-tile s's row 4 g + i is key PL g + 4 s + i of the
 // tile; a lane then owns PL consecutive keys, which are PL contiguous bytes of the value page, lie in one page
 // and have one scale of each side.  Dims likewise: a lane's 16 key bytes are two steps of the first contraction.
-// The loads of a wave's next tile are issued as soon as their registers are free: the keys' behind the first
-// product, the values' behind the second, the page numbers a tile earlier.
+// A lane's neighbours hold other rows of the page, so that loads from the page into these registers would take a
+// cache access per lane (1070 of a tile of 16 KB, which bound the many rows of action suffixes).  Each wave therefore
+// fetches its tiles by DMA into a part of LDS of its own, lanes side by side along the rows (eight suffixes of 50
+// tokens 25.4 -> 18.8 us), and reads the operands from there.  No barrier: as soon as a tile's keys (values) are in
+// registers, the next tile's follow into the same place; its page numbers come a tile earlier.
 //
 // Bound by HBM: one token each of 96 requests that hold 4096, 8 kv heads of 128, takes 147 us (5.5 TB/s), of 48 requests
 // 84 (4.8); with lengths from 1 to 4096 the last workgroups run with the GPU half empty (48 requests, 64 us, 3.7
 // TB/s).  More bytes in flight bring nothing there: two tiles of loads ahead 67 us, three waves a SIMD 79 and more.
-// Bound by the latency of a tile at few requests: 969 tokens of one kv head of 256, 7.6 us and 3.6 for the join.
+// Bound by the latency of a tile at few requests: 969 tokens of one kv head of 256, 6.9 us and 3.3 for the join.
 //
 // The value scale is folded into the weights before they are rounded to fp16: with x = logit * log2(e) the
 // running maximum is that of x + log2(scale_v), so that w = 2^(x - m) * scale_v stays within [0, 2^12] whatever
@@ -536,7 +595,8 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   typedef uint32_t VWords __attribute__((ext_vector_type(VW)));
   __shared__ int sh[5];
   __shared__ float sm[4][KV_RT], sl[4][KV_RT];
-  __shared__ __attribute__((aligned(16))) float so[4][KV_RT][HD + 4];
+  constexpr int HALF = TK * HD, AREA = 2 * HALF + 512, MEET = KV_RT * (HD + 4) * 4;  // bytes of a wave
+  __shared__ __attribute__((aligned(1024))) char lds[4 * (AREA > MEET ? AREA : MEET)];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / (a.KV * a.S), rest = blockIdx.x % (a.KV * a.S);
@@ -553,48 +613,46 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   if (split > 0 && t_begin >= tiles) return;
 
   const int32_t* table = a.table + (size_t)it.b * a.max_pages;
-  // pages of this lane's key row and of its own keys in tile t; -1: none that can be read
-  struct Pages {
-    int k, v;
+  // A wave's part of LDS: its tile's keys, values, page numbers and scales.  A tile is NG groups of 16 keys, each in
+  // one page.
+  constexpr int NG = TK / 16, NI = HALF / 1024, RPI = 1024 / HD;  // DMA instructions, key rows of one
+  char* const my_k = lds + w * AREA;
+  char* const my_v = my_k + HALF;
+  const int* const my_ids = reinterpret_cast<const int*>(my_v + HALF);
+  const float* const my_scales = reinterpret_cast<const float*>(my_v + HALF + 256);
+  const int vg = (lane & (NG - 1)) ^ (g & (NG - 1));  // the group whose numbers, scales and values this lane fetches
+  const int ko = lane / (HD / 16) * HD + ((lane % (HD / 16)) ^ k_turn<HD>(lane / (HD / 16))) * 16;
+  int ids[NG], id_mine = 0, id_own = 0;  // pages of the groups, of vg, of the lane's own keys; -1: none to be read
+  auto fetch_ids = [&](int t) {
+    t = min(t, t_end - 1);
+    dma4(table + min((TK * t + 16 * vg) >> a.psh, a.max_pages - 1), reinterpret_cast<const char*>(my_ids));
   };
-  auto pages_at = [&](int t) {
-    auto one = [&](int pos) {
-      const int pg = pos >> a.psh;
-      const int id = pg < a.max_pages ? load_global(table + pg) : -1;
-      return id >= 0 && id < a.num_pages ? id : -1;
-    };
-    return Pages{one(TK * t + PL * (r16 >> 2)), one(TK * t + PL * g)};
+  auto read_ids = [&]() {
+    auto sound = [&](int id) { return id >= 0 && id < a.num_pages ? id : -1; };
+#pragma unroll
+    for (int i = 0; i < NG; ++i) ids[i] = __builtin_amdgcn_readfirstlane(sound(my_ids[i]));  // lane i < NG has vg = i
+    id_mine = sound(my_ids[lane]);
+    id_own = sound(my_ids[PL * g >> 4]);
   };
-  u4 kr[SUB][NJ];
-  VWords vr[ND];
-  auto load_keys = [&](int t, int id) {
-    const int pos = TK * t + PL * (r16 >> 2) + (r16 & 3);
-    const uint8_t* p = a.kc + (((size_t)max(id, 0) * a.KV + h) * page + (pos & (page - 1))) * HD + 16 * g;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) kr[s][j] = load_global(reinterpret_cast<const u4*>(p + 4 * s * HD + 64 * j));
+  auto load_scales = [&]() {
+    dma4((lane < 32 ? a.ks : a.vs) + (size_t)max(id_mine, 0) * a.KV + h, reinterpret_cast<const char*>(my_scales));
   };
-  auto load_values = [&](int t, int id) {
-    const uint8_t* p = a.vc + (((size_t)max(id, 0) * a.KV + h) * HD + r16) * page + ((TK * t + PL * g) & (page - 1));
+  auto load_keys = [&](int t) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const VWords*>(p + (size_t)16 * d * page));
+    for (int i = 0; i < NI; ++i) {
+      const int grp = i * RPI / 16, pos = (TK * t + 16 * grp) & (page - 1);
+      const uint8_t* p = a.kc + (((size_t)max(ids[grp], 0) * a.KV + h) * page + pos + (i * RPI & 15)) * HD;
+      dma16(p, ko ^ 16 * k_turn<HD>(i * RPI), my_k + 1024 * i);
+    }
+  };
+  auto load_values = [&](int t) {
+    const uint8_t* p = a.vc + (((size_t)max(id_mine, 0) * a.KV + h) * HD + lane / NG) * page +
+                       ((TK * t + 16 * vg) & (page - 1));
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16(p + (size_t)(64 / NG * i) * page, my_v + 1024 * i);
   };
   int t = t_begin + w;
-  Pages now = {-1, -1}, next = {-1, -1};
-  float sk = 0.f, sv = 0.f;  // scales of the lane's keys
-  auto load_scales = [&](int id) {
-    const size_t i = (size_t)max(id, 0) * a.KV + h;
-    sk = load_global(a.ks + i);
-    sv = load_global(a.vs + i);
-  };
-  if (t < t_end) {
-    now = pages_at(t);
-    if (t + 4 < t_end) next = pages_at(t + 4);
-    load_scales(now.v);
-    load_keys(t, now.k);
-    load_values(t, now.v);
-  }
+  if (t < t_end) fetch_ids(t);
 
   // the query operand: row r16, dims 64 j + 16 g + 8 s .. + 7 for step 2 j + s
   V8 q[2 * NJ];
@@ -615,6 +673,19 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
         }
       }
   }
+#pragma unroll
+  for (int i = 0; i < 2 * NJ; ++i) wait_value(q[i]);  // no load of the compiler's is in flight in the loop
+  int own_page = 0;  // of the tile at hand
+  if (t < t_end) {
+    wait_dma<0>();
+    read_ids();
+    own_page = id_own;
+    wait_lds();
+    fetch_ids(t + 4);
+    load_scales();
+    load_keys(t);
+    load_values(t);
+  }
   f4 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = (f4){0.f, 0.f, 0.f, 0.f};
@@ -622,11 +693,26 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   bool poison = false;  // a NaN code was cleared
   for (; t < t_end; t += 4) {
     const int pv = TK * t + PL * g;
-    const float skc = sk * a.c, svc = sv;
     const bool more = t + 4 < t_end;
-    Pages after = {-1, -1};
-    if (t + 8 < t_end) after = pages_at(t + 8);
-
+    wait_dma<NI>();  // in flight behind it: the values
+    u4 kr[SUB][NJ];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int row = PL * (r16 >> 2) + 4 * s + (r16 & 3);
+        kr[s][j] = *reinterpret_cast<const u4*>(my_k + row * HD + (((4 * j + g) ^ k_turn<HD>(row)) * 16));
+      }
+    const float skc = my_scales[PL * g >> 4] * a.c, svc = my_scales[32 + ((PL * g >> 4) ^ (2 & (NG - 1)))];
+    const int now = own_page;
+    if (more) {
+      read_ids();
+      own_page = id_own;
+      wait_lds();
+      fetch_ids(t + 8);
+      load_scales();
+      load_keys(t + 4);
+    }
     f4 x[SUB];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
@@ -637,28 +723,8 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
         x[s] = mfma16(widen8<BF>(kr[s][j][2], kr[s][j][3]), q[2 * j + 1], x[s]);
       }
     }
-    if (more) {
-      load_scales(next.v);
-      load_keys(t + 4, next.k);
-    }
-    const int own = now.v < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
-    const bool edge = TK * t + TK > first || __any(now.v < 0);
-    if (edge) {
-      bool nan = false;
-#pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        const uint32_t keep = byte_mask(0, own - 4 * i);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          vr[d][i] &= keep;
-          // bytes that are NaN codes (0x7f or 0xff) to zero
-          const uint32_t bad = ((((vr[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
-          nan = nan || bad;
-          vr[d][i] &= ~bad;
-        }
-      }
-      poison = poison || __any(nan);
-    }
+    const int own = now < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
+    const bool edge = TK * t + TK > first || __any(now < 0);
     const float lsv = __builtin_amdgcn_logf(fmaxf(svc, 0x1p-64f)) - 12.0f;
     h8 p[PL / 8];
     float top = -INFINITY;
@@ -686,22 +752,52 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
         p[s >> 1][4 * (s & 1) + i] = (_Float16)(e * svc);
       }
     l = l * alpha + sum;
+    if (more) wait_dma<NI + 2>();  // behind the values: the next tile's keys, scales and page numbers
+    else wait_dma<0>();
+    VWords vr[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int dim = 16 * d + r16, piece = NG * dim + ((PL * g >> 4) ^ (dim * NG >> 4 & (NG - 1)));
+      vr[d] = *reinterpret_cast<const VWords*>(my_v + 16 * piece + (PL * g & 15));
+    }
+    if (more) {
+      wait_lds();
+      load_values(t + 4);
+    }
+    if (edge) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < VW; ++i) {
+        const uint32_t keep = byte_mask(0, own - 4 * i);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          vr[d][i] &= keep;
+          // bytes that are NaN codes (0x7f or 0xff) to zero
+          const uint32_t bad = ((((vr[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+          nan = nan || bad;
+          vr[d][i] &= ~bad;
+        }
+      }
+      poison = poison || __any(nan);
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       o[d] *= alpha;
 #pragma unroll
       for (int i = 0; i < PL / 8; ++i) o[d] = mfma16(widen8<false>(vr[d][2 * i], vr[d][2 * i + 1]), p[i], o[d]);
     }
-    if (more) load_values(t + 4, next.v);
-    now = next;
-    next = after;
   }
   if (poison)  // the tiles of this wave that hold keys from `first` on, or pages that are not there
     for (t = t_begin + w; t < t_end; t += 4) {
-      const int idv = pages_at(t).v;
+      const int pos = TK * t + PL * g, pg = pos >> a.psh;
+      int idv = pg < a.max_pages ? load_global(table + pg) : -1;
+      if (idv >= a.num_pages) idv = -1;
       if (!(TK * t + TK > first || __any(idv < 0))) continue;
-      load_values(t, idv);
-      const int own = idv < 0 ? 0 : clamp_i(kv_len - (TK * t + PL * g), 0, PL);
+      VWords vr[ND];
+      const uint8_t* p = a.vc + (((size_t)max(idv, 0) * a.KV + h) * HD + r16) * page + (pos & (page - 1));
+#pragma unroll
+      for (int d = 0; d < ND; ++d) vr[d] = load_global(reinterpret_cast<const VWords*>(p + (size_t)16 * d * page));
+      const int own = idv < 0 ? 0 : clamp_i(kv_len - pos, 0, PL);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         int at = 0x7fffffff;  // the first of the lane's keys whose value at dim 16 d + r16 is NaN
@@ -719,6 +815,7 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
 
   const size_t part0 = (((size_t)item * a.KV + h) * a.S + split) * KV_RT;  // of the partial results' rows
   // ---- the waves meet ------------------------------------------------------------------------------
+  float (*so)[KV_RT][HD + 4] = reinterpret_cast<float (*)[KV_RT][HD + 4]>(lds);  // once every wave is through its tiles
   l = xor_sum_16_32(l);
   if (g == 0) {
     sm[w][r16] = m;
@@ -853,13 +950,25 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   p.items = rows / KV_RT + B;
   const long long busy = std::max({1ll, (rows + KV_RT - 1) / KV_RT, (long long)std::min(B, tokens)}) * KV;
   const int tiles = std::max(1, max_kv / 64 + (max_kv % 64 != 0));
-  // Splits while the workgroups are resident at once, two to a CU: two requests of 131072 tokens take 38 us in 128 or
-  // 256 splits each, 45 in 512.  From 171 workgroups on none: two splits of 200 (eight suffixes of 50 tokens, 8 heads)
-  // take 28 us and their join among them, one 25.5; of 384 (48 requests of 8 kv heads) 70, one 64.  At least a tile
-  // for every wave.
-  const long long fit = 512 / busy, least = hd == 256 ? 2 : 4;
-  const long long want = fit < 3 ? 1 : std::min(fit, (tiles + least - 1) / least);
-  p.span = (int)((tiles + want - 1) / want);
+  // Splits: none, or as many as make one or two workgroups per CU, whichever costs least.  In rounds of the waves'
+  // tiles a workgroup costs two more to begin with, all of it half as much again where two share a CU, and the join's
+  // launch 2.5 and its reads.  Heads of 256: 5 suffixes of 50 tokens over 1018 take 18.3 us without, 24.7 with four
+  // splits, two of them 13.6 with four, 16.6 with eight; 200 requests of 4096 tokens 126 without, 95 with two (but 16 of
+  // them 19.5 with 16, 16.9 with 32).  Heads of 128: 24 requests of 4096 tokens 41.4 and 48.5, 16 of them 38.6 with two,
+  // 33.6 with four; a suffix 11.1 and 10.2; one workgroup per CU was never best there (8 requests 21.5, two per CU
+  // 17.4).
+  const int round = hd == 256 ? 2 : 4;  // tiles of 64 keys that the waves take at once
+  auto cut = [&](long long n) {
+    const long long want = std::max(1ll, std::min<long long>(n / busy, (tiles + round - 1) / round));
+    return (int)((tiles + want - 1) / want);
+  };
+  auto cost = [&](int span) {
+    const long long S = (tiles + span - 1) / span, groups = busy * S, rounds = 2 + (span + round - 1) / round;
+    return rounds * (groups > 256 ? 1.5 : 1.0) + (S > 1 ? 2.5 + groups * hd / 65536.0 : 0.0);
+  };
+  p.span = tiles;
+  for (const int n : {512, 256})
+    if ((n == 512 || hd == 256) && cost(cut(n)) < cost(p.span)) p.span = cut(n);
   p.S = (tiles + p.span - 1) / p.span;
   const size_t parts = (size_t)p.items * KV * p.S * KV_RT;
   p.o_floats = p.S > 1 ? parts * hd : 0;
