@@ -64,11 +64,12 @@ __device__ __forceinline__ f16v mfma32(Elem<true>::V8 a, Elem<true>::V8 b, f16v 
 
 // 16 bytes per lane from the buffer into LDS at lds + 16 lane.  In assembly, because the compiler waits for every
 // DMA in flight before a transposing LDS read, whose memory it does not know; it returns nothing into registers,
-// and the loop waits for it before the barrier after which the tile is read.
+// and the loop waits for it before the barrier after which the tile is read.  M0, which holds the LDS address, has to
+// be one wait state old.
 __device__ __forceinline__ void pr_dma16(u4 r, char* lds, int voff) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(r));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(r) : "m0");
 #endif
 }
 // four 16-bit elements of one column: per 16 lanes a 4 x 16 block, lane i giving the address of row i / 4,
