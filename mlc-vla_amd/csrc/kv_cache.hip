@@ -559,8 +559,8 @@ __device__ constexpr int k_turn(int r) {
 }
 
 // Row r of a request is token r / grp of its n new tokens and head h * grp + r % grp: the query heads of a kv
-// head share its keys.  A workgroup (4 waves) takes 16 such rows and one split of the keys; its waves take tiles of
-// TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
+// head share its keys.  A workgroup (NW waves) takes 16 such rows and one split of the keys; its waves take tiles
+// of TK keys in turn, each with its own running maximum and sum, and meet in LDS at the end.
 //
 // No data is shuffled between lanes.  S^T = K . Q^T and O^T = V^T . P^T on
 // v_mfma_f32_16x16x32: with lane = 16 g + r, S^T puts keys 4 g .. 4 g + 3 of each 16-key sub-tile and query row
@@ -587,16 +587,16 @@ __device__ constexpr int k_turn(int r) {
 //
 // A key or page that a row does not see has weight 0, which a NaN code behind it would turn into NaN.  In a tile
 // that not every row sees whole such codes are cleared, and at the end the rows that do see one are set to NaN.
-template <bool BF, int HD, int TK>
-__global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
+template <bool BF, int HD, int TK, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv_attn_kernel(const KvAttnArgs a) {
   typedef typename El<BF>::T T;
   typedef typename El<BF>::V8 V8;
   constexpr int NJ = HD / 64, ND = HD / 16, SUB = TK / 16, PL = TK / 4, VW = PL / 4;
   typedef uint32_t VWords __attribute__((ext_vector_type(VW)));
   __shared__ int sh[5];
-  __shared__ float sm[4][KV_RT], sl[4][KV_RT];
+  __shared__ float sm[NW][KV_RT], sl[NW][KV_RT];
   constexpr int HALF = TK * HD, AREA = 2 * HALF + 512, MEET = KV_RT * (HD + 4) * 4;  // bytes of a wave
-  __shared__ __attribute__((aligned(1024))) char lds[4 * (AREA > MEET ? AREA : MEET)];
+  __shared__ __attribute__((aligned(1024))) char lds[NW * (AREA > MEET ? AREA : MEET)];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / (a.KV * a.S), rest = blockIdx.x % (a.KV * a.S);
@@ -681,7 +681,7 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
     read_ids();
     own_page = id_own;
     wait_lds();
-    fetch_ids(t + 4);
+    fetch_ids(t + NW);
     load_scales();
     load_keys(t);
     load_values(t);
@@ -691,9 +691,9 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   for (int d = 0; d < ND; ++d) o[d] = (f4){0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   bool poison = false;  // a NaN code was cleared
-  for (; t < t_end; t += 4) {
+  for (; t < t_end; t += NW) {
     const int pv = TK * t + PL * g;
-    const bool more = t + 4 < t_end;
+    const bool more = t + NW < t_end;
     wait_dma<NI>();  // in flight behind it: the values
     u4 kr[SUB][NJ];
 #pragma unroll
@@ -709,9 +709,9 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
       read_ids();
       own_page = id_own;
       wait_lds();
-      fetch_ids(t + 8);
+      fetch_ids(t + 2 * NW);
       load_scales();
-      load_keys(t + 4);
+      load_keys(t + NW);
     }
     f4 x[SUB];
 #pragma unroll
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
     }
     if (more) {
       wait_lds();
-      load_values(t + 4);
+      load_values(t + NW);
     }
     if (edge) {
       bool nan = false;
@@ -788,7 +788,7 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
     }
   }
   if (poison)  // the tiles of this wave that hold keys from `first` on, or pages that are not there
-    for (t = t_begin + w; t < t_end; t += 4) {
+    for (t = t_begin + w; t < t_end; t += NW) {
       const int pos = TK * t + PL * g, pg = pos >> a.psh;
       int idv = pg < a.max_pages ? load_global(table + pg) : -1;
       if (idv >= a.num_pages) idv = -1;
@@ -824,12 +824,14 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   __syncthreads();
   float f;  // this wave's share of the workgroup's sum
   {
-    const float mx = fmaxf(fmaxf(sm[0][r16], sm[1][r16]), fmaxf(sm[2][r16], sm[3][r16]));
+    float mx = sm[0][r16];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sm[i][r16]);
     const float mu = mx == -INFINITY ? 0.f : mx;
     f = __builtin_amdgcn_exp2f(m - mu);
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += sl[i][r16] * __builtin_amdgcn_exp2f(sm[i][r16] - mu);
+    for (int i = 0; i < NW; ++i) sum += sl[i][r16] * __builtin_amdgcn_exp2f(sm[i][r16] - mu);
     if (a.S > 1) {
       if (w == 0 && g == 0 && row0 + r16 < rows) reinterpret_cast<f2*>(a.part_ml)[part0 + r16] = (f2){mx, sum};
     } else {
@@ -838,19 +840,16 @@ __global__ __launch_bounds__(KV_NT, 2) void kv_attn_kernel(const KvAttnArgs a) {
   }
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    f4 v = o[d];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = f == 0.f ? 0.f : v[i] * f;
-    *reinterpret_cast<f4*>(&so[w][r16][16 * d + 4 * g]) = v;
+    *reinterpret_cast<f4*>(&so[w][r16][16 * d + 4 * g]) = o[d] * f;  // a NaN stays, even under a share of zero
   }
   __syncthreads();
 #pragma unroll
-  for (int i = tid; i < KV_RT * HD / 4; i += KV_NT) {
+  for (int i = tid; i < KV_RT * HD / 4; i += 64 * NW) {
     const int row = i / (HD / 4), d = 4 * (i % (HD / 4));
     if (row0 + row >= rows) continue;
     f4 v = *reinterpret_cast<const f4*>(&so[0][row][d]);
 #pragma unroll
-    for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const f4*>(&so[k][row][d]);
+    for (int k = 1; k < NW; ++k) v += *reinterpret_cast<const f4*>(&so[k][row][d]);
     if (a.S > 1) {
       *reinterpret_cast<f4*>(a.part_o + (part0 + row) * HD + d) = v;
     } else {
@@ -911,7 +910,7 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a) {
     const f2 e = load_global(ml + (size_t)s * KV_RT);
     const float f = __builtin_amdgcn_exp2f(e[0] - mu);
     const f4 u = load_global(reinterpret_cast<const f4*>(a.part_o + (p0 + (size_t)s * KV_RT) * HD + d0 + d));
-    if (f != 0.f) v += u * f;
+    v += u * f;
     sum += e[1] * f;
   }
 #pragma unroll
@@ -941,6 +940,7 @@ __global__ __launch_bounds__(KV_NT) void kv_join_kernel(const KvAttnArgs a) {
 // How an attention call is cut: splits of the keys, from what the host knows.
 struct KvAttnPlan {
   int S, span;
+  bool wide;         // eight waves per workgroup
   long long items;  // tiles of 16 rows, at most
   size_t o_floats, bytes;
 };
@@ -950,25 +950,30 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   p.items = rows / KV_RT + B;
   const long long busy = std::max({1ll, (rows + KV_RT - 1) / KV_RT, (long long)std::min(B, tokens)}) * KV;
   const int tiles = std::max(1, max_kv / 64 + (max_kv % 64 != 0));
-  // Splits: none, or as many as make one or two workgroups per CU, whichever costs least.  In rounds of the waves'
-  // tiles a workgroup costs two more to begin with, all of it half as much again where two share a CU, and the join's
-  // launch 2.5 and its reads.  Heads of 256: 5 suffixes of 50 tokens over 1018 take 18.3 us without, 24.7 with four
-  // splits, two of them 13.6 with four, 16.6 with eight; 200 requests of 4096 tokens 126 without, 95 with two (but 16 of
-  // them 19.5 with 16, 16.9 with 32).  Heads of 128: 24 requests of 4096 tokens 41.4 and 48.5, 16 of them 38.6 with two,
-  // 33.6 with four; a suffix 11.1 and 10.2; one workgroup per CU was never best there (8 requests 21.5, two per CU
-  // 17.4).
-  const int round = hd == 256 ? 2 : 4;  // tiles of 64 keys that the waves take at once
+  // What costs least: four or eight waves per workgroup, or splits, as many as make one or two workgroups per CU.  In
+  // rounds of four waves' tiles a workgroup costs two more to begin with, all of it half as much again where eight
+  // waves share a CU, and the join's launch 2.5 and its reads.  Heads of 256: 8 suffixes of 50 tokens over 1018 take
+  // 18.7 us with four waves, 17.1 with eight, two suffixes 13.6 with four splits, 16.6 with eight and 16.2 with none;
+  // 200 requests of 4096 tokens 126 with four waves, 80 with eight, 95 with two splits; 128 of them 67 with four
+  // splits, 70 with none.  Heads of 128: 32 requests 43.6 with four waves, 38.4 with eight (24 of them 34.3 and 35.2); 16
+  // of them 33 with eight, 28 with four splits.  One workgroup per CU was never best there (8 requests 21.5, two 17.4).
+  const int round = hd == 256 ? 2 : 4;  // tiles of 64 keys that four waves take at once
   auto cut = [&](long long n) {
     const long long want = std::max(1ll, std::min<long long>(n / busy, (tiles + round - 1) / round));
     return (int)((tiles + want - 1) / want);
   };
-  auto cost = [&](int span) {
-    const long long S = (tiles + span - 1) / span, groups = busy * S, rounds = 2 + (span + round - 1) / round;
-    return rounds * (groups > 256 ? 1.5 : 1.0) + (S > 1 ? 2.5 + groups * hd / 65536.0 : 0.0);
+  auto cost = [&](int span, bool wide) {
+    const long long S = (tiles + span - 1) / span, groups = busy * S, at_once = wide ? 2 * round : round;
+    return (2 + (span + at_once - 1) / at_once) * (wide || groups > 256 ? 1.5 : 1.0) +
+           (S > 1 ? 2.5 + groups * hd / 65536.0 : 0.0);
   };
   p.span = tiles;
+  p.wide = busy <= 256 && cost(tiles, true) <= cost(tiles, false);
   for (const int n : {512, 256})
-    if ((n == 512 || hd == 256) && cost(cut(n)) < cost(p.span)) p.span = cut(n);
+    if ((n == 512 || hd == 256) && cost(cut(n), false) < cost(p.span, p.wide)) {
+      p.span = cut(n);
+      p.wide = false;
+    }
   p.S = (tiles + p.span - 1) / p.span;
   const size_t parts = (size_t)p.items * KV * p.S * KV_RT;
   p.o_floats = p.S > 1 ? parts * hd : 0;
@@ -1001,7 +1006,9 @@ template <bool BF, int HD>
 int kv_attn_launch(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_t st) {
   const unsigned grid = (unsigned)(p.items * a.KV * p.S);
   // tiles of 32 keys at head_dim 256: two waves fit a SIMD (131072 tokens 52 -> 38 us)
-  kv_attn_kernel<BF, HD, (HD == 256 ? 32 : 64)><<<grid, KV_NT, 0, st>>>(a);
+  constexpr int TK = HD == 256 ? 32 : 64;
+  if (p.wide) kv_attn_kernel<BF, HD, TK, 8><<<grid, 512, 0, st>>>(a);
+  else kv_attn_kernel<BF, HD, TK, 4><<<grid, 256, 0, st>>>(a);
   MLCV_HIP(hipGetLastError());
   if (p.S > 1) {
     const long long rows = (long long)a.tokens * a.H;

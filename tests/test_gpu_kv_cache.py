@@ -393,6 +393,30 @@ def test_kv_attention_nan_behind_the_mask(dt, hd):
     assert torch.isnan(got.torch[4].float()).all() and torch.isfinite(got.torch[:3].float()).all()
 
 
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("dt,hd", [("f16", 64), ("bf16", 128), ("f16", 256)])
+def test_kv_attention_suffixes(dt, hd, page):
+    """Many rows over long contexts, as action suffixes are: more waves to a workgroup, no splits."""
+    rng = np.random.default_rng(40)
+    past, new = [1018, 700, 0, 903, 65, 1200], [50, 50, 50, 0, 33, 50]
+    table, (kc, ks, vc, vs) = _paged(rng, past, new, 1, hd, page)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    lens = [p + n for p, n in zip(past, new)]
+    table[1, 3] = -1
+    kr, vr = kc.view(torch.uint8), vc.view(torch.uint8)
+    last = table[5, (lens[5] - 1) // page], (lens[5] - 1) % page + 1   # NaN behind a request's end
+    kr[last[0], :, last[1]:] = 0x7f
+    vr[last[0], :, :, last[1]:] = 0xff
+    q = _rows(rng, (cu[-1], 8, hd), TYPES[dt], 0.5)
+    for causal in (True, False):
+        got = _check_cached(q, cu, lens, table, (kc, ks, vc, vs), causal)
+        assert torch.isfinite(got.torch.float()).all()
+    vr[table[0, 0], 0, 5, 7] = 0x7f        # a value that every row of request 0 sees
+    got = _check_cached(q, cu, lens, table, (kc, ks, vc, vs), False)
+    bad = torch.isnan(got.torch.float())
+    assert bad[:50, :, 5].all() and int(bad.sum()) == 50 * 8
+
+
 def test_kv_attention_strides_and_workspace():
     rng = np.random.default_rng(4)
     past, new, hd = [900, 40], [2, 9], 128
