@@ -571,13 +571,14 @@ __device__ constexpr int k_turn(int r) {
 // A lane's neighbours hold other rows of the page, so that loads from the page into these registers would take a
 // cache access per lane (1070 of a tile of 16 KB, which bound the many rows of action suffixes).  Each wave therefore
 // fetches its tiles by DMA into a part of LDS of its own, lanes side by side along the rows (eight suffixes of 50
-// tokens 25.4 -> 18.8 us), and reads the operands from there.  No barrier: as soon as a tile's keys (values) are in
+// tokens 25.4 -> 18.6 us), and reads the operands from there.  No barrier: as soon as a tile's keys (values) are in
 // registers, the next tile's follow into the same place; its page numbers come a tile earlier.
 //
 // Bound by HBM: one token each of 96 requests that hold 4096, 8 kv heads of 128, takes 147 us (5.5 TB/s), of 48 requests
 // 84 (4.8); with lengths from 1 to 4096 the last workgroups run with the GPU half empty (48 requests, 64 us, 3.7
-// TB/s).  More bytes in flight bring nothing there: two tiles of loads ahead 67 us, three waves a SIMD 79 and more.
-// Bound by the latency of a tile at few requests: 969 tokens of one kv head of 256, 6.9 us and 3.3 for the join.
+// TB/s).  More bytes in flight bring nothing there: two tiles of loads ahead 67 us, three waves a SIMD 79 and
+// more (both before the DMA).
+// Bound by the latency of a tile at few requests: 969 tokens of one kv head of 256, 6.8 us and 3.3 for the join.
 //
 // The value scale is folded into the weights before they are rounded to fp16: with x = logit * log2(e) the
 // running maximum is that of x + log2(scale_v), so that w = 2^(x - m) * scale_v stays within [0, 2^12] whatever
