@@ -293,8 +293,8 @@ __device__ __forceinline__ uint32_t byte_mask(int lo, int hi) {
 // codes, so that the input is read once.  Where a head's page has fewer units than the workgroup threads, several
 // heads go side by side.  Keys leave as 8 bytes per position; values go through LDS to be turned to [hd][page] and
 // leave as 16-byte pieces.  A piece that is not wholly new is merged with what the page held.
-// Bound by HBM for long prompts (21447 tokens of 8 heads of 128 in pages of 32: 40.7 us, 3.2 TB/s), by the chain of loads
-// (cu, slots, tokens) for few tokens (64 requests of one: 7.4 us).
+// Bound by HBM for long prompts (21447 tokens of 8 heads of 128 in pages of 32: 40.7 us, 3.2 TB/s), by the chain of
+// loads (cu, slots, tokens) for few tokens (64 requests of one: 7.8 us).
 template <int HD, int UNITS>
 __global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
   constexpr int CH = HD / 8;                     // 8-dim pieces of a row
@@ -574,8 +574,8 @@ __device__ constexpr int k_turn(int r) {
 // tokens 25.4 -> 18.6 us), and reads the operands from there.  No barrier: as soon as a tile's keys (values) are in
 // registers, the next tile's follow into the same place; its page numbers come a tile earlier.
 //
-// Bound by HBM: one token each of 96 requests that hold 4096, 8 kv heads of 128, takes 147 us (5.5 TB/s), of 48 requests
-// 84 (4.8); with lengths from 1 to 4096 the last workgroups run with the GPU half empty (48 requests, 64 us, 3.7
+// Bound by HBM: one token each of 96 requests that hold 4096, 8 kv heads of 128, takes 147 us (5.5 TB/s), of 48
+// requests 84 (4.8); with lengths from 1 to 4096 the last workgroups run with the GPU half empty (48 requests, 64 us, 3.7
 // TB/s).  More bytes in flight bring nothing there: two tiles of loads ahead 67 us, three waves a SIMD 79 and
 // more (both before the DMA).
 // Bound by the latency of a tile at few requests: 969 tokens of one kv head of 256, 6.8 us and 3.3 for the join.
@@ -956,8 +956,10 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   // waves share a CU, and the join's launch 2.5 and its reads.  Heads of 256: 8 suffixes of 50 tokens over 1018 take
   // 18.7 us with four waves, 17.1 with eight, two suffixes 13.6 with four splits, 16.6 with eight and 16.2 with none;
   // 200 requests of 4096 tokens 126 with four waves, 80 with eight, 95 with two splits; 128 of them 67 with four
-  // splits, 70 with none.  Heads of 128: 32 requests 43.6 with four waves, 38.4 with eight (24 of them 34.3 and 35.2); 16
-  // of them 33 with eight, 28 with four splits.  One workgroup per CU was never best there (8 requests 21.5, two 17.4).
+  // splits, 70 with none.  Heads of 128: 32 requests 43.6 with four waves, 38.4 with eight (24 of them 34.3 and 35.2);
+  // 16 of them 33 with eight, 28 with four splits.  One workgroup per CU was never best there (8 requests 21.5, two
+  // 17.4).  Above 256 workgroups eight waves are slower: 16 suffixes 31.7 us (26.2), 500 requests of up to 500 tokens,
+  // heads of 64, 34 (25); though 96 long ones 58 (63).
   const int round = hd == 256 ? 2 : 4;  // tiles of 64 keys that four waves take at once
   auto cut = [&](long long n) {
     const long long want = std::max(1ll, std::min<long long>(n / busy, (tiles + round - 1) / round));
