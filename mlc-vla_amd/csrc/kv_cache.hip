@@ -704,8 +704,11 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attn_kernel(const KvAttnArgs a)
         const int row = PL * (r16 >> 2) + 4 * s + (r16 & 3);
         kr[s][j] = *reinterpret_cast<const u4*>(my_k + row * HD + (((4 * j + g) ^ k_turn<HD>(row)) * 16));
       }
-    const float skc = my_scales[PL * g >> 4] * a.c, svc = my_scales[32 + ((PL * g >> 4) ^ (2 & (NG - 1)))];
     const int now = own_page;
+    const int own = now < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
+    // the value scale of a page that holds none of them may be anything, NaN too: it would outlast the weight of 0
+    const float vscale = my_scales[32 + ((PL * g >> 4) ^ (2 & (NG - 1)))];
+    const float skc = my_scales[PL * g >> 4] * a.c, svc = own > 0 ? vscale : 0.f;
     if (more) {
       read_ids();
       own_page = id_own;
@@ -724,7 +727,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attn_kernel(const KvAttnArgs a)
         x[s] = mfma16(widen8<BF>(kr[s][j][2], kr[s][j][3]), q[2 * j + 1], x[s]);
       }
     }
-    const int own = now < 0 ? 0 : clamp_i(kv_len - pv, 0, PL);  // the lane's keys that are the request's
     const bool edge = TK * t + TK > first || __any(now < 0);
     const float lsv = __builtin_amdgcn_logf(fmaxf(svc, 0x1p-64f)) - 12.0f;
     h8 p[PL / 8];
