@@ -355,10 +355,11 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
  * keeps the tokens before the first new one: the scale then only grows, and their codes follow it
  * (rounded to nearest even, which a power of two leaves exact but for subnormal codes).  Positions
  * behind the last new one keep their codes.  Values past 448 * scale and infinities saturate, NaN
- * stays NaN.  A request's slots are a plan's: they follow one another within a page, and its pages
- * after the first begin at their position 0.  Of the tokens of a page, those from the first on whose
- * slot does not follow are not written; nor is a later page that begins elsewhere, nor a negative
- * slot.  No page may be written twice in a call (its contents are then undefined). */
+ * stays NaN.  A request's slots are a plan's: they follow one another within a page, its pages after
+ * the first begin at their position 0, and -1 stands for the tokens of a page that is not there.  Of
+ * the tokens of a page, those from the first on whose slot does not follow are not written; nor is a
+ * later page that begins elsewhere, nor a negative slot.  No page may be written twice in a call (its
+ * contents are then undefined). */
 int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head, const void* v, int32_t v_dtype,
                   int64_t v_tok, int64_t v_head, int32_t tokens, const int32_t* cu_seqlens, int32_t B,
                   const int32_t* slot_map, void* k_cache, float* k_scale, void* v_cache, float* v_scale,

@@ -305,7 +305,22 @@ __global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
   const int tid = threadIdx.x, page = 1 << a.psh, z = blockIdx.z;
   const Item it = find_item(a.cu, nullptr, a.B, a.tokens, blockIdx.x, 1, page, 2, sh);
   if (it.b < 0) return;
-  const int o0 = a.slots[it.c0] & (page - 1);  // of a negative slot: any value, the tokens are dropped below
+  int o0 = a.slots[it.c0];  // the request's first slot: its place within the page says where the others begin
+  if (o0 < 0) {
+    // its first page is not there.  For a later one, any slot of the 2 page - 1 < KV_NT tokens that can lie on it,
+    // wherever pages begin, says the same; if all are negative, there is nothing to be written.
+    if (it.i == 0) return;
+    if (tid == 0) follow = KV_NT;
+    __syncthreads();
+    const int near = (it.i - 1) * page + 1;
+    if (tid < min(it.n - near, 2 * page - 1) && a.slots[it.c0 + near + tid] >= 0) atomicMin(&follow, tid);
+    __syncthreads();
+    const int first = follow;
+    if (first == KV_NT) return;
+    o0 = a.slots[it.c0 + near + first] - near - first;
+    __syncthreads();  // follow is written again
+  }
+  o0 &= page - 1;
   const int start = it.i == 0 ? it.c0 : it.c0 + it.i * page - o0;
   const int stop = min(it.c0 + it.n, it.i == 0 ? it.c0 + page - o0 : start + page);
   if (start >= stop) return;

@@ -66,3 +66,75 @@ def test_kv_attention_scales_of_pages_not_in_use(dt, hd, page):
             bad_k[unused], bad_v[unused] = x, x
             for most in (None, 1, 10 ** 6):                # other cuts of the keys
                 _check(q, cu, lens, table, (kc, bad_k, vc, bad_v), causal, want, tol, max_kv=most)
+
+
+# ---- write -----------------------------------------------------------------------------------------
+
+
+def _check_only(x, cu, slots, written, cache):
+    """kv_write of x as keys and values under `slots`: what writing the token runs `written` (first token, first slot,
+    tokens; each within a page) one by one gives, and nothing else changes."""
+    kc, ks, vc, vs = cache
+    page = kc.shape[2]
+    k, v = (_host(kc), _host(ks)), (_host(vc).transpose(0, 1, 3, 2).copy(), _host(vs))
+    xh = _host(x)
+    for t, slot, n in written:
+        for data, scale in (k, v):
+            R.write(xh[t:t + n], [0, n], range(slot, slot + n), data, scale, page)
+    C.kv_write(x, x, _ints(cu), _ints(slots), *cache)
+    for got, want in ((kc, k[0]), (ks, k[1]), (vc, v[0].transpose(0, 1, 3, 2)), (vs, v[1])):
+        np.testing.assert_array_equal(_host(got), want)
+
+
+@pytest.mark.parametrize("hd,kv", [(64, 2), (128, 1), (256, 1)])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_write_behind_pages_that_are_not_there(hd, kv, page):
+    """A request whose first pages have numbers outside of the cache: its later tokens go where their slots say."""
+    rng = np.random.default_rng(page + hd)
+    for past, ids in ((0, [-1, 2]), (5, [-1, 3, -1, 1]), (page - 1, [-1, -1, 0, 2]), (0, [-1, -1, -1, 3]), (0, [1, -1, 2]),
+                      (3, [-1, -1])):
+        for n in (len(ids) * page - past, len(ids) * page - past - page + 1):
+            own = [ids[(past + t) // page] for t in range(n)]
+            slots = [-1 if i < 0 else i * page + (past + t) % page for t, i in enumerate(own)]
+            # two more requests around it, so that its tokens and pages do not begin at 0
+            slots = [4 * page, 4 * page + 1] + slots + [5 * page + 7]
+            written, t = [(0, 4 * page, 2), (2 + n, 5 * page + 7, 1)], 0
+            while t < n:
+                run = min(n - t, page - (past + t) % page)
+                if own[t] >= 0:
+                    written.append((2 + t, slots[2 + t], run))
+                t += run
+            x = _rows(rng, (n + 3, kv, hd), torch.float16)
+            _check_only(x, [0, 2, 2 + n, 3 + n], slots, written, _cache(rng, 6, kv, hd, page))
+
+
+def test_plan_write_and_attention_behind_a_page_that_is_not_there():
+    """The free list begins with a page outside of the cache: the plan gives its tokens no slots, the writer fills the
+    request's other page, and the attention sees that page alone."""
+    rng = np.random.default_rng(3)
+    hd, page = 64, 16
+    cache = _cache(rng, 4, 1, hd, page)
+    table = torch.full((1, 2), -1, dtype=torch.int32, device="cuda")
+    plan = C.kv_plan(_ints([0]), _ints([32]), table, _ints([99, 2]), num_pages=4, page_size=page, tokens=32)
+    assert plan.slot_map.numpy().tolist() == [-1] * 16 + list(range(32, 48)) and plan.kv_lens.numpy().tolist() == [32]
+    x = _rows(rng, (32, 1, hd), torch.float16, 0.5)
+    _check_only(x, [0, 32], plan.slot_map.numpy().tolist(), [(16, 32, 16)], cache)
+    q = _rows(rng, (32, 2, hd), torch.float16, 0.5)
+    want, tol = _want_cached(q, [0, 32], [32], table.cpu().numpy(), cache, True, hd ** -0.5)
+    _check(q, [0, 32], [32], table.cpu().numpy(), cache, True, want, tol)
+    assert (want[:16] == 0).all() and (want[16:] != 0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_write_keeps_nan_codes_of_a_page_that_grows(hd):
+    """NaN codes among the tokens that a page keeps stay NaN when its scale grows, and do not raise it."""
+    rng = np.random.default_rng(hd)
+    page = 32
+    kc, ks, vc, vs = _cache(rng, 3, 2, hd, page)
+    kr, vr = kc.view(torch.uint8), vc.view(torch.uint8)
+    kr[1, 0, 3, 5], kr[1, 1, 6, hd - 1], kr[1, 0, 20, 2] = 0x7f, 0xff, 0x7f    # the last one behind the new tokens
+    vr[1, 0, 5, 3], vr[1, 1, hd - 1, 6], vr[1, 0, 2, 20] = 0xff, 0x7f, 0xff
+    for size in (1.0, 1e4):                                                    # the second grows the page
+        x = _rows(rng, (9, 2, hd), torch.float32) * size
+        _check_only(x, [0, 9], range(page + 7, page + 16), [(0, page + 7, 9)], (kc, ks, vc, vs))
+    assert int(torch.isnan(kc.float()).sum()) == 3 and int(torch.isnan(vc.float()).sum()) == 3
