@@ -340,7 +340,8 @@ int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const vo
  * tokens do not fit into `tokens`, or the free pages do not last (every later one that needs a
  * page is then refused too): it takes no page, its kv_lens is 0 and its slots are -1.  So are the
  * slots behind the last request and those on a page outside [0, num_pages).  At most 4096
- * requests.  The outputs must not overlap the inputs. */
+ * requests.  No output may overlap an input or another output (-2): kv_lens can be the next call's
+ * past_lens, but not that call's kv_lens too. */
 int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
                  int32_t n_free, int32_t num_pages, int32_t page, int32_t* block_table, int32_t max_pages,
                  int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,

@@ -1001,6 +1001,20 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   return p;
 }
 
+// Whether one of the first `outs` arrays of ints shares memory with any other
+struct Ints {
+  const void* p;
+  int64_t n;
+};
+bool overlap(const Ints* a, int outs, int all) {
+  for (int i = 0; i < outs; ++i)
+    for (int j = i + 1; j < all; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(a[i].p), y = reinterpret_cast<uintptr_t>(a[j].p);
+      if (a[i].n > 0 && a[j].n > 0 && x < y + 4 * a[j].n && y < x + 4 * a[i].n) return true;
+    }
+  return false;
+}
+
 bool kv_page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
 bool kv_hd_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1059,6 +1073,10 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
   MLCV_REQUIRE(B <= KV_MAX_REQ, "more than 4096 requests");
   MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST && (int64_t)max_pages * page <= KV_MOST,
                "more than 2^31 - 256 slots");
+  // every workgroup reads the lengths, one writes kv_lens: a plan written over them would be read half new
+  const Ints arrays[] = {{block_table, (int64_t)B * max_pages}, {cu_seqlens, (int64_t)B + 1}, {kv_lens, B}, {slot_map, tokens},
+                         {status, 2}, {past_lens, B}, {new_lens, B}, {free_pages, n_free}};
+  MLCV_REQUIRE(!overlap(arrays, 5, 8), "outputs overlap the inputs or one another");
   PlanArgs a{past_lens, new_lens, free_pages, block_table, cu_seqlens, kv_lens, slot_map, status, B, n_free,
              num_pages, log2_of(page), max_pages, tokens, 0};
   a.slot_blocks = std::max(1, (int)(((int64_t)tokens + 4 * KV_NT - 1) / (4 * KV_NT)));

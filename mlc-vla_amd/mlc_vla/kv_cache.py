@@ -114,7 +114,8 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
     """Block tables and slot maps from request lengths (mlcv_kv_plan).
 
     past_lens, new_lens [B], block_table [B, max_pages] (its new entries are written), free_pages [F], all int32;
-    ``tokens``: the packed tokens of the call.  ``out``: a plan of the same sizes to write into."""
+    ``tokens``: the packed tokens of the call.  ``out``: a plan of the same sizes to write into; not the one whose
+    ``kv_lens`` are the call's past_lens (two plans in turn do)."""
     past, new, table, free = _t(past_lens), _t(new_lens), _t(block_table), _t(free_pages)
     dev = past.get_device()
     shape = table.shape

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import kvref as R
+from mlc_vla import _native as N
 from mlc_vla import kv_cache as C
 from test_gpu_kv_cache import F8, TYPES, _cache, _host, _ints, _rows, _say, _want_cached
 
@@ -138,3 +139,27 @@ def test_write_keeps_nan_codes_of_a_page_that_grows(hd):
         x = _rows(rng, (9, 2, hd), torch.float32) * size
         _check_only(x, [0, 9], range(page + 7, page + 16), [(0, page + 7, 9)], (kc, ks, vc, vs))
     assert int(torch.isnan(kc.float()).sum()) == 3 and int(torch.isnan(vc.float()).sum()) == 3
+
+
+# ---- plan ------------------------------------------------------------------------------------------
+
+
+def test_plans_in_turn():
+    """A plan's kv_lens as the next step's past_lens: into another plan, not over itself."""
+    lens, page, free = [15, 16, 40], 16, _ints(range(20))
+    table = torch.full((3, 8), -1, dtype=torch.int32, device="cuda")
+    cache = C.PagedKVCache(20, page, 1, 64)
+    plan = cache.plan(_ints([0, 0, 0]), _ints(lens), table, free, sum(lens))
+    used, new = int(plan.status.numpy()[0]), _ints([1, 1, 1])
+    plans = [C.KVPlan(*(torch.zeros(n, dtype=torch.int32, device="cuda") for n in (4, 3, 3, 2))) for _ in range(2)]
+    past = plan.kv_lens.torch
+    for i in range(18):
+        at = plans[i & 1]
+        cache.plan(past, new, table, free[used:], 3, out=at)
+        past, lens = at.kv_lens, [n + 1 for n in lens]
+        with pytest.raises(N.MlcvError, match="overlap"):
+            cache.plan(past, new, table, free[used:], 3, out=at)
+        used += int(at.status[0])
+        assert past.tolist() == lens and int(at.status[1]) == 0
+        want = [int(table[b, (n - 1) // page]) * page + (n - 1) % page for b, n in enumerate(lens)]
+        assert at.slot_map.tolist() == want and min(want) >= 0

@@ -109,3 +109,16 @@ def test_plain_write_is_what_the_format_says():
     want = torch.from_numpy(x).to(torch.float8_e4m3fn).double().numpy()
     assert np.array_equal(R.e4m3(x.astype(np.float64)), want)
     assert R.scale_for(448.0) == 1.0 and R.scale_for(448.1) == 2.0 and R.scale_for(0.0) == 2.0 ** -64
+
+
+@pytest.mark.parametrize("a,b", [("lens", "past"), ("cu", "past"), ("table", "new"), ("slots", "free"), ("status", "free"),
+                                 ("lens", "new"), ("table", "free"), ("cu", "lens"), ("slots", "table"), ("status", "cu")])
+def test_a_plan_over_its_own_lengths_is_refused(a, b):
+    """Every workgroup reads the lengths while one writes the plan's."""
+    ints = dict(past=2, new=2, free=4, table=8, cu=3, lens=2, slots=5, status=2)
+    at, p = {}, P
+    for name, n in ints.items():
+        at[name], p = p, p + 4 * n
+    for shift in (0, 4 * (ints[b] - 1), -4 * (ints[a] - 1)):
+        with pytest.raises(N.MlcvError, match="overlap"):
+            _plan(**{**at, a: at[b] + shift})
