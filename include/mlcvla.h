@@ -310,8 +310,8 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *   k_cache [num_pages][KV][page][hd]   v_cache [num_pages][KV][hd][page]  (token innermost)
  *   k_scale, v_scale [num_pages][KV] f32: x = code * scale, finite and positive on every page in use
  * both caches 16-byte aligned; at most 2^31 - 256 slots (num_pages * page), and as many positions of a
- * block table's row.  Slot s is token
- * s % page of page s / page. */
+ * block table's row, tokens of a write or of prompts, and query rows (tokens * H / KV) of an attention
+ * over the cache.  Slot s is token s % page of page s / page. */
 
 /* Attention over whole prompts: row i of a prompt of n tokens sees the keys [0, n) of its own prompt
  * (causal = 0), or [0, max(i + 1, min(bidir[b], n))) (causal = 1; bidir [B] or NULL for all 0): the

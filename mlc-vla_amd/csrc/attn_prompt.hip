@@ -469,6 +469,7 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
                                      int64_t o_tok, int64_t o_head, void* stream) {
   MLCV_REQUIRE(dtype == MLCV_DTYPE_F16 || dtype == MLCV_DTYPE_BF16, "q, k and v are float16 or bfloat16");
   MLCV_REQUIRE(tokens >= 0 && B >= 0, "negative size");
+  MLCV_REQUIRE(tokens <= INT32_MAX - 255, "more than 2^31 - 256 tokens");  // the last tile's rows and keys still are ints
   MLCV_REQUIRE(H > 0 && KV > 0 && H % KV == 0, "query heads must be a multiple of the kv heads");
   MLCV_REQUIRE(hd == 64 || hd == 128 || hd == 256, "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");

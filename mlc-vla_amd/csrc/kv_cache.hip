@@ -22,7 +22,9 @@ namespace {
 
 constexpr int KV_NT = 256;         // threads per workgroup of every kernel here
 constexpr int KV_RT = 16;          // query rows of an attention workgroup
-constexpr int64_t KV_MOST = INT32_MAX - 255;  // slots of a cache, positions of a row: the last tile's still are ints
+// Slots of a cache, positions of a row, tokens of a write, query rows of a kv head: the last tile's or page's positions
+// still are ints
+constexpr int64_t KV_MOST = INT32_MAX - 255;
 constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
 
 // ---- plan ------------------------------------------------------------------------------------------
@@ -1101,6 +1103,7 @@ int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head,
   MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE(KV <= 65535, "more than 65535 kv heads");
   MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST, "more than 2^31 - 256 slots");
+  MLCV_REQUIRE(tokens <= KV_MOST, "more than 2^31 - 256 tokens");
   MLCV_REQUIRE((int64_t)tokens / page + 2 * (int64_t)B <= INT32_MAX, "too many requests");
   MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
   WriteArgs a{};
@@ -1135,7 +1138,7 @@ static int kv_attn_sizes_ok(int32_t tokens, int32_t B, int32_t H, int32_t KV, in
   MLCV_REQUIRE(tokens >= 0 && B >= 0 && max_kv >= 0, "negative size");
   MLCV_REQUIRE(H > 0 && KV > 0 && H % KV == 0, "query heads must be a multiple of the kv heads");
   MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
-  MLCV_REQUIRE((int64_t)tokens * (H / KV) <= INT32_MAX, "more than 2^31 - 1 query rows of a kv head");
+  MLCV_REQUIRE((int64_t)tokens * (H / KV) <= KV_MOST, "more than 2^31 - 256 query rows of a kv head");
   const KvAttnPlan p = kv_attn_plan(tokens, std::max(B, 1), H, KV, hd, max_kv);
   MLCV_REQUIRE(p.items * KV * p.S <= INT32_MAX && (int64_t)tokens * H * (hd / 64) <= INT32_MAX, "too many workgroups");
   return 0;

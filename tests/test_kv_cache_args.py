@@ -122,3 +122,15 @@ def test_a_plan_over_its_own_lengths_is_refused(a, b):
     for shift in (0, 4 * (ints[b] - 1), -4 * (ints[a] - 1)):
         with pytest.raises(N.MlcvError, match="overlap"):
             _plan(**{**at, a: at[b] + shift})
+
+
+@pytest.mark.parametrize("fn,bad", [
+    (_write, dict(tokens=2 ** 31 - 255)), (_write, dict(tokens=2 ** 31 - 1)), (_prompt, dict(tokens=2 ** 31 - 255)),
+    (_prompt, dict(tokens=2 ** 31 - 1)), (_attn, dict(tokens=2 ** 30 - 100, ws=P, ws_bytes=1 << 62)),
+    (_attn, dict(tokens=2 ** 31 - 255, H=2, ws=P, ws_bytes=1 << 62)),
+])
+def test_tokens_near_the_largest_int_are_refused(fn, bad):
+    """The last tile or page reaches past the last token: its positions have to be ints as well.  (Tensors of a stride
+    of 0 have such sizes without the memory.)"""
+    with pytest.raises(N.MlcvError, match="2\\^31 - 256"):
+        fn(**bad)
