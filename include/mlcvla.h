@@ -321,7 +321,7 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *   aligned, out rows 8-byte; k and v tokens hd to 2^24 elements apart
  *   out = sum_j softmax_j(scale * q . k_j) v_j      float32 logits, statistics and sums; the weights
  *   are rounded to the tensors' type for the matrix cores
- * out may be q itself, but must not overlap k or v (nor, below, the cache).
+ * out may be q itself, but must not overlap k or v (nor, below, the cache); its rows lie apart (-2).
  * What a row does not see does not reach it, whatever it holds; a logit that it does see and that is
  * infinite can make it infinite or NaN. */
 int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,

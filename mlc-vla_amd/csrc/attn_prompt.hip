@@ -489,6 +489,7 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
                "rows of q, k and v must be 16-byte aligned");
   MLCV_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7) == 0 && o_tok % 4 == 0 && o_head % 4 == 0,
                "rows of out must be 8-byte aligned");
+  MLCV_REQUIRE(rows_apart(tokens, o_tok, H, o_head, hd), "rows of out overlap");
   // a tile of keys is addressed through one buffer with 32-bit offsets
   MLCV_REQUIRE(k_tok >= hd && v_tok >= hd && k_tok < (1 << 24) && v_tok < (1 << 24),
                "the tokens of k and v must be between head_dim and 2^24 elements apart");

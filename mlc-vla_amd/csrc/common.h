@@ -44,6 +44,20 @@ const char* get_error();
     if (_r != 0) return _r;                                                          \
   } while (0)
 
+// ---- argument checks (host) --------------------------------------------------
+// Whether no two rows of n elements of an output of `tokens` x `heads` rows share one: element strides tok and head,
+// of either sign.  Rows j heads apart are closest where the tokens between them make up for j * head.
+inline bool rows_apart(int64_t tokens, int64_t tok, int64_t heads, int64_t head, int64_t n) {
+  const __int128 t = tok < 0 ? -(__int128)tok : tok, h = head < 0 ? -(__int128)head : head;
+  if ((tokens > 1 && t < n) || (heads > 1 && h < n)) return false;
+  if (tokens <= 1 || heads <= 1 || t >= h * (heads - 1) + n || h >= t * (tokens - 1) + n) return true;
+  for (int64_t j = 1; j < heads; ++j) {
+    const __int128 d = h * j, i = d / t;
+    if ((i < tokens && d - i * t < n) || (i + 1 < tokens && (i + 1) * t - d < n)) return false;
+  }
+  return true;
+}
+
 // ---- device numerics helpers ----------------------------------------------
 // Fragment-major activation layout for the skinny GEMMs (rows m < 64, K % 32 == 0,
 // 64 x K halfs): the B operand of mfma16x16x32 f16 for k step ks and m tile mt is one

@@ -1169,6 +1169,7 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
   MLCV_REQUIRE(max_pages == 0 || num_pages == 0 || (block_table && k_cache && k_scale && v_cache && v_scale),
                "null cache");
   MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
+  MLCV_REQUIRE(rows_apart(tokens, o_tok, H, o_head, hd), "rows of out overlap");
   const KvAttnPlan p = kv_attn_plan(tokens, B, H, KV, hd, max_kv);
   MLCV_REQUIRE(p.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes),
                "workspace missing, not 16-byte aligned or too small");

@@ -134,3 +134,15 @@ def test_tokens_near_the_largest_int_are_refused(fn, bad):
     of 0 have such sizes without the memory.)"""
     with pytest.raises(N.MlcvError, match="2\\^31 - 256"):
         fn(**bad)
+
+
+@pytest.mark.parametrize("fn,bad", [
+    (_prompt, dict(o_tok=0)), (_prompt, dict(o_head=0)), (_prompt, dict(o_tok=60)), (_prompt, dict(o_head=-32)),
+    (_attn, dict(o_tok=0, ws=P, ws_bytes=1 << 62)), (_attn, dict(o_head=0, ws=P, ws_bytes=1 << 62)),
+    (_prompt, dict(o_tok=64, o_head=64)), (_prompt, dict(o_tok=192, o_head=128)), (_prompt, dict(o_tok=-256, o_head=300)),
+    (_attn, dict(o_tok=-63, ws=P, ws_bytes=1 << 62)), (_attn, dict(o_head=32, ws=P, ws_bytes=1 << 62)),
+])
+def test_rows_of_out_that_overlap_are_refused(fn, bad):
+    """An expanded tensor as out: rows of several tokens or heads would be written to one place."""
+    with pytest.raises(N.MlcvError, match="out overlap"):
+        fn(**bad)
