@@ -379,6 +379,9 @@ int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head,
  * them, that may overlap need their own). */
 int mlcv_kv_attention_workspace(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv,
                                 size_t* bytes);
+/* Test hook: how a call of these sizes is cut: splits of the keys, waves of a workgroup (4 or 8). */
+int mlcv_kv_attention_plan(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv,
+                           int32_t* splits, int32_t* waves);
 int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_head, int32_t tokens,
                       const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens, const int32_t* block_table,
                       int32_t max_pages, const void* k_cache, const float* k_scale, const void* v_cache,

@@ -1152,6 +1152,16 @@ int mlcv_kv_attention_workspace(int32_t tokens, int32_t B, int32_t H, int32_t KV
   return 0;
 }
 
+int mlcv_kv_attention_plan(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv, int32_t* splits,
+                           int32_t* waves) {
+  MLCV_REQUIRE(splits && waves, "null pointer");
+  MLCV_TRY(kv_attn_sizes_ok(tokens, B, H, KV, hd, max_kv));
+  const KvAttnPlan p = kv_attn_plan(tokens, std::max(B, 1), H, KV, hd, max_kv);
+  *splits = p.S;
+  *waves = p.wide ? 8 : 4;
+  return 0;
+}
+
 int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_head, int32_t tokens,
                       const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens, const int32_t* block_table,
                       int32_t max_pages, const void* k_cache, const float* k_scale, const void* v_cache,

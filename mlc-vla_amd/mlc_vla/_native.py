@@ -89,6 +89,7 @@ SIGNATURES = {
     "mlcv_kv_write": (ctypes.c_int, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
                                      _vp, _i32, _i32, _i32, _i32, _vp]),
     "mlcv_kv_attention_workspace": (ctypes.c_int, [_i32] * 6 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlcv_kv_attention_plan": (ctypes.c_int, [_i32] * 6 + [ctypes.POINTER(_i32)] * 2),
     "mlcv_kv_attention": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp,
                                          _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _i32, _i32, _vp, _i64, _i64,
                                          _vp, ctypes.c_size_t, _vp]),

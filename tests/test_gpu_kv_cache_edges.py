@@ -3,6 +3,8 @@ are not there.  Plain 64-bit forms and bounds as in test_gpu_kv_cache.py."""
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -163,3 +165,161 @@ def test_plans_in_turn():
         assert past.tolist() == lens and int(at.status[1]) == 0
         want = [int(table[b, (n - 1) // page]) * page + (n - 1) % page for b, n in enumerate(lens)]
         assert at.slot_map.tolist() == want and min(want) >= 0
+
+
+# ---- attention over the cache: every form of the kernel -------------------------------------------------
+
+
+def _plan(*sizes):
+    s, w = ctypes.c_int32(), ctypes.c_int32()
+    N.call("mlcv_kv_attention_plan", *sizes, ctypes.byref(s), ctypes.byref(w))
+    return s.value, w.value
+
+
+def _wanted(q, cu, lens, table, cache, causal):
+    """_want_cached by matrix products, for many rows: (outputs, bounds, seen [tokens][n keys of the request])."""
+    kc, ks, vc, vs = cache
+    page, kv, hd = kc.shape[2], kc.shape[1], kc.shape[3]
+    kf, vf = _host(kc) * _host(ks)[..., None, None], _host(vc).transpose(0, 1, 3, 2) * _host(vs)[..., None, None]
+    qh, scale, grp = _host(q), hd ** -0.5, q.shape[1] // kv
+    out, tol, seen = np.zeros(q.shape), np.zeros(q.shape), []
+    tiny = 2.0 ** -37 * 448 * float(vs.max())
+    for b, (a, z) in enumerate(zip(cu, cu[1:])):
+        n, total = z - a, int(lens[b])
+        ids = table[b][:-(-total // page)]
+        there = np.array([0 <= ids[t // page] < kc.shape[0] for t in range(total)])
+        at = [(ids[t // page] if there[t] else 0, t % page) for t in range(total)]
+        limit = np.array([total - n + i + 1 if causal else total for i in range(n)])
+        see = (np.arange(total)[None, :] < limit[:, None]) & there[None, :]
+        seen.append(see)
+        for h in range(q.shape[1]):
+            k, v = (np.stack([x[p, h // grp, o] for p, o in at]) for x in (kf, vf))
+            k[~there], v[~there] = 0, 0
+            with np.errstate(invalid="ignore"):
+                x = np.where(see, qh[a:z, h] @ k.T * scale, -np.inf)
+                p = np.where(see.any(1)[:, None], np.exp(x - x.max(1, keepdims=True)), 0)
+                p = np.where(see, p, 0) / np.maximum(p.sum(1, keepdims=True), 1e-300)
+            o, mass = p @ v, p @ np.abs(v)
+            big = np.where(see, np.abs(qh[a:z, h]) @ np.abs(k).T * scale, 0).max(1, initial=0)[:, None]
+            out[a:z, h] = o
+            tol[a:z, h] = R.bound(o, mass, big, q.dtype, max(int(there.sum()), 1), hd, torch.float16, tiny)
+    return out, tol, seen
+
+
+# new tokens of each request, their past, a bound on the lengths, and what the call is cut into
+FORMS = {
+    "four": ([50, 33, 0, 50, 1], [200, 250, 77, 0, 5], 300, (1, 4)),
+    "eight": ([50, 33, 50, 0, 17, 50], [968, 700, 0, 903, 65, 400], 1018, (1, 8)),
+    "few splits": ([1, 1, 2], [900, 1017, 63], 1018, None),
+    "many splits": ([1, 2], [9000, 3000], 9001, None),
+}
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,page", [(64, 16), (64, 128), (128, 64), (128, 32), (256, 16), (256, 128)])
+def test_kv_attention_every_form(form, dt, hd, page):
+    """Four waves per workgroup and eight, no splits, up to 16 of them and more: lengths of every kind, a hole, page
+    scales and codes that are not numbers in what no row sees, and then in what some do."""
+    new, past, most, cut = FORMS[form]
+    rng = np.random.default_rng(hd + page)
+    lens, cu = [p + n for p, n in zip(past, new)], [0] + np.cumsum(new).tolist()
+    splits, waves = _plan(cu[-1], len(new), 8, 1, hd, most)
+    assert (splits, waves) == cut if cut else (waves == 4 and (splits > 16 if form == "many splits" else 1 < splits <= 16))
+    table, (kc, ks, vc, vs), unused = _own_pages(rng, lens, 1, hd, page, 1 + -(-most // page))
+    table[1, 1] = -1
+    q = _rows(rng, (cu[-1], 8, hd), TYPES[dt], 0.5)
+    kr, vr = kc.view(torch.uint8), vc.view(torch.uint8)
+    want = {causal: _wanted(q, cu, lens, table, (kc, ks, vc, vs), causal) for causal in (True, False)}
+    ks[unused], vs[unused] = float("nan"), float("inf")
+    kr[unused], vr[unused] = 0x7f, 0xff
+    for b, n in enumerate(lens):                          # behind each request's end, on its last page
+        if n % page:
+            kr[table[b, n // page], :, n % page:] = 0xff
+            vr[table[b, n // page], :, :, n % page:] = 0x7f
+    for causal in (True, False):
+        _check(q, cu, lens, table, (kc, ks, vc, vs), causal, *want[causal][:2], max_kv=most)
+    # values that rows see: the last key of request 0 (its last row's alone, if causal) and its first key
+    for key, dim in ((lens[0] - 1, 3), (0, hd - 1)):
+        vr[table[0, key // page], 0, dim, key % page] = 0x7f
+        for causal in (True, False):
+            got = C.kv_attention(q, _ints(cu), _ints(lens), torch.from_numpy(table).cuda(), kc, ks, vc, vs, causal=causal,
+                                 max_kv=most)
+            out, tol, seen = want[causal]
+            bad = np.zeros(out.shape, bool)
+            for k, d in ((lens[0] - 1, 3), (0, hd - 1)) if key == 0 else ((key, dim),):
+                bad[:cu[1], :, d] |= seen[0][:, k][:, None]
+            g = _host(got.torch)
+            np.testing.assert_array_equal(np.isnan(g), bad)
+            assert (np.abs(g - out)[~bad] <= tol[~bad]).all()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,hd,page,past,new", [
+    (4, 1, 64, 16, [1000, 300, 7], [64, 200, 130]),
+    (8, 2, 128, 64, [1000, 0, 129], [65, 128, 257]),
+    (8, 1, 256, 32, [2000, 63], [64, 100]),
+    (6, 6, 128, 16, [15, 1], [513, 64]),
+    (20, 1, 64, 128, [500], [300]),
+])
+def test_kv_attention_chunks(dt, heads, kv, hd, page, past, new):
+    """64 and more new tokens of a request over its cached ones: a prompt that comes in pieces."""
+    rng = np.random.default_rng(hd + page)
+    lens, cu = [p + n for p, n in zip(past, new)], [0] + np.cumsum(new).tolist()
+    table, cache, _ = _own_pages(rng, lens, kv, hd, page, 2 + -(-max(lens) // page))
+    q = _rows(rng, (cu[-1], heads, hd), TYPES[dt], 0.5)
+    for causal in (True, False):
+        want, tol, _ = _wanted(q, cu, lens, table, cache, causal)
+        for most in (max(lens), 1, 10 ** 6):
+            _check(q, cu, lens, table, cache, causal, want, tol, max_kv=most)
+
+
+def test_wanted_is_the_plain_form():
+    """The products above against the rows one by one."""
+    rng = np.random.default_rng(1)
+    lens, cu = [40, 3, 70], [0, 5, 8, 9]
+    table, cache, _ = _own_pages(rng, lens, 2, 64, 16, 6)
+    table[2, 1] = -1
+    q = _rows(rng, (9, 4, 64), torch.float16)
+    for causal in (True, False):
+        a, at = _want_cached(q, cu, lens, table, cache, causal, 64 ** -0.5)
+        b, bt, _ = _wanted(q, cu, lens, table, cache, causal)
+        np.testing.assert_allclose(b, a, rtol=1e-10, atol=1e-10)
+        assert (bt >= at * (1 - 1e-9)).all()  # it counts every key of the request
+
+
+def test_requests_of_sound_offsets_beside_others():
+    """Offsets that descend or lie outside before and behind a request: its rows are what it alone gives, with splits of
+    the keys and without, and its tokens are written; nothing around the outputs and the cache is."""
+    rng = np.random.default_rng(17)
+    n, hd, page = 300, 64, 16
+    q, k, v = (_rows(rng, (n, h, hd), torch.float16, 0.5) for h in (2, 1, 1))
+    table, cache, _ = _own_pages(rng, [500, 500, 500], 1, hd, page, 32)
+    t = torch.from_numpy(table).cuda()
+    cu, lens, own = [250, 100, 299, 10 ** 6], [400, 450, 3], slice(100, 299)
+    store = torch.full((n + 64, 2, hd), 9.0, dtype=torch.float16, device="cuda")
+    out = store[32:32 + n]
+    C.prompt_attention(q, k, v, _ints(cu), out=out)
+    assert torch.equal(out[own], C.prompt_attention(q[own], k[own], v[own], _ints([0, 199])).torch)
+    assert (out[:100] == 9).all()
+    for most in (1, 512, 10 ** 6):
+        for causal in (True, False):
+            out.fill_(9.0)
+            C.kv_attention(q, _ints(cu), _ints(lens), t, *cache, out=out, max_kv=most, causal=causal)
+            want, tol, _ = _wanted(q[own], [0, 199], lens[1:2], table[1:2], cache, causal)
+            assert (np.abs(_host(out[own]) - want) <= tol).all()
+            assert (out[:100] == 9).all()
+    assert (store[:32] == 9).all() and (store[32 + n:] == 9).all()
+    # the writer: request 1's tokens to pages of their own, and a guard on both sides of each cache
+    whole = [torch.full((32 + 40 + 32,) + x.shape[1:], 3, dtype=torch.uint8, device="cuda").view(F8) if x.dtype == F8 else
+             torch.full((32 + 40 + 32,) + x.shape[1:], 3.0, device="cuda") for x in cache]
+    held = [x[32:72] for x in whole]
+    slots = [-1] * 100 + [16 * 3 + 5 + i for i in range(199)] + [16 * 30]
+    C.kv_write(k, v, _ints(cu), _ints(slots), *held)
+    alone = [x.clone() for x in whole]
+    for x in alone:
+        (x.view(torch.uint8) if x.dtype == F8 else x).fill_(3)
+    C.kv_write(k[own], v[own], _ints([0, 199]), _ints(slots[own]), *(x[32:72] for x in alone))
+    C.kv_write(k[299:], v[299:], _ints([0, 1]), _ints(slots[299:]), *(x[32:72] for x in alone))
+    for a, b in zip(whole, alone):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

@@ -146,3 +146,18 @@ def test_rows_of_out_that_overlap_are_refused(fn, bad):
     """An expanded tensor as out: rows of several tokens or heads would be written to one place."""
     with pytest.raises(N.MlcvError, match="out overlap"):
         fn(**bad)
+
+
+def test_attention_plan_query():
+    s, w = ctypes.c_int32(), ctypes.c_int32()
+    ask = lambda *a: N.call("mlcv_kv_attention_plan", *a, ctypes.byref(s), ctypes.byref(w)) or (s.value, w.value)  # noqa: E731
+    with pytest.raises(N.MlcvError, match="head_dim"):
+        ask(1, 1, 8, 1, 100, 10)
+    with pytest.raises(N.MlcvError, match="null"):
+        N.call("mlcv_kv_attention_plan", 1, 1, 8, 1, 64, 10, None, None)
+    assert ask(0, 0, 8, 1, 64, 0) == (1, 4)
+    for hd in (64, 128, 256):
+        assert ask(400, 8, 8, 1, hd, 1018) == (1, 8)                            # action suffixes: no splits, no workspace
+        assert C.kv_attention_workspace(400, 8, 8, 1, hd, 1018) == 0
+        assert ask(1, 1, 8, 1, hd, 9000)[0] > 16 and ask(2, 2, 8, 1, hd, 1018)[0] in range(2, 17)
+        assert ask(16 * 300, 300, 8, 1, hd, 4096) == (1, 4)
