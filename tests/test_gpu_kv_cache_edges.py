@@ -323,3 +323,82 @@ def test_requests_of_sound_offsets_beside_others():
     C.kv_write(k[299:], v[299:], _ints([0, 1]), _ints(slots[299:]), *(x[32:72] for x in alone))
     for a, b in zip(whole, alone):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---- together ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_kv_attention_over_its_own_queries(form, hd):
+    """out = q, as the documentation allows, in every form of the kernel."""
+    new, past, most, _ = FORMS[form]
+    rng = np.random.default_rng(hd)
+    lens, cu = [p + n for p, n in zip(past, new)], [0] + np.cumsum(new).tolist()
+    table, cache, _ = _own_pages(rng, lens, 1, hd, 64, 1 + -(-most // 64))
+    wide = _rows(rng, (cu[-1], 12, hd), torch.float16, 0.5)
+    args = (_ints(cu), _ints(lens), torch.from_numpy(table).cuda(), *cache)
+    want = C.kv_attention(wide[:, 2:10], *args, max_kv=most).torch
+    rest = wide[:, 10:].clone()
+    q = wide[:, 2:10]                                    # a slice of wider rows
+    assert torch.equal(C.kv_attention(q, *args, max_kv=most, out=q).torch, want) and torch.equal(q, want)
+    assert torch.equal(wide[:, 10:], rest)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("heads", [4, 64])               # few rows: shared by two waves; many
+def test_prompt_attention_over_its_own_queries(hd, heads):
+    rng = np.random.default_rng(hd)
+    lens = [1, 130, 200, 63]
+    cu = _ints([0] + np.cumsum(lens).tolist())
+    q, k, v = (_rows(rng, (sum(lens) + 2, h, hd), torch.bfloat16, 0.5) for h in (heads, 2, 2))
+    want, rest = C.prompt_attention(q, k, v, cu).torch[:-2], q[-2:].clone()
+    assert torch.equal(C.prompt_attention(q, k, v, cu, out=q).torch[:-2], want) and torch.equal(q[-2:], rest)
+
+
+def test_captured_step_whose_lengths_grow():
+    """One graph of a decode step, replayed as its requests grow over page ends: the lengths, the table and the list of
+    free pages stay on the device and are the next replay's; every replay against eager calls on caches of their own."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    page, kv, heads, hd, lens = 16, 2, 8, 64, [30, 1, 47]
+    rand = lambda n, h: torch.randn((n, h, hd), generator=g, device="cuda").half()  # noqa: E731
+    caches = [C.PagedKVCache(40, page, kv, hd) for _ in range(2)]
+    tables = [torch.full((3, 8), -1, dtype=torch.int32, device="cuda") for _ in range(2)]
+    free, new, past = _ints(range(39, -1, -1)), _ints([1, 1, 1]), _ints(lens)
+    k, v = rand(sum(lens), kv), rand(sum(lens), kv)
+    for cache, table in zip(caches, tables):
+        plan = cache.plan(_ints([0, 0, 0]), past, table, free, sum(lens))
+        cache.write(k, v, plan)
+    used = int(plan.status.numpy()[0])
+    left = torch.cat([free[used:], free[:used]])          # the list that the graph takes pages from the front of
+    at = torch.arange(left.numel(), device="cuda")
+    q, k, v = rand(3, heads), rand(3, kv), rand(3, kv)
+
+    def step(cache, table, past, left):
+        plan = cache.plan(past, new, table, left, 3)
+        cache.write(k, v, plan)
+        return plan, cache.attention(q, plan, table).torch
+
+    spare = [t.clone() for t in (caches[0].k.view(torch.uint8), caches[0].v.view(torch.uint8), caches[0].k_scale,
+                                 caches[0].v_scale, tables[0])]
+    step(caches[0], tables[0], past, left)                # as a capture asks for; then back
+    for a, b in zip((caches[0].k.view(torch.uint8), caches[0].v.view(torch.uint8), caches[0].k_scale, caches[0].v_scale,
+                     tables[0]), spare):
+        a.copy_(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, out = step(caches[0], tables[0], past, left)
+        past.copy_(plan.kv_lens.torch)
+        left.copy_(left[(at + plan.status.torch[:1]) % left.numel()])
+    own_past, own_left = past.clone(), left.clone()
+    for i in range(40):
+        for x in (q, k, v):
+            x.copy_(rand(3, x.shape[1]))
+        want_plan, want = step(caches[1], tables[1], own_past, own_left)
+        own_past, own_left = want_plan.kv_lens.torch, own_left.roll(-int(want_plan.status.torch[0]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert past.tolist() == [n + i + 1 for n in lens] and want_plan.status.torch[1] == 0
+        assert torch.equal(out, want) and torch.equal(tables[0], tables[1]) and torch.equal(left, own_left)
+        for a, b in zip(caches[0].pages(), caches[1].pages()):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
