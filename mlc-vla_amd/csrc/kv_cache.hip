@@ -25,6 +25,7 @@ constexpr int KV_RT = 16;          // query rows of an attention workgroup
 // Slots of a cache, positions of a row, tokens of a write, query rows of a kv head: the last tile's or page's positions
 // still are ints
 constexpr int64_t KV_MOST = INT32_MAX - 255;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
 
 // ---- plan ------------------------------------------------------------------------------------------
@@ -1173,7 +1174,7 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
   MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
   MLCV_REQUIRE(num_pages >= 0 && max_pages >= 0 && (int64_t)num_pages * page <= KV_MOST &&
                    (int64_t)max_pages * page <= KV_MOST, "more than 2^31 - 256 slots");
-  MLCV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
+  MLCV_REQUIRE(scale > 0.f && scale * LOG2E < INFINITY, "scale must be positive and below 2.3e38");
   if (tokens == 0 || B == 0) return 0;
   MLCV_REQUIRE(q && cu_seqlens && kv_lens && out, "null pointer");
   MLCV_REQUIRE(max_pages == 0 || num_pages == 0 || (block_table && k_cache && k_scale && v_cache && v_scale),
@@ -1211,7 +1212,7 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
   a.q_vec = aligned16(q) && q_tok % 8 == 0 && q_head % 8 == 0;
   a.S = p.S;
   a.span = p.span;
-  a.c = scale * 1.4426950408889634f;
+  a.c = scale * LOG2E;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool bf = dtype == MLCV_DTYPE_BF16;
   if (hd == 64) return bf ? kv_attn_launch<true, 64>(a, p, st) : kv_attn_launch<false, 64>(a, p, st);

@@ -161,3 +161,12 @@ def test_attention_plan_query():
         assert C.kv_attention_workspace(400, 8, 8, 1, hd, 1018) == 0
         assert ask(1, 1, 8, 1, hd, 9000)[0] > 16 and ask(2, 2, 8, 1, hd, 1018)[0] in range(2, 17)
         assert ask(16 * 300, 300, 8, 1, hd, 4096) == (1, 4)
+
+
+@pytest.mark.parametrize("fn,bad,what", [
+    (_prompt, dict(scale=3e38), "scale"), (_attn, dict(scale=2.4e38, ws=P, ws_bytes=1 << 62), "scale"),
+])
+def test_what_a_launch_cannot_hold_is_refused(fn, bad, what):
+    """A scale whose product with log2(e) is infinite."""
+    with pytest.raises(N.MlcvError, match="invalid argument.*" + what):
+        fn(**bad)
