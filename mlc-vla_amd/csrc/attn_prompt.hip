@@ -480,7 +480,7 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
   // 24.5 -> 19.4, of 64: 17.6 -> 13.7.  At 256 workgroups it is level (heads of 64 and 128) or 1.28 times slower.
   const bool split = ((int64_t)tokens + PR_ROWS - 1) / PR_ROWS * H <= 128;
   const int64_t items = (int64_t)tokens / (split ? PR_ROWS / 2 : PR_ROWS) + B;
-  MLCV_REQUIRE(items * H <= INT32_MAX, "too many workgroups");
+  MLCV_REQUIRE(items * H <= UINT32_MAX / PR_NT, "too many workgroups");  // a launch holds less than 2^32 threads
   if (tokens == 0 || B == 0) return 0;
   MLCV_REQUIRE(q && k && v && cu_seqlens && out, "null pointer");
   auto fits = [](const void* p, int64_t tok, int64_t head) {

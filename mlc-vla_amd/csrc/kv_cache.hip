@@ -1105,7 +1105,7 @@ int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head,
   MLCV_REQUIRE(KV <= 65535, "more than 65535 kv heads");
   MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST, "more than 2^31 - 256 slots");
   MLCV_REQUIRE(tokens <= KV_MOST, "more than 2^31 - 256 tokens");
-  MLCV_REQUIRE((int64_t)tokens / page + 2 * (int64_t)B <= INT32_MAX, "too many requests");
+  MLCV_REQUIRE((int64_t)tokens / page + 2 * (int64_t)B <= UINT32_MAX / KV_NT, "too many requests");
   MLCV_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the cache must be 16-byte aligned");
   WriteArgs a{};
   a.x[0] = k;
@@ -1141,7 +1141,9 @@ static int kv_attn_sizes_ok(int32_t tokens, int32_t B, int32_t H, int32_t KV, in
   MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
   MLCV_REQUIRE((int64_t)tokens * (H / KV) <= KV_MOST, "more than 2^31 - 256 query rows of a kv head");
   const KvAttnPlan p = kv_attn_plan(tokens, std::max(B, 1), H, KV, hd, max_kv);
-  MLCV_REQUIRE(p.items * KV * p.S <= INT32_MAX && (int64_t)tokens * H * (hd / 64) <= INT32_MAX, "too many workgroups");
+  // a launch holds less than 2^32 threads
+  MLCV_REQUIRE(p.items * KV * p.S <= UINT32_MAX / (p.wide ? 512 : 256) &&
+                   (p.S == 1 || (int64_t)tokens * H * (hd / 64) <= UINT32_MAX / KV_NT), "too many workgroups");
   return 0;
 }
 

@@ -165,8 +165,11 @@ def test_attention_plan_query():
 
 @pytest.mark.parametrize("fn,bad,what", [
     (_prompt, dict(scale=3e38), "scale"), (_attn, dict(scale=2.4e38, ws=P, ws_bytes=1 << 62), "scale"),
+    (_prompt, dict(tokens=1 << 27, H=64, KV=64, o_tok=4096), "workgroups"),
+    (_attn, dict(tokens=1 << 22, H=64, KV=64, o_tok=4096, max_kv=64), "workgroups"),
+    (_write, dict(B=1 << 23, tokens=1 << 20), "requests"),
 ])
 def test_what_a_launch_cannot_hold_is_refused(fn, bad, what):
-    """A scale whose product with log2(e) is infinite."""
+    """A scale whose product with log2(e) is infinite; grids of 2^32 threads and more."""
     with pytest.raises(N.MlcvError, match="invalid argument.*" + what):
         fn(**bad)
