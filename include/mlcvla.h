@@ -300,7 +300,8 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *
  * No counterpart in the reference, which serves one request over a dense cache.  Tokens of B
  * requests are packed one after another: request b owns tokens [cu_seqlens[b], cu_seqlens[b+1])
- * of a call, B + 1 int32 on the device, ascending from 0.  Every length stays on the device; the
+ * of a call, B + 1 int32 on the device, ascending from 0 (rows between offsets that do not ascend are
+ * left undefined, or as they were).  Every length stays on the device; the
  * entry points do not synchronize, allocate or keep anything between calls, and can be captured.
  * Sizes, types, strides and alignment are checked on the host (-2).  Lengths and indices are
  * device data: they are brought into range in the kernels, which neither read nor write outside
@@ -322,8 +323,8 @@ int mlcv_tile_linear(const void* x, int32_t M, int32_t K, const void* w, int32_t
  *   out = sum_j softmax_j(scale * q . k_j) v_j      float32 logits, statistics and sums; the weights
  *   are rounded to the tensors' type for the matrix cores
  * out may be q itself, but must not overlap k or v (nor, below, the cache); its rows lie apart (-2).
- * What a row does not see does not reach it, whatever it holds; a logit that it does see and that is
- * infinite can make it infinite or NaN. */
+ * What a row does not see does not reach it, whatever it holds; a logit or a value that it does see and
+ * that is infinite can make it infinite or NaN. */
 int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                           const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int32_t tokens,
                           const int32_t* cu_seqlens, int32_t B, int32_t H, int32_t KV, int32_t hd, float scale,
@@ -370,11 +371,15 @@ int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head,
  * of kv_lens[b] cached tokens; query t sees the keys [0, kv_lens[b] - n + t + 1) (causal = 1) or all
  * kv_lens[b] of them (0, the action suffix).  q, out: element (t, h, d) at t * tok + h * head + d,
  * MLCV_DTYPE_F16 or _BF16; query head h reads kv head h / (H / KV).
- *   out = sum_j softmax_j(scale * q . k_j) v_j     float32 sums and statistics; the weights are
- *   rounded to fp16 (2^-11 of each, below the output's rounding) for the matrix cores
+ *   out = sum_j softmax_j(scale * q . k_j) v_j     float32 sums and statistics; each weight times its
+ *   page's value scale is rounded to fp16 for the matrix cores: by 2^-11 of itself, below the output's
+ *   rounding, down to 2^-26 of the row's largest such product, and by up to 2^-37 of that largest below
+ *   it (weights of the largest size on pages whose scale is 2^26 below another's fall there)
  * A query that sees nothing gives zeros; so does one whose request was refused (kv_lens 0).  Pages
- * outside [0, num_pages) count as not seen.  max_kv: a bound on kv_lens for the plan of the work
- * (larger lengths are still right, only slower).  workspace: mlcv_kv_attention_workspace bytes of
+ * outside [0, num_pages) count as not seen, and scales and codes of pages that hold none of a request's
+ * tokens may be anything.  max_kv: a bound on kv_lens by which the keys are split over the GPU: lengths
+ * above it are still right, but they and a bound far above the lengths are slower (8 requests of 969
+ * tokens, one kv head of 256: 10 us with max_kv 969, 10 with 3876, 18 with 32768, 26 with 131072).  workspace: mlcv_kv_attention_workspace bytes of
  * device memory, 16-byte aligned, for this call alone while it runs (calls, captured ones among
  * them, that may overlap need their own). */
 int mlcv_kv_attention_workspace(int32_t tokens, int32_t B, int32_t H, int32_t KV, int32_t hd, int32_t max_kv,

@@ -478,6 +478,7 @@ extern "C" int mlcv_prompt_attention(const void* q, int64_t q_tok, int64_t q_hea
   // Few rows: workgroups of 64 rows, whose waves share them by keys, while even those leave no CU two of them
   // (up to 128 workgroups of 128 rows).  One prompt of 968 tokens, 8 heads of 256: 43.9 -> 32.2 us; 16 heads of 128:
   // 24.5 -> 19.4, of 64: 17.6 -> 13.7.  At 256 workgroups it is level (heads of 64 and 128) or 1.28 times slower.
+  // The sides cross between: ragged prompts of heads of 256 are 1.08 times faster with 64 rows at 160 workgroups, level at 184.
   const bool split = ((int64_t)tokens + PR_ROWS - 1) / PR_ROWS * H <= 128;
   const int64_t items = (int64_t)tokens / (split ? PR_ROWS / 2 : PR_ROWS) + B;
   MLCV_REQUIRE(items * H <= UINT32_MAX / PR_NT, "too many workgroups");  // a launch holds less than 2^32 threads

@@ -68,7 +68,9 @@ struct PlanArgs {
 // follow those of the requests before it, and slot = table[pos / page] * page + pos % page.
 // Every workgroup runs the same scan over the requests (two loads and a prefix sum per 256 of them, which costs
 // less than a second launch that waits for the first), then fills its own part of the slot map or of the table.
-// Bound by launch and load latency: 3.2 us for 16 requests of one new token, 9.0 for 256 of up to 1168 (170000 tokens).
+// Bound by launch and load latency: 3.1 us for 16 requests of one new token, 8.9 for 256 of up to 1168 (170000 tokens).
+// The scan is the smaller part of that: 256 requests of one token take 0.3 us more than 16.  A thread's four slots cost 1.2
+// us each, as their chains of search, length and page number run one after another.
 __global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
   extern __shared__ int sm[];
   __shared__ long long part[KV_NT / 64];
@@ -296,8 +298,11 @@ __device__ __forceinline__ uint32_t byte_mask(int lo, int hi) {
 // codes, so that the input is read once.  Where a head's page has fewer units than the workgroup threads, several
 // heads go side by side.  Keys leave as 8 bytes per position; values go through LDS to be turned to [hd][page] and
 // leave as 16-byte pieces.  A piece that is not wholly new is merged with what the page held.
-// Bound by HBM for long prompts (21447 tokens of 8 heads of 128 in pages of 32: 40.7 us, 3.2 TB/s), by the chain of
-// loads (cu, slots, tokens) for few tokens (64 requests of one: 7.8 us).
+// Bound by the chain of loads (cu, slots, tokens, the page's old codes), for few tokens (64 requests of one: 8.0 us) as
+// for long prompts: 21447 tokens of 8 heads of 128 in pages of 32 take 40.7 us, 3.2 of the 5.2 TB/s of a copy, with the waves
+// waiting 58% of their time.  The type is settled in the kernel, so that every type pays for float32's loads: 120
+// registers and four waves a SIMD (UNITS = 2: 177, two waves; 4: 282, one).  The turn's stores meet on LDS banks (rows of
+// page + 16 bytes: 8 to 32 lanes of a store on one), about a tenth of the time of those prompts.
 template <int HD, int UNITS>
 __global__ __launch_bounds__(KV_NT) void kv_write_kernel(const WriteArgs a) {
   constexpr int CH = HD / 8;                     // 8-dim pieces of a row

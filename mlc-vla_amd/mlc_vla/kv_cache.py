@@ -195,7 +195,9 @@ def kv_attention(q, cu_seqlens, kv_lens, block_table, k_cache, k_scale, v_cache,
                  scale: Optional[float] = None, max_kv: Optional[int] = None, out=None, workspace=None) -> Tensor:
     """Attention of the last tokens of each request, q [tokens, H, hd], over its cached keys and values
     (mlcv_kv_attention).  ``scale``: 1 / sqrt(hd) if not given; ``max_kv``: a bound on kv_lens (default: the
-    block table's width); ``workspace``: uint8 tensor of ``kv_attention_workspace`` bytes (default: allocated here)."""
+    block table's width; one far above the lengths, as a wide table's, splits the keys badly: up to 3.6 times the
+    time); ``out``: rows behind the last request are left as they were, so by default they are not initialized;
+    ``workspace``: uint8 tensor of ``kv_attention_workspace`` bytes (default: allocated here)."""
     q, cu, lens, table = _t(q), _t(cu_seqlens), _t(kv_lens), _t(block_table)
     kc, ks, vc, vs = _t(k_cache), _t(k_scale), _t(v_cache), _t(v_scale)
     dev, shape, name = q.get_device(), kc.shape, _NAME.get(q.dtype)
@@ -240,7 +242,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, bidir=None, sc
                      out=None) -> Tensor:
     """Attention of packed prompts, q [tokens, H, hd], k and v [tokens, KV, hd] in float16 or bfloat16
     (mlcv_prompt_attention).  ``bidir`` [B] int32: the first tokens of each prompt that all see one another.  Rows
-    that are not 16-byte aligned, and tokens that share keys or values, are copied first."""
+    that are not 16-byte aligned, and tokens that share keys or values, are copied first.  ``out``: 8-byte aligned
+    rows; those behind the last prompt are left as they were, so by default they are not initialized."""
     q, k, v, cu = _t(q), _t(k), _t(v), _t(cu_seqlens)
     dev, dt, name = q.get_device(), q.dtype, _NAME.get(q.dtype)
     tokens, heads, hd = q.shape if q.dim() == 3 else (-1,) * 3
