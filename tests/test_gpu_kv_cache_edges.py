@@ -187,17 +187,17 @@ def _wanted(q, cu, lens, table, cache, causal):
     for b, (a, z) in enumerate(zip(cu, cu[1:])):
         n, total = z - a, int(lens[b])
         ids = table[b][:-(-total // page)]
-        there = np.array([0 <= ids[t // page] < kc.shape[0] for t in range(total)])
+        there = np.array([0 <= ids[t // page] < kc.shape[0] for t in range(total)], bool)
         at = [(ids[t // page] if there[t] else 0, t % page) for t in range(total)]
         limit = np.array([total - n + i + 1 if causal else total for i in range(n)])
         see = (np.arange(total)[None, :] < limit[:, None]) & there[None, :]
         seen.append(see)
         for h in range(q.shape[1]):
-            k, v = (np.stack([x[p, h // grp, o] for p, o in at]) for x in (kf, vf))
+            k, v = (np.array([x[p, h // grp, o] for p, o in at]).reshape(total, hd) for x in (kf, vf))
             k[~there], v[~there] = 0, 0
             with np.errstate(invalid="ignore"):
                 x = np.where(see, qh[a:z, h] @ k.T * scale, -np.inf)
-                p = np.where(see.any(1)[:, None], np.exp(x - x.max(1, keepdims=True)), 0)
+                p = np.where(see.any(1)[:, None], np.exp(x - x.max(1, keepdims=True, initial=-np.inf)), 0)
                 p = np.where(see, p, 0) / np.maximum(p.sum(1, keepdims=True), 1e-300)
             o, mass = p @ v, p @ np.abs(v)
             big = np.where(see, np.abs(qh[a:z, h]) @ np.abs(k).T * scale, 0).max(1, initial=0)[:, None]
