@@ -39,7 +39,7 @@ extern "C" {
  * reference runs in float32; the other entry points and options of the step forms report that
  * they are not built for them. */
 #define MLCV_DTYPE_F32 2
-/* bfloat16: the tensors of the request entry points (mlcv_kv_*, mlcv_prompt_attention) only */
+/* bfloat16: the tensors of the request entry points (mlcv_kv_*, mlcv_prompt_attention, mlcv_qk_rope) only */
 #define MLCV_DTYPE_BF16 3
 #define MLCV_QUANT_NONE 0
 #define MLCV_QUANT_Q4F16_1 1
@@ -393,6 +393,25 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
                       const float* v_scale, int32_t num_pages, int32_t page, int32_t H, int32_t KV, int32_t hd,
                       float scale, int32_t causal, int32_t max_kv, void* out, int64_t o_tok, int64_t o_head,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Queries and keys before they are attended or cached: the RMS norm of each head (norm = 1) and the rotation to the
+ * token's position, in one pass.
+ *   y = x / sqrt(mean(x^2) + eps) * (w + w_offset)     (y = x with norm = 0; a NULL weight stands for factors of 1;
+ *                                                       Gemma's weights take w_offset = 1)
+ *   (y_i, y_{i + rotary/2}) -> (y_i cos - y_{i + rotary/2} sin, y_{i + rotary/2} cos + y_i sin), i < rotary / 2, of the angle
+ *   position * theta^(-2 i / rotary); dims from `rotary` on (a multiple of 16, 0 to hd) stay y
+ * q, k and their outs: element (t, h, d) at t * tok + h * head + d elements, MLCV_DTYPE_F16, _BF16 or _F32 throughout (any
+ * strides; where all rows are 16-byte aligned they are read faster); hd 64, 128 or 256; weights [hd] of that type or
+ * _F32.  float32 between the load and one rounding at the end, the angles of far positions in more.
+ * The position of a token is positions[t] (any int32), or, with positions NULL, its place in the cache as
+ * mlcv_kv_attention has it: kv_lens[b] - n + i for token i of request b's n (a refused request's, with kv_lens 0, are
+ * negative); rows behind the last request are then left as they were.  An out may be its own input (same strides); it
+ * must not overlap the other input or output, and its rows lie apart (-2). */
+int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                 int32_t dtype, int32_t tokens, const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens,
+                 const int32_t* positions, int32_t H, int32_t KV, int32_t hd, int32_t rotary, double theta, int32_t norm,
+                 const void* q_weight, const void* k_weight, int32_t w_dtype, float w_offset, float eps, void* q_out,
+                 int64_t qo_tok, int64_t qo_head, void* k_out, int64_t ko_tok, int64_t ko_head, void* stream);
 
 /* Enqueue `iters` launches of one operation of denoise_step_kv on `stream`, on the
  * context's current buffers (benchmarking / profiling only; no counterpart in the

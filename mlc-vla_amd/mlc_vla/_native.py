@@ -95,6 +95,9 @@ SIGNATURES = {
                                          _vp, ctypes.c_size_t, _vp]),
     "mlcv_prompt_attention": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32,
                                              _i32, _i32, _i32, ctypes.c_float, _i32, _vp, _vp, _i64, _i64, _vp]),
+    "mlcv_qk_rope": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32,
+                                    _i32, ctypes.c_double, _i32, _vp, _vp, _i32, ctypes.c_float, ctypes.c_float, _vp,
+                                    _i64, _i64, _vp, _i64, _i64, _vp]),
     "mlcv_bench_op": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
 }
 

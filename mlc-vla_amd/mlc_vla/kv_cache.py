@@ -5,6 +5,7 @@ requests are packed one after another, ``cu_seqlens`` [B + 1] int32 says where e
 length stays on the device: nothing here synchronizes, so a serving step can be captured into a graph.
 
     plan = kv_plan(past, new, table, free, num_pages=..., page_size=64, tokens=T)   # slots of the new tokens
+    q, k = qk_rope(q, k, plan.cu_seqlens, plan.kv_lens)                             # turned to their positions
     out = prompt_attention(q, k, v, plan.cu_seqlens)                                # a prompt's own attention
     cache.write(k, v, plan, layer)                                                  # into the pages
     out = cache.attention(q, plan, table, layer)                                    # later tokens
@@ -18,7 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -29,6 +30,7 @@ _F16, _BF16, _F32, _I32, _U8 = torch.float16, torch.bfloat16, torch.float32, tor
 _F8 = torch.float8_e4m3fn
 _CODE = {_F16: N.MLCV_DTYPE_F16, _F32: N.MLCV_DTYPE_F32, _BF16: N.MLCV_DTYPE_BF16}
 _NAME = {_F16: "float16", _BF16: "bfloat16"}
+_ANY_NAME = {_F16: "float16", _BF16: "bfloat16", _F32: "float32"}
 
 
 class KVPlan(NamedTuple):
@@ -146,6 +148,67 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
           page_size, table.data_ptr(), wide, cu.data_ptr(), lens.data_ptr(), slots.data_ptr(), tokens,
           status.data_ptr())
     return out
+
+
+def qk_rope(q, k, cu_seqlens=None, kv_lens=None, *, positions=None, theta: float = 10000.0,
+            rotary_dim: Optional[int] = None, norm: bool = False, q_weight=None, k_weight=None,
+            weight_offset: float = 1.0, eps: float = 1e-6, out=None) -> Tuple[Tensor, Tensor]:
+    """Norm of each head (optional) and rotation of queries [tokens, H, hd] and keys [tokens, KV, hd] (float16, bfloat16 or
+    float32, any strides with contiguous rows), in one pass (mlcv_qk_rope).
+
+    The tokens' places in the cache, from a plan's ``cu_seqlens`` and ``kv_lens``, or ``positions`` [tokens] int32.
+    ``rotary_dim``: the first dims of a head that are turned (default: all); ``norm``: each head is divided by its root mean
+    square, and times ``weight_offset`` + its weight [hd] (of the type of q or float32) where there is one.  ``out``: two
+    tensors; they may be q and k themselves.  Rows behind the last request are left as they were, so by default they are
+    not initialized."""
+    q, k = _t(q), _t(k)
+    dev, dt = q.get_device(), q.dtype
+    code = _CODE.get(dt)
+    tokens, heads, hd = q.shape if q.dim() == 3 else (-1,) * 3
+    kv = k.shape[1] if k.dim() == 3 else -1
+    if not (code and k.dtype is dt and k.shape == (tokens, kv, hd) and dev >= 0 and k.get_device() == dev
+            and (q.stride(2) == k.stride(2) == 1 or not tokens * hd)):
+        t, d = (tokens, hd) if q.dim() == 3 else (None, None)
+        _refuse("qk_rope", dev, (("q", q, _CODE, (None,) * 3, False), ("k", k, (dt,), (t, None, d), False)))
+    n, cu, lens, pos = 0, None, None, None
+    if positions is None:
+        if cu_seqlens is None or kv_lens is None:
+            _bad("qk_rope", "positions", "or cu_seqlens and kv_lens are needed")
+        c, m = _t(cu_seqlens), _t(kv_lens)
+        n = m.shape[0] if m.dim() == 1 else -1
+        if not (c.dtype is _I32 and m.dtype is _I32 and c.shape == (n + 1,) and c.is_contiguous() and m.is_contiguous()
+                and c.get_device() == m.get_device() == dev):
+            _refuse("qk_rope", dev, (("kv_lens", m, (_I32,), (None,), True), ("cu_seqlens", c, (_I32,), (n + 1,), True)))
+        cu, lens = c.data_ptr(), m.data_ptr()
+    else:
+        if cu_seqlens is not None or kv_lens is not None:
+            _bad("qk_rope", "positions", "and cu_seqlens or kv_lens exclude one another")
+        p = _t(positions)
+        if not (p.dtype is _I32 and p.shape == (tokens,) and p.is_contiguous() and p.get_device() == dev):
+            _refuse("qk_rope", dev, (("positions", p, (_I32,), (tokens,), True),))
+        pos = p.data_ptr()
+    wt, at = code, [None, None]
+    if q_weight is not None or k_weight is not None:
+        if not norm:
+            _bad("qk_rope", "q_weight" if q_weight is not None else "k_weight", "goes with norm")
+        ws = [None if w is None else _t(w) for w in (q_weight, k_weight)]
+        wt = _F32 if any(w is not None and w.dtype is _F32 for w in ws) else dt
+        for i, w in enumerate(ws):
+            if w is None:
+                continue
+            if not (w.dtype is wt and w.shape == (hd,) and w.is_contiguous() and w.get_device() == dev):
+                _refuse("qk_rope", dev, (("qk"[i] + "_weight", w, (wt,), (hd,), True),))
+            at[i] = w.data_ptr()
+        wt = _CODE[wt]
+    qo, ko = (_like(q), _like(k)) if out is None else (_given("qk_rope", x, y, dev) for x, y in zip(out, (q, k)))
+    qt, qh, _ = q.stride()
+    kt, kh, _ = k.stride()
+    qot, qoh, _ = qo.stride()
+    kot, koh, _ = ko.stride()
+    _call("mlcv_qk_rope", dev, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, code, tokens, cu, n, lens, pos, heads, kv, hd,
+          hd if rotary_dim is None else rotary_dim, theta, norm, at[0], at[1], wt, weight_offset, eps, qo.data_ptr(), qot,
+          qoh, ko.data_ptr(), kot, koh)
+    return Tensor(qo, _ANY_NAME[dt]), Tensor(ko, _ANY_NAME[dt])
 
 
 def _cache_wanted(kc, ks, vc, vs):

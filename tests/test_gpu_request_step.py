@@ -1,0 +1,192 @@
+"""What a decode step of several requests needs around its attention, on the GPU: norm and rotation of queries and keys
+(kv_cache.qk_rope) against plain implementations in 64 bits (stepref.py, which derives the tolerances)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import stepref as S
+from mlc_vla import _native as N
+from mlc_vla import kv_cache as C
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+@pytest.fixture(autouse=True)
+def _named(request):
+    print(request.node.name, flush=True)
+
+
+def _ints(v):
+    return torch.tensor(list(v), dtype=torch.int32, device="cuda")
+
+
+def _host(t):
+    return t.detach().cpu().to(torch.float64).numpy()
+
+
+def _randn(rng, shape, dt, scale=1.0):
+    return torch.from_numpy(scale * rng.standard_normal(shape)).to(dt).cuda()
+
+
+# ---- norm and rotation ---------------------------------------------------------------------------------
+
+
+def _check_rope(q, k, pos, there, got, rd, theta, norm, ws, offset, eps):
+    for x, y, w in zip((q, k), got, ws):
+        hd = x.shape[2]
+        want, size = S.rope(_host(x), pos, rd, theta, norm, None if w is None else _host(w), offset, eps)
+        tol = S.rope_bound(want, size, x.dtype, hd, pos, norm)
+        y = _host(y.torch)
+        assert (np.abs(y - want) <= tol)[there].all(), np.max((np.abs(y - want) / tol)[there])
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("hd,heads,kv,rd", [(64, 1, 1, 64), (64, 14, 2, 32), (128, 8, 8, 128), (128, 5, 1, 112),
+                                            (256, 8, 1, 256), (256, 3, 3, 16), (256, 2, 1, 0)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_qk_rope(dt, hd, heads, kv, rd, norm):
+    rng = np.random.default_rng(hd + heads + rd + norm)
+    past, new = [0, 131071, 5, 700, 3], [3, 1, 0, 70, 2]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    lens = [p + n for p, n in zip(past, new)]
+    tokens = int(cu[-1]) + 2  # two rows behind the last request
+    q, k = _randn(rng, (tokens, heads, hd), TYPES[dt], 3.0), _randn(rng, (tokens, kv, hd), TYPES[dt])
+    ws = [None, None]
+    if norm:
+        ws = [_randn(rng, hd, TYPES[dt], 0.3), None if rd == 16 else _randn(rng, hd, TYPES[dt], 0.3)]
+    got = C.qk_rope(q, k, _ints(cu), _ints(lens), theta=500000.0, rotary_dim=rd, norm=norm, q_weight=ws[0], k_weight=ws[1])
+    pos, there = S.places(cu, lens, tokens)
+    _check_rope(q, k, pos, there, got, rd, 500000.0, norm, ws, 1.0, 1e-6)
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_qk_rope_given_positions(dt):
+    """Any int32: far, negative, the same twice; weights in float32, no offset, another eps."""
+    rng = np.random.default_rng(1)
+    pos = np.array([0, 1, -1, 7, 7, 131072, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31] + list(range(100, 600)))
+    q, k = _randn(rng, (len(pos), 4, 128), TYPES[dt]), _randn(rng, (len(pos), 2, 128), TYPES[dt])
+    ws = [torch.from_numpy(1 + 0.1 * rng.standard_normal(128)).float().cuda() for _ in range(2)]
+    for norm, w in ((False, [None, None]), (True, ws), (True, [None, None])):
+        got = C.qk_rope(q, k, positions=_ints(pos), norm=norm, q_weight=w[0], k_weight=w[1], weight_offset=0.0, eps=1e-3)
+        _check_rope(q, k, pos, np.ones(len(pos), bool), got, 128, 10000.0, norm, w, 0.0, 1e-3)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_qk_rope_strides(hd, dt):
+    """Views of a fused projection, rows off 16 bytes, head-major tensors, in place, into given tensors."""
+    rng = np.random.default_rng(hd)
+    t, h, kv = 37, 6, 2
+    pos = _ints(range(1000, 1000 + t))
+    base = _randn(rng, (t, h + 2 * kv, hd), TYPES[dt])
+    q, k = base[:, :h], base[:, h:h + kv]
+    want = [x.torch.clone() for x in C.qk_rope(q.contiguous(), k.contiguous(), positions=pos, norm=True)]
+    assert all(torch.equal(a.torch, b) for a, b in zip(C.qk_rope(q, k, positions=pos, norm=True), want))
+    odd = torch.zeros(t * (h + kv) * hd + 3, dtype=TYPES[dt], device="cuda")[3:].view(t, h + kv, hd)
+    odd.copy_(base[:, :h + kv])
+    assert all(torch.equal(a.torch, b) for a, b in zip(C.qk_rope(odd[:, :h], odd[:, h:], positions=pos, norm=True), want))
+    qh, kh = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k))
+    outs = [torch.zeros((n, t, hd + 8), dtype=TYPES[dt], device="cuda").transpose(0, 1)[..., 8:] for n in (h, kv)]
+    got = C.qk_rope(qh, kh, positions=pos, norm=True, out=outs)
+    assert all(torch.equal(a.torch, b) and a.torch.data_ptr() == o.data_ptr() for a, b, o in zip(got, want, outs))
+    v = base[:, h + kv:].clone()
+    C.qk_rope(q, k, positions=pos, norm=True, out=(q, k))  # in place
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(base[:, h + kv:], v)
+
+
+def test_qk_rope_rows_behind_the_last_request():
+    """They stay as they were; so does everything where no offset says whose a token is."""
+    rng = np.random.default_rng(3)
+    q, k = _randn(rng, (9, 2, 64), torch.float16), _randn(rng, (9, 1, 64), torch.float16)
+    outs = [torch.full_like(x, 7.0) for x in (q, k)]
+    C.qk_rope(q, k, _ints([0, 2, 5]), _ints([2, 9]), out=outs)
+    assert all((o[5:] == 7).all() and (o[:5] != 7).any(-1).all() for o in outs)
+    for cu in ([9, 9, 9], [-5, -1, 0]):
+        outs = [torch.full_like(x, 7.0) for x in (q, k)]
+        C.qk_rope(q, k, _ints(cu), _ints([2, 9]), out=outs)
+        assert all((o == 7).all() for o in outs)
+    # no tokens, no requests
+    C.qk_rope(q[:0], k[:0], _ints([0, 0]), _ints([4]))
+    outs = [torch.full_like(x, 7.0) for x in (q, k)]
+    C.qk_rope(q, k, _ints([0]), _ints([]), out=outs)
+    assert all((o == 7).all() for o in outs)
+
+
+@pytest.mark.parametrize("b", [1, 63, 64, 65, 127, 4095, 4097, 9000])
+def test_qk_rope_of_many_requests(b):
+    """The search for a token's request; some bring no tokens."""
+    rng = np.random.default_rng(b)
+    new = rng.integers(0, 3, b)
+    new[0] = 1
+    cu = np.concatenate([[0], np.cumsum(new)])
+    lens = rng.integers(0, 5000, b) + new
+    tokens = int(cu[-1])
+    q, k = _randn(rng, (tokens, 1, 64), torch.float32), _randn(rng, (tokens, 1, 64), torch.float32)
+    pos, there = S.places(cu, lens, tokens)
+    got = C.qk_rope(q, k, _ints(cu), _ints(lens))
+    same = C.qk_rope(q, k, positions=_ints(pos))
+    assert all(torch.equal(x.torch, y.torch) for x, y in zip(got, same))
+    _check_rope(q, k, pos, there, got, 64, 10000.0, False, (None, None), 1.0, 1e-6)
+
+
+def test_qk_rope_values_of_every_size():
+    """Zeros, subnormals, the largest values, infinities and NaN stay within their head."""
+    q = torch.zeros((6, 2, 64), dtype=torch.float16, device="cuda")
+    q[1], q[2, 0], q[3, 0, 5], q[4, 0, 5] = 6e-8, 6e4, float("inf"), float("nan")
+    k = torch.ones((6, 1, 64), dtype=torch.float16, device="cuda")
+    pos = _ints([0] * 6)
+    got = C.qk_rope(q, k, positions=pos)[0].torch
+    assert torch.equal(got[:3], q[:3]) and torch.isfinite(got[3:, 1]).all()
+    assert got[3, 0, 5].isinf() and got[4, 0, 5].isnan()
+    got = C.qk_rope(q, k, positions=pos, norm=True)[0].torch
+    assert (got[0] == 0).all() and torch.isfinite(got[:3]).all() and (got[2, 0] == 1).all()
+    # 6e-8^2 is far below eps: x / sqrt(eps)
+    assert (got[1] - 5.96e-8 * 1e3).abs().max() < 1e-6
+
+
+def test_qk_rope_rotates_as_the_model_does():
+    """The rotation of the joint attention's oracle."""
+    from oracle import pi0_oracle as O
+
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((40, 8, 256)).astype(np.float32)
+    cos, sin = O.make_rope_np(40, 256, 10000.0, 0)
+    want = O.apply_rope(x, cos, sin, O.Prec("f64"))
+    t = torch.from_numpy(x).cuda()
+    got = C.qk_rope(t, t[:, :1], positions=_ints(range(40)))[0].torch
+    # its table holds float32 angles: at position 39 half a step is 2^-19
+    assert np.abs(_host(got) - want).max() <= 2.0 ** -18 * 2 * np.abs(x).max()
+
+
+def test_qk_rope_arguments():
+    rng = np.random.default_rng(9)
+    q, k = _randn(rng, (4, 4, 64), torch.float16), _randn(rng, (4, 2, 64), torch.float16)
+    cu, lens, pos, w = _ints([0, 4]), _ints([4]), _ints(range(4)), _randn(rng, 64, torch.float16)
+    C.qk_rope(q, k, cu, lens)
+    for args, kw, what in (
+            ((q, k), {}, "positions"), ((q, k, cu), {}, "positions"), ((q, k, cu, lens), dict(positions=pos), "exclude"),
+            ((q, k.float(), cu, lens), {}, "k has dtype"), ((q, k[:3], cu, lens), {}, "k expects shape"),
+            ((q, k[..., :32], cu, lens), {}, "k expects shape"), ((q[0], k, cu, lens), {}, "q expects shape"),
+            ((q.int(), k, cu, lens), {}, "q has dtype"), ((q[..., ::2], k[..., ::2], cu, lens), {}, "contiguous rows"),
+            ((q, k, cu, _ints([4, 4])), {}, "cu_seqlens expects"), ((q, k, cu.long(), lens), {}, "cu_seqlens has dtype"),
+            ((q, k, cu.cpu(), lens), {}, "cu_seqlens is not on"), ((q, k), dict(positions=pos[:3]), "positions expects"),
+            ((q, k), dict(positions=pos.long()), "positions has dtype"),
+            ((q, k, cu, lens), dict(q_weight=w), "goes with norm"),
+            ((q, k, cu, lens), dict(norm=True, q_weight=w[:32]), "q_weight expects"),
+            ((q, k, cu, lens), dict(norm=True, q_weight=w, k_weight=w.float()), "q_weight has dtype"),
+            ((q, k, cu, lens), dict(norm=True, k_weight=w.bfloat16()), "k_weight has dtype"),
+            ((q, k, cu, lens), dict(out=(q, k[:3])), "out expects")):
+        with pytest.raises(ValueError, match=what):
+            C.qk_rope(*args, **kw)
+    for kw, what in ((dict(rotary_dim=24), "rotary"), (dict(rotary_dim=80), "rotary"), (dict(rotary_dim=-16), "rotary"),
+                     (dict(theta=0.5), "theta"), (dict(theta=float("nan")), "theta"), (dict(norm=True, eps=-1.0), "eps"),
+                     (dict(norm=True, eps=float("nan")), "eps"),
+                     (dict(norm=True, q_weight=w, weight_offset=float("inf")), "w_offset"),
+                     (dict(out=(q[:1].expand(4, 4, 64), k)), "out overlap")):
+        with pytest.raises(N.MlcvError, match=what):
+            C.qk_rope(q, k, cu, lens, **kw)
