@@ -39,7 +39,8 @@ extern "C" {
  * reference runs in float32; the other entry points and options of the step forms report that
  * they are not built for them. */
 #define MLCV_DTYPE_F32 2
-/* bfloat16: the tensors of the request entry points (mlcv_kv_*, mlcv_prompt_attention, mlcv_qk_rope) only */
+/* bfloat16: the tensors of the request entry points (mlcv_kv_*, mlcv_prompt_attention, mlcv_qk_rope,
+ * mlcv_token_logprobs) only */
 #define MLCV_DTYPE_BF16 3
 #define MLCV_QUANT_NONE 0
 #define MLCV_QUANT_Q4F16_1 1
@@ -412,6 +413,20 @@ int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, in
                  const int32_t* positions, int32_t H, int32_t KV, int32_t hd, int32_t rotary, double theta, int32_t norm,
                  const void* q_weight, const void* k_weight, int32_t w_dtype, float w_offset, float eps, void* q_out,
                  int64_t qo_tok, int64_t qo_head, void* k_out, int64_t ko_tok, int64_t ko_head, void* stream);
+
+/* Log probabilities from logits: row r, element i at r * stride + i elements (any stride), MLCV_DTYPE_F16, _BF16 or _F32;
+ *   log p(i) = z_i - log(sum_j exp(z_j)),  z = scale * x        scale between 1e-6 and 1e6 (one over the temperature)
+ *   logprobs [rows][given]      of tokens [rows][given]; 0 for a token outside [0, vocab) (padding)
+ *   entropy [rows]              -sum p log p (NULL: not wanted)
+ *   top_ids, top_logprobs [rows][top]   the `top` (up to 64) largest logits in descending order, equal ones by their index
+ * all in float32, read in one pass.  Masked logits (-inf) have probability 0 and rank behind the others; a row of them alone has
+ * entropy 0 and log probabilities of -inf.  A row with a NaN or +inf has NaN for its probabilities and entropy; NaN ranks
+ * last.  Logits of the type's lowest value are ordinary ones.  workspace: mlcv_token_logprobs_workspace bytes of device
+ * memory, 16-byte aligned, for this call alone while it runs.  Outputs must not overlap the inputs. */
+int mlcv_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, size_t* bytes);
+int mlcv_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, float scale,
+                        const int32_t* tokens, int32_t given, float* logprobs, float* entropy, int32_t top,
+                        int32_t* top_ids, float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Enqueue `iters` launches of one operation of denoise_step_kv on `stream`, on the
  * context's current buffers (benchmarking / profiling only; no counterpart in the

@@ -98,6 +98,9 @@ SIGNATURES = {
     "mlcv_qk_rope": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32,
                                     _i32, ctypes.c_double, _i32, _vp, _vp, _i32, ctypes.c_float, ctypes.c_float, _vp,
                                     _i64, _i64, _vp, _i64, _i64, _vp]),
+    "mlcv_token_logprobs_workspace": (ctypes.c_int, [_i32] * 3 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlcv_token_logprobs": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i32, ctypes.c_float, _vp, _i32, _vp, _vp, _i32, _vp,
+                                           _vp, _vp, ctypes.c_size_t, _vp]),
     "mlcv_bench_op": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
 }
 

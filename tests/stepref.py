@@ -49,3 +49,48 @@ def rope_bound(out, size, dtype, hd, pos, norm):
            + (9 + (hd + 8 if norm else 0)) * E32)
     f = torch.finfo(dtype)
     return f.eps / 2 * np.abs(out) + rel * size * (1 + f.eps) + f.smallest_normal * f.eps / 2
+
+
+def logprobs(x, scale, tokens, top):
+    """x [rows, vocab] float64 -> (log probabilities of tokens [rows, n] or None, entropy, ids, their log probabilities)."""
+    rows, vocab = x.shape
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        z = x * scale
+        m = z.max(1, keepdims=True)
+        e = np.exp(z - np.where(np.isfinite(m), m, 0.0))
+        s = e.sum(1, keepdims=True)
+        lp = (z - np.where(np.isfinite(m), m, 0.0)) - np.log(s)  # m + ln s would lose ln s next to logits of 1e38
+        p = e / s
+        h = -np.where(p > 0, p * lp, 0.0).sum(1)
+    lp[lp < -np.finfo(np.float32).max] = -np.inf  # what the results' type cannot hold
+    none, bad = (m == -np.inf)[:, 0], np.isnan(x).any(1) | (x == np.inf).any(1)
+    lp[none], h[none] = -np.inf, 0.0
+    lp[bad], h[bad] = np.nan, np.nan
+    got = None
+    if tokens is not None:
+        there = (tokens >= 0) & (tokens < vocab)
+        got = np.where(there, np.take_along_axis(lp, np.where(there, tokens, 0), 1), 0.0)
+    # largest first, equal ones by their index, NaN behind -inf
+    rank = np.where(np.isnan(x), -np.inf, x)
+    ids = np.stack([np.lexsort((np.arange(vocab), np.isnan(r), -q))[:top] for r, q in zip(x, rank)]) \
+        if rows else np.zeros((0, top), int)
+    return got, h, ids, np.take_along_axis(lp, ids, 1)
+
+
+def logprobs_bound(x, scale, vocab):
+    """(bound of each log probability given its value, bound of the entropy), per row, as functions of what is compared.
+    With w the spread of scaled logits that carry weight (those further than 104 below the largest are below the smallest
+    float32) and u = 2^-24:
+      exponents     scale * log2(e) rounded (1 u of |z|, of every term the same factor but for its distance from the
+                    largest: w), one fused product (w), the hardware's exponential 2 u: a weight is off by (2 w + 2) u
+      sums          up to vocab terms of one sign, in chains of at most vocab / 256 + 32: that many u
+      logarithm     2 u of ln s (at most ln vocab), and of a log probability the subtraction, product and sum: 3 u of it"""
+    with np.errstate(invalid="ignore", over="ignore"):
+        z = x * scale
+        m = np.max(np.where(np.isfinite(z), z, -np.inf), 1, keepdims=True)
+        d = np.where(np.isfinite(z), m - z, 0.0)
+    w = np.where(d < 104, d, 0.0).max(1)
+    chain = vocab / 256 + 32
+    rel = (2 * w + 2 + chain + 8) * E32           # of s, and of u
+    base = 1.1 * (rel + 2 * E32 * np.log(vocab + 1))
+    return (lambda lp: base[:, None] + 4 * E32 * np.abs(lp)), base + 2 * rel * (np.log(vocab) + 1) + 4 * E32 * np.log(vocab + 1)

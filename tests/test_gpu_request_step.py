@@ -1,5 +1,5 @@
 """What a decode step of several requests needs around its attention, on the GPU: norm and rotation of queries and keys
-(kv_cache.qk_rope) against plain implementations in 64 bits (stepref.py, which derives the tolerances)."""
+(kv_cache.qk_rope), log probabilities (logits.token_logprobs), against plain implementations in 64 bits (stepref.py, which derives the tolerances)."""
 
 from __future__ import annotations
 
@@ -10,6 +10,7 @@ import torch
 import stepref as S
 from mlc_vla import _native as N
 from mlc_vla import kv_cache as C
+from mlc_vla import logits as L
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +191,173 @@ def test_qk_rope_arguments():
                      (dict(out=(q[:1].expand(4, 4, 64), k)), "out overlap")):
         with pytest.raises(N.MlcvError, match=what):
             C.qk_rope(q, k, cu, lens, **kw)
+
+
+# ---- log probabilities -----------------------------------------------------------------------------------
+
+
+def _check_logprobs(x, scale, tokens, top, **kw):
+    host, vocab = _host(x), x.shape[1]
+    ids = None if tokens is None else tokens.cpu().numpy().reshape(len(host), -1)
+    want, h, top_ids, top_lp = S.logprobs(host, float(np.float32(scale)), ids, top)
+    tol, tol_h = S.logprobs_bound(host, scale, vocab)
+    got = L.token_logprobs(x, tokens, top=top, scale=scale, **kw)
+
+    def near(g, w, t):
+        g = g.torch.cpu().double().numpy().reshape(w.shape)
+        fin = np.isfinite(w)
+        np.testing.assert_array_equal(g[~fin], w[~fin])
+        with np.errstate(invalid="ignore"):
+            assert (np.abs(g - w) <= t)[fin].all(), np.max((np.abs(g - w) / t)[fin])
+
+    near(got.entropy, h, tol_h)
+    assert (got.logprobs is None) == (tokens is None) and (got.top_ids is None) == (not top)
+    if tokens is not None:
+        assert got.logprobs.shape == tuple(tokens.shape)
+        near(got.logprobs, want, tol(np.where(np.isfinite(want), want, 0.0)))
+    if top:
+        np.testing.assert_array_equal(got.top_ids.numpy(), top_ids)
+        near(got.top_logprobs, top_lp, tol(np.where(np.isfinite(top_lp), top_lp, 0.0)))
+    return got
+
+
+def _tokens(rng, rows, n, vocab):
+    t = rng.integers(-1, vocab + 1, (rows, n) if n > 1 else rows)
+    return torch.from_numpy(t.astype(np.int32)).cuda()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab,top,n", [
+    (1, 1, 1, 1), (3, 2, 2, 2), (1, 7, 5, 1), (9, 64, 64, 1), (5, 333, 20, 3), (130, 4096, 1, 1), (2, 4097, 64, 1),
+    (3, 16391, 20, 5), (1, 50257, 20, 1), (40, 50257, 8, 1), (2, 257152, 64, 70), (1, 1000, 0, 1), (3, 70001, 0, 0),
+    (1100, 5001, 3, 1)])
+def test_token_logprobs(dt, rows, vocab, top, n):
+    rng = np.random.default_rng(vocab + rows)
+    x = rng.standard_normal((rows, vocab)) * 3
+    x[np.arange(rows), rng.integers(0, vocab, rows)] += 9
+    x = torch.from_numpy(x).to(TYPES[dt]).cuda()
+    _check_logprobs(x, 1.0 if rows != 5 else 0.7, _tokens(rng, rows, n, vocab) if n else None, top)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [100, 5000, 33000])
+def test_token_logprobs_order(dt, vocab):
+    """Ascending, descending, all equal, two values, zeros of both signs: ties go to the lowest index."""
+    rng = np.random.default_rng(vocab)
+    up = np.arange(vocab) / vocab * 20 - 10
+    x = np.stack([up, -up, np.full(vocab, 1.5), rng.integers(0, 2, vocab) * 1.0, np.where(rng.random(vocab) < 0.5, 0.0, -0.0),
+                  np.sort(rng.standard_normal(vocab)), np.where(np.arange(vocab) % 64 < 8, up, -20.0)])
+    x = torch.from_numpy(x).to(TYPES[dt]).cuda()
+    for top in (1, 20, 64):
+        _check_logprobs(x, 1.0, _tokens(rng, len(x), 2, vocab), top)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [50, 9001])
+def test_token_logprobs_masks(dt, vocab):
+    """-inf and the type's lowest value as masks: of some logits, of all but a few, of all; NaN and +inf in a row."""
+    rng = np.random.default_rng(vocab)
+    low, t = torch.finfo(TYPES[dt]).min, vocab - 3
+    x = torch.from_numpy(rng.standard_normal((14, vocab)) * 2).to(TYPES[dt])
+    x[0, 5:] = -np.inf
+    x[1, :t] = -np.inf
+    x[2] = -np.inf
+    x[3, 5:] = low
+    x[4, :t] = low
+    x[5] = low
+    x[6] = torch.finfo(TYPES[dt]).max
+    x[7, 3] = np.nan
+    x[8, t] = np.inf
+    x[9] = np.nan
+    x[10, ::2], x[10, 1::2] = -np.inf, np.nan
+    x[11, 2], x[11, 3:] = low, -np.inf
+    x[12, 0] = np.nan
+    x[12, 1:] = -np.inf
+    x[13, :7], x[13, 7:] = torch.finfo(TYPES[dt]).max, -np.inf
+    x = x.cuda()
+    for scale in (1.0, 4.0):
+        for top in (0, 1, 20, 50):
+            _check_logprobs(x, scale, _tokens(rng, len(x), 3, vocab), top)
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 30.0, 1e6])
+def test_token_logprobs_temperatures(dt, scale):
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.standard_normal((3, 6000)) * 5).to(TYPES[dt]).cuda()
+    _check_logprobs(x, scale, _tokens(rng, 3, 4, 6000), 10)
+
+
+def test_token_logprobs_of_certain_rows():
+    """A row that is almost certain keeps the digits of its entropy: every term has one sign."""
+    x = torch.full((8, 5000), -30.0, device="cuda")
+    gap = torch.tensor([4.0, 8, 12, 16, 20, 24, 28, 30], device="cuda")
+    x[:, 17] = gap
+    got = _check_logprobs(x, 1.0, torch.full((8,), 17, dtype=torch.int32, device="cuda"), 2)
+    _, h, _, _ = S.logprobs(_host(x), 1.0, None, 2)
+    # ln s: the largest term's exponential is off by 2^-23, s by 2^-24 of about 1; every other term by (5000 / 256 + 200) 2^-24
+    np.testing.assert_allclose(got.entropy.numpy(), h, rtol=1e-4, atol=2.0 ** -22)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [37, 4099, 30011])
+def test_token_logprobs_strides(dt, vocab):
+    """Rows at every offset from 16 bytes, a padded vocabulary, one row for all, rows backwards; given outputs."""
+    rng = np.random.default_rng(vocab)
+    whole = torch.from_numpy(rng.standard_normal((9, vocab + 13)) * 3).to(TYPES[dt]).cuda()
+    whole[:, vocab:] = float("nan")  # never looked at
+    tokens = _tokens(rng, 9, 1, vocab)
+    for off in range(9):
+        _check_logprobs(whole[:, off:vocab], 1.0, tokens, 7)
+    flat = whole.flatten()[13:]
+    flat = torch.where(torch.isnan(flat), 0.0, flat).to(TYPES[dt])
+    _check_logprobs(flat[:8 * (vocab + 13)].view(8, vocab + 13)[:, 5:vocab + 5], 1.0, tokens[:8], 7)
+    _check_logprobs(whole[:1, :vocab].expand(9, vocab), 1.0, tokens, 7)
+    made = _check_logprobs(whole[:, :vocab], 1.0, tokens, 7)
+    n = L.token_logprobs_workspace(9, vocab, 7)
+    given = L.TokenLogprobs(*(torch.zeros_like(t.torch) for t in made))
+    ws = torch.zeros(n + 64, dtype=torch.uint8, device="cuda")
+    again = L.token_logprobs(whole[:, :vocab], tokens, top=7, out=given, workspace=ws)
+    assert again is given and all(torch.equal(a, b.torch) for a, b in zip(given, made)) and (ws[n:] == 0).all()
+
+
+def test_token_logprobs_past_32_bit_offsets():
+    """Rows behind 2^32 bytes and 2^31 elements."""
+    rows, vocab = 8400, 257152
+    x = torch.empty((rows, vocab), dtype=torch.float16, device="cuda")
+    x.fill_(-5.0)
+    hot = torch.arange(rows, device="cuda") * 29 % vocab
+    x[torch.arange(rows, device="cuda"), hot] = 9.0
+    got = L.token_logprobs(x, hot.to(torch.int32), top=2)
+    want = -np.log1p((vocab - 1) * np.exp(-14.0))
+    assert torch.equal(got.top_ids.torch[:, 0], hot.to(torch.int32))
+    assert torch.equal(got.top_ids.torch[:, 1], (hot == 0).to(torch.int32))
+    assert (got.logprobs.torch - want).abs().max() < 1e-4 and torch.equal(got.logprobs.torch, got.top_logprobs.torch[:, 0])
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_token_logprobs_arguments():
+    x = torch.zeros((3, 100), dtype=torch.float16, device="cuda")
+    t = _ints([1, 2, 3])
+    made = L.token_logprobs(x, t, top=4)
+    for args, kw, what in (
+            ((x[0],), {}, "logits expects"), ((x.int(),), {}, "logits has dtype"), ((x[:, ::2],), {}, "contiguous rows"),
+            ((x.cpu(),), {}, "device"), ((x, t[:2]), {}, "tokens expects"), ((x, t.long()), {}, "tokens has dtype"),
+            ((x, t.cpu()), {}, "tokens is not on"), ((x, t), dict(top=-1), "top"),
+            ((x,), dict(top=4, out=made), "nothing to hold"), ((x, t), dict(out=made), "nothing to hold"),
+            ((x, t), dict(top=3, out=made), "top_ids expects"),
+            ((x, t), dict(top=4, out=made._replace(entropy=None)), "entropy is missing")):
+        with pytest.raises(ValueError, match=what):
+            L.token_logprobs(*args, **kw)
+    for kw, what in ((dict(top=65), "top must"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(scale=-1.0), "scale")):
+        with pytest.raises(N.MlcvError, match=what):
+            L.token_logprobs(x, t, **kw)
+    with pytest.raises(N.MlcvError, match="bad size"):
+        L.token_logprobs(x[:, :0])
+    big = torch.zeros((2, 50000), device="cuda")
+    assert L.token_logprobs_workspace(2, 50000, 5) > 64
+    with pytest.raises(N.MlcvError, match="workspace"):
+        L.token_logprobs(big, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"), top=5)
+    assert L.token_logprobs(x[:0], t[:0], top=2).top_ids.shape == (0, 2)

@@ -8,6 +8,7 @@ import torch
 
 from mlc_vla import _native as N
 from mlc_vla import kv_cache as C
+from mlc_vla import logits as L
 
 P = 4096  # a pointer that is never followed
 
@@ -20,7 +21,22 @@ def _rope(**kw):
     N.call("mlcv_qk_rope", *a.values())
 
 
+def _logprobs(**kw):
+    a = dict(logits=P, dtype=1, stride=100, rows=3, vocab=100, scale=1.0, tokens=P, given=1, lp=P, entropy=P, top=4, ids=P,
+             tlp=P, ws=None, ws_bytes=0, stream=None)
+    a.update(kw)
+    N.call("mlcv_token_logprobs", *a.values())
+
+
 @pytest.mark.parametrize("fn,bad,what", [
+    (_logprobs, dict(dtype=0), "float"), (_logprobs, dict(rows=-1), "size"), (_logprobs, dict(vocab=0), "size"),
+    (_logprobs, dict(vocab=2 ** 31 - 1), "vocab"), (_logprobs, dict(top=65), "top"), (_logprobs, dict(vocab=3), "top"),
+    (_logprobs, dict(top=-1), "top"), (_logprobs, dict(given=-1), "size"), (_logprobs, dict(scale=0.0), "scale"),
+    (_logprobs, dict(scale=float("inf")), "scale"), (_logprobs, dict(scale=float("nan")), "scale"),
+    (_logprobs, dict(logits=None), "null"), (_logprobs, dict(tokens=None), "null"), (_logprobs, dict(lp=None), "null"),
+    (_logprobs, dict(ids=None), "null"), (_logprobs, dict(tlp=None), "null"), (_logprobs, dict(logits=P + 1), "aligned"),
+    (_logprobs, dict(vocab=257152), "workspace"), (_logprobs, dict(vocab=257152, ws=P + 8, ws_bytes=1 << 40), "workspace"),
+    (_logprobs, dict(vocab=257152, ws=P, ws_bytes=100), "workspace"), (_logprobs, dict(rows=2 ** 30), "rows"),
     (_rope, dict(dtype=4), "float"), (_rope, dict(tokens=-1), "size"), (_rope, dict(H=0), "size"),
     (_rope, dict(KV=0), "size"), (_rope, dict(B=-1), "size"), (_rope, dict(hd=80), "head_dim"),
     (_rope, dict(rotary=40), "rotary"), (_rope, dict(rotary=80), "rotary"), (_rope, dict(theta=0.0), "theta"),
@@ -39,6 +55,7 @@ def test_refused(fn, bad, what):
 def test_empty_calls_do_nothing():
     _rope(tokens=0)
     _rope(B=0)
+    _logprobs(rows=0)
 
 
 def test_host_tensors_are_refused():
@@ -46,3 +63,14 @@ def test_host_tensors_are_refused():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="device"):
         C.qk_rope(x, x, positions=i)
+    with pytest.raises(ValueError, match="device"):
+        L.token_logprobs(x[0])
+
+
+def test_workspace_of_logprobs():
+    assert L.token_logprobs_workspace(0, 257152, 5) == 0 and L.token_logprobs_workspace(2000, 257152, 5) == 0
+    one = L.token_logprobs_workspace(1, 257152, 0)
+    assert one > 0 and L.token_logprobs_workspace(1, 257152, 64) == one // 16 * (16 + 8 * 64)
+    assert L.token_logprobs_workspace(1, 4096, 64) == 0
+    with pytest.raises(N.MlcvError, match="null"):
+        N.call("mlcv_token_logprobs_workspace", 1, 100, 1, None)
