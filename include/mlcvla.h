@@ -349,6 +349,13 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
                  int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,
                  void* stream);
 
+/* mlcv_kv_plan with the number of free pages on the device: the first min(n_free, *free_count) entries of free_pages are free
+ * (free_count NULL: all n_free), as mlcv_kv_free leaves them. */
+int mlcv_kv_plan_counted(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
+                         int32_t n_free, const int32_t* free_count, int32_t num_pages, int32_t page,
+                         int32_t* block_table, int32_t max_pages, int32_t* cu_seqlens, int32_t* kv_lens,
+                         int32_t* slot_map, int32_t tokens, int32_t* status, void* stream);
+
 /* Write the new tokens' keys and values into their slots.  k, v: element (t, h, d) at
  * t * k_tok + h * k_head + d elements (any strides; rows of 16-byte alignment are read faster),
  * each of MLCV_DTYPE_F16, _BF16 or _F32 -- mlcv_prefill's float32 keys and float16 values
@@ -394,6 +401,50 @@ int mlcv_kv_attention(const void* q, int32_t dtype, int64_t q_tok, int64_t q_hea
                       const float* v_scale, int32_t num_pages, int32_t page, int32_t H, int32_t KV, int32_t hd,
                       float scale, int32_t causal, int32_t max_kv, void* out, int64_t o_tok, int64_t o_head,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages change hands.  The pages in use are those of the first ceil(kv_lens[b] / page) entries of each row of the block
+ * table [B][max_pages] (lengths are brought into 0 .. max_pages * page; entries outside [0, num_pages) count as none; up to
+ * 4096 rows); rows may share pages, and no count of references is kept.  Entries may not be shared by requests that still write to
+ * them: full pages are safe.  A request that a plan has refused holds what it held: its length is then the old one.
+ *
+ * mlcv_kv_free: free_pages [num_pages] becomes the pages that no row holds, ascending, then -1; free_count [1] how many there
+ * are.  A plan or a fork takes pages from the front; between them the list is made anew.  workspace:
+ * mlcv_kv_free_workspace bytes, 16-byte aligned, for this call alone while it runs (so below). */
+int mlcv_kv_free_workspace(int32_t num_pages, size_t* bytes);
+int mlcv_kv_free(const int32_t* block_table, int32_t B, int32_t max_pages, const int32_t* kv_lens, int32_t num_pages,
+                 int32_t page, int32_t* free_pages, int32_t* free_count, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* Copy pages of all layers, codes and scales: page src[i] of the first cache to page dst[i] of the second (which may be the
+ * first).  Caches [layers][pages][...] as above.  Pairs with a number outside of their pool are passed over.  No page may be
+ * written twice, nor written and read, in one call (what it then holds is undefined). */
+int mlcv_kv_copy(const int32_t* src, const int32_t* dst, int32_t n, void* k_cache, float* k_scale, void* v_cache,
+                 float* v_scale, int32_t num_pages, void* k_into, float* k_scale_into, void* v_into,
+                 float* v_scale_into, int32_t pages_into, int32_t layers, int32_t page, int32_t KV, int32_t hd,
+                 void* stream);
+
+/* Requests that go on from the tokens of others: row i of new_table [n][max_pages] holds the pages of row parents[i], new_lens[i]
+ * is its length; entries behind are -1, and a parent outside [0, B) gives an empty row.  Full pages are shared.  A last page that
+ * is not full stays with the first row of its parent; every other row gets a copy of it (all layers) on a page from the
+ * front of free_pages, in the order of the rows.  Rows for which the free pages do not last are refused: empty, length 0.
+ *   status [2]: pages taken; rows refused.  copies [2 n]: where the copied pages come from and go to (scratch)
+ * The old table is done with: to keep a request beside its forks, let it be a row of its own.  At most 4096 rows of either table.  No
+ * output may overlap an input or another output (-2). */
+int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, int32_t B, int32_t max_pages,
+                 const int32_t* kv_lens, const int32_t* free_pages, int32_t n_free, const int32_t* free_count,
+                 void* k_cache, float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages,
+                 int32_t page, int32_t KV, int32_t hd, int32_t* new_table, int32_t* new_lens, int32_t* status,
+                 int32_t* copies, void* stream);
+
+/* Make a pool dense: with m pages in use, those numbered m and above move, in ascending order, to the free ones below m, in all
+ * layers; new_table (which may be block_table) has their new numbers.  The pages from m on are free then.  Entries behind a
+ * row's length stay as they are.
+ *   status [2]: m; pages moved */
+int mlcv_kv_compact_workspace(int32_t num_pages, size_t* bytes);
+int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, const int32_t* kv_lens, void* k_cache,
+                    float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages, int32_t page,
+                    int32_t KV, int32_t hd, int32_t* new_table, int32_t* status, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 /* Queries and keys before they are attended or cached: the RMS norm of each head (norm = 1) and the rotation to the
  * token's position, in one pass.

@@ -11,6 +11,7 @@
 // Values are held token-innermost because the attention's second product contracts over tokens: its matrix
 // operand is then 16 contiguous bytes per lane, as is the first product's over the head dim.
 #include "kernels.h"
+#include "kv_args.h"
 #include "mlcvla.h"
 
 #include <algorithm>
@@ -22,30 +23,9 @@ namespace {
 
 constexpr int KV_NT = 256;         // threads per workgroup of every kernel here
 constexpr int KV_RT = 16;          // query rows of an attention workgroup
-// Slots of a cache, positions of a row, tokens of a write, query rows of a kv head: the last tile's or page's positions
-// still are ints
-constexpr int64_t KV_MOST = INT32_MAX - 255;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int KV_MAX_REQ = 4096;   // requests of one plan: two ints each in LDS
 
 // ---- plan ------------------------------------------------------------------------------------------
-
-// Inclusive prefix sums of one value per thread over the workgroup (KV_NT threads); `part` holds a sum per wave.
-__device__ __forceinline__ long long block_scan(long long v, long long* part) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 63) part[w] = v;
-  __syncthreads();
-  long long before = 0;
-#pragma unroll
-  for (int i = 0; i < KV_NT / 64 - 1; ++i) before += i < w ? part[i] : 0;
-  __syncthreads();
-  return v + before;
-}
 
 // The last index b in [0, n) with a[b] <= v (a ascending, a[0] <= v).
 __device__ __forceinline__ int last_le(const int* a, int n, int v) {
@@ -59,7 +39,7 @@ __device__ __forceinline__ int last_le(const int* a, int n, int v) {
 }
 
 struct PlanArgs {
-  const int32_t *past, *fresh, *free_pages;
+  const int32_t *past, *fresh, *free_pages, *free_count;
   int32_t *table, *cu, *kv_lens, *slots, *status;
   int32_t B, n_free, num_pages, psh, max_pages, tokens, slot_blocks;
 };
@@ -78,6 +58,7 @@ __global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
   int* scu = sm;                // [B + 1] first token of each request
   int* sbase = sm + a.B + 1;    // [B + 1] first page it takes from the free list; ~base where it is refused
   const int tid = threadIdx.x, page = 1 << a.psh;
+  const int n_free = a.free_count ? clamp_i(*a.free_count, 0, a.n_free) : a.n_free;
   if (tid == 0) sbad = sused = 0;
   __syncthreads();
   long long tok0 = 0, pg0 = 0;
@@ -87,17 +68,17 @@ __global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
     const bool in = b < a.B;
     const long long p = in ? a.past[b] : 0, q = in ? a.fresh[b] : 0;
     const long long qn = q > 0 ? q : 0;
-    const long long end = block_scan(qn, part) + tok0;
+    const long long end = block_scan<KV_NT>(qn, part) + tok0;
     const long long had = (p + page - 1) >> a.psh, has = (p + qn + page - 1) >> a.psh;
     const bool fits = in && p >= 0 && q >= 0 && has <= a.max_pages && end <= a.tokens;
     const long long need = fits ? has - had : 0;
-    const long long pend = block_scan(need, part) + pg0;
-    const bool ok = fits && (need == 0 || pend <= a.n_free);
+    const long long pend = block_scan<KV_NT>(need, part) + pg0;
+    const bool ok = fits && (need == 0 || pend <= n_free);
     if (in) {
       const long long first = end - qn;
       scu[b] = (int)(first < a.tokens ? first : a.tokens);
       // pages past the free list are never indexed: a refused request has no slots and no table entries
-      const long long base = pend - need < a.n_free ? pend - need : a.n_free;
+      const long long base = pend - need < n_free ? pend - need : n_free;
       sbase[b] = ok ? (int)base : ~(int)base;
       bad += !ok;
       if (ok && need > 0) used = (int)pend;  // granted: at most n_free; ascending over b
@@ -121,7 +102,7 @@ __global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
   if (used) atomicMax(&sused, used);
   if (tid == 0) {
     scu[a.B] = (int)(tok0 < a.tokens ? tok0 : a.tokens);
-    sbase[a.B] = (int)(pg0 < a.n_free ? pg0 : a.n_free);
+    sbase[a.B] = (int)(pg0 < n_free ? pg0 : n_free);
   }
   __syncthreads();
   if ((int)blockIdx.x < a.slot_blocks) {  // slots
@@ -169,7 +150,6 @@ __global__ __launch_bounds__(KV_NT) void kv_plan_kernel(const PlanArgs a) {
 // ceil(n * mul / div) items (extra = 1), or one more for a first page that is not empty (extra = 2), so that
 // floor(tokens * mul / div) + extra * B items always do; the few that are left over end at once.
 // Every thread tests its own b: one round of loads instead of a chain of dependent ones.
-__device__ __forceinline__ int clamp_i(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 struct Item {
   int b, c0, n;  // request, its first token and number of tokens; b = -1: none
   int i;         // the item's number within its request
@@ -1009,25 +989,6 @@ KvAttnPlan kv_attn_plan(int tokens, int B, int H, int KV, int hd, int max_kv) {
   return p;
 }
 
-// Whether one of the first `outs` arrays of ints shares memory with any other
-struct Ints {
-  const void* p;
-  int64_t n;
-};
-bool overlap(const Ints* a, int outs, int all) {
-  for (int i = 0; i < outs; ++i)
-    for (int j = i + 1; j < all; ++j) {
-      const uintptr_t x = reinterpret_cast<uintptr_t>(a[i].p), y = reinterpret_cast<uintptr_t>(a[j].p);
-      if (a[i].n > 0 && a[j].n > 0 && x < y + 4 * a[j].n && y < x + 4 * a[i].n) return true;
-    }
-  return false;
-}
-
-bool kv_page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
-bool kv_hd_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int log2_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
-
 template <int HD>
 int kv_write_launch(const WriteArgs& a, hipStream_t st) {
   const int page = 1 << a.psh;
@@ -1068,10 +1029,10 @@ using namespace mlcv;
 
 extern "C" {
 
-int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
-                 int32_t n_free, int32_t num_pages, int32_t page, int32_t* block_table, int32_t max_pages,
-                 int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,
-                 void* stream) {
+int mlcv_kv_plan_counted(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
+                         int32_t n_free, const int32_t* free_count, int32_t num_pages, int32_t page,
+                         int32_t* block_table, int32_t max_pages, int32_t* cu_seqlens, int32_t* kv_lens,
+                         int32_t* slot_map, int32_t tokens, int32_t* status, void* stream) {
   MLCV_REQUIRE(B >= 0 && n_free >= 0 && num_pages >= 0 && max_pages >= 0 && tokens >= 0, "negative size");
   MLCV_REQUIRE(cu_seqlens && status, "null output");
   MLCV_REQUIRE(B == 0 || (past_lens && new_lens && kv_lens && (block_table || max_pages == 0)), "null request array");
@@ -1083,9 +1044,10 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
                "more than 2^31 - 256 slots");
   // every workgroup reads the lengths, one writes kv_lens: a plan written over them would be read half new
   const Ints arrays[] = {{block_table, (int64_t)B * max_pages}, {cu_seqlens, (int64_t)B + 1}, {kv_lens, B}, {slot_map, tokens},
-                         {status, 2}, {past_lens, B}, {new_lens, B}, {free_pages, n_free}};
-  MLCV_REQUIRE(!overlap(arrays, 5, 8), "outputs overlap the inputs or one another");
-  PlanArgs a{past_lens, new_lens, free_pages, block_table, cu_seqlens, kv_lens, slot_map, status, B, n_free,
+                         {status, 2}, {past_lens, B}, {new_lens, B}, {free_pages, n_free},
+                         {free_count, free_count ? 1 : 0}};
+  MLCV_REQUIRE(!overlap(arrays, 5, 9), "outputs overlap the inputs or one another");
+  PlanArgs a{past_lens, new_lens, free_pages, free_count, block_table, cu_seqlens, kv_lens, slot_map, status, B, n_free,
              num_pages, log2_of(page), max_pages, tokens, 0};
   a.slot_blocks = std::max(1, (int)(((int64_t)tokens + 4 * KV_NT - 1) / (4 * KV_NT)));
   // a request takes at most new / page + 1 pages
@@ -1094,6 +1056,14 @@ int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, c
   kv_plan_kernel<<<grid, KV_NT, (size_t)2 * (B + 1) * sizeof(int), reinterpret_cast<hipStream_t>(stream)>>>(a);
   MLCV_HIP(hipGetLastError());
   return 0;
+}
+
+int mlcv_kv_plan(const int32_t* past_lens, const int32_t* new_lens, int32_t B, const int32_t* free_pages,
+                 int32_t n_free, int32_t num_pages, int32_t page, int32_t* block_table, int32_t max_pages,
+                 int32_t* cu_seqlens, int32_t* kv_lens, int32_t* slot_map, int32_t tokens, int32_t* status,
+                 void* stream) {
+  return mlcv_kv_plan_counted(past_lens, new_lens, B, free_pages, n_free, nullptr, num_pages, page, block_table,
+                              max_pages, cu_seqlens, kv_lens, slot_map, tokens, status, stream);
 }
 
 int mlcv_kv_write(const void* k, int32_t k_dtype, int64_t k_tok, int64_t k_head, const void* v, int32_t v_dtype,

@@ -1,0 +1,537 @@
+// The pages of the paged key/value cache change hands: which ones no request holds (mlcv_kv_free), requests that go on
+// from another's tokens (mlcv_kv_fork), a pool made dense (mlcv_kv_compact), pages copied (mlcv_kv_copy).
+//
+// Nothing counts references: the pages in use are the ones that the block table's rows hold, and are found anew by each
+// call.  Shared pages need no bookkeeping then, and nothing can drift.  Two requests may share a page as long as
+// neither writes to it, which is so for pages that are full; a fork copies the one that is not.
+#include "kernels.h"
+#include "kv_args.h"
+#include "mlcvla.h"
+
+#include <algorithm>
+
+namespace mlcv {
+
+namespace {
+
+constexpr int MK_NT = 1024;   // threads of a workgroup that marks
+constexpr int LS_NT = 256;    // of one that lists
+constexpr int LS_BLOCK = 4096;  // pages that it lists: 64 groups of 64
+constexpr int CP_NT = 256;    // of one that copies
+constexpr int FK_NT = 256;    // of one that forks
+
+// ---- pages in use ------------------------------------------------------------------------------------
+
+struct MarkArgs {
+  const int32_t *table, *lens;
+  uint32_t* words;   // a bit for each page in use, whole slices
+  int32_t* counts;   // of the pages in use, per LS_BLOCK
+  int32_t B, max_pages, psh, num_pages, slice;
+};
+
+// Each workgroup reads the whole table and marks the pages of its slice in LDS: reading it over costs less than a pass that
+// clears a bitmap in memory before another sets bits in it by atomics.
+__global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a) {
+  extern __shared__ int dyn[];
+  __shared__ int most;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [slice / 32]
+  int* held = dyn + (a.slice >> 5);                   // [B] entries of each row in use
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (tid == 0) most = 0;
+  for (int i = tid; i < a.slice >> 5; i += MK_NT) bits[i] = 0u;
+  __syncthreads();
+  int mine = 0;
+  for (int b = tid; b < a.B; b += MK_NT) {
+    const int len = clamp_i(a.lens[b], 0, a.max_pages << a.psh), n = (int)(((int64_t)len + (1 << a.psh) - 1) >> a.psh);
+    held[b] = n;
+    mine = max(mine, n);
+  }
+  if (mine) atomicMax(&most, mine);
+  __syncthreads();
+  // items of 4 rows x 256 entries, 16 loads in flight per lane
+  const int p0 = (int)blockIdx.x * a.slice;
+  const int wide = (most + 255) >> 8, items = ((a.B + 3) >> 2) * wide;
+  for (int it = w; it < items; it += MK_NT / 64) {
+    const int b0 = it / wide * 4, j0 = (it % wide) * 256 + lane;
+    int id[16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int b = b0 + r, n = b < a.B ? held[b] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 64 * i;
+        id[4 * r + i] = j < n ? load_global(a.table + (int64_t)b * a.max_pages + j) : -1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t at = (uint32_t)id[i] - (uint32_t)p0;
+      if (id[i] >= 0 && id[i] < a.num_pages && at < (uint32_t)a.slice) atomicOr(&bits[at >> 5], 1u << (at & 31));
+    }
+  }
+  __syncthreads();
+  // 128 words of a block: two waves' lanes
+  for (int i = tid; i < a.slice >> 5; i += MK_NT) {
+    const uint32_t v = bits[i];
+    a.words[(size_t)blockIdx.x * (a.slice >> 5) + i] = v;
+    int n = __popc(v);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+    if (lane == 0) held[i >> 6] = n;  // the rows' numbers are not needed any more
+  }
+  __syncthreads();
+  for (int i = tid; i < a.slice / LS_BLOCK; i += MK_NT)
+    a.counts[(size_t)blockIdx.x * (a.slice / LS_BLOCK) + i] = held[2 * i] + held[2 * i + 1];
+}
+
+struct ListArgs {
+  const uint32_t* words;
+  const int32_t* counts;
+  int32_t num_pages, blocks;
+  int32_t *free_pages, *free_count;       // the free list, or
+  int32_t *to, *holes, *from, *status;    // a dense pool's moves: page from[r] goes to holes[r], to[from[r]] = r
+};
+
+// A workgroup lists the pages of one block.  With u(p) the pages in use before p: free page p is number p - u(p) of the
+// list; with `live` of them in all, a page in use from there on is move number u(p) - u(live), and a free one before it
+// hole number p - u(p).
+template <bool MOVES>
+__global__ __launch_bounds__(LS_NT) void list_kernel(const ListArgs a) {
+  __shared__ int before[LS_BLOCK / 64], sum[3];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, mine = blockIdx.x;
+  if (tid < 3) sum[tid] = 0;
+  __syncthreads();
+  int lower = 0, all = 0;
+  for (int i = tid; i < a.blocks; i += LS_NT) {
+    const int n = a.counts[i];
+    lower += i < mine ? n : 0;
+    all += n;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lower += __shfl_xor(lower, o);
+    all += __shfl_xor(all, o);
+  }
+  if (lane == 0) {
+    atomicAdd(&sum[0], lower);
+    atomicAdd(&sum[1], all);
+  }
+  const uint64_t* groups = reinterpret_cast<const uint64_t*>(a.words) + (size_t)mine * (LS_BLOCK / 64);
+  if (w == 0) {
+    int n = __popcll(groups[lane]), v = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(v, o);
+      if (lane >= o) v += u;
+    }
+    before[lane] = v - n;
+  }
+  __syncthreads();
+  const int base = sum[0], live = sum[1];
+  int used_low = 0;  // pages in use before page `live`
+  if constexpr (MOVES) {
+    const int lb = live / LS_BLOCK, lp = live % LS_BLOCK;
+    int n = 0;
+    for (int i = tid; i < lb; i += LS_NT) n += a.counts[i];
+    if (tid < LS_BLOCK / 64 && lb < a.blocks) {
+      const uint64_t g = reinterpret_cast<const uint64_t*>(a.words)[(size_t)lb * (LS_BLOCK / 64) + tid];
+      const int cut = clamp_i(lp - 64 * tid, 0, 64);
+      n += __popcll(cut == 64 ? g : g & ((1ull << cut) - 1));
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+    if (lane == 0) atomicAdd(&sum[2], n);
+    __syncthreads();
+    used_low = sum[2];
+  }
+#pragma unroll 4
+  for (int q = w; q < LS_BLOCK / 64; q += LS_NT / 64) {
+    const int p = mine * LS_BLOCK + 64 * q + lane;
+    if (p >= a.num_pages) continue;
+    const uint64_t g = groups[q];
+    const bool used = (g >> lane) & 1;
+    const int u = base + before[q] +
+                  (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(g >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)g, 0));
+    if constexpr (MOVES) {
+      if (used && p >= live) {
+        a.from[u - used_low] = p;
+        a.to[p] = u - used_low;
+      }
+      if (!used && p < live) a.holes[p - u] = p;
+    } else {
+      if (!used) a.free_pages[p - u] = p;
+      if (p >= a.num_pages - live) a.free_pages[p] = -1;
+    }
+  }
+  if (mine == 0 && tid == 0) {
+    if constexpr (MOVES) {
+      a.status[0] = live;
+      a.status[1] = live - used_low;
+    } else {
+      *a.free_count = a.num_pages - live;
+    }
+  }
+}
+
+// Slices of the pages, one for each workgroup that marks: blocks of 4096 pages, more where there would be over 1024 of them
+int mark_slice(int num_pages) {
+  const int64_t blocks = std::max<int64_t>(1, ((int64_t)num_pages + LS_BLOCK - 1) / LS_BLOCK);
+  return (int)((blocks + 1023) / 1024) * LS_BLOCK;
+}
+struct MarkSizes {
+  int slice, slices, blocks;
+  size_t words, counts;  // ints
+};
+MarkSizes mark_sizes(int num_pages) {
+  MarkSizes m;
+  m.slice = mark_slice(num_pages);
+  m.slices = std::max(1, (int)(((int64_t)num_pages + m.slice - 1) / m.slice));
+  m.blocks = m.slices * (m.slice / LS_BLOCK);
+  m.words = (size_t)m.slices * (m.slice / 32);
+  m.counts = ((size_t)m.blocks + 3) / 4 * 4;
+  return m;
+}
+int mark_launch(const int32_t* table, const int32_t* lens, int B, int max_pages, int page, int num_pages,
+                const MarkSizes& m, uint32_t* words, int32_t* counts, hipStream_t st) {
+  const MarkArgs a{table, lens, words, counts, B, max_pages, log2_of(page), num_pages, m.slice};
+  const size_t lds = (size_t)(m.slice / 32 + std::max(B, m.slice / 2048)) * 4;
+  mark_kernel<<<(unsigned)m.slices, MK_NT, lds, st>>>(a);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+// ---- copying -----------------------------------------------------------------------------------------
+
+struct Pool {
+  uint8_t* data[2];  // keys, values [layers][pages][page_bytes]
+  float* scale[2];   // [layers][pages][KV]
+  int32_t pages;
+};
+struct CopyArgs {
+  Pool from, into;
+  const int32_t *src, *dst, *count;  // count: how many of them there are (null: most)
+  int32_t most, layers, KV, page_bytes, pieces;
+};
+constexpr int CP_PIECE = 8192;  // bytes that a wave moves at a time: 8 loads of 16 per lane
+
+// Units of one page, layer, side and piece; a wave takes one after another.
+__device__ __forceinline__ void copy_pages(const CopyArgs& a, long long unit, long long step) {
+  const int lane = threadIdx.x & 63;
+  const int n = a.count ? clamp_i(*a.count, 0, a.most) : a.most;
+  const int per = a.layers * 2 * a.pieces;
+  const long long units = (long long)n * per;
+  for (; unit < units; unit += step) {
+    const int i = (int)(unit / per), rest = (int)(unit - (long long)i * per);
+    const int piece = rest % a.pieces, z = (rest / a.pieces) & 1, y = rest / a.pieces >> 1;
+    const int s = a.src[i], d = a.dst[i];
+    if (s < 0 || s >= a.from.pages || d < 0 || d >= a.into.pages) continue;
+    const long long ps = (long long)y * a.from.pages + s, pd = (long long)y * a.into.pages + d;
+    const u4* p = reinterpret_cast<const u4*>(a.from.data[z] + ps * a.page_bytes + piece * CP_PIECE) + lane;
+    u4* q = reinterpret_cast<u4*>(a.into.data[z] + pd * a.page_bytes + piece * CP_PIECE) + lane;
+    const int left = min(CP_PIECE, a.page_bytes - piece * CP_PIECE) / 16 - lane;
+    u4 v[CP_PIECE / 1024];
+#pragma unroll
+    for (int k = 0; k < CP_PIECE / 1024; ++k)
+      if (64 * k < left) v[k] = load_global(p + 64 * k);
+#pragma unroll
+    for (int k = 0; k < CP_PIECE / 1024; ++k)
+      if (64 * k < left) q[64 * k] = v[k];
+    if (piece == 0)
+      for (int h = lane; h < a.KV; h += 64) a.into.scale[z][pd * a.KV + h] = a.from.scale[z][ps * a.KV + h];
+  }
+}
+
+__global__ __launch_bounds__(CP_NT) void copy_kernel(const CopyArgs a) {
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  copy_pages(a, (long long)blockIdx.x * (CP_NT / 64) + w, (long long)gridDim.x * (CP_NT / 64));
+}
+
+struct RenameArgs {
+  const int32_t *table, *lens, *to, *holes, *status;
+  int32_t* out;
+  int32_t B, max_pages, psh, num_pages, groups;
+};
+// The moves of a dense pool, and in the first `groups` workgroups the table's new page numbers: a row each, in turn
+__global__ __launch_bounds__(CP_NT) void move_kernel(const CopyArgs a, const RenameArgs t) {
+  if ((int)blockIdx.x >= t.groups) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    copy_pages(a, (long long)(blockIdx.x - t.groups) * (CP_NT / 64) + w, (long long)(gridDim.x - t.groups) * (CP_NT / 64));
+    return;
+  }
+  const int live = t.status[0];
+  for (int b = blockIdx.x; b < t.B; b += t.groups) {
+    const int len = clamp_i(t.lens[b], 0, t.max_pages << t.psh), n = (int)(((int64_t)len + (1 << t.psh) - 1) >> t.psh);
+    for (int j = threadIdx.x; j < t.max_pages; j += CP_NT) {
+      const int64_t at = (int64_t)b * t.max_pages + j;
+      int id = t.table[at];
+      if (j < n && id >= live && id < t.num_pages) id = t.holes[t.to[id]];
+      t.out[at] = id;
+    }
+  }
+}
+
+// workgroups for `most` pages: as many as the GPU holds at once, or fewer
+unsigned copy_groups(const CopyArgs& a) {
+  const int64_t units = (int64_t)a.most * a.layers * 2 * a.pieces;
+  return (unsigned)std::min<int64_t>((units + CP_NT / 64 - 1) / (CP_NT / 64), 2048);
+}
+
+// ---- forks -------------------------------------------------------------------------------------------
+
+struct ForkArgs {
+  const int32_t *parents, *table, *lens, *free_pages, *free_count;
+  int32_t *out, *out_lens, *status, *src, *dst;
+  int32_t N, B, max_pages, psh, n_free;
+};
+
+// Row i of the new table goes on from row parents[i].  The first of a parent's rows keeps its last page, if that is not
+// full; the others take a free one each, in their order.  Every workgroup finds this out for all rows (as the
+// plan's do), then writes its own.
+__global__ __launch_bounds__(FK_NT) void fork_kernel(const ForkArgs a) {
+  extern __shared__ int sm[];
+  __shared__ long long part[FK_NT / 64], carry;
+  __shared__ int lost;
+  int* first = sm;        // [B] the first row of each parent
+  int* fresh = sm + a.B;  // [N] number of the free page that a row takes; -1: none; -2: refused
+  const int tid = threadIdx.x, lane = tid & 63, page = 1 << a.psh;
+  const int n_free = a.free_count ? clamp_i(*a.free_count, 0, a.n_free) : a.n_free;
+  for (int b = tid; b < a.B; b += FK_NT) first[b] = INT32_MAX;
+  if (tid == 0) lost = 0;
+  __syncthreads();
+  for (int i = tid; i < a.N; i += FK_NT) {
+    const int p = a.parents[i];
+    if (p >= 0 && p < a.B) atomicMin(&first[p], i);
+  }
+  __syncthreads();
+  long long taken = 0;
+  int refused = 0;
+  for (int i0 = 0; i0 < a.N; i0 += FK_NT) {
+    const int i = i0 + tid, p = i < a.N ? a.parents[i] : -1;
+    const bool there = p >= 0 && p < a.B;
+    const int len = there ? clamp_i(a.lens[p], 0, a.max_pages << a.psh) : 0;
+    const bool need = there && (len & (page - 1)) && first[p] != i;
+    const long long end = block_scan<FK_NT>(need, part) + taken;
+    const bool ok = !need || end <= n_free;
+    refused += !ok;
+    if (i < a.N) fresh[i] = !ok ? -2 : need ? (int)end - 1 : -1;
+    if (blockIdx.x == 0 && i < a.N) {
+      a.out_lens[i] = ok ? len : 0;
+      if (need && ok) {
+        a.src[end - 1] = a.table[(int64_t)p * a.max_pages + (len >> a.psh)];
+        a.dst[end - 1] = a.free_pages[end - 1];
+      }
+    }
+    if (tid == FK_NT - 1) carry = end;
+    __syncthreads();
+    taken = carry;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0) {
+    if (refused) atomicAdd(&lost, refused);
+    __syncthreads();
+    if (tid == 0) {
+      a.status[0] = (int)(taken < n_free ? taken : n_free);
+      a.status[1] = lost;
+    }
+  }
+  // a wave for each row
+  for (int i = blockIdx.x * (FK_NT / 64) + (tid >> 6); i < a.N; i += gridDim.x * (FK_NT / 64)) {
+    const int p = a.parents[i], f = fresh[i];
+    const bool there = p >= 0 && p < a.B && f != -2;
+    const int len = there ? clamp_i(a.lens[p], 0, a.max_pages << a.psh) : 0;
+    const int n = (int)(((int64_t)len + page - 1) >> a.psh);
+    for (int j = lane; j < a.max_pages; j += 64) {
+      int id = j < n ? a.table[(int64_t)p * a.max_pages + j] : -1;
+      if (f >= 0 && j == n - 1) id = a.free_pages[f];
+      a.out[(int64_t)i * a.max_pages + j] = id;
+    }
+  }
+}
+
+int pages_ok(int32_t num_pages, int32_t page, int32_t max_pages, int32_t B) {
+  MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
+  MLCV_REQUIRE(num_pages >= 0 && max_pages >= 0 && B >= 0, "negative size");
+  MLCV_REQUIRE((int64_t)num_pages * page <= KV_MOST && (int64_t)max_pages * page <= KV_MOST,
+               "more than 2^31 - 256 slots");
+  MLCV_REQUIRE(B <= KV_MAX_REQ, "more than 4096 requests");
+  return 0;
+}
+
+// The copying part of a call; `a`'s lists are the caller's
+int pool_ok(CopyArgs& a, void* k, float* ks, void* v, float* vs, int32_t num_pages, void* k2, float* ks2, void* v2,
+            float* vs2, int32_t num_pages2, int32_t layers, int32_t page, int32_t KV, int32_t hd) {
+  MLCV_REQUIRE(kv_page_ok(page), "page must be 16, 32, 64 or 128");
+  MLCV_REQUIRE(kv_hd_ok(hd), "head_dim must be 64, 128 or 256");
+  MLCV_REQUIRE(layers > 0 && layers <= 65535 && KV > 0 && KV <= 65535, "layers and kv heads must be 1 to 65535");
+  MLCV_REQUIRE((num_pages == 0 || (k && ks && v && vs)) && (num_pages2 == 0 || (k2 && ks2 && v2 && vs2)), "null cache");
+  MLCV_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k2) && aligned16(v2), "the cache must be 16-byte aligned");
+  a.from = Pool{{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v)}, {ks, vs}, num_pages};
+  a.into = Pool{{static_cast<uint8_t*>(k2), static_cast<uint8_t*>(v2)}, {ks2, vs2}, num_pages2};
+  MLCV_REQUIRE((int64_t)KV * page * hd <= 1 << 30, "a page of more than 2^30 bytes");
+  a.layers = layers;
+  a.KV = KV;
+  a.page_bytes = KV * page * hd;
+  a.pieces = (a.page_bytes + CP_PIECE - 1) / CP_PIECE;
+  MLCV_REQUIRE((int64_t)a.layers * 2 * a.pieces <= INT32_MAX, "too many layers and heads");
+  return 0;
+}
+
+size_t compact_ints(int32_t num_pages) {
+  const MarkSizes m = mark_sizes(num_pages);
+  return m.words + m.counts + 3 * (size_t)num_pages;
+}
+
+}  // namespace
+}  // namespace mlcv
+
+using namespace mlcv;
+
+extern "C" {
+
+int mlcv_kv_free_workspace(int32_t num_pages, size_t* bytes) {
+  MLCV_REQUIRE(bytes, "null pointer");
+  MLCV_REQUIRE(num_pages >= 0 && num_pages <= KV_MOST / 16, "bad num_pages");
+  const MarkSizes m = mark_sizes(num_pages);
+  *bytes = (m.words + m.counts) * 4;
+  return 0;
+}
+
+int mlcv_kv_free(const int32_t* block_table, int32_t B, int32_t max_pages, const int32_t* kv_lens, int32_t num_pages,
+                 int32_t page, int32_t* free_pages, int32_t* free_count, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  MLCV_TRY(pages_ok(num_pages, page, max_pages, B));
+  MLCV_REQUIRE(free_count && (num_pages == 0 || free_pages), "null output");
+  MLCV_REQUIRE(B == 0 || (kv_lens && (block_table || max_pages == 0)), "null request array");
+  const MarkSizes m = mark_sizes(num_pages);
+  MLCV_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= (m.words + m.counts) * 4,
+               "workspace missing, not 16-byte aligned or too small");
+  const Ints arrays[] = {{free_pages, num_pages}, {free_count, 1}, {workspace, (int64_t)(m.words + m.counts)},
+                         {block_table, (int64_t)B * max_pages}, {kv_lens, B}};
+  MLCV_REQUIRE(!overlap(arrays, 3, 5), "outputs overlap the inputs or one another");
+  uint32_t* words = static_cast<uint32_t*>(workspace);
+  int32_t* counts = reinterpret_cast<int32_t*>(words + m.words);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  MLCV_TRY(mark_launch(block_table, kv_lens, B, max_pages, page, num_pages, m, words, counts, st));
+  ListArgs l{};
+  l.words = words;
+  l.counts = counts;
+  l.num_pages = num_pages;
+  l.blocks = m.blocks;
+  l.free_pages = free_pages;
+  l.free_count = free_count;
+  list_kernel<false><<<(unsigned)m.blocks, LS_NT, 0, st>>>(l);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+int mlcv_kv_copy(const int32_t* src, const int32_t* dst, int32_t n, void* k_cache, float* k_scale, void* v_cache,
+                 float* v_scale, int32_t num_pages, void* k_into, float* k_scale_into, void* v_into,
+                 float* v_scale_into, int32_t pages_into, int32_t layers, int32_t page, int32_t KV, int32_t hd,
+                 void* stream) {
+  MLCV_REQUIRE(n >= 0, "negative size");
+  MLCV_TRY(pages_ok(num_pages, page, 0, 0));
+  MLCV_TRY(pages_ok(pages_into, page, 0, 0));
+  CopyArgs a{};
+  MLCV_TRY(pool_ok(a, k_cache, k_scale, v_cache, v_scale, num_pages, k_into, k_scale_into, v_into, v_scale_into,
+                   pages_into, layers, page, KV, hd));
+  if (n == 0 || num_pages == 0 || pages_into == 0) return 0;
+  MLCV_REQUIRE(src && dst, "null pointer");
+  a.src = src;
+  a.dst = dst;
+  a.most = n;
+  copy_kernel<<<copy_groups(a), CP_NT, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, int32_t B, int32_t max_pages,
+                 const int32_t* kv_lens, const int32_t* free_pages, int32_t n_free, const int32_t* free_count,
+                 void* k_cache, float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages,
+                 int32_t page, int32_t KV, int32_t hd, int32_t* new_table, int32_t* new_lens, int32_t* status,
+                 int32_t* copies, void* stream) {
+  MLCV_TRY(pages_ok(num_pages, page, max_pages, B));
+  MLCV_REQUIRE(n >= 0 && n_free >= 0, "negative size");
+  MLCV_REQUIRE(n <= KV_MAX_REQ, "more than 4096 requests");
+  CopyArgs a{};
+  MLCV_TRY(pool_ok(a, k_cache, k_scale, v_cache, v_scale, num_pages, k_cache, k_scale, v_cache, v_scale, num_pages,
+                   layers, page, KV, hd));
+  MLCV_REQUIRE(status, "null output");
+  MLCV_REQUIRE(n == 0 || (parents && new_lens && copies && (new_table || max_pages == 0)), "null row array");
+  MLCV_REQUIRE(B == 0 || (kv_lens && (block_table || max_pages == 0)), "null request array");
+  MLCV_REQUIRE(n_free == 0 || free_pages, "null free_pages");
+  const Ints arrays[] = {{new_table, (int64_t)n * max_pages}, {new_lens, n}, {status, 2}, {copies, 2 * (int64_t)n},
+                         {parents, n}, {block_table, (int64_t)B * max_pages}, {kv_lens, B}, {free_pages, n_free},
+                         {free_count, free_count ? 1 : 0}};
+  MLCV_REQUIRE(!overlap(arrays, 4, 9), "outputs overlap the inputs or one another");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const ForkArgs f{parents, block_table, kv_lens, free_pages, free_count, new_table, new_lens, status, copies,
+                   copies + n, n, B, max_pages, log2_of(page), n_free};
+  const unsigned grid = (unsigned)std::max(1, std::min((n + FK_NT / 64 - 1) / (FK_NT / 64), 256));
+  fork_kernel<<<grid, FK_NT, (size_t)(B + n) * 4, st>>>(f);
+  MLCV_HIP(hipGetLastError());
+  a.src = copies;
+  a.dst = copies + n;
+  a.count = status;
+  a.most = std::min(n, n_free);
+  if (a.most == 0 || num_pages == 0) return 0;
+  copy_kernel<<<copy_groups(a), CP_NT, 0, st>>>(a);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+int mlcv_kv_compact_workspace(int32_t num_pages, size_t* bytes) {
+  MLCV_REQUIRE(bytes, "null pointer");
+  MLCV_REQUIRE(num_pages >= 0 && num_pages <= KV_MOST / 16, "bad num_pages");
+  *bytes = compact_ints(num_pages) * 4;
+  return 0;
+}
+
+int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, const int32_t* kv_lens, void* k_cache,
+                    float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages, int32_t page,
+                    int32_t KV, int32_t hd, int32_t* new_table, int32_t* status, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  MLCV_TRY(pages_ok(num_pages, page, max_pages, B));
+  CopyArgs a{};
+  MLCV_TRY(pool_ok(a, k_cache, k_scale, v_cache, v_scale, num_pages, k_cache, k_scale, v_cache, v_scale, num_pages,
+                   layers, page, KV, hd));
+  MLCV_REQUIRE(status, "null output");
+  MLCV_REQUIRE(B == 0 || (kv_lens && ((block_table && new_table) || max_pages == 0)), "null request array");
+  const size_t ints = compact_ints(num_pages);
+  MLCV_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= ints * 4,
+               "workspace missing, not 16-byte aligned or too small");
+  // the table may become the new one in place
+  const int64_t entries = (int64_t)B * max_pages;
+  const Ints arrays[] = {{new_table, entries}, {status, 2}, {workspace, (int64_t)ints}, {kv_lens, B},
+                         {block_table, new_table == block_table ? 0 : entries}};
+  MLCV_REQUIRE(!overlap(arrays, 3, 5), "outputs overlap the inputs or one another");
+  const MarkSizes m = mark_sizes(num_pages);
+  uint32_t* words = static_cast<uint32_t*>(workspace);
+  int32_t* counts = reinterpret_cast<int32_t*>(words + m.words);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  MLCV_TRY(mark_launch(block_table, kv_lens, B, max_pages, page, num_pages, m, words, counts, st));
+  ListArgs l{};
+  l.words = words;
+  l.counts = counts;
+  l.num_pages = num_pages;
+  l.blocks = m.blocks;
+  l.to = counts + m.counts;
+  l.holes = l.to + num_pages;
+  l.from = l.holes + num_pages;
+  l.status = status;
+  list_kernel<true><<<(unsigned)m.blocks, LS_NT, 0, st>>>(l);
+  MLCV_HIP(hipGetLastError());
+  a.src = l.from;
+  a.dst = l.holes;
+  a.count = status + 1;
+  // every move has a hole: at most half of the pages move
+  a.most = num_pages / 2;
+  const RenameArgs t{block_table, kv_lens, l.to, l.holes, status, new_table, B, max_pages, log2_of(page), num_pages,
+                     std::min(B, 256)};
+  const unsigned grid = t.groups + (a.most ? copy_groups(a) : 0);
+  if (grid == 0) return 0;
+  move_kernel<<<grid, CP_NT, 0, st>>>(a, t);
+  MLCV_HIP(hipGetLastError());
+  return 0;
+}
+
+}  // extern "C"

@@ -9,6 +9,8 @@ length stays on the device: nothing here synchronizes, so a serving step can be 
     out = prompt_attention(q, k, v, plan.cu_seqlens)                                # a prompt's own attention
     cache.write(k, v, plan, layer)                                                  # into the pages
     out = cache.attention(q, plan, table, layer)                                    # later tokens
+    free = cache.free(table, lens)                                                  # pages that no request holds
+    fork = cache.fork(parents, table, lens, *free)                                  # beams: who goes on from whom
 
 Every function body is one call into ``libmlcvla_hip.so`` (include/mlcvla.h says what each computes);
 tensors are ``runtime.Tensor`` or torch tensors on one HIP device, on whose current stream the work runs.
@@ -40,6 +42,28 @@ class KVPlan(NamedTuple):
     kv_lens: Tensor     # [B] cached tokens after the new ones are written; 0: the request was refused
     slot_map: Tensor    # [tokens] slot of each new token, -1: none
     status: Tensor      # [2] pages taken from the front of the free list; requests refused
+
+
+class KVFree(NamedTuple):
+    """What ``kv_free`` made: see mlcv_kv_free."""
+
+    free_pages: Tensor  # [num_pages] the free pages, ascending, then -1
+    free_count: Tensor  # [1] how many there are
+
+
+class KVFork(NamedTuple):
+    """What ``kv_fork`` made: see mlcv_kv_fork."""
+
+    block_table: Tensor  # [N, max_pages]
+    kv_lens: Tensor      # [N]; 0: the row was refused, or its parent is none
+    status: Tensor       # [2] pages taken from the front of the free list; rows refused
+
+
+class KVCompact(NamedTuple):
+    """What ``kv_compact`` made: see mlcv_kv_compact."""
+
+    block_table: Tensor  # [B, max_pages] with the pages' new numbers
+    status: Tensor       # [2] pages in use, now the first of the pool; pages moved
 
 
 # A call's checks take longer than the kernels of its smallest sizes: each function first looks at everything it
@@ -111,12 +135,22 @@ def _given(fn: str, out, q: torch.Tensor, dev: int) -> torch.Tensor:
     return o
 
 
+def _count(fn: str, free_count, dev: int) -> Optional[int]:
+    if free_count is None:
+        return None
+    c = _t(free_count)
+    if not (c.dtype is _I32 and c.shape == (1,) and c.get_device() == dev):
+        _refuse(fn, dev, (("free_count", c, (_I32,), (1,), True),))
+    return c.data_ptr()
+
+
 def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, page_size: int, tokens: int,
-            out: Optional[KVPlan] = None) -> KVPlan:
+            free_count=None, out: Optional[KVPlan] = None) -> KVPlan:
     """Block tables and slot maps from request lengths (mlcv_kv_plan).
 
     past_lens, new_lens [B], block_table [B, max_pages] (its new entries are written), free_pages [F], all int32;
-    ``tokens``: the packed tokens of the call.  ``out``: a plan of the same sizes to write into; not the one whose
+    ``tokens``: the packed tokens of the call.  ``free_count`` [1] int32: how many of free_pages are free, as ``kv_free``
+    leaves it (mlcv_kv_plan_counted; default: all).  ``out``: a plan of the same sizes to write into; not the one whose
     ``kv_lens`` are the call's past_lens (two plans in turn do)."""
     past, new, table, free = _t(past_lens), _t(new_lens), _t(block_table), _t(free_pages)
     dev = past.get_device()
@@ -144,9 +178,9 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
                         for t in (cu, lens, slots, status))):
             _refuse("kv_plan", dev, tuple(("out." + f, t, (_I32,), (k,), True) for f, t, k in
                                           zip(KVPlan._fields, (cu, lens, slots, status), (n + 1, n, tokens, 2))))
-    _call("mlcv_kv_plan", dev, past.data_ptr(), new.data_ptr(), n, free.data_ptr(), free.shape[0], num_pages,
-          page_size, table.data_ptr(), wide, cu.data_ptr(), lens.data_ptr(), slots.data_ptr(), tokens,
-          status.data_ptr())
+    _call("mlcv_kv_plan_counted", dev, past.data_ptr(), new.data_ptr(), n, free.data_ptr(), free.shape[0],
+          _count("kv_plan", free_count, dev), num_pages, page_size, table.data_ptr(), wide, cu.data_ptr(),
+          lens.data_ptr(), slots.data_ptr(), tokens, status.data_ptr())
     return out
 
 
@@ -338,6 +372,151 @@ def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, bidir=None, sc
     return Tensor(o, name)
 
 
+def _pool(fn: str, k, k_scale, v, v_scale):
+    """The four tensors of a cache, of one layer or (with one more dim in front) several, and (device, layers, pages, KV,
+    page, hd)."""
+    c = tuple(_t(x) for x in (k, k_scale, v, v_scale))
+    kc, ks, vc, vs = c
+    dev, shape = kc.get_device(), tuple(kc.shape)
+    size = (1,) + shape if len(shape) == 4 else shape if len(shape) == 5 else (-1,) * 5
+    pages, kv, page, hd = size[1:]
+    top = shape[:-2]
+    if not (kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and size[0] >= 0
+            and vc.shape == top + (hd, page) and ks.shape == top and vs.shape == top and kc.is_contiguous()
+            and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and dev >= 0 and ks.get_device() == vc.get_device() == vs.get_device() == dev):
+        _refuse(fn, dev, (("k_cache", kc, (_F8,), shape if len(shape) == 5 else (None,) * 4, True),
+                          ("k_scale", ks, (_F32,), top, True), ("v_cache", vc, (_F8,), top + (hd, page), True),
+                          ("v_scale", vs, (_F32,), top, True)))
+    return c, (dev,) + size
+
+
+def _rows(fn: str, block_table, kv_lens, dev: int):
+    """(table, lengths, rows, entries of a row)"""
+    table, lens = _t(block_table), _t(kv_lens)
+    n, wide = table.shape if table.dim() == 2 else (-1, 0)
+    if not (table.dtype is _I32 and lens.dtype is _I32 and lens.shape == (n,) and table.is_contiguous()
+            and lens.is_contiguous() and dev >= 0 and table.get_device() == lens.get_device() == dev):
+        b = table.shape[0] if table.dim() else None
+        _refuse(fn, dev, (("block_table", table, (_I32,), (None, None), True), ("kv_lens", lens, (_I32,), (b,), True)))
+    return table, lens, n, wide
+
+
+def _outs(fn: str, dev: int, out, shapes):
+    """The tensors of ``out`` (a named tuple) checked for their shapes."""
+    ts = tuple(_t(x) for x in out)
+    if len(ts) != len(shapes):
+        _bad(fn, "out", f"is not {len(shapes)} tensors")
+    for name, t, s in zip(out._fields, ts, shapes):
+        if not (t.dtype is _I32 and t.shape == s and t.is_contiguous() and t.get_device() == dev):
+            _refuse(fn, dev, (("out." + name, t, (_I32,), s, True),))
+    return ts
+
+
+@functools.lru_cache(maxsize=256)
+def _pages_workspace(name: str, num_pages: int) -> int:
+    n = ctypes.c_size_t()
+    N.call(name, num_pages, ctypes.byref(n))
+    return n.value
+
+
+def kv_free_workspace(num_pages: int) -> int:
+    """Bytes of workspace of ``kv_free`` (mlcv_kv_free_workspace)."""
+    return _pages_workspace("mlcv_kv_free_workspace", num_pages)
+
+
+def kv_compact_workspace(num_pages: int) -> int:
+    """Bytes of workspace of ``kv_compact`` (mlcv_kv_compact_workspace)."""
+    return _pages_workspace("mlcv_kv_compact_workspace", num_pages)
+
+
+def _space(fn: str, workspace, size: int, like: torch.Tensor, dev: int):
+    if workspace is None:
+        return torch.empty(size, dtype=_U8, device=like.device), size
+    w = _t(workspace)
+    if not (w.dtype is _U8 and w.is_contiguous() and w.get_device() == dev):
+        _refuse(fn, dev, (("workspace", w, (_U8,), (None,), True),))
+    return w, w.numel()
+
+
+def kv_free(block_table, kv_lens, *, num_pages: int, page_size: int, out: Optional[KVFree] = None,
+            workspace=None) -> KVFree:
+    """The pages that no row of block_table [B, max_pages] holds, as the free list of the next plan or fork
+    (mlcv_kv_free).  A finished request's length is 0; one that a plan refused still has its old length."""
+    dev = _t(block_table).get_device()
+    table, lens, n, wide = _rows("kv_free", block_table, kv_lens, dev)
+    if not 0 <= num_pages < 1 << 27:
+        _bad("kv_free", "num_pages", "is negative or past 2^27 - 1")
+    if out is None:
+        pages, count = torch.empty(num_pages + 1, dtype=_I32, device=table.device).split((num_pages, 1))
+        out = KVFree(Tensor(pages, "int32"), Tensor(count, "int32"))
+    else:
+        pages, count = _outs("kv_free", dev, out, ((num_pages,), (1,)))
+    ws, size = _space("kv_free", workspace, kv_free_workspace(num_pages), table, dev)
+    _call("mlcv_kv_free", dev, table.data_ptr(), n, wide, lens.data_ptr(), num_pages, page_size, pages.data_ptr(),
+          count.data_ptr(), ws.data_ptr(), size)
+    return out
+
+
+def kv_copy(src, dst, k_cache, k_scale, v_cache, v_scale, *, into=None) -> None:
+    """Copy pages src [n] to pages dst [n] (int32), in all layers, within a cache or ``into`` the four tensors of another
+    (mlcv_kv_copy).  Caches of one layer [pages, KV, page, hd] or of all [layers, pages, KV, page, hd]."""
+    cache, (dev, layers, pages, kv, page, hd) = _pool("kv_copy", k_cache, k_scale, v_cache, v_scale)
+    to, size = (cache, None) if into is None else _pool("kv_copy", *into)
+    if size is not None and (size[:2] != (dev, layers) or size[3:] != (kv, page, hd)):
+        _bad("kv_copy", "into", "is a cache of other layers, heads or pages")
+    s, d = _t(src), _t(dst)
+    n = s.shape[0] if s.dim() == 1 else -1
+    if not (s.dtype is _I32 and d.dtype is _I32 and d.shape == (n,) and s.is_contiguous() and d.is_contiguous()
+            and s.get_device() == d.get_device() == dev):
+        _refuse("kv_copy", dev, (("src", s, (_I32,), (None,), True), ("dst", d, (_I32,), (n,), True)))
+    _call("mlcv_kv_copy", dev, s.data_ptr(), d.data_ptr(), n, *(t.data_ptr() for t in cache), pages,
+          *(t.data_ptr() for t in to), pages if size is None else size[2], layers, page, kv, hd)
+
+
+def kv_fork(parents, block_table, kv_lens, free_pages, k_cache, k_scale, v_cache, v_scale, *, free_count=None,
+            out: Optional[KVFork] = None) -> KVFork:
+    """Rows that go on from the requests ``parents`` [N] int32 of block_table [B, max_pages] (mlcv_kv_fork): beams,
+    samples of one prompt.  Full pages are shared; of a last page that is not full all rows but the first of its parent get a
+    copy, on pages from the front of ``free_pages``, of which ``free_count`` [1] are free (default: all).  The old table
+    is done with; a request that stays beside its forks is a row of its own."""
+    cache, (dev, layers, pages, kv, page, hd) = _pool("kv_fork", k_cache, k_scale, v_cache, v_scale)
+    table, lens, b, wide = _rows("kv_fork", block_table, kv_lens, dev)
+    p, free = _t(parents), _t(free_pages)
+    if not (p.dtype is _I32 and free.dtype is _I32 and p.dim() == 1 and free.dim() == 1 and p.is_contiguous()
+            and free.is_contiguous() and p.get_device() == free.get_device() == dev):
+        _refuse("kv_fork", dev, (("parents", p, (_I32,), (None,), True), ("free_pages", free, (_I32,), (None,), True)))
+    n = p.shape[0]
+    if out is None:
+        t, m, status, copies = torch.empty(n * wide + 3 * n + 2, dtype=_I32, device=table.device).split(
+            (n * wide, n, 2, 2 * n))
+        out = KVFork(Tensor(t.view(n, wide), "int32"), Tensor(m, "int32"), Tensor(status, "int32"))
+    else:
+        t, m, status = _outs("kv_fork", dev, out, ((n, wide), (n,), (2,)))
+        copies = torch.empty(2 * n, dtype=_I32, device=table.device)
+    _call("mlcv_kv_fork", dev, p.data_ptr(), n, table.data_ptr(), b, wide, lens.data_ptr(), free.data_ptr(),
+          free.shape[0], _count("kv_fork", free_count, dev), *(x.data_ptr() for x in cache), layers, pages, page, kv, hd,
+          t.data_ptr(), m.data_ptr(), status.data_ptr(), copies.data_ptr())
+    return out
+
+
+def kv_compact(block_table, kv_lens, k_cache, k_scale, v_cache, v_scale, *, out: Optional[KVCompact] = None,
+               workspace=None) -> KVCompact:
+    """Move the pages in use to the front of the pool, in all layers (mlcv_kv_compact); ``out``: its block table may be
+    the given one."""
+    cache, (dev, layers, pages, kv, page, hd) = _pool("kv_compact", k_cache, k_scale, v_cache, v_scale)
+    table, lens, n, wide = _rows("kv_compact", block_table, kv_lens, dev)
+    if out is None:
+        t, status = torch.empty(n * wide + 2, dtype=_I32, device=table.device).split((n * wide, 2))
+        out = KVCompact(Tensor(t.view(n, wide), "int32"), Tensor(status, "int32"))
+    else:
+        t, status = _outs("kv_compact", dev, out, ((n, wide), (2,)))
+    ws, size = _space("kv_compact", workspace, kv_compact_workspace(pages), table, dev)
+    _call("mlcv_kv_compact", dev, table.data_ptr(), n, wide, lens.data_ptr(), *(x.data_ptr() for x in cache), layers,
+          pages, page, kv, hd, t.data_ptr(), status.data_ptr(), ws.data_ptr(), size)
+    return out
+
+
 class PagedKVCache:
     """The pages of every layer of a model: ``num_pages`` pages of ``page_size`` tokens (16, 32, 64 or 128) in
     float8_e4m3fn with their scales.  A block table's page numbers are the same in every layer."""
@@ -358,9 +537,26 @@ class PagedKVCache:
         """(k_cache, k_scale, v_cache, v_scale) of one layer."""
         return self.k[layer], self.k_scale[layer], self.v[layer], self.v_scale[layer]
 
-    def plan(self, past_lens, new_lens, block_table, free_pages, tokens: int, out: Optional[KVPlan] = None) -> KVPlan:
+    def all_layers(self):
+        """(k_cache, k_scale, v_cache, v_scale) of all layers, each with a dim of layers in front."""
+        return self.k, self.k_scale, self.v, self.v_scale
+
+    def plan(self, past_lens, new_lens, block_table, free_pages, tokens: int, out: Optional[KVPlan] = None,
+             free_count=None) -> KVPlan:
         return kv_plan(past_lens, new_lens, block_table, free_pages, num_pages=self.num_pages,
-                       page_size=self.page_size, tokens=tokens, out=out)
+                       page_size=self.page_size, tokens=tokens, free_count=free_count, out=out)
+
+    def free(self, block_table, kv_lens, **options) -> KVFree:
+        return kv_free(block_table, kv_lens, num_pages=self.num_pages, page_size=self.page_size, **options)
+
+    def fork(self, parents, block_table, kv_lens, free_pages, free_count=None, **options) -> KVFork:
+        return kv_fork(parents, block_table, kv_lens, free_pages, *self.all_layers(), free_count=free_count, **options)
+
+    def compact(self, block_table, kv_lens, **options) -> KVCompact:
+        return kv_compact(block_table, kv_lens, *self.all_layers(), **options)
+
+    def copy(self, src, dst, into: Optional["PagedKVCache"] = None) -> None:
+        kv_copy(src, dst, *self.all_layers(), into=None if into is None else into.all_layers())
 
     def write(self, k, v, plan: KVPlan, layer: int = 0) -> None:
         kv_write(k, v, plan.cu_seqlens, plan.slot_map, *self.pages(layer))

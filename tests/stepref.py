@@ -94,3 +94,53 @@ def logprobs_bound(x, scale, vocab):
     rel = (2 * w + 2 + chain + 8) * E32           # of s, and of u
     base = 1.1 * (rel + 2 * E32 * np.log(vocab + 1))
     return (lambda lp: base[:, None] + 4 * E32 * np.abs(lp)), base + 2 * rel * (np.log(vocab) + 1) + 4 * E32 * np.log(vocab + 1)
+
+
+def used_pages(table, lens, num_pages, page):
+    """(pages in use, which entries of the table hold one)."""
+    b, wide = table.shape
+    held = np.arange(wide)[None, :] < -(-np.clip(lens, 0, wide * page) // page)[:, None]
+    held &= (table >= 0) & (table < num_pages)
+    return np.unique(table[held]), held
+
+
+def free(table, lens, num_pages, page):
+    used, _ = used_pages(table, lens, num_pages, page)
+    rest = np.setdiff1d(np.arange(num_pages), used)
+    return np.concatenate([rest, np.full(num_pages - len(rest), -1)]), len(rest)
+
+
+def fork(parents, table, lens, free_pages, page):
+    """What mlcv_kv_fork documents, row by row: (table, lengths, status, pairs of pages copied)."""
+    b, wide = table.shape
+    out, got = np.full((len(parents), wide), -1), np.zeros(len(parents), int)
+    seen, pairs, refused = set(), [], 0
+    for i, p in enumerate(parents):
+        if not 0 <= p < b:
+            continue
+        n = int(np.clip(lens[p], 0, wide * page))
+        has = -(-n // page)
+        if n % page and p in seen:
+            if len(pairs) == len(free_pages):
+                refused += 1
+                continue
+            out[i, :has] = table[p, :has]
+            out[i, has - 1] = free_pages[len(pairs)]
+            pairs.append((table[p, has - 1], free_pages[len(pairs)]))
+        else:
+            out[i, :has] = table[p, :has]
+        seen.add(p)
+        got[i] = n
+    return out, got, np.array([len(pairs), refused]), pairs
+
+
+def compact(table, lens, num_pages, page):
+    """(table, status, pairs of pages moved)."""
+    used, held = used_pages(table, lens, num_pages, page)
+    m = len(used)
+    src = used[used >= m]
+    dst = np.setdiff1d(np.arange(m), used)
+    to = dict(zip(src.tolist(), dst.tolist()))
+    out = table.copy()
+    out[held] = [to.get(int(e), int(e)) for e in table[held]]
+    return out, np.array([m, len(src)]), list(zip(src, dst))

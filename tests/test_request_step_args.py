@@ -3,6 +3,8 @@ call."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -28,7 +30,55 @@ def _logprobs(**kw):
     N.call("mlcv_token_logprobs", *a.values())
 
 
+def _free(**kw):
+    a = dict(table=P, B=2, max_pages=4, lens=2 * P, num_pages=8, page=16, free=3 * P, count=4 * P, ws=5 * P, ws_bytes=1 << 40,
+             stream=None)
+    a.update(kw)
+    N.call("mlcv_kv_free", *a.values())
+
+
+def _copy(**kw):
+    a = dict(src=P, dst=P, n=2, k=P, ks=P, v=P, vs=P, num_pages=8, k2=P, ks2=P, v2=P, vs2=P, pages2=8, layers=2, page=16, KV=1,
+             hd=64, stream=None)
+    a.update(kw)
+    N.call("mlcv_kv_copy", *a.values())
+
+
+def _fork(**kw):
+    a = dict(parents=P, n=3, table=2 * P, B=2, max_pages=4, lens=3 * P, free=4 * P, n_free=5, count=5 * P, k=P, ks=P, v=P, vs=P,
+             layers=2, num_pages=8, page=16, KV=1, hd=64, out=6 * P, out_lens=7 * P, status=8 * P, copies=9 * P, stream=None)
+    a.update(kw)
+    N.call("mlcv_kv_fork", *a.values())
+
+
+def _compact(**kw):
+    a = dict(table=P, B=2, max_pages=4, lens=2 * P, k=P, ks=P, v=P, vs=P, layers=2, num_pages=8, page=16, KV=1, hd=64, out=3 * P,
+             status=4 * P, ws=5 * P, ws_bytes=1 << 40, stream=None)
+    a.update(kw)
+    N.call("mlcv_kv_compact", *a.values())
+
+
 @pytest.mark.parametrize("fn,bad,what", [
+    (_free, dict(page=48), "page"), (_free, dict(num_pages=-1), "negative"), (_free, dict(B=4097), "4096"),
+    (_free, dict(num_pages=2 ** 28), "slots"), (_free, dict(max_pages=2 ** 28), "slots"), (_free, dict(free=None), "null"),
+    (_free, dict(count=None), "null"), (_free, dict(lens=None), "null"), (_free, dict(table=None), "null"),
+    (_free, dict(ws=None), "workspace"), (_free, dict(ws=P + 8), "workspace"), (_free, dict(ws_bytes=64), "workspace"),
+    (_free, dict(free=P), "overlap"), (_free, dict(count=2 * P + 4), "overlap"), (_free, dict(free=3 * P, count=3 * P + 28), "overlap"),
+    (_copy, dict(page=8), "page"), (_copy, dict(hd=96), "head_dim"), (_copy, dict(n=-1), "negative"),
+    (_copy, dict(layers=0), "layers"), (_copy, dict(KV=0), "layers"), (_copy, dict(k=None), "null"),
+    (_copy, dict(vs2=None), "null"), (_copy, dict(src=None), "null"), (_copy, dict(v=P + 8), "aligned"),
+    (_copy, dict(k2=P + 1), "aligned"), (_copy, dict(num_pages=2 ** 28), "slots"), (_copy, dict(pages2=-1), "negative"),
+    (_copy, dict(KV=65535, page=128, hd=256), "2\\^30"),
+    (_fork, dict(n=-1), "negative"), (_fork, dict(n=4097), "4096"), (_fork, dict(B=4097), "4096"), (_fork, dict(page=24), "page"),
+    (_fork, dict(status=None), "null"), (_fork, dict(parents=None), "null"), (_fork, dict(out=None), "null"),
+    (_fork, dict(out_lens=None), "null"), (_fork, dict(copies=None), "null"), (_fork, dict(lens=None), "null"),
+    (_fork, dict(free=None), "free_pages"), (_fork, dict(k=None), "null"), (_fork, dict(hd=32), "head_dim"),
+    (_fork, dict(out=2 * P + 28), "overlap"), (_fork, dict(out_lens=P), "overlap"), (_fork, dict(copies=4 * P), "overlap"),
+    (_fork, dict(status=5 * P), "overlap"), (_fork, dict(out_lens=9 * P), "overlap"),
+    (_compact, dict(page=24), "page"), (_compact, dict(ws_bytes=8), "workspace"), (_compact, dict(out=None), "null"),
+    (_compact, dict(status=None), "null"), (_compact, dict(lens=None), "null"), (_compact, dict(v=None), "null"),
+    (_compact, dict(out=P + 4), "overlap"), (_compact, dict(status=2 * P), "overlap"), (_compact, dict(ws=P), "overlap"),
+    (_compact, dict(layers=70000), "layers"), (_compact, dict(B=5000), "4096"),
     (_logprobs, dict(dtype=0), "float"), (_logprobs, dict(rows=-1), "size"), (_logprobs, dict(vocab=0), "size"),
     (_logprobs, dict(vocab=2 ** 31 - 1), "vocab"), (_logprobs, dict(top=65), "top"), (_logprobs, dict(vocab=3), "top"),
     (_logprobs, dict(top=-1), "top"), (_logprobs, dict(given=-1), "size"), (_logprobs, dict(scale=0.0), "scale"),
@@ -56,6 +106,9 @@ def test_empty_calls_do_nothing():
     _rope(tokens=0)
     _rope(B=0)
     _logprobs(rows=0)
+    _copy(n=0)
+    _copy(num_pages=0)
+    _copy(pages2=0)
 
 
 def test_host_tensors_are_refused():
@@ -74,3 +127,15 @@ def test_workspace_of_logprobs():
     assert L.token_logprobs_workspace(1, 4096, 64) == 0
     with pytest.raises(N.MlcvError, match="null"):
         N.call("mlcv_token_logprobs_workspace", 1, 100, 1, None)
+
+
+def test_workspaces_of_the_pages():
+    for n in (0, 1, 4096, 4097, 2 ** 22, 2 ** 22 + 1, 2 ** 26):
+        blocks = max(1, -(-n // 4096))
+        assert blocks * 516 <= C.kv_free_workspace(n) <= 2 * blocks * 516 + 16
+        assert C.kv_compact_workspace(n) == C.kv_free_workspace(n) + 12 * n
+    for name in ("mlcv_kv_free_workspace", "mlcv_kv_compact_workspace"):
+        with pytest.raises(N.MlcvError, match="null"):
+            N.call(name, 5, None)
+        with pytest.raises(N.MlcvError, match="num_pages"):
+            N.call(name, -1, ctypes.byref(ctypes.c_size_t()))
