@@ -5,14 +5,19 @@
 // row that is almost certain keeps its digits; the sums are rebased where the maximum grows.  float32 throughout.
 //
 // Alternatives are ranked by a 64-bit key, the logit's bits in an order of integers over the complement of its index:
-// no two are equal, and equal logits rank by their index.  A wave holds its best 64 sorted, one per lane, and
-// appends what passes the k-th of them to a buffer of its own; 64 at a time are sorted and merged by the bitonic
-// network.  Of n logits in random order about k ln(n / k) pass.
+// no two are equal, and equal logits rank by their index.  A wave holds its best 64 sorted, one per lane.  A logit that passes
+// the threshold is inserted; where many do, as at the row's beginning, they are sorted and merged by the bitonic network.  The
+// threshold is the wave's k-th best, or the least that the waves of the row know to be below k.
+//
+// Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 100 us, 5.1 TB/s, as a copy has), with about
+// 11 vector instructions per logit beside it (a quarter of them the exponential's); for few rows by the latency of selecting
+// (16 rows: 9.1 us in 512 workgroups and 4.7 in the join; without alternatives 8.6 in all).
 #include "kernels.h"
 #include "mlcvla.h"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mlcv {
 
@@ -21,6 +26,8 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int LP_W = 4;         // waves per workgroup
+constexpr int LP_U = 4;         // chunks of 8 logits in flight per lane
+constexpr int LP_GROUP = 64 * LP_W * LP_U;
 constexpr int LP_JW = 8;        // waves per workgroup of the join
 constexpr int LP_TOP = 64;      // most alternatives: one per lane
 constexpr float LN2 = 0.6931471805599453f;
@@ -70,26 +77,68 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// one step of the bitonic network: lanes `stride` apart, the larger key to the lower lane where down
-__device__ __forceinline__ u64 exchange(u64 v, int stride, bool down, int lane) {
-  const u64 o = __shfl_xor(v, stride);
-  return (((lane & stride) == 0) == down) == (v > o) ? v : o;
+// v of lane ^ M, M < 16, within the registers: the crossbar of LDS takes four times as long
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  auto dpp = [](uint32_t x, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true);
+  };
+  if constexpr (M == 1) return dpp(v, std::integral_constant<int, 0xb1>());   // quads [1 0 3 2]
+  if constexpr (M == 2) return dpp(v, std::integral_constant<int, 0x4e>());   // quads [2 3 0 1]
+  if constexpr (M == 4) return dpp(dpp(v, std::integral_constant<int, 0x1b>()), std::integral_constant<int, 0x141>());  // 3 ^ 7
+  if constexpr (M == 8) return dpp(v, std::integral_constant<int, 0x128>());  // rows of 16 turned by 8
 }
-__device__ __forceinline__ u64 sort64(u64 v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int s = size >> 1; s > 0; s >>= 1) v = exchange(v, s, (lane & size) == 0, lane);
-  return v;
+// one step of the bitonic network over lanes S apart
+template <int S>
+__device__ __forceinline__ u64 exchange(u64 v, bool larger) {
+  const uint32_t l = (uint32_t)v, h = (uint32_t)(v >> 32);
+  u64 a = v, b;
+  if constexpr (S < 16) {
+    b = (u64)lane_xor<S>(h) << 32 | lane_xor<S>(l);
+  } else {  // both lanes of a pair receive the lower lane's and the upper's
+    const auto x = S == 16 ? __builtin_amdgcn_permlane16_swap(l, l, false, false) : __builtin_amdgcn_permlane32_swap(l, l, false, false);
+    const auto y = S == 16 ? __builtin_amdgcn_permlane16_swap(h, h, false, false) : __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    a = (u64)y[0] << 32 | x[0];
+    b = (u64)y[1] << 32 | x[1];
+  }
+  return (a > b) == larger ? a : b;
 }
-// the best 64 of two sorted lists, sorted
-__device__ __forceinline__ u64 merge64(u64 a, u64 b, int lane) {
-  const u64 o = __shfl(b, 63 - lane);
-  a = a > o ? a : o;
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) a = exchange(a, s, true, lane);
-  return a;
+// The same for values alone: a third of the instructions.  Falling.
+template <int S>
+__device__ __forceinline__ float exchange(float v, bool larger) {
+  const uint32_t b = __float_as_uint(v);
+  float x = v, y;
+  if constexpr (S < 16) {
+    y = __uint_as_float(lane_xor<S>(b));
+  } else {
+    const auto z = S == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false) : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    x = __uint_as_float(z[0]);
+    y = __uint_as_float(z[1]);
+  }
+  return larger ? fmaxf(x, y) : fminf(x, y);
 }
+
+// lanes SIZE / 2, SIZE / 4, .. 1 apart: each run of SIZE lanes, first falling then rising (or the reverse), becomes sorted
+template <int SIZE, class V>
+__device__ __forceinline__ V settle(V v, bool falling, int lane) {
+  if constexpr (SIZE >= 64) v = exchange<32>(v, ((lane & 32) == 0) == falling);
+  if constexpr (SIZE >= 32) v = exchange<16>(v, ((lane & 16) == 0) == falling);
+  if constexpr (SIZE >= 16) v = exchange<8>(v, ((lane & 8) == 0) == falling);
+  if constexpr (SIZE >= 8) v = exchange<4>(v, ((lane & 4) == 0) == falling);
+  if constexpr (SIZE >= 4) v = exchange<2>(v, ((lane & 2) == 0) == falling);
+  return exchange<1>(v, ((lane & 1) == 0) == falling);
+}
+template <class V>
+__device__ __forceinline__ V sort64(V v, bool falling, int lane) {
+  v = settle<2>(v, (lane & 2) == 0, lane);
+  v = settle<4>(v, (lane & 4) == 0, lane);
+  v = settle<8>(v, (lane & 8) == 0, lane);
+  v = settle<16>(v, (lane & 16) == 0, lane);
+  v = settle<32>(v, ((lane & 32) == 0) == falling, lane);
+  return settle<64>(v, falling, lane);
+}
+// the best 64 of a falling and a rising list, falling
+__device__ __forceinline__ u64 merge64(u64 a, u64 b, int lane) { return settle<64>(a > b ? a : b, true, lane); }
 
 // Sums relative to a maximum.  y = x * ce - mc in one fused operation: ce is c, but 2^-20 where c |m| would leave float32's
 // range; logits of that size are equal or 2^70 apart.
@@ -116,90 +165,157 @@ __device__ __forceinline__ void rebase(Sums& v, float m, Base b, float c) {
   v.m = m;
 }
 
-template <bool TOP>
+// the largest float32 below a finite one; -inf stays
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x == -INFINITY ? x : x == 0.f ? __uint_as_float(0x80000001u) : __uint_as_float(x > 0.f ? b - 1 : b + 1);
+}
+
+template <bool TOP, int WPR>
 struct Scan {
   Sums v;       // the maximum is the wave's, the sums each lane's
   Base base;
   float c, thr;  // what a logit has to pass to matter beyond the sums
   u64 list;
-  u64* buf;
-  int k, pend, lane;
+  u64* buf;            // 576 keys of the wave
+  volatile float* kw;  // of each wave of the row, its (k / WPR)-th best (rounded up) so far
+  int k, w, lane;
 
-  __device__ __forceinline__ void init(float c_, int k_, u64* buf_, int lane_) {
+  __device__ __forceinline__ void init(float c_, int k_, u64* buf_, volatile float* kw_, int w_, int lane_) {
     c = c_;
     k = k_;
     buf = buf_;
+    kw = kw_;
+    w = w_;
     lane = lane_;
     v.m = thr = -INFINITY;
+    // Values that the compiler does not know: where it knows the -inf, it turns x > -inf into "x differs from -inf", and the
+    // ballot of that into an instruction which is true for NaN.
+    asm volatile("" : "+v"(v.m), "+v"(thr));
     v.s = v.u = 0.f;
     base = base_of(v.m, c);
     list = 0;
-    pend = 0;
   }
-  // `n` <= 64 of the buffer's keys into the list
-  __device__ __forceinline__ void take(int n) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    list = merge64(list, sort64(lane < n ? buf[lane] : 0, lane), lane);
-    const u64 rest = lane < pend - n ? buf[n + lane] : 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (lane < pend - n) buf[lane] = rest;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    pend -= n;
-  }
-  // logits x of indices i0 .. + 7; `big` the largest; some lane's passes thr
-  __device__ __forceinline__ void look(const float (&x)[8], int i0, float big) {
+  __device__ __forceinline__ void raise(float big) {
+    if (!__any(big > v.m)) return;
     const float wm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(big))));
-    if (wm > v.m) {
-      base = base_of(wm, c);
-      rebase(v, wm, base, c);
+    base = base_of(wm, c);
+    rebase(v, wm, base, c);
+  }
+  // one key of the wave's into the list
+  __device__ __forceinline__ void insert(u64 key) {
+    const int at = __popcll(__ballot(list > key));
+    const uint32_t l = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)list, 0x138, 0xf, 0xf, true);  // of the lane before
+    const uint32_t h = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(list >> 32), 0x138, 0xf, 0xf, true);
+    list = lane < at ? list : lane == at ? key : (u64)h << 32 | l;
+  }
+  // the buffer's keys from the last n <= 64 of its first `pend` on into the list
+  __device__ __forceinline__ void take(int n, int pend) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    list = merge64(list, sort64(lane < n ? buf[pend - n + lane] : 0, false, lane), lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // What the wave now knows.  Its own k-th best: later logits have to be larger, as equal ones rank behind.  And where
+  // every wave of the row has ceil(k / WPR) of at least some value, k have: equal ones may still rank before those.
+  __device__ __forceinline__ void publish() {
+    const u64 kth = lane_of(list, k - 1);
+    if (kth) thr = fmaxf(thr, value_of(kth));
+    if constexpr (WPR > 1) {
+      const u64 mine = lane_of(list, (k + WPR - 1) / WPR - 1);
+      if (mine && lane == 0) kw[w] = value_of(mine);
     }
+  }
+  __device__ __forceinline__ void listen() {
+    if constexpr (WPR > 1) {
+      float low = kw[0];
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) low = fminf(low, kw[i]);
+      thr = fmaxf(thr, below(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(low)))));
+    }
+  }
+  // Logits x[n] of indices i0[n] .. + 7, the largest of each big[n], of all `top`; some lane's passes thr.
+  template <int U>
+  __device__ __forceinline__ void look(const float (&x)[U][8], const int (&i0)[U], const float (&big)[U], float top) {
+    raise(top);
     if constexpr (!TOP) {
       thr = v.m;
       return;
     }
-    // All of this block is compared with the threshold from before it: equal logits of it may have lower indices than
-    // those that are taken first.
-    const float t0 = thr;
-    int all = 0;
+    listen();
+    const u64 lanes = __ballot(top > thr);
+    if (!lanes) return;
+    float bar = thr;  // where many lanes have something, the k-th of their largest bounds what can matter
+    if (__popcll(lanes) > 16)
+      bar = fmaxf(bar, below(__uint_as_float(__builtin_amdgcn_readlane(
+                           __float_as_uint(sort64(fmaxf(top, -INFINITY), true, lane)), k - 1))));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) all += __popcll(__ballot(x[e] > t0));
-    u64 low = 0;
-    if (all > 64) {  // the k-th of the lanes' best bounds what can matter
-      int at = 0;
+    for (int n = 0; n < U; ++n) {
+      // All of a chunk is compared with one threshold: equal logits of it may have lower indices than those that are
+      // taken first.
+      const float t0 = fmaxf(bar, thr);
+      if (!__any(big[n] > t0)) continue;
+      u64 b[8];
+      int all = 0;
 #pragma unroll
-      for (int e = 7; e >= 0; --e) at = x[e] == big ? e : at;
-      low = lane_of(sort64(big > t0 ? key_of(big, i0 + at) : 0, lane), k - 1);
+      for (int e = 0; e < 8; ++e) {
+        b[e] = __ballot(x[n][e] > t0);
+        all += __popcll(b[e]);
+      }
+      if (all <= 12) {  // one by one
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          for (; b[e]; b[e] &= b[e] - 1) {
+            const int l = __builtin_ctzll(b[e]);
+            const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[n][e]), l));
+            insert(key_of(y, (uint32_t)(__builtin_amdgcn_readlane(i0[n], l) + e)));
+          }
+      } else {  // 64 at a time
+        int pend = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if ((b[e] >> lane) & 1)
+            buf[pend + __builtin_amdgcn_mbcnt_hi((uint32_t)(b[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b[e], 0))] =
+                key_of(x[n][e], i0[n] + e);
+          pend += __popcll(b[e]);
+        }
+        for (; pend > 0; pend -= 64) take(min(pend, 64), pend);
+      }
+      publish();
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const u64 key = key_of(x[e], i0 + e);
-      const bool ok = x[e] > t0 && key >= low;
-      const u64 b = __ballot(ok);
-      if (!b) continue;
-      if (ok) buf[pend + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0))] = key;
-      pend += __popcll(b);
-      if (pend >= 64) take(64);
-    }
-    const u64 kth = lane_of(list, k - 1), bound = kth > low ? kth : low;
-    if (bound) thr = fmaxf(thr, value_of(bound));
   }
-  __device__ __forceinline__ void add(const float (&x)[8], int i0) {
-    const float big = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(big > thr)) look(x, i0, big);
-    float s[8], u[8];
+  // Before the first look: the waves of a row tell one another the ceil(k / WPR)-th of their lanes' largest.
+  __device__ __forceinline__ void meet(float top) {
+    const float v = sort64(fmaxf(top, -INFINITY), true, lane);
+    if (lane == (k + WPR - 1) / WPR - 1) kw[w] = v;
+    __syncthreads();
+  }
+  template <int U>
+  __device__ __forceinline__ void add(const float (&x)[U][8], const int (&i0)[U], bool begin) {
+    float big[U], top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __builtin_fmaf(x[e], base.ce, -base.mc);
-      s[e] = __builtin_amdgcn_exp2f(y);
-      u[e] = fmaxf(y, -1000.f);  // a masked logit's y is -inf, its weight 0
+    for (int n = 0; n < U; ++n) {
+      const float* y = x[n];
+      big[n] = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+      top = n ? fmaxf(top, big[n]) : big[n];
     }
-    v.s += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    if constexpr (TOP && WPR > 1)
+      if (begin) meet(top);
+    if (__any(top > thr)) look<U>(x, i0, big, top);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v.u = __builtin_fmaf(-u[e], s[e], v.u);
+    for (int n = 0; n < U; ++n) {
+      float s[8], u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = __builtin_fmaf(x[n][e], base.ce, -base.mc);
+        s[e] = __builtin_amdgcn_exp2f(y);
+        u[e] = fmaxf(y, -1000.f);  // a masked logit's y is -inf, its weight 0
+      }
+      v.s += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.u = __builtin_fmaf(-u[e], s[e], v.u);
+    }
   }
   __device__ __forceinline__ void end() {
-    if constexpr (TOP)
-      if (pend) take(pend);
     v.s = wave_sum(v.s);
     v.u = wave_sum(v.u);
   }
@@ -251,9 +367,10 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 lis
 template <int TYPE, bool TOP, int WPR>
 __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
   typedef typename LpType<TYPE>::T T;
-  constexpr int V = sizeof(T) / 2, U = 4;  // 16-byte loads of a chunk, chunks in flight
-  __shared__ u64 buf[LP_W][TOP ? 128 : 1];
+  constexpr int V = sizeof(T) / 2, U = LP_U;  // 16-byte loads of a chunk, chunks in flight
+  __shared__ u64 buf[LP_W][TOP ? 63 + 8 * 64 + 1 : 1];
   __shared__ Sums part[LP_W];
+  __shared__ float kw[LP_W];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = WPR == 1 ? blockIdx.x * LP_W + w : blockIdx.x / a.S;
   const int split = WPR == 1 ? 0 : blockIdx.x % a.S;
@@ -262,40 +379,45 @@ __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
   const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int chunks = (int)(((int64_t)a.vocab + off + 7) >> 3);
   const int last = (int)min((int64_t)chunks, (int64_t)(split + 1) * a.per);
-  const int first = (int)((int64_t)split * a.per) + (WPR == 1 ? 0 : w) * 64 + lane;
-  Scan<TOP> scan;
-  scan.init(a.c, a.k, buf[w], lane);
-  // whole chunks, as long as every lane of the wave has U of them
-  int at = first;
-  const int whole = min(last, (int)(((int64_t)a.vocab + off) >> 3));  // chunks before this one end within the row
-  auto any_chunk = [&](int ch) {
-    float z[8];
-    const int64_t i0 = (int64_t)ch * 8 - off;
+  const int first = (int)((int64_t)split * a.per) + (WPR == 1 ? 0 : w) * 64;
+  Scan<TOP, WPR> scan;
+  scan.init(a.c, a.k, buf[w], kw, w, lane);
+  const int whole = (int)(((int64_t)a.vocab + off) >> 3);  // chunks from here on end behind the row
+  // a wave without chunks takes one round too, as the waves meet in it
+  for (int at = first; at == first || at < last; at += 64 * WPR * U) {
+    float z[U][8];
+    int at0[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      z[e] = ch < last && i0 + e >= 0 && i0 + e < a.vocab ? (float)load_global(x + i0 + e) : -INFINITY;
-    scan.add(z, (int)i0);
-  };
-  if (off && at - lane == 0) {  // the first chunk begins before the row
-    any_chunk(at);
-    at += 64 * WPR;
-  }
-  for (; at - lane + 64 * WPR * (U - 1) + 63 < whole; at += 64 * WPR * U) {
-    u4 raw[U][V];
+    for (int n = 0; n < U; ++n) at0[n] = (at + 64 * WPR * n + lane) * 8 - off;
+    if (at + 64 * WPR * (U - 1) + 63 < min(last, whole) && (at > 0 || !off)) {
+      u4 raw[U][V];
 #pragma unroll
-    for (int n = 0; n < U; ++n)
+      for (int n = 0; n < U; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        raw[n][i] = load_global(reinterpret_cast<const u4*>(x + ((int64_t)(at + 64 * WPR * n) * 8 - off)) + i);
+        for (int i = 0; i < V; ++i) raw[n][i] = load_global(reinterpret_cast<const u4*>(x + at0[n]) + i);
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
-      float z[8];
+      for (int n = 0; n < U; ++n)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = (float)reinterpret_cast<const T*>(raw[n])[e];
-      scan.add(z, (at + 64 * WPR * n) * 8 - off);
+        for (int e = 0; e < 8; ++e) z[n][e] = (float)reinterpret_cast<const T*>(raw[n])[e];
+    } else {  // the row's ends
+#pragma unroll
+      for (int n = 0; n < U; ++n) {
+        const int ch = at + 64 * WPR * n + lane;
+        u4 raw[V];
+        if (ch < last && ch < whole && at0[n] >= 0) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) raw[i] = load_global(reinterpret_cast<const u4*>(x + at0[n]) + i);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[n][e] = (float)reinterpret_cast<const T*>(raw)[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            z[n][e] = ch < last && at0[n] + e >= 0 && at0[n] + e < a.vocab ? (float)load_global(x + at0[n] + e) : -INFINITY;
+        }
+      }
     }
+    scan.template add<U>(z, at0, at == first);
   }
-  for (; at - lane < last; at += 64 * WPR) any_chunk(at);
   scan.end();
   if constexpr (WPR > 1) {
     if constexpr (TOP) buf[w][lane] = scan.list;
@@ -317,7 +439,7 @@ __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
     scan.v = v;
     if constexpr (TOP)
 #pragma unroll
-      for (int i = 1; i < LP_W; ++i) scan.list = merge64(scan.list, buf[i][lane], lane);
+      for (int i = 1; i < LP_W; ++i) scan.list = merge64(scan.list, buf[i][63 - lane], lane);
     if (a.S > 1) {
       const int64_t o = (int64_t)row * a.S + split;
       if (lane == 0) *reinterpret_cast<f4*>(a.stats + 4 * o) = (f4){v.m, v.s, v.u, 0.f};
@@ -336,15 +458,25 @@ __global__ __launch_bounds__(64 * LP_JW) void logprobs_join_kernel(const LpArgs 
   const int64_t o = (int64_t)row * a.S;
   u64 list = 0;
   if (a.k) {
-    for (int s = w; s < a.S; s += LP_JW) {
-      const u64 key = lane < a.k ? load_global(a.keys + (o + s) * a.k + lane) : 0;
-      list = s == w ? key : merge64(list, key, lane);
+    constexpr int Q = 4;  // lists on their way at once
+    for (int s0 = w; s0 < a.S; s0 += Q * LP_JW) {
+      u64 key[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int s = s0 + q * LP_JW;
+        // the first as it is, the others from their end
+        const int at = s == w ? lane : 63 - lane;
+        key[q] = s < a.S && at < a.k ? load_global(a.keys + (o + s) * a.k + at) : 0;
+      }
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        if (s0 + q * LP_JW < a.S) list = s0 + q * LP_JW == w ? key[q] : merge64(list, key[q], lane);
     }
     lists[w][lane] = list;
 #pragma unroll
     for (int h = LP_JW / 2; h > 0; h >>= 1) {
       __syncthreads();
-      if (w < h) lists[w][lane] = list = merge64(list, lists[w + h][lane], lane);
+      if (w < h) lists[w][lane] = list = merge64(list, lists[w + h][63 - lane], lane);
     }
   }
   if (w > 0) return;
@@ -370,11 +502,20 @@ struct LpPlan {
 };
 LpPlan lp_plan(int rows, int vocab, int k) {
   LpPlan p;
-  p.wpr = vocab <= 4096 ? 1 : LP_W;
+  // A wave for each row where there are enough of them, as it selects once and not four times: 4000 rows of 4096, 8192 and
+  // 32000 logits take 20.7, 31.4 and 72.6 us, with four waves 31.0, 32.2 and 77.9; 2000 of 8192 21.8 and 20.4, 1000 of 4096
+  // 12.5 and 12.9, 64 of 4096 11.5 and 8.7.  Up to 2048 logits are one round of one wave.
+  p.wpr = vocab <= 2048 || rows >= (vocab <= 4096 ? 1000 : 4000) ? 1 : LP_W;
   const int chunks = (int)(((int64_t)vocab + 7 + 7) >> 3);
-  // as many splits as make four workgroups per CU, of 8192 logits at least
-  int S = p.wpr == 1 ? 1 : std::max(1, std::min((1024 + rows - 1) / rows, chunks / 1024));
+  // Splits that make about 1200 workgroups, of a round of loads (8192 logits) at least, and none of less than three rounds,
+  // where the join's launch costs more.  257152 logits, 20 alternatives (5 from 150 rows on): 16 rows 15.6 us with 32
+  // splits, 17.4 with 16, 51.9 with one; 64 rows 25.2, 23.7, 56.3; 300 rows 47.0 with 4, 49.3 with 8, 53.3 with 2, 65.1 with one; 1001
+  // rows 110.8 with one, 120.4 with 2.  32000 logits: 64 rows 13.1 with 4, 16.7 with one; 16384: 16 rows 13.4 with 2, 10.1
+  // with one.
+  const int rounds = (int)(((int64_t)vocab + 8 * LP_GROUP - 1) / (8 * LP_GROUP));
+  int S = p.wpr == 1 || rounds < 3 ? 1 : std::max(1, std::min((int)((1200 + (int64_t)rows / 2) / rows), rounds));
   p.per = (chunks + S - 1) / S;
+  if (S > 1) p.per = (p.per + LP_GROUP - 1) / LP_GROUP * LP_GROUP;  // only the last split ends within a round of loads
   p.S = (chunks + p.per - 1) / p.per;
   p.bytes = p.S > 1 ? (size_t)rows * p.S * (16 + 8 * (size_t)k) : 0;
   return p;

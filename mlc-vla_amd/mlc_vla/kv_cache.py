@@ -124,7 +124,7 @@ def _aligned(t: torch.Tensor, low: int) -> torch.Tensor:
 
 
 def _like(q: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
 def _given(fn: str, out, q: torch.Tensor, dev: int) -> torch.Tensor:

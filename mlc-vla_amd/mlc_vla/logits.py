@@ -27,6 +27,9 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[Tensor]  # [rows, top]
 
 
+_OUT = ("float32", "float32", "int32", "float32")
+
+
 @functools.lru_cache(maxsize=4096)
 def token_logprobs_workspace(rows: int, vocab: int, top: int) -> int:
     """Bytes of workspace of ``token_logprobs`` for these sizes (mlcv_token_logprobs_workspace)."""
@@ -64,10 +67,14 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, scale: float = 1.0, out
         # one allocation: given tokens, entropy, alternatives' ids and log probabilities
         n = rows * given
         f = torch.empty(n + rows * (1 + 2 * top), dtype=_F32, device=x.device)
-        lp, h, ids, tlp = f.split((n, rows, rows * top, rows * top))
-        out = TokenLogprobs(None if tokens is None else Tensor(lp.view(shape), "float32"), Tensor(h, "float32"),
-                            Tensor(ids.view(_I32).view(rows, top), "int32") if top else None,
-                            Tensor(tlp.view(rows, top), "float32") if top else None)
+        h = f.as_strided((rows,), (1,), n)
+        lp = ids = tlp = None
+        if at is not None:
+            lp = f.as_strided(shape, (1,) if len(shape) == 1 else (given, 1))
+        if top:
+            ids = f.view(_I32).as_strided((rows, top), (top, 1), n + rows)
+            tlp = f.as_strided((rows, top), (top, 1), n + rows * (1 + top))
+        out = TokenLogprobs(*(None if o is None else Tensor(o, d) for o, d in zip((lp, h, ids, tlp), _OUT)))
     else:
         lp, h, ids, tlp = (None if o is None else _t(o) for o in out)
         for name, o, dt, want in (("logprobs", lp, _F32, shape), ("entropy", h, _F32, (rows,)),

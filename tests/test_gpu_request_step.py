@@ -230,7 +230,7 @@ def _tokens(rng, rows, n, vocab):
 @pytest.mark.parametrize("rows,vocab,top,n", [
     (1, 1, 1, 1), (3, 2, 2, 2), (1, 7, 5, 1), (9, 64, 64, 1), (5, 333, 20, 3), (130, 4096, 1, 1), (2, 4097, 64, 1),
     (3, 16391, 20, 5), (1, 50257, 20, 1), (40, 50257, 8, 1), (2, 257152, 64, 70), (1, 1000, 0, 1), (3, 70001, 0, 0),
-    (1100, 5001, 3, 1)])
+    (1100, 5001, 3, 1), (4100, 4500, 3, 1), (1000, 4000, 20, 0), (17, 16385, 2, 1)])
 def test_token_logprobs(dt, rows, vocab, top, n):
     rng = np.random.default_rng(vocab + rows)
     x = rng.standard_normal((rows, vocab)) * 3
