@@ -14,11 +14,12 @@ namespace mlcv {
 
 namespace {
 
-constexpr int MK_NT = 1024;   // threads of a workgroup that marks
-constexpr int LS_NT = 256;    // of one that lists
-constexpr int LS_BLOCK = 4096;  // pages that it lists: 64 groups of 64
+constexpr int MK_NT = 1024;   // threads of a workgroup that marks or lists pages
+constexpr int LS_BLOCK = 4096;  // pages that one lists: 64 groups of 64
+constexpr int MK_PARTS = 4;     // parts of the table, where a pool has up to MK_FEW blocks
+constexpr int MK_FEW = 64;
 constexpr int CP_NT = 256;    // of one that copies
-constexpr int FK_NT = 256;    // of one that forks
+constexpr int FK_NT = 512;    // of one that forks
 
 // ---- pages in use ------------------------------------------------------------------------------------
 
@@ -26,97 +27,39 @@ struct MarkArgs {
   const int32_t *table, *lens;
   uint32_t* words;   // a bit for each page in use, whole slices
   int32_t* counts;   // of the pages in use, per LS_BLOCK
-  int32_t B, max_pages, psh, num_pages, slice;
+  int32_t B, max_pages, psh, num_pages, slice, vec;  // vec: rows are 16-byte aligned
 };
-
-// Each workgroup reads the whole table and marks the pages of its slice in LDS: reading it over costs less than a pass that
-// clears a bitmap in memory before another sets bits in it by atomics.
-__global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a) {
-  extern __shared__ int dyn[];
-  __shared__ int most;
-  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [slice / 32]
-  int* held = dyn + (a.slice >> 5);                   // [B] entries of each row in use
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (tid == 0) most = 0;
-  for (int i = tid; i < a.slice >> 5; i += MK_NT) bits[i] = 0u;
-  __syncthreads();
-  int mine = 0;
-  for (int b = tid; b < a.B; b += MK_NT) {
-    const int len = clamp_i(a.lens[b], 0, a.max_pages << a.psh), n = (int)(((int64_t)len + (1 << a.psh) - 1) >> a.psh);
-    held[b] = n;
-    mine = max(mine, n);
-  }
-  if (mine) atomicMax(&most, mine);
-  __syncthreads();
-  // items of 4 rows x 256 entries, 16 loads in flight per lane
-  const int p0 = (int)blockIdx.x * a.slice;
-  const int wide = (most + 255) >> 8, items = ((a.B + 3) >> 2) * wide;
-  for (int it = w; it < items; it += MK_NT / 64) {
-    const int b0 = it / wide * 4, j0 = (it % wide) * 256 + lane;
-    int id[16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int b = b0 + r, n = b < a.B ? held[b] : 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 64 * i;
-        id[4 * r + i] = j < n ? load_global(a.table + (int64_t)b * a.max_pages + j) : -1;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t at = (uint32_t)id[i] - (uint32_t)p0;
-      if (id[i] >= 0 && id[i] < a.num_pages && at < (uint32_t)a.slice) atomicOr(&bits[at >> 5], 1u << (at & 31));
-    }
-  }
-  __syncthreads();
-  // 128 words of a block: two waves' lanes
-  for (int i = tid; i < a.slice >> 5; i += MK_NT) {
-    const uint32_t v = bits[i];
-    a.words[(size_t)blockIdx.x * (a.slice >> 5) + i] = v;
-    int n = __popc(v);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
-    if (lane == 0) held[i >> 6] = n;  // the rows' numbers are not needed any more
-  }
-  __syncthreads();
-  for (int i = tid; i < a.slice / LS_BLOCK; i += MK_NT)
-    a.counts[(size_t)blockIdx.x * (a.slice / LS_BLOCK) + i] = held[2 * i] + held[2 * i + 1];
-}
-
 struct ListArgs {
   const uint32_t* words;
   const int32_t* counts;
-  int32_t num_pages, blocks;
+  int32_t num_pages, blocks, parts;
   int32_t *free_pages, *free_count;       // the free list, or
   int32_t *to, *holes, *from, *status;    // a dense pool's moves: page from[r] goes to holes[r], to[from[r]] = r
 };
 
-// A workgroup lists the pages of one block.  With u(p) the pages in use before p: free page p is number p - u(p) of the
-// list; with `live` of them in all, a page in use from there on is move number u(p) - u(live), and a free one before it
-// hole number p - u(p).
+// The wave's sum in every lane, in the registers
+template <int CTRL>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int wave_add(int v) {
+  v = dpp_add<0xb1>(v);   // lane ^ 1
+  v = dpp_add<0x4e>(v);   // ^ 2
+  v = dpp_add<0x141>(v);  // the other four of eight
+  v = dpp_add<0x140>(v);  // the other eight of sixteen
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = (int)(a[0] + a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return (int)(b[0] + b[1]);
+}
+
+// One block's pages, by a workgroup that has its groups of 64 bits in LDS.  With u(p) the pages in use before p: free page p is
+// number p - u(p) of the list; with `live` of them in all, a page in use from there on is move number u(p) - u(live), and a
+// free one before it hole number p - u(p).
 template <bool MOVES>
-__global__ __launch_bounds__(LS_NT) void list_kernel(const ListArgs a) {
-  __shared__ int before[LS_BLOCK / 64], sum[3];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, mine = blockIdx.x;
-  if (tid < 3) sum[tid] = 0;
-  __syncthreads();
-  int lower = 0, all = 0;
-  for (int i = tid; i < a.blocks; i += LS_NT) {
-    const int n = a.counts[i];
-    lower += i < mine ? n : 0;
-    all += n;
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    lower += __shfl_xor(lower, o);
-    all += __shfl_xor(all, o);
-  }
-  if (lane == 0) {
-    atomicAdd(&sum[0], lower);
-    atomicAdd(&sum[1], all);
-  }
-  const uint64_t* groups = reinterpret_cast<const uint64_t*>(a.words) + (size_t)mine * (LS_BLOCK / 64);
+__device__ __forceinline__ void list_block(const ListArgs& a, const uint64_t* groups, int* before, int mine, int base,
+                                           int live, int used_low) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   if (w == 0) {
     int n = __popcll(groups[lane]), v = n;
 #pragma unroll
@@ -127,26 +70,9 @@ __global__ __launch_bounds__(LS_NT) void list_kernel(const ListArgs a) {
     before[lane] = v - n;
   }
   __syncthreads();
-  const int base = sum[0], live = sum[1];
-  int used_low = 0;  // pages in use before page `live`
-  if constexpr (MOVES) {
-    const int lb = live / LS_BLOCK, lp = live % LS_BLOCK;
-    int n = 0;
-    for (int i = tid; i < lb; i += LS_NT) n += a.counts[i];
-    if (tid < LS_BLOCK / 64 && lb < a.blocks) {
-      const uint64_t g = reinterpret_cast<const uint64_t*>(a.words)[(size_t)lb * (LS_BLOCK / 64) + tid];
-      const int cut = clamp_i(lp - 64 * tid, 0, 64);
-      n += __popcll(cut == 64 ? g : g & ((1ull << cut) - 1));
-    }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
-    if (lane == 0) atomicAdd(&sum[2], n);
-    __syncthreads();
-    used_low = sum[2];
-  }
-#pragma unroll 4
-  for (int q = w; q < LS_BLOCK / 64; q += LS_NT / 64) {
-    const int p = mine * LS_BLOCK + 64 * q + lane;
+  for (int i = 0; i < LS_BLOCK / MK_NT; ++i) {
+    const int q = w + i * (MK_NT / 64), p = mine * LS_BLOCK + 64 * q + lane;
     if (p >= a.num_pages) continue;
     const uint64_t g = groups[q];
     const bool used = (g >> lane) & 1;
@@ -173,13 +99,190 @@ __global__ __launch_bounds__(LS_NT) void list_kernel(const ListArgs a) {
   }
 }
 
+// A workgroup reads the whole table, or one of MK_PARTS parts of it, and marks the pages of its slice in LDS: reading it over
+// costs less than a pass that clears a bitmap in memory before another sets bits in it by atomics.  Bound by its own
+// instructions, about 12 per 64 entries: 512 rows of 256 entries over 262144 pages take 18.3 us with the whole table for each of
+// 64 workgroups, 9.0 in four parts, whose bits the listing workgroups put together.
+// A pool of one block is listed by the same workgroup (THEN: 1 the free list, 2 the moves), a larger one by a second launch.
+template <int THEN>
+__global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const ListArgs l) {
+  extern __shared__ __attribute__((aligned(16))) int dyn[];
+  __shared__ int most, sum[2], before[LS_BLOCK / 64];
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [slice / 32]
+  int* held = dyn + (a.slice >> 5);                   // [B] entries of each row in use
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (tid == 0) most = sum[0] = sum[1] = 0;
+  for (int i = tid; i < a.slice >> 5; i += MK_NT) bits[i] = 0u;
+  __syncthreads();
+  int mine = 0;
+  for (int b = tid; b < a.B; b += MK_NT) {
+    const int len = clamp_i(a.lens[b], 0, a.max_pages << a.psh), n = (int)(((int64_t)len + (1 << a.psh) - 1) >> a.psh);
+    held[b] = n;
+    mine = max(mine, n);
+  }
+  if (mine) atomicMax(&most, mine);
+  __syncthreads();
+  // Items of 4 rows x 256 entries.  An item's loads are issued without branches (from within the table, used or not), and the
+  // next one's before it is marked: with a branch around each load the compiler waits for all of them between items.
+  const int p0 = (int)blockIdx.x * a.slice;
+  const uint32_t many = (uint32_t)clamp_i(a.num_pages - p0, 0, a.slice);  // pages of the slice; a page before it wraps
+  const int wide = (most + 255) >> 8, items = ((a.B + 3) >> 2) * wide;
+  auto fetch = [&](int it, uint32_t (&v)[16]) {
+    const int b0 = it / wide * 4, j0 = (it % wide) * 256;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int32_t* row = a.table + (int64_t)min(b0 + r, a.B - 1) * a.max_pages;
+      if (a.vec) {
+        const u4 x = load_global(reinterpret_cast<const u4*>(row + min(j0 + 4 * lane, a.max_pages - 4)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * r + i] = x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * r + i] = (uint32_t)load_global(row + min(j0 + lane + 64 * i, a.max_pages - 1));
+      }
+    }
+  };
+  auto mark = [&](int it, const uint32_t (&v)[16]) {
+    const int b0 = it / wide * 4, j0 = (it % wide) * 256;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = b0 + r < a.B ? held[b0 + r] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = a.vec ? j0 + 4 * lane + i : j0 + lane + 64 * i;
+        const uint32_t at = v[4 * r + i] - (uint32_t)p0;
+        if (j < n && at < many) atomicOr(&bits[at >> 5], 1u << (at & 31));
+      }
+    }
+  };
+  const int begin = (int)blockIdx.y * (MK_NT / 64) + w, step = (int)gridDim.y * (MK_NT / 64);
+  if (begin < items) {
+    uint32_t one[16], two[16];
+    fetch(begin, one);
+    for (int it = begin; it < items; it += 2 * step) {
+      fetch(min(it + step, items - 1), two);
+      mark(it, one);
+      fetch(min(it + 2 * step, items - 1), one);
+      if (it + step < items) mark(it + step, two);
+    }
+  }
+  __syncthreads();
+  if constexpr (THEN == 0) {
+    // 128 words of a block: two waves' lanes
+    for (int i = tid; i < a.slice >> 5; i += MK_NT) {
+      const uint32_t v = bits[i];
+      a.words[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * (a.slice >> 5) + i] = v;
+      const int n = wave_add(__popc(v));
+      if (lane == 0) held[i >> 6] = n;  // the rows' numbers are not needed any more
+    }
+    if (gridDim.y > 1) return;
+    __syncthreads();
+    for (int i = tid; i < a.slice / LS_BLOCK; i += MK_NT)
+      a.counts[(size_t)blockIdx.x * (a.slice / LS_BLOCK) + i] = held[2 * i] + held[2 * i + 1];
+  } else {
+    const uint64_t* groups = reinterpret_cast<const uint64_t*>(bits);
+    if (w == 0) {
+      const uint64_t g = groups[lane];
+      const int live = wave_add(__popcll(g)), cut = clamp_i(live - 64 * lane, 0, 64);
+      const int low = wave_add(__popcll(cut == 64 ? g : g & ((1ull << cut) - 1)));
+      if (lane == 0) {
+        sum[0] = live;
+        sum[1] = low;
+      }
+    }
+    __syncthreads();
+    list_block<THEN == 2>(l, groups, before, 0, 0, sum[0], sum[1]);
+  }
+}
+
+// a word's bits for pages before p, its first page being at
+__device__ __forceinline__ int used_before(uint32_t word, int at, int p) {
+  const int cut = clamp_i(p - at, 0, 32);
+  return __popc(cut == 32 ? word : word & ((1u << cut) - 1));
+}
+
+template <bool MOVES>
+__global__ __launch_bounds__(MK_NT) void list_kernel(const ListArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t groups[LS_BLOCK / 32];
+  __shared__ int before[LS_BLOCK / 64], sum[3];
+  const int tid = threadIdx.x, lane = tid & 63, mine = blockIdx.x;
+  if (tid < 3) sum[tid] = 0;
+  __syncthreads();
+  int lower = 0, all = 0, low = 0;  // pages in use: before this block, of the pool, before page number `live`
+  if (a.parts > 1) {
+    // few blocks: every workgroup puts the parts of the whole pool together, 8 words per thread at most
+    constexpr int Q = MK_FEW * (LS_BLOCK / 128) / MK_NT;
+    const int quads = a.blocks * (LS_BLOCK / 128);
+    u4 v[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = min(tid + q * MK_NT, quads - 1);
+      u4 x[MK_PARTS];
+#pragma unroll
+      for (int k = 0; k < MK_PARTS; ++k)
+        x[k] = load_global(reinterpret_cast<const u4*>(a.words) + (size_t)k * quads + i);
+      v[q] = x[0];
+#pragma unroll
+      for (int k = 1; k < MK_PARTS; ++k) v[q] |= x[k];
+      if (tid + q * MK_NT >= quads) v[q] = (u4){0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = tid + q * MK_NT, n = __popc(v[q][0]) + __popc(v[q][1]) + __popc(v[q][2]) + __popc(v[q][3]);
+      const int block = i / (LS_BLOCK / 128);
+      all += n;
+      lower += block < mine ? n : 0;
+      if (block == mine) reinterpret_cast<u4*>(groups)[i % (LS_BLOCK / 128)] = v[q];
+    }
+    lower = wave_add(lower);
+    all = wave_add(all);
+    if (lane == 0 && all) {
+      atomicAdd(&sum[0], lower);
+      atomicAdd(&sum[1], all);
+    }
+    __syncthreads();
+    if constexpr (MOVES) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low += used_before(v[q][e], (tid + q * MK_NT) * 128 + 32 * e, sum[1]);
+    }
+  } else {
+    if (tid < LS_BLOCK / 32) groups[tid] = a.words[(size_t)mine * (LS_BLOCK / 32) + tid];
+    for (int i = tid; i < a.blocks; i += MK_NT) {
+      const int n = a.counts[i];
+      lower += i < mine ? n : 0;
+      all += n;
+    }
+    lower = wave_add(lower);
+    all = wave_add(all);
+    if (lane == 0 && all) {
+      atomicAdd(&sum[0], lower);
+      atomicAdd(&sum[1], all);
+    }
+    __syncthreads();
+    if constexpr (MOVES) {
+      const int live = sum[1], lb = live / LS_BLOCK;
+      for (int i = tid; i < lb; i += MK_NT) low += a.counts[i];
+      if (tid < LS_BLOCK / 32 && lb < a.blocks)
+        low += used_before(a.words[(size_t)lb * (LS_BLOCK / 32) + tid], lb * LS_BLOCK + 32 * tid, live);
+    }
+  }
+  if constexpr (MOVES) {
+    low = wave_add(low);
+    if (lane == 0 && low) atomicAdd(&sum[2], low);
+    __syncthreads();
+  }
+  list_block<MOVES>(a, reinterpret_cast<const uint64_t*>(groups), before, mine, sum[0], sum[1], sum[2]);
+}
+
 // Slices of the pages, one for each workgroup that marks: blocks of 4096 pages, more where there would be over 1024 of them
 int mark_slice(int num_pages) {
   const int64_t blocks = std::max<int64_t>(1, ((int64_t)num_pages + LS_BLOCK - 1) / LS_BLOCK);
   return (int)((blocks + 1023) / 1024) * LS_BLOCK;
 }
 struct MarkSizes {
-  int slice, slices, blocks;
+  int slice, slices, blocks, parts;
   size_t words, counts;  // ints
 };
 MarkSizes mark_sizes(int num_pages) {
@@ -187,15 +290,32 @@ MarkSizes mark_sizes(int num_pages) {
   m.slice = mark_slice(num_pages);
   m.slices = std::max(1, (int)(((int64_t)num_pages + m.slice - 1) / m.slice));
   m.blocks = m.slices * (m.slice / LS_BLOCK);
-  m.words = (size_t)m.slices * (m.slice / 32);
+  m.parts = m.blocks > 1 && m.blocks <= MK_FEW ? MK_PARTS : 1;
+  m.words = (size_t)m.parts * m.slices * (m.slice / 32);
   m.counts = ((size_t)m.blocks + 3) / 4 * 4;
   return m;
 }
-int mark_launch(const int32_t* table, const int32_t* lens, int B, int max_pages, int page, int num_pages,
-                const MarkSizes& m, uint32_t* words, int32_t* counts, hipStream_t st) {
-  const MarkArgs a{table, lens, words, counts, B, max_pages, log2_of(page), num_pages, m.slice};
+// Finds the pages in use and lists the free ones, or a dense pool's moves; l: what is to be written
+template <bool MOVES>
+int list_launch(const int32_t* table, const int32_t* lens, int B, int max_pages, int page, int num_pages,
+                const MarkSizes& m, int32_t* workspace, ListArgs l, hipStream_t st) {
+  uint32_t* words = reinterpret_cast<uint32_t*>(workspace);
+  int32_t* counts = workspace + m.words;
+  const MarkArgs a{table, lens, words, counts, B, max_pages, log2_of(page), num_pages, m.slice,
+                   aligned16(table) && max_pages % 4 == 0};
   const size_t lds = (size_t)(m.slice / 32 + std::max(B, m.slice / 2048)) * 4;
-  mark_kernel<<<(unsigned)m.slices, MK_NT, lds, st>>>(a);
+  l.words = words;
+  l.counts = counts;
+  l.num_pages = num_pages;
+  l.blocks = m.blocks;
+  l.parts = m.parts;
+  if (m.blocks == 1) {
+    mark_kernel<MOVES ? 2 : 1><<<1, MK_NT, lds, st>>>(a, l);
+  } else {
+    mark_kernel<0><<<dim3(m.slices, m.parts), MK_NT, lds, st>>>(a, l);
+    MLCV_HIP(hipGetLastError());
+    list_kernel<MOVES><<<(unsigned)m.blocks, MK_NT, 0, st>>>(l);
+  }
   MLCV_HIP(hipGetLastError());
   return 0;
 }
@@ -408,20 +528,11 @@ int mlcv_kv_free(const int32_t* block_table, int32_t B, int32_t max_pages, const
   const Ints arrays[] = {{free_pages, num_pages}, {free_count, 1}, {workspace, (int64_t)(m.words + m.counts)},
                          {block_table, (int64_t)B * max_pages}, {kv_lens, B}};
   MLCV_REQUIRE(!overlap(arrays, 3, 5), "outputs overlap the inputs or one another");
-  uint32_t* words = static_cast<uint32_t*>(workspace);
-  int32_t* counts = reinterpret_cast<int32_t*>(words + m.words);
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  MLCV_TRY(mark_launch(block_table, kv_lens, B, max_pages, page, num_pages, m, words, counts, st));
   ListArgs l{};
-  l.words = words;
-  l.counts = counts;
-  l.num_pages = num_pages;
-  l.blocks = m.blocks;
   l.free_pages = free_pages;
   l.free_count = free_count;
-  list_kernel<false><<<(unsigned)m.blocks, LS_NT, 0, st>>>(l);
-  MLCV_HIP(hipGetLastError());
-  return 0;
+  return list_launch<false>(block_table, kv_lens, B, max_pages, page, num_pages, m, static_cast<int32_t*>(workspace), l,
+                            reinterpret_cast<hipStream_t>(stream));
 }
 
 int mlcv_kv_copy(const int32_t* src, const int32_t* dst, int32_t n, void* k_cache, float* k_scale, void* v_cache,
@@ -505,21 +616,13 @@ int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, co
                          {block_table, new_table == block_table ? 0 : entries}};
   MLCV_REQUIRE(!overlap(arrays, 3, 5), "outputs overlap the inputs or one another");
   const MarkSizes m = mark_sizes(num_pages);
-  uint32_t* words = static_cast<uint32_t*>(workspace);
-  int32_t* counts = reinterpret_cast<int32_t*>(words + m.words);
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  MLCV_TRY(mark_launch(block_table, kv_lens, B, max_pages, page, num_pages, m, words, counts, st));
   ListArgs l{};
-  l.words = words;
-  l.counts = counts;
-  l.num_pages = num_pages;
-  l.blocks = m.blocks;
-  l.to = counts + m.counts;
+  l.to = static_cast<int32_t*>(workspace) + m.words + m.counts;
   l.holes = l.to + num_pages;
   l.from = l.holes + num_pages;
   l.status = status;
-  list_kernel<true><<<(unsigned)m.blocks, LS_NT, 0, st>>>(l);
-  MLCV_HIP(hipGetLastError());
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  MLCV_TRY(list_launch<true>(block_table, kv_lens, B, max_pages, page, num_pages, m, static_cast<int32_t*>(workspace), l, st));
   a.src = l.from;
   a.dst = l.holes;
   a.count = status + 1;
