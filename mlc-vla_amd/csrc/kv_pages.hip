@@ -332,9 +332,12 @@ struct CopyArgs {
   const int32_t *src, *dst, *count;  // count: how many of them there are (null: most)
   int32_t most, layers, KV, page_bytes, pieces;
 };
-constexpr int CP_PIECE = 8192;  // bytes that a wave moves at a time: 8 loads of 16 per lane
+constexpr int CP_PIECE = 2048;  // bytes that a wave moves at a time: 2 loads of 16 per lane
 
-// Units of one page, layer, side and piece; a wave takes one after another.
+// Units of one page, layer, side and piece; a wave takes one after another.  Bound by memory: 4001 pages of 32 KB of two layers
+// take 99.6 us, 5.3 TB/s read and written.  Small units in many waves, and stores past the caches, which leaves those to pages that
+// are read several times: 8 KB per wave and plain stores take 103.4 us, 431 pages forked from 64 in 6 layers 28.1 (20.3), a
+// pool of 12000 pages of 32 KB made dense (2954 move) 51.1 (41.6); 1 KB per wave 110, 26 and 52.
 __device__ __forceinline__ void copy_pages(const CopyArgs& a, long long unit, long long step) {
   const int lane = threadIdx.x & 63;
   const int n = a.count ? clamp_i(*a.count, 0, a.most) : a.most;
@@ -355,7 +358,7 @@ __device__ __forceinline__ void copy_pages(const CopyArgs& a, long long unit, lo
       if (64 * k < left) v[k] = load_global(p + 64 * k);
 #pragma unroll
     for (int k = 0; k < CP_PIECE / 1024; ++k)
-      if (64 * k < left) q[64 * k] = v[k];
+      if (64 * k < left) __builtin_nontemporal_store(v[k], q + 64 * k);
     if (piece == 0)
       for (int h = lane; h < a.KV; h += 64) a.into.scale[z][pd * a.KV + h] = a.from.scale[z][ps * a.KV + h];
   }
@@ -390,10 +393,11 @@ __global__ __launch_bounds__(CP_NT) void move_kernel(const CopyArgs a, const Ren
   }
 }
 
-// workgroups for `most` pages: as many as the GPU holds at once, or fewer
+// Workgroups for `most` pages, of which there may be fewer: up to 16384.  With 2048 (about what the GPU holds at once) the
+// copies above take 101.2, 20.4 and 43.0 us.
 unsigned copy_groups(const CopyArgs& a) {
   const int64_t units = (int64_t)a.most * a.layers * 2 * a.pieces;
-  return (unsigned)std::min<int64_t>((units + CP_NT / 64 - 1) / (CP_NT / 64), 2048);
+  return (unsigned)std::min<int64_t>((units + CP_NT / 64 - 1) / (CP_NT / 64), 16384);
 }
 
 // ---- forks -------------------------------------------------------------------------------------------

@@ -448,7 +448,8 @@ def kv_free(block_table, kv_lens, *, num_pages: int, page_size: int, out: Option
     if not 0 <= num_pages < 1 << 27:
         _bad("kv_free", "num_pages", "is negative or past 2^27 - 1")
     if out is None:
-        pages, count = torch.empty(num_pages + 1, dtype=_I32, device=table.device).split((num_pages, 1))
+        both = torch.empty(num_pages + 1, dtype=_I32, device=table.device)
+        pages, count = both.as_strided((num_pages,), (1,)), both.as_strided((1,), (1,), num_pages)
         out = KVFree(Tensor(pages, "int32"), Tensor(count, "int32"))
     else:
         pages, count = _outs("kv_free", dev, out, ((num_pages,), (1,)))
@@ -488,9 +489,10 @@ def kv_fork(parents, block_table, kv_lens, free_pages, k_cache, k_scale, v_cache
         _refuse("kv_fork", dev, (("parents", p, (_I32,), (None,), True), ("free_pages", free, (_I32,), (None,), True)))
     n = p.shape[0]
     if out is None:
-        t, m, status, copies = torch.empty(n * wide + 3 * n + 2, dtype=_I32, device=table.device).split(
-            (n * wide, n, 2, 2 * n))
-        out = KVFork(Tensor(t.view(n, wide), "int32"), Tensor(m, "int32"), Tensor(status, "int32"))
+        copies = torch.empty(2 * n + n * wide + n + 2, dtype=_I32, device=table.device)  # and the outputs
+        t, m = copies.as_strided((n, wide), (wide, 1), 2 * n), copies.as_strided((n,), (1,), n * (wide + 2))
+        status = copies.as_strided((2,), (1,), n * (wide + 3))
+        out = KVFork(Tensor(t, "int32"), Tensor(m, "int32"), Tensor(status, "int32"))
     else:
         t, m, status = _outs("kv_fork", dev, out, ((n, wide), (n,), (2,)))
         copies = torch.empty(2 * n, dtype=_I32, device=table.device)
@@ -507,8 +509,9 @@ def kv_compact(block_table, kv_lens, k_cache, k_scale, v_cache, v_scale, *, out:
     cache, (dev, layers, pages, kv, page, hd) = _pool("kv_compact", k_cache, k_scale, v_cache, v_scale)
     table, lens, n, wide = _rows("kv_compact", block_table, kv_lens, dev)
     if out is None:
-        t, status = torch.empty(n * wide + 2, dtype=_I32, device=table.device).split((n * wide, 2))
-        out = KVCompact(Tensor(t.view(n, wide), "int32"), Tensor(status, "int32"))
+        both = torch.empty(n * wide + 2, dtype=_I32, device=table.device)
+        t, status = both.as_strided((n, wide), (wide, 1)), both.as_strided((2,), (1,), n * wide)
+        out = KVCompact(Tensor(t, "int32"), Tensor(status, "int32"))
     else:
         t, status = _outs("kv_compact", dev, out, ((n, wide), (2,)))
     ws, size = _space("kv_compact", workspace, kv_compact_workspace(pages), table, dev)
