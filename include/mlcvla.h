@@ -427,14 +427,14 @@ int mlcv_kv_copy(const int32_t* src, const int32_t* dst, int32_t n, void* k_cach
  * is its length; entries behind are -1, and a parent outside [0, B) gives an empty row.  Full pages are shared.  A last page that
  * is not full stays with the first row of its parent; every other row gets a copy of it (all layers) on a page from the
  * front of free_pages, in the order of the rows.  Rows for which the free pages do not last are refused: empty, length 0.
- *   status [2]: pages taken; rows refused.  copies [2 n]: where the copied pages come from and go to (scratch)
+ *   status [2]: pages taken; rows refused
  * The old table is done with: to keep a request beside its forks, let it be a row of its own.  At most 4096 rows of either table.  No
  * output may overlap an input or another output (-2). */
 int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, int32_t B, int32_t max_pages,
                  const int32_t* kv_lens, const int32_t* free_pages, int32_t n_free, const int32_t* free_count,
                  void* k_cache, float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages,
                  int32_t page, int32_t KV, int32_t hd, int32_t* new_table, int32_t* new_lens, int32_t* status,
-                 int32_t* copies, void* stream);
+                 void* stream);
 
 /* Make a pool dense: with m pages in use, those numbered m and above move, in ascending order, to the free ones below m, in all
  * layers; new_table (which may be block_table) has their new numbers.  The pages from m on are free then.  Entries behind a
@@ -454,11 +454,12 @@ int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, co
  *   position * theta^(-2 i / rotary); dims from `rotary` on (a multiple of 16, 0 to hd) stay y
  * q, k and their outs: element (t, h, d) at t * tok + h * head + d elements, MLCV_DTYPE_F16, _BF16 or _F32 throughout (any
  * strides; where all rows are 16-byte aligned they are read faster); hd 64, 128 or 256; weights [hd] of that type or
- * _F32.  float32 between the load and one rounding at the end, the angles of far positions in more.
+ * _F32.  float32 between the load and one rounding at the end, the angles of far positions in more (so a head whose squares sum
+ * past float32's range is normed to zeros).
  * The position of a token is positions[t] (any int32), or, with positions NULL, its place in the cache as
  * mlcv_kv_attention has it: kv_lens[b] - n + i for token i of request b's n (a refused request's, with kv_lens 0, are
- * negative); rows behind the last request are then left as they were.  An out may be its own input (same strides); it
- * must not overlap the other input or output, and its rows lie apart (-2). */
+ * negative); rows behind the last request are then left as they were.  An out may be its own input, with its strides; it
+ * must not otherwise overlap the other input or output, and its rows lie apart (-2). */
 int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                  int32_t dtype, int32_t tokens, const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens,
                  const int32_t* positions, int32_t H, int32_t KV, int32_t hd, int32_t rotary, double theta, int32_t norm,

@@ -53,14 +53,10 @@ __device__ __forceinline__ int wave_add(int v) {
   return (int)(b[0] + b[1]);
 }
 
-// One block's pages, by a workgroup that has its groups of 64 bits in LDS.  With u(p) the pages in use before p: free page p is
-// number p - u(p) of the list; with `live` of them in all, a page in use from there on is move number u(p) - u(live), and a
-// free one before it hole number p - u(p).
-template <bool MOVES>
-__device__ __forceinline__ void list_block(const ListArgs& a, const uint64_t* groups, int* before, int mine, int base,
-                                           int live, int used_low) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (w == 0) {
+// before[q]: bits of the block's groups before group q
+__device__ __forceinline__ void groups_before(const uint64_t* groups, int* before) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < 64) {
     int n = __popcll(groups[lane]), v = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -70,6 +66,16 @@ __device__ __forceinline__ void list_block(const ListArgs& a, const uint64_t* gr
     before[lane] = v - n;
   }
   __syncthreads();
+}
+
+// One block's pages, by a workgroup that has its groups of 64 bits in LDS.  With u(p) the pages in use before p: free page p is
+// number p - u(p) of the list; with `live` of them in all, a page in use from there on is move number u(p) - u(live), and a
+// free one before it hole number p - u(p).
+template <bool MOVES>
+__device__ __forceinline__ void list_block(const ListArgs& a, const uint64_t* groups, int* before, int mine, int base,
+                                           int live, int used_low) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  groups_before(groups, before);
 #pragma unroll
   for (int i = 0; i < LS_BLOCK / MK_NT; ++i) {
     const int q = w + i * (MK_NT / 64), p = mine * LS_BLOCK + 64 * q + lane;
@@ -104,14 +110,12 @@ __device__ __forceinline__ void list_block(const ListArgs& a, const uint64_t* gr
 // instructions, about 12 per 64 entries: 512 rows of 256 entries over 262144 pages take 18.3 us with the whole table for each of
 // 64 workgroups, 9.0 in four parts, whose bits the listing workgroups put together.
 // A pool of one block is listed by the same workgroup (THEN: 1 the free list, 2 the moves), a larger one by a second launch.
-template <int THEN>
-__global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const ListArgs l) {
-  extern __shared__ __attribute__((aligned(16))) int dyn[];
-  __shared__ int most, sum[2], before[LS_BLOCK / 64];
-  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [slice / 32]
-  int* held = dyn + (a.slice >> 5);                   // [B] entries of each row in use
+// bits [slice / 32] in LDS: the pages in use of the slice from p0 on, as far as the rows of this part of `parts` have them; held
+// [B]: entries of each row in use
+__device__ __forceinline__ void mark_slice_bits(const MarkArgs& a, uint32_t* bits, int* held, int p0, int part, int parts) {
+  __shared__ int most;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (tid == 0) most = sum[0] = sum[1] = 0;
+  if (tid == 0) most = 0;
   for (int i = tid; i < a.slice >> 5; i += MK_NT) bits[i] = 0u;
   __syncthreads();
   int mine = 0;
@@ -124,7 +128,6 @@ __global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const Lis
   __syncthreads();
   // Items of 4 rows x 256 entries.  An item's loads are issued without branches (from within the table, used or not), and the
   // next one's before it is marked: with a branch around each load the compiler waits for all of them between items.
-  const int p0 = (int)blockIdx.x * a.slice;
   const uint32_t many = (uint32_t)clamp_i(a.num_pages - p0, 0, a.slice);  // pages of the slice; a page before it wraps
   const int wide = (most + 255) >> 8, items = ((a.B + 3) >> 2) * wide;
   auto fetch = [&](int it, uint32_t (&v)[16]) {
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const Lis
       }
     }
   };
-  const int begin = (int)blockIdx.y * (MK_NT / 64) + w, step = (int)gridDim.y * (MK_NT / 64);
+  const int begin = part * (MK_NT / 64) + w, step = parts * (MK_NT / 64);
   if (begin < items) {
     uint32_t one[16], two[16];
     fetch(begin, one);
@@ -167,6 +170,31 @@ __global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const Lis
     }
   }
   __syncthreads();
+}
+
+// Of a pool of one block, whose groups of 64 bits are in LDS: pages in use, and those of them before page number `live`
+__device__ __forceinline__ void count_block(const uint64_t* groups, int* sum) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < 64) {
+    const uint64_t g = groups[lane];
+    const int live = wave_add(__popcll(g)), cut = clamp_i(live - 64 * lane, 0, 64);
+    const int low = wave_add(__popcll(cut == 64 ? g : g & ((1ull << cut) - 1)));
+    if (lane == 0) {
+      sum[0] = live;
+      sum[1] = low;
+    }
+  }
+  __syncthreads();
+}
+
+template <int THEN>
+__global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const ListArgs l) {
+  extern __shared__ __attribute__((aligned(16))) int dyn[];
+  __shared__ int sum[2], before[LS_BLOCK / 64];
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [slice / 32]
+  int* held = dyn + (a.slice >> 5);                   // [B]
+  const int tid = threadIdx.x, lane = tid & 63;
+  mark_slice_bits(a, bits, held, (int)blockIdx.x * a.slice, blockIdx.y, gridDim.y);
   if constexpr (THEN == 0) {
     // 128 words of a block: two waves' lanes
     for (int i = tid; i < a.slice >> 5; i += MK_NT) {
@@ -181,16 +209,7 @@ __global__ __launch_bounds__(MK_NT) void mark_kernel(const MarkArgs a, const Lis
       a.counts[(size_t)blockIdx.x * (a.slice / LS_BLOCK) + i] = held[2 * i] + held[2 * i + 1];
   } else {
     const uint64_t* groups = reinterpret_cast<const uint64_t*>(bits);
-    if (w == 0) {
-      const uint64_t g = groups[lane];
-      const int live = wave_add(__popcll(g)), cut = clamp_i(live - 64 * lane, 0, 64);
-      const int low = wave_add(__popcll(cut == 64 ? g : g & ((1ull << cut) - 1)));
-      if (lane == 0) {
-        sum[0] = live;
-        sum[1] = low;
-      }
-    }
-    __syncthreads();
+    count_block(groups, sum);
     list_block<THEN == 2>(l, groups, before, 0, 0, sum[0], sum[1]);
   }
 }
@@ -338,15 +357,17 @@ constexpr int CP_PIECE = 2048;  // bytes that a wave moves at a time: 2 loads of
 // take 99.6 us, 5.3 TB/s read and written.  Small units in many waves, and stores past the caches, which leaves those to pages that
 // are read several times: 8 KB per wave and plain stores take 103.4 us, 431 pages forked from 64 in 6 layers 28.1 (20.3), a
 // pool of 12000 pages of 32 KB made dense (2954 move) 51.1 (41.6); 1 KB per wave 110, 26 and 52.
-__device__ __forceinline__ void copy_pages(const CopyArgs& a, long long unit, long long step) {
+// pair(i) gives pages (from, into) number i of n.
+template <class Pair>
+__device__ __forceinline__ void copy_pages(const CopyArgs& a, int n, long long unit, long long step, Pair pair) {
   const int lane = threadIdx.x & 63;
-  const int n = a.count ? clamp_i(*a.count, 0, a.most) : a.most;
   const int per = a.layers * 2 * a.pieces;
   const long long units = (long long)n * per;
   for (; unit < units; unit += step) {
     const int i = (int)(unit / per), rest = (int)(unit - (long long)i * per);
     const int piece = rest % a.pieces, z = (rest / a.pieces) & 1, y = rest / a.pieces >> 1;
-    const int s = a.src[i], d = a.dst[i];
+    const int2 p2 = pair(i);
+    const int s = p2.x, d = p2.y;
     if (s < 0 || s >= a.from.pages || d < 0 || d >= a.into.pages) continue;
     const long long ps = (long long)y * a.from.pages + s, pd = (long long)y * a.into.pages + d;
     const u4* p = reinterpret_cast<const u4*>(a.from.data[z] + ps * a.page_bytes + piece * CP_PIECE) + lane;
@@ -363,10 +384,15 @@ __device__ __forceinline__ void copy_pages(const CopyArgs& a, long long unit, lo
       for (int h = lane; h < a.KV; h += 64) a.into.scale[z][pd * a.KV + h] = a.from.scale[z][ps * a.KV + h];
   }
 }
+// pairs from the lists
+__device__ __forceinline__ void copy_listed(const CopyArgs& a, long long unit, long long step) {
+  const int n = a.count ? clamp_i(*a.count, 0, a.most) : a.most;
+  copy_pages(a, n, unit, step, [&](int i) { return make_int2(a.src[i], a.dst[i]); });
+}
 
 __global__ __launch_bounds__(CP_NT) void copy_kernel(const CopyArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  copy_pages(a, (long long)blockIdx.x * (CP_NT / 64) + w, (long long)gridDim.x * (CP_NT / 64));
+  copy_listed(a, (long long)blockIdx.x * (CP_NT / 64) + w, (long long)gridDim.x * (CP_NT / 64));
 }
 
 struct RenameArgs {
@@ -378,7 +404,7 @@ struct RenameArgs {
 __global__ __launch_bounds__(CP_NT) void move_kernel(const CopyArgs a, const RenameArgs t) {
   if ((int)blockIdx.x >= t.groups) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    copy_pages(a, (long long)(blockIdx.x - t.groups) * (CP_NT / 64) + w, (long long)(gridDim.x - t.groups) * (CP_NT / 64));
+    copy_listed(a, (long long)(blockIdx.x - t.groups) * (CP_NT / 64) + w, (long long)(gridDim.x - t.groups) * (CP_NT / 64));
     return;
   }
   const int live = t.status[0];
@@ -393,6 +419,50 @@ __global__ __launch_bounds__(CP_NT) void move_kernel(const CopyArgs a, const Ren
   }
 }
 
+// A small pool made dense in one launch: every workgroup finds the moves for itself, keeps them in LDS, and does its share.  The
+// new table must not be the old one, which others still read.  16 requests on 185 of 512 pages, 113 of which move, in 2 layers:
+// a call takes 12.7 us (7.2 on the GPU), with a launch for the moves before that of the copies 15.6 (4.9 and 3.3).
+__global__ __launch_bounds__(MK_NT) void dense_kernel(const MarkArgs a, const CopyArgs c, int32_t* out, int32_t* status) {
+  extern __shared__ __attribute__((aligned(16))) int dyn[];
+  __shared__ int sum[2], before[LS_BLOCK / 64];
+  __shared__ uint16_t from[LS_BLOCK / 2], holes[LS_BLOCK / 2];
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);  // [LS_BLOCK / 32]
+  int* held = dyn + LS_BLOCK / 32;                    // [B]
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  mark_slice_bits(a, bits, held, 0, 0, 1);
+  const uint64_t* groups = reinterpret_cast<const uint64_t*>(bits);
+  count_block(groups, sum);
+  groups_before(groups, before);
+  const int live = sum[0], used_low = sum[1], moves = live - used_low;
+  auto used = [&](int p) { return before[p >> 6] + __popcll(groups[p >> 6] & ((1ull << (p & 63)) - 1)); };  // before page p
+#pragma unroll
+  for (int i = 0; i < LS_BLOCK / MK_NT; ++i) {
+    const int p = tid + i * MK_NT;
+    if (p >= a.num_pages) continue;
+    const bool in_use = (groups[p >> 6] >> (p & 63)) & 1;
+    if (in_use && p >= live) from[used(p) - used_low] = (uint16_t)p;
+    if (!in_use && p < live) holes[p - used(p)] = (uint16_t)p;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) {
+    status[0] = live;
+    status[1] = moves;
+  }
+  const int wave = blockIdx.x * (MK_NT / 64) + w, waves = gridDim.x * (MK_NT / 64);
+  for (int b = wave; b < a.B; b += waves) {
+    const int n = held[b];
+    for (int j = lane; j < a.max_pages; j += 64) {
+      const int64_t at = (int64_t)b * a.max_pages + j;
+      int id = a.table[at];
+      if (j < n && id >= live && id < a.num_pages) id = holes[used(id) - used_low];
+      out[at] = id;
+    }
+  }
+  copy_pages(c, moves, wave, waves, [&](int i) {
+    return make_int2(__builtin_amdgcn_readfirstlane((int)from[i]), __builtin_amdgcn_readfirstlane((int)holes[i]));
+  });
+}
+
 // Workgroups for `most` pages, of which there may be fewer: up to 16384.  With 2048 (about what the GPU holds at once) the
 // copies above take 101.2, 20.4 and 43.0 us.
 unsigned copy_groups(const CopyArgs& a) {
@@ -404,20 +474,23 @@ unsigned copy_groups(const CopyArgs& a) {
 
 struct ForkArgs {
   const int32_t *parents, *table, *lens, *free_pages, *free_count;
-  int32_t *out, *out_lens, *status, *src, *dst;
+  int32_t *out, *out_lens, *status;
   int32_t N, B, max_pages, psh, n_free;
 };
 
 // Row i of the new table goes on from row parents[i].  The first of a parent's rows keeps its last page, if that is not
 // full; the others take a free one each, in their order.  Every workgroup finds this out for all rows (as the
-// plan's do), then writes its own.
-__global__ __launch_bounds__(FK_NT) void fork_kernel(const ForkArgs a) {
+// plan's do), then writes its own and copies its share of the pages: for few rows that takes as long as a second launch
+// would, a call for 16 rows of 4 requests and 12 pages in 18 layers takes 13.4 us in one launch (5.9 on the GPU), 17.5 in two (3.0
+// and 5.3); for 512 rows and 431 pages in 6 layers 22.5 and 20.3.
+__global__ __launch_bounds__(FK_NT) void fork_kernel(const ForkArgs a, const CopyArgs c) {
   extern __shared__ int sm[];
   __shared__ long long part[FK_NT / 64], carry;
   __shared__ int lost;
-  int* first = sm;        // [B] the first row of each parent
-  int* fresh = sm + a.B;  // [N] number of the free page that a row takes; -1: none; -2: refused
-  const int tid = threadIdx.x, lane = tid & 63, page = 1 << a.psh;
+  int* first = sm;              // [B] the first row of each parent
+  int* fresh = sm + a.B;        // [N] number of the free page that a row takes; -1: none; -2: refused
+  int* from = sm + a.B + a.N;   // [N] of each free page taken, the page that is copied there
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), page = 1 << a.psh;
   const int n_free = a.free_count ? clamp_i(*a.free_count, 0, a.n_free) : a.n_free;
   for (int b = tid; b < a.B; b += FK_NT) first[b] = INT32_MAX;
   if (tid == 0) lost = 0;
@@ -438,28 +511,24 @@ __global__ __launch_bounds__(FK_NT) void fork_kernel(const ForkArgs a) {
     const bool ok = !need || end <= n_free;
     refused += !ok;
     if (i < a.N) fresh[i] = !ok ? -2 : need ? (int)end - 1 : -1;
-    if (blockIdx.x == 0 && i < a.N) {
-      a.out_lens[i] = ok ? len : 0;
-      if (need && ok) {
-        a.src[end - 1] = a.table[(int64_t)p * a.max_pages + (len >> a.psh)];
-        a.dst[end - 1] = a.free_pages[end - 1];
-      }
-    }
+    if (need && ok) from[end - 1] = a.table[(int64_t)p * a.max_pages + (len >> a.psh)];
+    if (blockIdx.x == 0 && i < a.N) a.out_lens[i] = ok ? len : 0;
     if (tid == FK_NT - 1) carry = end;
     __syncthreads();
     taken = carry;
     __syncthreads();
   }
+  const int got = (int)(taken < n_free ? taken : n_free);
   if (blockIdx.x == 0) {
     if (refused) atomicAdd(&lost, refused);
     __syncthreads();
     if (tid == 0) {
-      a.status[0] = (int)(taken < n_free ? taken : n_free);
+      a.status[0] = got;
       a.status[1] = lost;
     }
   }
   // a wave for each row
-  for (int i = blockIdx.x * (FK_NT / 64) + (tid >> 6); i < a.N; i += gridDim.x * (FK_NT / 64)) {
+  for (int i = blockIdx.x * (FK_NT / 64) + w; i < a.N; i += gridDim.x * (FK_NT / 64)) {
     const int p = a.parents[i], f = fresh[i];
     const bool there = p >= 0 && p < a.B && f != -2;
     const int len = there ? clamp_i(a.lens[p], 0, a.max_pages << a.psh) : 0;
@@ -470,6 +539,8 @@ __global__ __launch_bounds__(FK_NT) void fork_kernel(const ForkArgs a) {
       a.out[(int64_t)i * a.max_pages + j] = id;
     }
   }
+  copy_pages(c, got, (long long)blockIdx.x * (FK_NT / 64) + w, (long long)gridDim.x * (FK_NT / 64),
+             [&](int i) { return make_int2(__builtin_amdgcn_readfirstlane(from[i]), a.free_pages[i]); });
 }
 
 int pages_ok(int32_t num_pages, int32_t page, int32_t max_pages, int32_t B) {
@@ -563,7 +634,7 @@ int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, 
                  const int32_t* kv_lens, const int32_t* free_pages, int32_t n_free, const int32_t* free_count,
                  void* k_cache, float* k_scale, void* v_cache, float* v_scale, int32_t layers, int32_t num_pages,
                  int32_t page, int32_t KV, int32_t hd, int32_t* new_table, int32_t* new_lens, int32_t* status,
-                 int32_t* copies, void* stream) {
+                 void* stream) {
   MLCV_TRY(pages_ok(num_pages, page, max_pages, B));
   MLCV_REQUIRE(n >= 0 && n_free >= 0, "negative size");
   MLCV_REQUIRE(n <= KV_MAX_REQ, "more than 4096 requests");
@@ -571,25 +642,19 @@ int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, 
   MLCV_TRY(pool_ok(a, k_cache, k_scale, v_cache, v_scale, num_pages, k_cache, k_scale, v_cache, v_scale, num_pages,
                    layers, page, KV, hd));
   MLCV_REQUIRE(status, "null output");
-  MLCV_REQUIRE(n == 0 || (parents && new_lens && copies && (new_table || max_pages == 0)), "null row array");
+  MLCV_REQUIRE(n == 0 || (parents && new_lens && (new_table || max_pages == 0)), "null row array");
   MLCV_REQUIRE(B == 0 || (kv_lens && (block_table || max_pages == 0)), "null request array");
   MLCV_REQUIRE(n_free == 0 || free_pages, "null free_pages");
-  const Ints arrays[] = {{new_table, (int64_t)n * max_pages}, {new_lens, n}, {status, 2}, {copies, 2 * (int64_t)n},
-                         {parents, n}, {block_table, (int64_t)B * max_pages}, {kv_lens, B}, {free_pages, n_free},
+  const Ints arrays[] = {{new_table, (int64_t)n * max_pages}, {new_lens, n}, {status, 2}, {parents, n}, {block_table, (int64_t)B * max_pages}, {kv_lens, B}, {free_pages, n_free},
                          {free_count, free_count ? 1 : 0}};
-  MLCV_REQUIRE(!overlap(arrays, 4, 9), "outputs overlap the inputs or one another");
+  MLCV_REQUIRE(!overlap(arrays, 3, 8), "outputs overlap the inputs or one another");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const ForkArgs f{parents, block_table, kv_lens, free_pages, free_count, new_table, new_lens, status, copies,
-                   copies + n, n, B, max_pages, log2_of(page), n_free};
-  const unsigned grid = (unsigned)std::max(1, std::min((n + FK_NT / 64 - 1) / (FK_NT / 64), 256));
-  fork_kernel<<<grid, FK_NT, (size_t)(B + n) * 4, st>>>(f);
-  MLCV_HIP(hipGetLastError());
-  a.src = copies;
-  a.dst = copies + n;
-  a.count = status;
-  a.most = std::min(n, n_free);
-  if (a.most == 0 || num_pages == 0) return 0;
-  copy_kernel<<<copy_groups(a), CP_NT, 0, st>>>(a);
+  const ForkArgs f{parents, block_table, kv_lens, free_pages, free_count, new_table, new_lens, status, n, B, max_pages,
+                   log2_of(page), n_free};
+  // a wave for each row, and for each unit of the pages as far as the GPU holds them at once
+  const int64_t units = num_pages ? (int64_t)std::min(n, n_free) * layers * 2 * a.pieces : 0;
+  const int64_t waves = std::max<int64_t>({1, std::min(n, 2048), std::min<int64_t>(units, 8192)});
+  fork_kernel<<<(unsigned)((waves + FK_NT / 64 - 1) / (FK_NT / 64)), FK_NT, (size_t)(B + 2 * n) * 4, st>>>(f, a);
   MLCV_HIP(hipGetLastError());
   return 0;
 }
@@ -620,18 +685,28 @@ int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, co
                          {block_table, new_table == block_table ? 0 : entries}};
   MLCV_REQUIRE(!overlap(arrays, 3, 5), "outputs overlap the inputs or one another");
   const MarkSizes m = mark_sizes(num_pages);
+  // every move has a hole: at most half of the pages move
+  a.most = num_pages / 2;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (m.blocks == 1 && new_table != block_table && ((int64_t)B + 3) / 4 * ((max_pages + 255) / 256) <= 2 * (MK_NT / 64)) {
+    // the table is marked in two rounds of a workgroup's waves at most
+    const MarkArgs k{block_table, kv_lens, nullptr, nullptr, B, max_pages, log2_of(page), num_pages, m.slice,
+                     aligned16(block_table) && max_pages % 4 == 0};
+    const int64_t waves = std::max<int64_t>({1, B, std::min<int64_t>((int64_t)a.most * layers * 2 * a.pieces, 8192)});
+    dense_kernel<<<(unsigned)((waves + MK_NT / 64 - 1) / (MK_NT / 64)), MK_NT, (size_t)(LS_BLOCK / 32 + B) * 4, st>>>(
+        k, a, new_table, status);
+    MLCV_HIP(hipGetLastError());
+    return 0;
+  }
   ListArgs l{};
   l.to = static_cast<int32_t*>(workspace) + m.words + m.counts;
   l.holes = l.to + num_pages;
   l.from = l.holes + num_pages;
   l.status = status;
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   MLCV_TRY(list_launch<true>(block_table, kv_lens, B, max_pages, page, num_pages, m, static_cast<int32_t*>(workspace), l, st));
   a.src = l.from;
   a.dst = l.holes;
   a.count = status + 1;
-  // every move has a hole: at most half of the pages move
-  a.most = num_pages / 2;
   const RenameArgs t{block_table, kv_lens, l.to, l.holes, status, new_table, B, max_pages, log2_of(page), num_pages,
                      std::min(B, 256)};
   const unsigned grid = t.groups + (a.most ? copy_groups(a) : 0);

@@ -71,12 +71,6 @@ __device__ __forceinline__ u64 lane_of(u64 v, int lane) {
   return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
-
 // v of lane ^ M, M < 16, within the registers: the crossbar of LDS takes four times as long
 template <int M>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
@@ -88,6 +82,28 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
   if constexpr (M == 4) return dpp(dpp(v, std::integral_constant<int, 0x1b>()), std::integral_constant<int, 0x141>());  // 3 ^ 7
   if constexpr (M == 8) return dpp(v, std::integral_constant<int, 0x128>());  // rows of 16 turned by 8
 }
+// f over all lanes, in every lane
+template <class F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+  auto dpp = [](float x, auto ctrl) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = f(v, dpp(v, std::integral_constant<int, 0xb1>()));   // lane ^ 1
+  v = f(v, dpp(v, std::integral_constant<int, 0x4e>()));   // ^ 2
+  v = f(v, dpp(v, std::integral_constant<int, 0x141>()));  // the other four of eight
+  v = f(v, dpp(v, std::integral_constant<int, 0x140>()));  // the other eight of sixteen
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float all_max(float v) {
+  return wave_all(v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float all_sum(float v) {
+  return wave_all(v, [](float x, float y) { return x + y; });
+}
+
 // one step of the bitonic network over lanes S apart
 template <int S>
 __device__ __forceinline__ u64 exchange(u64 v, bool larger) {
@@ -198,7 +214,7 @@ struct Scan {
   }
   __device__ __forceinline__ void raise(float big) {
     if (!__any(big > v.m)) return;
-    const float wm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(big))));
+    const float wm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(all_max(big))));
     base = base_of(wm, c);
     rebase(v, wm, base, c);
   }
@@ -316,14 +332,23 @@ struct Scan {
     }
   }
   __device__ __forceinline__ void end() {
-    v.s = wave_sum(v.s);
-    v.u = wave_sum(v.u);
+    v.s = all_sum(v.s);
+    v.u = all_sum(v.u);
   }
 };
 
-// The row's results by one wave, from its sums and its sorted best.
+// The logit of a row's given token number i, and whether there is one
 template <int TYPE>
-__device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 list, int lane) {
+__device__ __forceinline__ float given_logit(const LpArgs& a, int row, int i, bool& there) {
+  typedef typename LpType<TYPE>::T T;
+  const int t = i < a.given ? a.tokens[(int64_t)row * a.given + i] : -1;
+  there = t >= 0 && t < a.vocab;
+  return there ? (float)load_global(static_cast<const T*>(a.x) + (int64_t)row * a.stride + t) : 0.f;
+}
+
+// The row's results by one wave, from its sums and its sorted best; z0, there: given_logit of token number `lane`.
+template <int TYPE>
+__device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 list, int lane, float z0, bool there) {
   typedef typename LpType<TYPE>::T T;
   const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
   // the sums are relative to the rounded mc; its distance from m c counts where the two meet
@@ -333,9 +358,8 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 lis
   auto lp = [&](float z) { return v.s == 0.f ? -INFINITY : (z - v.m) * a.scale - ls; };
   if (lane == 0 && a.entropy) a.entropy[row] = v.s == 0.f ? 0.f : le + LN2 * (v.u / v.s);
   for (int i = lane; i < a.given; i += 64) {
-    const int64_t at = (int64_t)row * a.given + i;
-    const int t = a.tokens[at];
-    a.lp[at] = t >= 0 && t < a.vocab ? lp((float)load_global(x + t)) : 0.f;
+    if (i != lane) z0 = given_logit<TYPE>(a, row, i, there);
+    a.lp[(int64_t)row * a.given + i] = there ? lp(z0) : 0.f;
   }
   if (!a.k) return;
   int32_t* ids = a.top_ids + (int64_t)row * a.k;
@@ -447,7 +471,9 @@ __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
       return;
     }
   }
-  finish<TYPE>(a, row, scan.v, scan.list, lane);
+  bool there;
+  const float z0 = given_logit<TYPE>(a, row, lane, there);
+  finish<TYPE>(a, row, scan.v, scan.list, lane, z0, there);
 }
 
 // The splits of a row: a workgroup per row, its waves take splits in turn and meet in pairs.
@@ -457,6 +483,14 @@ __global__ __launch_bounds__(64 * LP_JW) void logprobs_join_kernel(const LpArgs 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x;
   const int64_t o = (int64_t)row * a.S;
   u64 list = 0;
+  // the sums and the given tokens are on their way while the lists are merged
+  f4 p = {-INFINITY, 0.f, 0.f, 0.f};
+  float z0 = 0.f;
+  bool there = false;
+  if (w == 0) {
+    if (lane < a.S) p = load_global(reinterpret_cast<const f4*>(a.stats) + o + lane);
+    z0 = given_logit<TYPE>(a, row, lane, there);
+  }
   if (a.k) {
     constexpr int Q = 4;  // lists on their way at once
     for (int s0 = w; s0 < a.S; s0 += Q * LP_JW) {
@@ -482,17 +516,16 @@ __global__ __launch_bounds__(64 * LP_JW) void logprobs_join_kernel(const LpArgs 
   if (w > 0) return;
   Sums v{-INFINITY, 0.f, 0.f};
   for (int s0 = 0; s0 < a.S; s0 += 64) {
-    const int s = s0 + lane;
-    const f4 p = s < a.S ? load_global(reinterpret_cast<const f4*>(a.stats) + o + s) : (f4){-INFINITY, 0.f, 0.f, 0.f};
-    const float m = fmaxf(v.m, wave_max(p[0]));
+    if (s0 > 0) p = s0 + lane < a.S ? load_global(reinterpret_cast<const f4*>(a.stats) + o + s0 + lane) : (f4){-INFINITY, 0.f, 0.f, 0.f};
+    const float m = fmaxf(v.m, all_max(p[0]));
     const Base b = base_of(m, a.c);
     Sums q{p[0], p[1], p[2]};
     rebase(q, m, b, a.c);
     rebase(v, m, b, a.c);
-    v.s += wave_sum(q.s);
-    v.u += wave_sum(q.u);
+    v.s += all_sum(q.s);
+    v.u += all_sum(q.u);
   }
-  finish<TYPE>(a, row, v, list, lane);
+  finish<TYPE>(a, row, v, list, lane, z0, there);
 }
 
 // How a call is cut: waves of a row (1 or 4), splits of it and their chunks

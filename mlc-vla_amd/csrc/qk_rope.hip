@@ -71,14 +71,16 @@ struct Piece {
   }
 };
 
+// What is fused is written out below, so that every form of the kernel rounds alike.
+//
 // sin and cos of 2 pi r, |r| <= 1/2: the nearest quarter turn is taken off, which leaves |x| <= pi / 4, where the Taylor
 // polynomials to x^9 and x^10 end within 2e-9
 __device__ __forceinline__ void turn(float r, float& s, float& c) {
   const float n = __builtin_rintf(4.0f * r);
-  const float x = (r - 0.25f * n) * 6.283185307179586f, z = x * x;
-  const float sx = x * (1.0f + z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880)))));
-  const float cx =
-      1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 - z * (1.0f / 3628800)))));
+  const float x = __builtin_fmaf(-0.25f, n, r) * 6.283185307179586f, z = x * x;
+  auto f = [](float a, float b, float c) { return __builtin_fmaf(a, b, c); };
+  const float sx = x * f(z, f(z, f(z, f(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+  const float cx = f(z, f(z, f(z, f(z, f(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
   const int q = (int)n;
   const float a = q & 1 ? cx : sx, b = q & 1 ? sx : cx;
   s = q & 2 ? -a : a;
@@ -166,17 +168,28 @@ __global__ __launch_bounds__(RP_NT) void qk_rope_kernel(const RopeArgs a) {
       if constexpr (NORM) {
         float sq = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sq += x[e] * x[e];
+        for (int e = 0; e < 16; ++e) sq = __builtin_fmaf(x[e], x[e], sq);
 #pragma unroll
         for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor(sq, o);
-        const float n = 1.0f / sqrtf(sq * (1.0f / HD) + a.eps);
+        const float n = 1.0f / sqrtf(__builtin_fmaf(sq, 1.0f / HD, a.eps));
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = x[e] * n * (z ? w[1][e] : w[0][e]);
       }
+      if (a.rd == HD || rot) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u.v[e] = (T)(x[e] * c[e] - x[8 + e] * s[e]);
-        v.v[e] = (T)(x[8 + e] * c[e] + x[e] * s[e]);
+        for (int e = 0; e < 8; ++e) {
+          float y0 = __builtin_fmaf(x[e], c[e], -(x[8 + e] * s[e])), y1 = __builtin_fmaf(x[8 + e], c[e], x[e] * s[e]);
+          // rounded to float32 first everywhere: some forms would get an instruction that rounds to 16 bits at once
+          asm("" : "+v"(y0), "+v"(y1));
+          u.v[e] = (T)y0;
+          v.v[e] = (T)y1;
+        }
+      } else if constexpr (NORM) {  // not rotated: by an angle of 0 an infinite neighbour would make it NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          u.v[e] = (T)x[e];
+          v.v[e] = (T)x[8 + e];
+        }
       }
       T* o = static_cast<T*>(z ? a.out[1] : a.out[0]) + (int64_t)t * (z ? a.otok[1] : a.otok[0]) +
              (int64_t)h * (z ? a.ohead[1] : a.ohead[0]);
@@ -238,6 +251,12 @@ extern "C" int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const 
   MLCV_REQUIRE(q && k && q_out && k_out && (positions || (cu_seqlens && kv_lens)), "null pointer");
   // the last round of a wave's tokens still is an int
   MLCV_REQUIRE(tokens <= INT32_MAX - 16384, "more than 2^31 - 16385 tokens");
+  auto in_place = [&](int64_t tok, int64_t otok, int64_t heads, int64_t head, int64_t ohead) {
+    return (tokens == 1 || tok == otok) && (heads == 1 || head == ohead);
+  };
+  MLCV_REQUIRE((q != q_out || in_place(q_tok, qo_tok, H, q_head, qo_head)) &&
+                   (k != k_out || in_place(k_tok, ko_tok, KV, k_head, ko_head)),
+               "an out that is its input must have its strides");
   MLCV_REQUIRE(rows_apart(tokens, qo_tok, H, qo_head, hd) && rows_apart(tokens, ko_tok, KV, ko_head, hd),
                "rows of out overlap");
   RopeArgs a{};

@@ -92,7 +92,7 @@ SIGNATURES = {
     "mlcv_kv_free": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "mlcv_kv_copy": (ctypes.c_int, [_vp, _vp, _i32] + [_vp] * 4 + [_i32] + [_vp] * 4 + [_i32] * 5 + [_vp]),
     "mlcv_kv_fork": (ctypes.c_int, [_vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp] + [_i32] * 5
-                     + [_vp] * 5),
+                     + [_vp] * 4),
     "mlcv_kv_compact_workspace": (ctypes.c_int, [_i32, ctypes.POINTER(ctypes.c_size_t)]),
     "mlcv_kv_compact": (ctypes.c_int, [_vp, _i32, _i32] + [_vp] * 5 + [_i32] * 5 + [_vp] * 3 + [ctypes.c_size_t, _vp]),
     "mlcv_kv_write": (ctypes.c_int, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp,

@@ -135,9 +135,7 @@ def _given(fn: str, out, q: torch.Tensor, dev: int) -> torch.Tensor:
     return o
 
 
-def _count(fn: str, free_count, dev: int) -> Optional[int]:
-    if free_count is None:
-        return None
+def _count(fn: str, free_count, dev: int) -> int:
     c = _t(free_count)
     if not (c.dtype is _I32 and c.shape == (1,) and c.get_device() == dev):
         _refuse(fn, dev, (("free_count", c, (_I32,), (1,), True),))
@@ -179,7 +177,7 @@ def kv_plan(past_lens, new_lens, block_table, free_pages, *, num_pages: int, pag
             _refuse("kv_plan", dev, tuple(("out." + f, t, (_I32,), (k,), True) for f, t, k in
                                           zip(KVPlan._fields, (cu, lens, slots, status), (n + 1, n, tokens, 2))))
     _call("mlcv_kv_plan_counted", dev, past.data_ptr(), new.data_ptr(), n, free.data_ptr(), free.shape[0],
-          _count("kv_plan", free_count, dev), num_pages, page_size, table.data_ptr(), wide, cu.data_ptr(),
+          None if free_count is None else _count("kv_plan", free_count, dev), num_pages, page_size, table.data_ptr(), wide, cu.data_ptr(),
           lens.data_ptr(), slots.data_ptr(), tokens, status.data_ptr())
     return out
 
@@ -234,7 +232,12 @@ def qk_rope(q, k, cu_seqlens=None, kv_lens=None, *, positions=None, theta: float
                 _refuse("qk_rope", dev, (("qk"[i] + "_weight", w, (wt,), (hd,), True),))
             at[i] = w.data_ptr()
         wt = _CODE[wt]
-    qo, ko = (_like(q), _like(k)) if out is None else (_given("qk_rope", x, y, dev) for x, y in zip(out, (q, k)))
+    if out is None:
+        qo, ko = _like(q), _like(k)
+    else:
+        if len(out) != 2:
+            _bad("qk_rope", "out", "is not two tensors")
+        qo, ko = _given("qk_rope", out[0], q, dev), _given("qk_rope", out[1], k, dev)
     qt, qh, _ = q.stride()
     kt, kh, _ = k.stride()
     qot, qoh, _ = qo.stride()
@@ -373,13 +376,12 @@ def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, bidir=None, sc
 
 
 def _pool(fn: str, k, k_scale, v, v_scale):
-    """The four tensors of a cache, of one layer or (with one more dim in front) several, and (device, layers, pages, KV,
-    page, hd)."""
-    c = tuple(_t(x) for x in (k, k_scale, v, v_scale))
-    kc, ks, vc, vs = c
+    """A cache's four tensors, of one layer or (with one more dim in front) several: their addresses, and (device, layers,
+    pages, KV, page, hd)."""
+    kc, ks, vc, vs = _t(k), _t(k_scale), _t(v), _t(v_scale)
     dev, shape = kc.get_device(), tuple(kc.shape)
     size = (1,) + shape if len(shape) == 4 else shape if len(shape) == 5 else (-1,) * 5
-    pages, kv, page, hd = size[1:]
+    _, pages, kv, page, hd = size
     top = shape[:-2]
     if not (kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and size[0] >= 0
             and vc.shape == top + (hd, page) and ks.shape == top and vs.shape == top and kc.is_contiguous()
@@ -388,18 +390,20 @@ def _pool(fn: str, k, k_scale, v, v_scale):
         _refuse(fn, dev, (("k_cache", kc, (_F8,), shape if len(shape) == 5 else (None,) * 4, True),
                           ("k_scale", ks, (_F32,), top, True), ("v_cache", vc, (_F8,), top + (hd, page), True),
                           ("v_scale", vs, (_F32,), top, True)))
-    return c, (dev,) + size
+    return (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()), (dev,) + size
 
 
-def _rows(fn: str, block_table, kv_lens, dev: int):
-    """(table, lengths, rows, entries of a row)"""
+def _rows(fn: str, block_table, kv_lens, dev: Optional[int] = None):
+    """(table, lengths, device, rows, entries of a row)"""
     table, lens = _t(block_table), _t(kv_lens)
+    if dev is None:
+        dev = table.get_device()
     n, wide = table.shape if table.dim() == 2 else (-1, 0)
     if not (table.dtype is _I32 and lens.dtype is _I32 and lens.shape == (n,) and table.is_contiguous()
             and lens.is_contiguous() and dev >= 0 and table.get_device() == lens.get_device() == dev):
         b = table.shape[0] if table.dim() else None
         _refuse(fn, dev, (("block_table", table, (_I32,), (None, None), True), ("kv_lens", lens, (_I32,), (b,), True)))
-    return table, lens, n, wide
+    return table, lens, dev, n, wide
 
 
 def _outs(fn: str, dev: int, out, shapes):
@@ -413,18 +417,19 @@ def _outs(fn: str, dev: int, out, shapes):
     return ts
 
 
-@functools.lru_cache(maxsize=256)
 def _pages_workspace(name: str, num_pages: int) -> int:
     n = ctypes.c_size_t()
     N.call(name, num_pages, ctypes.byref(n))
     return n.value
 
 
+@functools.lru_cache(maxsize=256)
 def kv_free_workspace(num_pages: int) -> int:
     """Bytes of workspace of ``kv_free`` (mlcv_kv_free_workspace)."""
     return _pages_workspace("mlcv_kv_free_workspace", num_pages)
 
 
+@functools.lru_cache(maxsize=256)
 def kv_compact_workspace(num_pages: int) -> int:
     """Bytes of workspace of ``kv_compact`` (mlcv_kv_compact_workspace)."""
     return _pages_workspace("mlcv_kv_compact_workspace", num_pages)
@@ -443,8 +448,7 @@ def kv_free(block_table, kv_lens, *, num_pages: int, page_size: int, out: Option
             workspace=None) -> KVFree:
     """The pages that no row of block_table [B, max_pages] holds, as the free list of the next plan or fork
     (mlcv_kv_free).  A finished request's length is 0; one that a plan refused still has its old length."""
-    dev = _t(block_table).get_device()
-    table, lens, n, wide = _rows("kv_free", block_table, kv_lens, dev)
+    table, lens, dev, n, wide = _rows("kv_free", block_table, kv_lens)
     if not 0 <= num_pages < 1 << 27:
         _bad("kv_free", "num_pages", "is negative or past 2^27 - 1")
     if out is None:
@@ -471,8 +475,8 @@ def kv_copy(src, dst, k_cache, k_scale, v_cache, v_scale, *, into=None) -> None:
     if not (s.dtype is _I32 and d.dtype is _I32 and d.shape == (n,) and s.is_contiguous() and d.is_contiguous()
             and s.get_device() == d.get_device() == dev):
         _refuse("kv_copy", dev, (("src", s, (_I32,), (None,), True), ("dst", d, (_I32,), (n,), True)))
-    _call("mlcv_kv_copy", dev, s.data_ptr(), d.data_ptr(), n, *(t.data_ptr() for t in cache), pages,
-          *(t.data_ptr() for t in to), pages if size is None else size[2], layers, page, kv, hd)
+    _call("mlcv_kv_copy", dev, s.data_ptr(), d.data_ptr(), n, *cache, pages, *to, pages if size is None else size[2],
+          layers, page, kv, hd)
 
 
 def kv_fork(parents, block_table, kv_lens, free_pages, k_cache, k_scale, v_cache, v_scale, *, free_count=None,
@@ -482,23 +486,22 @@ def kv_fork(parents, block_table, kv_lens, free_pages, k_cache, k_scale, v_cache
     copy, on pages from the front of ``free_pages``, of which ``free_count`` [1] are free (default: all).  The old table
     is done with; a request that stays beside its forks is a row of its own."""
     cache, (dev, layers, pages, kv, page, hd) = _pool("kv_fork", k_cache, k_scale, v_cache, v_scale)
-    table, lens, b, wide = _rows("kv_fork", block_table, kv_lens, dev)
+    table, lens, _, b, wide = _rows("kv_fork", block_table, kv_lens, dev)
     p, free = _t(parents), _t(free_pages)
     if not (p.dtype is _I32 and free.dtype is _I32 and p.dim() == 1 and free.dim() == 1 and p.is_contiguous()
             and free.is_contiguous() and p.get_device() == free.get_device() == dev):
         _refuse("kv_fork", dev, (("parents", p, (_I32,), (None,), True), ("free_pages", free, (_I32,), (None,), True)))
     n = p.shape[0]
     if out is None:
-        copies = torch.empty(2 * n + n * wide + n + 2, dtype=_I32, device=table.device)  # and the outputs
-        t, m = copies.as_strided((n, wide), (wide, 1), 2 * n), copies.as_strided((n,), (1,), n * (wide + 2))
-        status = copies.as_strided((2,), (1,), n * (wide + 3))
+        both = torch.empty(n * wide + n + 2, dtype=_I32, device=table.device)
+        t, m = both.as_strided((n, wide), (wide, 1)), both.as_strided((n,), (1,), n * wide)
+        status = both.as_strided((2,), (1,), n * (wide + 1))
         out = KVFork(Tensor(t, "int32"), Tensor(m, "int32"), Tensor(status, "int32"))
     else:
         t, m, status = _outs("kv_fork", dev, out, ((n, wide), (n,), (2,)))
-        copies = torch.empty(2 * n, dtype=_I32, device=table.device)
     _call("mlcv_kv_fork", dev, p.data_ptr(), n, table.data_ptr(), b, wide, lens.data_ptr(), free.data_ptr(),
-          free.shape[0], _count("kv_fork", free_count, dev), *(x.data_ptr() for x in cache), layers, pages, page, kv, hd,
-          t.data_ptr(), m.data_ptr(), status.data_ptr(), copies.data_ptr())
+          free.shape[0], None if free_count is None else _count("kv_fork", free_count, dev), *cache, layers, pages, page, kv,
+          hd, t.data_ptr(), m.data_ptr(), status.data_ptr())
     return out
 
 
@@ -507,7 +510,7 @@ def kv_compact(block_table, kv_lens, k_cache, k_scale, v_cache, v_scale, *, out:
     """Move the pages in use to the front of the pool, in all layers (mlcv_kv_compact); ``out``: its block table may be
     the given one."""
     cache, (dev, layers, pages, kv, page, hd) = _pool("kv_compact", k_cache, k_scale, v_cache, v_scale)
-    table, lens, n, wide = _rows("kv_compact", block_table, kv_lens, dev)
+    table, lens, _, n, wide = _rows("kv_compact", block_table, kv_lens, dev)
     if out is None:
         both = torch.empty(n * wide + 2, dtype=_I32, device=table.device)
         t, status = both.as_strided((n, wide), (wide, 1)), both.as_strided((2,), (1,), n * wide)
@@ -515,8 +518,8 @@ def kv_compact(block_table, kv_lens, k_cache, k_scale, v_cache, v_scale, *, out:
     else:
         t, status = _outs("kv_compact", dev, out, ((n, wide), (2,)))
     ws, size = _space("kv_compact", workspace, kv_compact_workspace(pages), table, dev)
-    _call("mlcv_kv_compact", dev, table.data_ptr(), n, wide, lens.data_ptr(), *(x.data_ptr() for x in cache), layers,
-          pages, page, kv, hd, t.data_ptr(), status.data_ptr(), ws.data_ptr(), size)
+    _call("mlcv_kv_compact", dev, table.data_ptr(), n, wide, lens.data_ptr(), *cache, layers, pages, page, kv, hd,
+          t.data_ptr(), status.data_ptr(), ws.data_ptr(), size)
     return out
 
 

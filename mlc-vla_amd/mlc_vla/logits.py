@@ -27,9 +27,6 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[Tensor]  # [rows, top]
 
 
-_OUT = ("float32", "float32", "int32", "float32")
-
-
 @functools.lru_cache(maxsize=4096)
 def token_logprobs_workspace(rows: int, vocab: int, top: int) -> int:
     """Bytes of workspace of ``token_logprobs`` for these sizes (mlcv_token_logprobs_workspace)."""
@@ -68,13 +65,15 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, scale: float = 1.0, out
         n = rows * given
         f = torch.empty(n + rows * (1 + 2 * top), dtype=_F32, device=x.device)
         h = f.as_strided((rows,), (1,), n)
-        lp = ids = tlp = None
+        lp = ids = tlp = given_lp = top_ids = top_lp = None
         if at is not None:
             lp = f.as_strided(shape, (1,) if len(shape) == 1 else (given, 1))
+            given_lp = Tensor(lp, "float32")
         if top:
             ids = f.view(_I32).as_strided((rows, top), (top, 1), n + rows)
             tlp = f.as_strided((rows, top), (top, 1), n + rows * (1 + top))
-        out = TokenLogprobs(*(None if o is None else Tensor(o, d) for o, d in zip((lp, h, ids, tlp), _OUT)))
+            top_ids, top_lp = Tensor(ids, "int32"), Tensor(tlp, "float32")
+        out = TokenLogprobs(given_lp, Tensor(h, "float32"), top_ids, top_lp)
     else:
         lp, h, ids, tlp = (None if o is None else _t(o) for o in out)
         for name, o, dt, want in (("logprobs", lp, _F32, shape), ("entropy", h, _F32, (rows,)),

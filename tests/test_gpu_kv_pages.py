@@ -258,7 +258,7 @@ def _check_compact(rng, table, lens, pages, page, kv=1, hd=64, layers=2, place=F
 
 @pytest.mark.parametrize("b,most,page,pages,hd,kv", [
     (1, 1, 16, 1, 64, 1), (2, 40, 16, 9, 64, 1), (16, 300, 16, 512, 256, 1), (5, 300, 128, 64, 128, 3), (40, 90, 32, 400, 64, 2),
-    (64, 900, 16, 4096, 64, 1), (300, 300, 16, 9001, 64, 1), (17, 4000, 64, 20000, 64, 1)])
+    (64, 900, 16, 4096, 64, 1), (300, 300, 16, 9001, 64, 1), (17, 4000, 64, 20000, 64, 1), (200, 60, 16, 900, 64, 1), (3, 14000, 16, 3000, 64, 1)])
 @pytest.mark.parametrize("place", [False, True])
 def test_compact(b, most, page, pages, hd, kv, place):
     rng = np.random.default_rng(pages + b)

@@ -150,6 +150,21 @@ def test_qk_rope_values_of_every_size():
     assert (got[1] - 5.96e-8 * 1e3).abs().max() < 1e-6
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_qk_rope_dims_that_are_not_turned(norm):
+    """They know nothing of one another: an infinity stays where it is (but for the norm, which is its head's)."""
+    x = torch.ones((3, 2, 128), device="cuda")
+    x[0, 0, 40], x[1, 1, 127], x[2, 0, 3] = float("inf"), float("nan"), float("inf")
+    got = C.qk_rope(x, x[:, :1], positions=_ints([5, 6, 0]), rotary_dim=32, norm=norm)[0].torch
+    bad = ~torch.isfinite(got)
+    if norm:
+        assert not bad[0, 1].any() and not bad[1, 0].any() and not bad[2, 1].any()
+    else:
+        want = torch.zeros_like(bad)
+        want[0, 0, 40] = want[1, 1, 127] = want[2, 0, 3] = want[2, 0, 19] = True  # 3 and 19 are a pair: inf * 0
+        assert torch.equal(bad, want) and torch.equal(got[..., 32:].nan_to_num(7.0), x[..., 32:].nan_to_num(7.0))
+
+
 def test_qk_rope_rotates_as_the_model_does():
     """The rotation of the joint attention's oracle."""
     from oracle import pi0_oracle as O
@@ -181,14 +196,17 @@ def test_qk_rope_arguments():
             ((q, k, cu, lens), dict(norm=True, q_weight=w[:32]), "q_weight expects"),
             ((q, k, cu, lens), dict(norm=True, q_weight=w, k_weight=w.float()), "q_weight has dtype"),
             ((q, k, cu, lens), dict(norm=True, k_weight=w.bfloat16()), "k_weight has dtype"),
-            ((q, k, cu, lens), dict(out=(q, k[:3])), "out expects")):
+            ((q, k, cu, lens), dict(out=(q, k[:3])), "out expects"),
+            ((q, k, cu, lens), dict(out=(q, k, k)), "two tensors")):
         with pytest.raises(ValueError, match=what):
             C.qk_rope(*args, **kw)
     for kw, what in ((dict(rotary_dim=24), "rotary"), (dict(rotary_dim=80), "rotary"), (dict(rotary_dim=-16), "rotary"),
                      (dict(theta=0.5), "theta"), (dict(theta=float("nan")), "theta"), (dict(norm=True, eps=-1.0), "eps"),
                      (dict(norm=True, eps=float("nan")), "eps"),
                      (dict(norm=True, q_weight=w, weight_offset=float("inf")), "w_offset"),
-                     (dict(out=(q[:1].expand(4, 4, 64), k)), "out overlap")):
+                     (dict(out=(q[:1].expand(4, 4, 64), k)), "must have its strides"),
+                     (dict(out=(q.clone()[:1].expand(4, 4, 64), k)), "out overlap"),
+                     (dict(out=(q.transpose(0, 1), k)), "must have its strides")):
         with pytest.raises(N.MlcvError, match=what):
             C.qk_rope(q, k, cu, lens, **kw)
 

@@ -17,8 +17,8 @@ P = 4096  # a pointer that is never followed
 
 def _rope(**kw):
     a = dict(q=P, q_tok=256, q_head=64, k=P, k_tok=128, k_head=64, dtype=1, tokens=5, cu=P, B=2, lens=P, pos=None, H=4,
-             KV=2, hd=64, rotary=64, theta=1e4, norm=0, qw=None, kw=None, w_dtype=1, w_offset=1.0, eps=1e-6, qo=P,
-             qo_tok=256, qo_head=64, ko=P, ko_tok=128, ko_head=64, stream=None)
+             KV=2, hd=64, rotary=64, theta=1e4, norm=0, qw=None, kw=None, w_dtype=1, w_offset=1.0, eps=1e-6, qo=2 * P,
+             qo_tok=256, qo_head=64, ko=3 * P, ko_tok=128, ko_head=64, stream=None)
     a.update(kw)
     N.call("mlcv_qk_rope", *a.values())
 
@@ -46,7 +46,7 @@ def _copy(**kw):
 
 def _fork(**kw):
     a = dict(parents=P, n=3, table=2 * P, B=2, max_pages=4, lens=3 * P, free=4 * P, n_free=5, count=5 * P, k=P, ks=P, v=P, vs=P,
-             layers=2, num_pages=8, page=16, KV=1, hd=64, out=6 * P, out_lens=7 * P, status=8 * P, copies=9 * P, stream=None)
+             layers=2, num_pages=8, page=16, KV=1, hd=64, out=6 * P, out_lens=7 * P, status=8 * P, stream=None)
     a.update(kw)
     N.call("mlcv_kv_fork", *a.values())
 
@@ -71,10 +71,10 @@ def _compact(**kw):
     (_copy, dict(KV=65535, page=128, hd=256), "2\\^30"),
     (_fork, dict(n=-1), "negative"), (_fork, dict(n=4097), "4096"), (_fork, dict(B=4097), "4096"), (_fork, dict(page=24), "page"),
     (_fork, dict(status=None), "null"), (_fork, dict(parents=None), "null"), (_fork, dict(out=None), "null"),
-    (_fork, dict(out_lens=None), "null"), (_fork, dict(copies=None), "null"), (_fork, dict(lens=None), "null"),
+    (_fork, dict(out_lens=None), "null"), (_fork, dict(lens=None), "null"),
     (_fork, dict(free=None), "free_pages"), (_fork, dict(k=None), "null"), (_fork, dict(hd=32), "head_dim"),
-    (_fork, dict(out=2 * P + 28), "overlap"), (_fork, dict(out_lens=P), "overlap"), (_fork, dict(copies=4 * P), "overlap"),
-    (_fork, dict(status=5 * P), "overlap"), (_fork, dict(out_lens=9 * P), "overlap"),
+    (_fork, dict(out=2 * P + 28), "overlap"), (_fork, dict(out_lens=P), "overlap"), (_fork, dict(out=4 * P - 8), "overlap"),
+    (_fork, dict(status=5 * P), "overlap"), (_fork, dict(out_lens=8 * P), "overlap"),
     (_compact, dict(page=24), "page"), (_compact, dict(ws_bytes=8), "workspace"), (_compact, dict(out=None), "null"),
     (_compact, dict(status=None), "null"), (_compact, dict(lens=None), "null"), (_compact, dict(v=None), "null"),
     (_compact, dict(out=P + 4), "overlap"), (_compact, dict(status=2 * P), "overlap"), (_compact, dict(ws=P), "overlap"),
@@ -95,6 +95,7 @@ def _compact(**kw):
     (_rope, dict(norm=1, kw=P, w_offset=float("nan")), "w_offset"), (_rope, dict(pos=P), "positions"),
     (_rope, dict(cu=None, lens=None), "positions"), (_rope, dict(lens=None), "null"), (_rope, dict(q=None), "null"),
     (_rope, dict(ko=None), "null"), (_rope, dict(tokens=2 ** 31 - 1), "2\\^31"), (_rope, dict(B=2 ** 31 - 1), "requests"),
+    (_rope, dict(qo=P, qo_tok=512), "strides"), (_rope, dict(ko=P, ko_head=-64), "strides"),
     (_rope, dict(H=2 ** 30), "heads"), (_rope, dict(qo_tok=0), "out overlap"), (_rope, dict(ko_head=32), "out overlap"),
 ])
 def test_refused(fn, bad, what):
