@@ -6,7 +6,7 @@
 // float32 angle is off by 2^-8 of a radian.  They are float64 products in turns, of which whole turns are taken off before
 // they become float32.
 //
-// Bound by memory for many tokens (24124 tokens of 40 heads of 128 in bf16: 92.4 us, 5.35 TB/s read and written; a copy reaches
+// Bound by memory for many tokens (24000 tokens of 40 heads of 128 in bf16: 91 us, 5.4 TB/s read and written; a copy reaches
 // 5.2), by latency for few (16 tokens of 9 heads of 256: 4 us).
 #include "kernels.h"
 #include "mlcvla.h"
@@ -26,6 +26,7 @@ struct RopeArgs {
   int64_t tok[2], head[2], otok[2], ohead[2];  // element strides
   const int32_t *cu, *kv_lens, *pos;
   int32_t tokens, B, H, rows, rd, w_f32;  // rows: heads of both
+  int32_t pack;                           // tokens that a wave takes at once
   float eps, offset;
   // turns per position of pair i = 8 j + e: one[e] times oct[b] for each bit b of j
   double oct[4], one[8];
@@ -46,15 +47,21 @@ struct RopeType<MLCV_DTYPE_F32> {
   typedef float T;
 };
 
-// 8 elements at p, by 16-byte loads and stores past the caches, as each element is read and written once, or one by one
-template <class T, bool VEC>
+// How a row is read: one by one, by 16-byte loads, or by such loads past the caches
+enum RopeLoads { RP_SINGLE, RP_WIDE, RP_FAR };
+
+// 8 elements at p; 16-byte stores go past the caches
+template <class T, int LOADS>
 struct Piece {
+  static constexpr bool VEC = LOADS != RP_SINGLE;
   T v[8] __attribute__((aligned(16)));
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<u4*>(v)[i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p) + i);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const u4* q = reinterpret_cast<const u4*>(p) + i;
+        reinterpret_cast<u4*>(v)[i] = LOADS == RP_FAR ? __builtin_nontemporal_load(q) : load_global(q);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = load_global(p + i);
@@ -102,63 +109,108 @@ __device__ __forceinline__ int find_request(const int32_t* cu, int B, int t, int
 }
 
 // A lane takes the dims 8 j .. + 7 and their partners rd / 2 further on of one head (two neighbouring pieces where they
-// are not rotated), so a wave 64 * 16 / HD heads of a token at a time, and a pair never leaves its lane.
-template <int TYPE, int HD, bool NORM, bool VEC>
-__global__ __launch_bounds__(RP_NT) void qk_rope_kernel(const RopeArgs a) {
+// are not rotated), so a wave 1024 / HD heads at a time, and a pair never leaves its lane: heads of one token, one round after
+// another, or of a.pack tokens at once where they have few.  Sines and cosines are computed once per token and pair, spread
+// over the lanes, and handed round through LDS; by each lane for its own pairs they are four to sixteen times as many
+// (100000 tokens of 3 heads of 64, one token at a time: 76 us; now 21.8).
+template <int TYPE, int HD, bool NORM, int LOADS>
+__global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
   typedef typename RopeType<TYPE>::T T;
   constexpr int LPH = HD / 16, NG = 64 / LPH;  // lanes of a head, heads at once
+  __shared__ double freq[HD / 2];              // turns per position
+  __shared__ __attribute__((aligned(16))) float sc[RP_NT / 64][2][NG * HD / 2];  // of each wave's tokens: sines, cosines
+  __shared__ __attribute__((aligned(16))) float wt[NORM ? 2 * HD : 1];
   const int lane = threadIdx.x & 63, g = lane / LPH, j = lane % LPH;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = a.rd / 2;  // pairs
   const bool rot = j < a.rd / 16;
-  const int lo = rot ? 8 * j : a.rd + 16 * (j - a.rd / 16), hi = rot ? lo + a.rd / 2 : lo + 8;
+  const int lo = rot ? 8 * j : a.rd + 16 * (j - a.rd / 16), hi = rot ? lo + half : lo + 8;
+  for (int i = threadIdx.x; i < half; i += RP_NT) {
+    double f = 1.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f = (i & 7) == e ? a.one[e] : f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) f *= (i >> (3 + b)) & 1 ? a.oct[b] : 1.0;
+    freq[i] = f;
+  }
+  if constexpr (NORM)
+    for (int i = threadIdx.x; i < 2 * HD; i += RP_NT) {
+      const int z = i / HD, d = i % HD;
+      wt[i] = !a.w[z] ? 1.0f
+                      : a.offset + (a.w_f32 ? load_global(static_cast<const float*>(a.w[z]) + d)
+                                            : (float)load_global(static_cast<const T*>(a.w[z]) + d));
+    }
+  __syncthreads();
 
-  double f[8];
-  {
-    double at = rot ? 1.0 : 0.0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) at *= (j >> b) & 1 ? a.oct[b] : 1.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = at * a.one[e];
+  // this lane's token of a block, and its head of the first round
+  const int mine = a.pack > 1 ? g / a.rows : 0, row0 = a.pack > 1 ? g - mine * a.rows : g;
+  const bool has = mine < a.pack && row0 < a.rows;
+  // up to 64 requests: their offsets and lengths stay in the lanes
+  int cu0 = 0, cu1 = 0, lens = 0;
+  if (!a.pos && lane < a.B) {
+    cu0 = load_global(a.cu + lane);
+    cu1 = load_global(a.cu + lane + 1);
+    lens = load_global(a.kv_lens + lane);
   }
-  float w[2][16];
-  if constexpr (NORM) {
-#pragma unroll
-    for (int z = 0; z < 2; ++z)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = e < 8 ? lo + e : hi + e - 8;
-        w[z][e] = !a.w[z] ? 1.0f
-                          : a.offset + (a.w_f32 ? load_global(static_cast<const float*>(a.w[z]) + d)
-                                                : (float)load_global(static_cast<const T*>(a.w[z]) + d));
-      }
-  }
-  const int waves = gridDim.x * (RP_NT / 64);
-  for (int t = __builtin_amdgcn_readfirstlane(blockIdx.x * (RP_NT / 64) + (threadIdx.x >> 6)); t < a.tokens;
-       t += waves) {
-    int64_t pos;
-    if (a.pos) {
-      pos = a.pos[t];
-    } else {
-      const int b = find_request(a.cu, a.B, t, lane);
-      if (b < 0) continue;
-      const int next = a.cu[b + 1];
-      if (next <= t) continue;  // behind the last request
-      pos = (int64_t)a.kv_lens[b] - ((int64_t)next - t);
-    }
-    float c[8], s[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double p = (double)pos * f[e];
-      turn((float)__builtin_fma((double)pos, f[e], -__builtin_rint(p)), s[e], c[e]);
-    }
-    for (int r0 = 0; r0 < a.rows; r0 += NG) {
-      const int row = r0 + g;
-      if (row >= a.rows) continue;
+  const int step = (int)gridDim.x * (RP_NT / 64) * a.pack;
+  for (int t0 = ((int)blockIdx.x * (RP_NT / 64) + w) * a.pack; t0 < a.tokens; t0 += step) {
+    const int t = t0 + mine;
+    Piece<T, LOADS> u, v;
+    auto in = [&](int row) {
       const int z = row >= a.H, h = z ? row - a.H : row;
       const T* p = static_cast<const T*>(z ? a.x[1] : a.x[0]) + (int64_t)t * (z ? a.tok[1] : a.tok[0]) +
                    (int64_t)h * (z ? a.head[1] : a.head[0]);
-      Piece<T, VEC> u, v;
       u.load(p + lo);
       v.load(p + hi);
+    };
+    bool there = has && t < a.tokens;
+    if (there) in(row0);  // on their way while the angles are found
+    int64_t pos = 0;      // this lane's token's
+    bool behind = false;
+    for (int i = 0; i < a.pack; ++i) {
+      const int ti = min(t0 + i, a.tokens - 1);
+      int64_t p = 0;
+      bool none = false;
+      if (a.pos) {
+        p = a.pos[ti];
+      } else {
+        int next = 0, len = 0;
+        if (a.B <= 64) {
+          const unsigned long long le = __ballot(lane < a.B && cu0 <= ti);
+          const int b = le ? 63 - __builtin_clzll(le) : 0;
+          next = le ? __builtin_amdgcn_readlane(cu1, b) : ti;
+          len = __builtin_amdgcn_readlane(lens, b);
+        } else {
+          const int b = find_request(a.cu, a.B, ti, lane);
+          next = b < 0 ? ti : a.cu[b + 1];
+          len = b < 0 ? 0 : a.kv_lens[b];
+        }
+        none = ti >= next;  // before the first request or behind the last
+        p = (int64_t)len - ((int64_t)next - ti);
+      }
+      // the pairs of this token
+      for (int k = lane; k < half; k += 64) {
+        const double f = freq[k], turns = (double)p * f;
+        float s, c;
+        turn((float)__builtin_fma((double)p, f, -__builtin_rint(turns)), s, c);
+        sc[w][0][i * half + k] = s;
+        sc[w][1][i * half + k] = c;
+      }
+      if (mine == i) behind = none;
+    }
+    there = there && !behind;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float s[8], c[8];
+    const int at = rot ? mine * half + 8 * j : 0;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(&sc[w][0][at + e]);
+      *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(&sc[w][1][at + e]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int row = row0; there && row < a.rows; row += NG) {
+      if (row != row0) in(row);
+      const int z = row >= a.H, h = z ? row - a.H : row;
       float x[16];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -173,7 +225,11 @@ __global__ __launch_bounds__(RP_NT) void qk_rope_kernel(const RopeArgs a) {
         for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor(sq, o);
         const float n = 1.0f / sqrtf(__builtin_fmaf(sq, 1.0f / HD, a.eps));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = x[e] * n * (z ? w[1][e] : w[0][e]);
+        for (int e = 0; e < 16; e += 4) {
+          const f4 y = *reinterpret_cast<const f4*>(wt + z * HD + (e < 8 ? lo + e : hi + e - 8));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[e + i] = x[e + i] * n * y[i];
+        }
       }
       if (a.rd == HD || rot) {
 #pragma unroll
@@ -199,27 +255,26 @@ __global__ __launch_bounds__(RP_NT) void qk_rope_kernel(const RopeArgs a) {
   }
 }
 
-template <int TYPE, int HD>
-int rope_launch(const RopeArgs& a, bool norm, bool vec, hipStream_t st) {
-  // What the GPU holds at once, four waves a SIMD, so that a wave's frequencies and weights serve many tokens and all end
-  // together: 24124 tokens of 40 heads of 128 in bf16 with norms take 92.4 us with 1024 workgroups, 98.7 with 2048, 108.9 with
-  // 512.  (Plain stores and loads 100.0, and 106.5 with 2048.)
-  const unsigned grid = (unsigned)std::min(((int64_t)a.tokens + 3) / 4, (int64_t)1024);
-  if (norm) {
-    if (vec) qk_rope_kernel<TYPE, HD, true, true><<<grid, RP_NT, 0, st>>>(a);
-    else qk_rope_kernel<TYPE, HD, true, false><<<grid, RP_NT, 0, st>>>(a);
-  } else {
-    if (vec) qk_rope_kernel<TYPE, HD, false, true><<<grid, RP_NT, 0, st>>>(a);
-    else qk_rope_kernel<TYPE, HD, false, false><<<grid, RP_NT, 0, st>>>(a);
-  }
+template <int TYPE, int HD, bool NORM>
+int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
+  a.pack = std::max(1, 64 / (HD / 16) / a.rows);
+  // What the GPU holds at once, five waves a SIMD, each taking tokens in turn: 24000 tokens of 40 heads of 128 with norms take
+  // 90.9 us with 1280 workgroups, 91.9 with 1024, 30000 of 9 heads of 256 57.1 and 60.1; with twice as many it is 96 and 67.
+  const unsigned grid = (unsigned)std::min(((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack), (int64_t)1280);
+  // Inputs that the GPU's L2 caches (32 MB) can hold are loaded through them, as the projection may just have written them: 3000
+  // tokens of 40 heads of 128 in bf16 (31 MB) 13.8 us, past the caches 16.7; 6000 31.5 and 30.3, 24000 100.5 and 94.8.
+  const bool far = (int64_t)a.tokens * a.rows * HD * (TYPE == MLCV_DTYPE_F32 ? 4 : 2) > (int64_t)40 << 20;
+  if (!vec) qk_rope_kernel<TYPE, HD, NORM, RP_SINGLE><<<grid, RP_NT, 0, st>>>(a);
+  else if (far) qk_rope_kernel<TYPE, HD, NORM, RP_FAR><<<grid, RP_NT, 0, st>>>(a);
+  else qk_rope_kernel<TYPE, HD, NORM, RP_WIDE><<<grid, RP_NT, 0, st>>>(a);
   MLCV_HIP(hipGetLastError());
   return 0;
 }
 template <int TYPE>
 int rope_launch(const RopeArgs& a, int hd, bool norm, bool vec, hipStream_t st) {
-  return hd == 64    ? rope_launch<TYPE, 64>(a, norm, vec, st)
-         : hd == 128 ? rope_launch<TYPE, 128>(a, norm, vec, st)
-                     : rope_launch<TYPE, 256>(a, norm, vec, st);
+  if (hd == 64) return norm ? rope_launch<TYPE, 64, true>(a, vec, st) : rope_launch<TYPE, 64, false>(a, vec, st);
+  if (hd == 128) return norm ? rope_launch<TYPE, 128, true>(a, vec, st) : rope_launch<TYPE, 128, false>(a, vec, st);
+  return norm ? rope_launch<TYPE, 256, true>(a, vec, st) : rope_launch<TYPE, 256, false>(a, vec, st);
 }
 
 }  // namespace
@@ -249,8 +304,8 @@ extern "C" int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const 
   MLCV_REQUIRE(!positions != !(cu_seqlens || kv_lens) || tokens == 0, "positions, or cu_seqlens and kv_lens");
   if (tokens == 0 || (!positions && B == 0)) return 0;
   MLCV_REQUIRE(q && k && q_out && k_out && (positions || (cu_seqlens && kv_lens)), "null pointer");
-  // the last round of a wave's tokens still is an int
-  MLCV_REQUIRE(tokens <= INT32_MAX - 16384, "more than 2^31 - 16385 tokens");
+  // the last round of a wave's tokens (at most 4096 waves' 16) still is an int
+  MLCV_REQUIRE(tokens <= INT32_MAX - 65536, "more than 2^31 - 65537 tokens");
   auto in_place = [&](int64_t tok, int64_t otok, int64_t heads, int64_t head, int64_t ohead) {
     return (tokens == 1 || tok == otok) && (heads == 1 || head == ohead);
   };

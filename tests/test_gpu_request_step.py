@@ -48,7 +48,8 @@ def _check_rope(q, k, pos, there, got, rd, theta, norm, ws, offset, eps):
 
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("hd,heads,kv,rd", [(64, 1, 1, 64), (64, 14, 2, 32), (128, 8, 8, 128), (128, 5, 1, 112),
-                                            (256, 8, 1, 256), (256, 3, 3, 16), (256, 2, 1, 0)])
+                                            (256, 8, 1, 256), (256, 3, 3, 16), (256, 2, 1, 0), (64, 1, 1, 48), (64, 2, 1, 16),
+                                            (128, 2, 1, 96), (256, 1, 1, 256)])
 @pytest.mark.parametrize("norm", [False, True])
 def test_qk_rope(dt, hd, heads, kv, rd, norm):
     rng = np.random.default_rng(hd + heads + rd + norm)
