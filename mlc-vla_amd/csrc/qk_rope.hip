@@ -50,30 +50,31 @@ struct RopeType<MLCV_DTYPE_F32> {
 // How a row is read: one by one, by 16-byte loads, or by such loads past the caches
 enum RopeLoads { RP_SINGLE, RP_WIDE, RP_FAR };
 
-// 8 elements at p; 16-byte stores go past the caches
+// 4 elements at p and 4 at p + gap (16-bit types: 8 in a row); 16-byte stores go past the caches
 template <class T, int LOADS>
 struct Piece {
   static constexpr bool VEC = LOADS != RP_SINGLE;
   T v[8] __attribute__((aligned(16)));
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void load(const T* p, int gap) {
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        const u4* q = reinterpret_cast<const u4*>(p) + i;
+        const u4* q = reinterpret_cast<const u4*>(p + i * gap);
         reinterpret_cast<u4*>(v)[i] = LOADS == RP_FAR ? __builtin_nontemporal_load(q) : load_global(q);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = load_global(p + i);
+      for (int i = 0; i < 8; ++i) v[i] = load_global(p + (i < 4 ? i : i - 4 + gap));
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
+  __device__ __forceinline__ void store(T* p, int gap) const {
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(reinterpret_cast<const u4*>(v)[i], reinterpret_cast<u4*>(p) + i);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        __builtin_nontemporal_store(reinterpret_cast<const u4*>(v)[i], reinterpret_cast<u4*>(p + i * gap));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = v[i];
+      for (int i = 0; i < 8; ++i) p[i < 4 ? i : i - 4 + gap] = v[i];
     }
   }
 };
@@ -108,11 +109,11 @@ __device__ __forceinline__ int find_request(const int32_t* cu, int B, int t, int
   }
 }
 
-// A lane takes the dims 8 j .. + 7 and their partners rd / 2 further on of one head (two neighbouring pieces where they
-// are not rotated), so a wave 1024 / HD heads at a time, and a pair never leaves its lane: heads of one token, one round after
-// another, or of a.pack tokens at once where they have few.  Sines and cosines are computed once per token and pair, spread
-// over the lanes, and handed round through LDS; by each lane for its own pairs they are four to sixteen times as many
-// (100000 tokens of 3 heads of 64, one token at a time: 76 us; now 21.8).
+// A lane takes 8 dims of one head and their partners rd / 2 further on (16 dims that are not rotated, where there are such),
+// so a wave 1024 / HD heads at a time, and a pair never leaves its lane: heads of one token, one round after another, or of
+// a.pack tokens at once where they have few.  Sines and cosines are computed once per token and pair, spread over the lanes,
+// and handed round through LDS; by each lane for its own pairs they are four to sixteen times as many (100000 tokens of 3
+// heads of 64, one token at a time: 76 us; now 23.1).
 template <int TYPE, int HD, bool NORM, int LOADS>
 __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
   typedef typename RopeType<TYPE>::T T;
@@ -123,8 +124,13 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
   const int lane = threadIdx.x & 63, g = lane / LPH, j = lane % LPH;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = a.rd / 2;  // pairs
-  const bool rot = j < a.rd / 16;
-  const int lo = rot ? 8 * j : a.rd + 16 * (j - a.rd / 16), hi = rot ? lo + half : lo + 8;
+  const int turned = a.rd / 16;  // lanes of a head that are
+  const bool rot = j < turned;
+  // Element e < 8 of the lane is dim lo + (e < 4 ? e : e - 4 + gap), element 8 + e the same from hi on.  float32: in fours, so
+  // that neighbouring lanes' 16-byte pieces are neighbours (12000 tokens of 40 heads of 128: 113.4 -> 97.8 us).
+  constexpr bool FOURS = sizeof(T) == 4;
+  const int step8 = FOURS ? 4 : 8, gap = FOURS ? 4 * (rot ? turned : LPH - turned) : 4;
+  const int lo = rot ? step8 * j : a.rd + step8 * (j - turned), hi = rot ? lo + half : lo + 8 * (LPH - turned);
   for (int i = threadIdx.x; i < half; i += RP_NT) {
     double f = 1.0;
 #pragma unroll
@@ -160,8 +166,8 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
       const int z = row >= a.H, h = z ? row - a.H : row;
       const T* p = static_cast<const T*>(z ? a.x[1] : a.x[0]) + (int64_t)t * (z ? a.tok[1] : a.tok[0]) +
                    (int64_t)h * (z ? a.head[1] : a.head[0]);
-      u.load(p + lo);
-      v.load(p + hi);
+      u.load(p + lo, gap);
+      v.load(p + hi, gap);
     };
     bool there = has && t < a.tokens;
     if (there) in(row0);  // on their way while the angles are found
@@ -201,11 +207,12 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
     there = there && !behind;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float s[8], c[8];
-    const int at = rot ? mine * half + 8 * j : 0;
+    const int at = rot ? mine * half + lo : 0;
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
-      *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(&sc[w][0][at + e]);
-      *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(&sc[w][1][at + e]);
+      const int k = e && rot ? at + gap : at;
+      *reinterpret_cast<f4*>(s + e) = *reinterpret_cast<const f4*>(&sc[w][0][k]);
+      *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(&sc[w][1][k]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (int row = row0; there && row < a.rows; row += NG) {
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
         const float n = 1.0f / sqrtf(__builtin_fmaf(sq, 1.0f / HD, a.eps));
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const f4 y = *reinterpret_cast<const f4*>(wt + z * HD + (e < 8 ? lo + e : hi + e - 8));
+          const f4 y = *reinterpret_cast<const f4*>(wt + z * HD + (e < 8 ? lo : hi) + (e & 4 ? gap : 0));
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[e + i] = x[e + i] * n * y[i];
         }
@@ -249,8 +256,8 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
       }
       T* o = static_cast<T*>(z ? a.out[1] : a.out[0]) + (int64_t)t * (z ? a.otok[1] : a.otok[0]) +
              (int64_t)h * (z ? a.ohead[1] : a.ohead[0]);
-      u.store(o + lo);
-      v.store(o + hi);
+      u.store(o + lo, gap);
+      v.store(o + hi, gap);
     }
   }
 }
