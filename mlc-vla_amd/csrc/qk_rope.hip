@@ -26,7 +26,7 @@ struct RopeArgs {
   int64_t tok[2], head[2], otok[2], ohead[2];  // element strides
   const int32_t *cu, *kv_lens, *pos;
   int32_t tokens, B, H, rows, rd, w_f32;  // rows: heads of both
-  int32_t pack;                           // tokens that a wave takes at once
+  int32_t pack, part;                     // tokens that a wave takes at once; heads of one that it takes
   float eps, offset;
   // turns per position of pair i = 8 j + e: one[e] times oct[b] for each bit b of j
   double oct[4], one[8];
@@ -47,20 +47,20 @@ struct RopeType<MLCV_DTYPE_F32> {
   typedef float T;
 };
 
-// How a row is read: one by one, by 16-byte loads, or by such loads past the caches
-enum RopeLoads { RP_SINGLE, RP_WIDE, RP_FAR };
+// How a row is read and written: element by element; by 16 bytes; stores past the caches; loads too
+enum RopeAccess { RP_SINGLE, RP_WIDE, RP_FAR_STORES, RP_FAR };
 
-// 4 elements at p and 4 at p + gap (16-bit types: 8 in a row); 16-byte stores go past the caches
-template <class T, int LOADS>
+// 4 elements at p and 4 at p + gap (16-bit types: 8 in a row)
+template <class T, int ACCESS>
 struct Piece {
-  static constexpr bool VEC = LOADS != RP_SINGLE;
+  static constexpr bool VEC = ACCESS != RP_SINGLE;
   T v[8] __attribute__((aligned(16)));
   __device__ __forceinline__ void load(const T* p, int gap) {
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
         const u4* q = reinterpret_cast<const u4*>(p + i * gap);
-        reinterpret_cast<u4*>(v)[i] = LOADS == RP_FAR ? __builtin_nontemporal_load(q) : load_global(q);
+        reinterpret_cast<u4*>(v)[i] = ACCESS == RP_FAR ? __builtin_nontemporal_load(q) : load_global(q);
       }
     } else {
 #pragma unroll
@@ -70,8 +70,11 @@ struct Piece {
   __device__ __forceinline__ void store(T* p, int gap) const {
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        __builtin_nontemporal_store(reinterpret_cast<const u4*>(v)[i], reinterpret_cast<u4*>(p + i * gap));
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        u4* q = reinterpret_cast<u4*>(p + i * gap);
+        if constexpr (ACCESS == RP_WIDE) *q = reinterpret_cast<const u4*>(v)[i];
+        else __builtin_nontemporal_store(reinterpret_cast<const u4*>(v)[i], q);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[i < 4 ? i : i - 4 + gap] = v[i];
@@ -114,7 +117,7 @@ __device__ __forceinline__ int find_request(const int32_t* cu, int B, int t, int
 // a.pack tokens at once where they have few.  Sines and cosines are computed once per token and pair, spread over the lanes,
 // and handed round through LDS; by each lane for its own pairs they are four to sixteen times as many (100000 tokens of 3
 // heads of 64, one token at a time: 76 us; now 23.1).
-template <int TYPE, int HD, bool NORM, int LOADS>
+template <int TYPE, int HD, bool NORM, int ACCESS>
 __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
   typedef typename RopeType<TYPE>::T T;
   constexpr int LPH = HD / 16, NG = 64 / LPH;  // lanes of a head, heads at once
@@ -148,20 +151,23 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
     }
   __syncthreads();
 
-  // this lane's token of a block, and its head of the first round
-  const int mine = a.pack > 1 ? g / a.rows : 0, row0 = a.pack > 1 ? g - mine * a.rows : g;
-  const bool has = mine < a.pack && row0 < a.rows;
-  // up to 64 requests: their offsets and lengths stay in the lanes
+  // this lane's token of a block, its head of the first round, and the heads up to which the wave goes
+  const int from = (int)blockIdx.y * a.part, to = min(a.rows, from + a.part);
+  const int mine = a.pack > 1 ? g / a.rows : 0, row0 = a.pack > 1 ? g - mine * a.rows : g + from;
+  const bool has = mine < a.pack && row0 < to;
+  // Up to 64 requests: their offsets and lengths stay in the lanes.  Up to 4096: every `stride`-th offset does, and a token's
+  // request is found by one more round of loads.
+  const int stride = (a.B + 63) >> 6;
   int cu0 = 0, cu1 = 0, lens = 0;
-  if (!a.pos && lane < a.B) {
-    cu0 = load_global(a.cu + lane);
-    cu1 = load_global(a.cu + lane + 1);
-    lens = load_global(a.kv_lens + lane);
+  if (!a.pos && lane * (int64_t)stride < a.B) {
+    cu0 = load_global(a.cu + lane * stride);
+    cu1 = load_global(a.cu + lane * stride + 1);
+    lens = load_global(a.kv_lens + lane * stride);
   }
   const int step = (int)gridDim.x * (RP_NT / 64) * a.pack;
   for (int t0 = ((int)blockIdx.x * (RP_NT / 64) + w) * a.pack; t0 < a.tokens; t0 += step) {
     const int t = t0 + mine;
-    Piece<T, LOADS> u, v;
+    Piece<T, ACCESS> u, v;
     auto in = [&](int row) {
       const int z = row >= a.H, h = z ? row - a.H : row;
       const T* p = static_cast<const T*>(z ? a.x[1] : a.x[0]) + (int64_t)t * (z ? a.tok[1] : a.tok[0]) +
@@ -171,8 +177,8 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
     };
     bool there = has && t < a.tokens;
     if (there) in(row0);  // on their way while the angles are found
-    int64_t pos = 0;      // this lane's token's
     bool behind = false;
+    int next = 0, len = 0;  // of the request of the last token looked up
     for (int i = 0; i < a.pack; ++i) {
       const int ti = min(t0 + i, a.tokens - 1);
       int64_t p = 0;
@@ -180,16 +186,24 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
       if (a.pos) {
         p = a.pos[ti];
       } else {
-        int next = 0, len = 0;
-        if (a.B <= 64) {
-          const unsigned long long le = __ballot(lane < a.B && cu0 <= ti);
-          const int b = le ? 63 - __builtin_clzll(le) : 0;
-          next = le ? __builtin_amdgcn_readlane(cu1, b) : ti;
-          len = __builtin_amdgcn_readlane(lens, b);
-        } else {
-          const int b = find_request(a.cu, a.B, ti, lane);
-          next = b < 0 ? ti : a.cu[b + 1];
-          len = b < 0 ? 0 : a.kv_lens[b];
+        if (i == 0 || ti >= next) {
+          const unsigned long long le = __ballot(lane * (int64_t)stride < a.B && cu0 <= ti);
+          const int at = le ? 63 - __builtin_clzll(le) : 0;
+          if (stride == 1) {
+            next = le ? __builtin_amdgcn_readlane(cu1, at) : ti;
+            len = __builtin_amdgcn_readlane(lens, at);
+          } else if (stride <= 64) {
+            const int k = min(at * stride + lane, a.B - 1);
+            const int c0 = load_global(a.cu + k), c1 = load_global(a.cu + k + 1), l = load_global(a.kv_lens + k);
+            const unsigned long long in = __ballot(lane < stride && c0 <= ti);
+            const int b = in ? 63 - __builtin_clzll(in) : 0;
+            next = le && in ? __builtin_amdgcn_readlane(c1, b) : ti;
+            len = __builtin_amdgcn_readlane(l, b);
+          } else {
+            const int b = find_request(a.cu, a.B, ti, lane);
+            next = b < 0 ? ti : a.cu[b + 1];
+            len = b < 0 ? 0 : a.kv_lens[b];
+          }
         }
         none = ti >= next;  // before the first request or behind the last
         p = (int64_t)len - ((int64_t)next - ti);
@@ -215,7 +229,7 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
       *reinterpret_cast<f4*>(c + e) = *reinterpret_cast<const f4*>(&sc[w][1][k]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int row = row0; there && row < a.rows; row += NG) {
+    for (int row = row0; there && row < to; row += NG) {
       if (row != row0) in(row);
       const int z = row >= a.H, h = z ? row - a.H : row;
       float x[16];
@@ -264,16 +278,27 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
 
 template <int TYPE, int HD, bool NORM>
 int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
-  a.pack = std::max(1, 64 / (HD / 16) / a.rows);
+  constexpr int NG = 64 / (HD / 16);
+  a.pack = std::max(1, NG / a.rows);
   // What the GPU holds at once, five waves a SIMD, each taking tokens in turn: 24000 tokens of 40 heads of 128 with norms take
   // 90.9 us with 1280 workgroups, 91.9 with 1024, 30000 of 9 heads of 256 57.1 and 60.1; with twice as many it is 96 and 67.
-  const unsigned grid = (unsigned)std::min(((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack), (int64_t)1280);
-  // Inputs that the GPU's L2 caches (32 MB) can hold are loaded through them, as the projection may just have written them: 3000
-  // tokens of 40 heads of 128 in bf16 (31 MB) 13.8 us, past the caches 16.7; 6000 31.5 and 30.3, 24000 100.5 and 94.8.
+  // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 5.8 us, with one 14.1).
+  const int64_t most = 1280, groups = ((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack);
+  const int rounds = (a.rows + NG - 1) / NG, parts = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, most / groups));
+  a.part = (rounds + parts - 1) / parts * NG;
+  const dim3 grid((unsigned)std::min(groups, most), (unsigned)((a.rows + a.part - 1) / a.part));
+  // Past the caches, as far as it pays: stores where each covers whole 64 bytes (16 for each lane of a head that is rotated,
+  // and of those that are not), loads where each covers whole lines of 128, and of inputs that the GPU's L2 caches (32 MB)
+  // cannot hold: smaller ones the projection may just have written.  Plain, stores and all past the caches:
+  //   24000 tokens of 40 heads of 128, bf16 108.4, 100.5, 94.8 us       3000 of them (31 MB) 16, 13.8, 16.7; 6000 -, 31.5, 30.3
+  //   100000 of 16 of 64, f16 92.2, 89.3, 94.2                          60000 of 8 of 64, float32 56.3, 55.8, 59.7
+  //   and with 48 dims of 64 rotated 66.4, 107.6, 118.2                 24000 of 40 with 112 of 128 rotated 108.7, 124.2, 139.0
+  const int turned = a.rd, rest = HD - a.rd;  // bytes of a store: 16 for each 16 dims
   const bool far = (int64_t)a.tokens * a.rows * HD * (TYPE == MLCV_DTYPE_F32 ? 4 : 2) > (int64_t)40 << 20;
   if (!vec) qk_rope_kernel<TYPE, HD, NORM, RP_SINGLE><<<grid, RP_NT, 0, st>>>(a);
-  else if (far) qk_rope_kernel<TYPE, HD, NORM, RP_FAR><<<grid, RP_NT, 0, st>>>(a);
-  else qk_rope_kernel<TYPE, HD, NORM, RP_WIDE><<<grid, RP_NT, 0, st>>>(a);
+  else if (turned % 64 || rest % 64) qk_rope_kernel<TYPE, HD, NORM, RP_WIDE><<<grid, RP_NT, 0, st>>>(a);
+  else if (!far || turned % 128 || rest % 128) qk_rope_kernel<TYPE, HD, NORM, RP_FAR_STORES><<<grid, RP_NT, 0, st>>>(a);
+  else if constexpr (HD > 64) qk_rope_kernel<TYPE, HD, NORM, RP_FAR><<<grid, RP_NT, 0, st>>>(a);
   MLCV_HIP(hipGetLastError());
   return 0;
 }
