@@ -9,9 +9,9 @@
 // the threshold is inserted; where many do, as at the row's beginning, they are sorted and merged by the bitonic network.  The
 // threshold is the wave's k-th best, or the least that the waves of the row know to be below k.
 //
-// Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 100 us, 5.1 TB/s, as a copy has), with about
-// 11 vector instructions per logit beside it (a quarter of them the exponential's); for few rows by the latency of selecting
-// (16 rows: 9.1 us in 512 workgroups and 4.7 in the join; without alternatives 8.6 in all).
+// Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 93.6 us, 5.5 TB/s; with loads that stay in
+// the caches 100.3), with about 11 vector instructions per logit beside it (the exponential counts four); for few rows by the
+// latency of selecting (16 rows: 9.1 us in 512 workgroups and 3.8 in the join; without alternatives 8.6 in all).
 #include "kernels.h"
 #include "mlcvla.h"
 
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
 #pragma unroll
       for (int n = 0; n < U; ++n)
 #pragma unroll
-        for (int i = 0; i < V; ++i) raw[n][i] = load_global(reinterpret_cast<const u4*>(x + at0[n]) + i);
+        for (int i = 0; i < V; ++i) raw[n][i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(x + at0[n]) + i);
 #pragma unroll
       for (int n = 0; n < U; ++n)
 #pragma unroll
