@@ -473,8 +473,9 @@ int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, in
  *   top_ids, top_logprobs [rows][top]   the `top` (up to 64) largest logits in descending order, equal ones by their index
  * all in float32, read in one pass.  Masked logits (-inf) have probability 0 and rank behind the others; a row of them alone has
  * entropy 0 and log probabilities of -inf.  A row with a NaN or +inf has NaN for its probabilities and entropy; NaN ranks
- * last.  Logits of the type's lowest value are ordinary ones.  workspace: mlcv_token_logprobs_workspace bytes of device
- * memory, 16-byte aligned, for this call alone while it runs.  Outputs must not overlap the inputs. */
+ * last.  Logits of the type's lowest value are ordinary ones.  A log probability below float32's range is -inf.
+ * workspace: mlcv_token_logprobs_workspace bytes of device memory, 16-byte aligned, for this call alone while it runs.
+ * Outputs must not overlap the inputs. */
 int mlcv_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, size_t* bytes);
 int mlcv_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, float scale,
                         const int32_t* tokens, int32_t given, float* logprobs, float* entropy, int32_t top,

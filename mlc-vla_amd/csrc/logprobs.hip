@@ -10,7 +10,7 @@
 // threshold is the wave's k-th best, or the least that the waves of the row know to be below k.
 //
 // Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 93.6 us, 5.5 TB/s; with loads that stay in
-// the caches 100.3), with about 11 vector instructions per logit beside it (the exponential counts four); for few rows by the
+// the caches 100.3), with 9.5 vector instructions per logit and lane beside it; for few rows by the
 // latency of selecting (16 rows: 9.1 us in 512 workgroups and 3.8 in the join; without alternatives 8.6 in all).
 #include "kernels.h"
 #include "mlcvla.h"
@@ -536,15 +536,15 @@ struct LpPlan {
 LpPlan lp_plan(int rows, int vocab, int k) {
   LpPlan p;
   // A wave for each row where there are enough of them, as it selects once and not four times: 4000 rows of 4096, 8192 and
-  // 32000 logits take 20.7, 31.4 and 72.6 us, with four waves 31.0, 32.2 and 77.9; 2000 of 8192 21.8 and 20.4, 1000 of 4096
-  // 12.5 and 12.9, 64 of 4096 11.5 and 8.7.  Up to 2048 logits are one round of one wave.
+  // 32000 logits take 19.9, 29.6 and 70.8 us, with four waves 29.3, 31.5 and 75.4; 2000 of 8192 21.8 and 19.6, 1000 of 4096
+  // 12.5 and 12.4, 64 of 4096 11.1 and 8.3.  Up to 2048 logits are one round of one wave.
   p.wpr = vocab <= 2048 || rows >= (vocab <= 4096 ? 1000 : 4000) ? 1 : LP_W;
   const int chunks = (int)(((int64_t)vocab + 7 + 7) >> 3);
   // Splits that make about 1200 workgroups, of a round of loads (8192 logits) at least, and none of less than three rounds,
-  // where the join's launch costs more.  257152 logits, 20 alternatives (5 from 150 rows on): 16 rows 15.6 us with 32
-  // splits, 17.4 with 16, 51.9 with one; 64 rows 25.2, 23.7, 56.3; 300 rows 47.0 with 4, 49.3 with 8, 53.3 with 2, 65.1 with one; 1001
-  // rows 110.8 with one, 120.4 with 2.  32000 logits: 64 rows 13.1 with 4, 16.7 with one; 16384: 16 rows 13.4 with 2, 10.1
-  // with one.
+  // where the join's launch costs more.  257152 logits, 20 alternatives (5 from 300 rows on): 16 rows 14.3 us with 32
+  // splits, 16.1 with 16, 57.6 with one; 64 rows 23.4, 22.3 and 59.2; 300 rows 44.6 with 4, 46.8 with 8, 51.1 with 2, 62.8 with
+  // one; 1001 rows 103.2 with one, 111.5 with 2 (the same logits again, in a graph).  32000 logits: 64 rows 12.7 with 4, 17.5
+  // with one; 16384: 16 rows 12.9 with 2, 9.9 with one.
   const int rounds = (int)(((int64_t)vocab + 8 * LP_GROUP - 1) / (8 * LP_GROUP));
   int S = p.wpr == 1 || rounds < 3 ? 1 : std::max(1, std::min((int)((1200 + (int64_t)rows / 2) / rows), rounds));
   p.per = (chunks + S - 1) / S;

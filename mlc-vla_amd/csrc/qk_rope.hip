@@ -282,7 +282,7 @@ int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
   a.pack = std::max(1, NG / a.rows);
   // What the GPU holds at once, five waves a SIMD, each taking tokens in turn: 24000 tokens of 40 heads of 128 with norms take
   // 90.9 us with 1280 workgroups, 91.9 with 1024, 30000 of 9 heads of 256 57.1 and 60.1; with twice as many it is 96 and 67.
-  // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 5.8 us, with one 14.1).
+  // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 7.2 us, with one 14.1).
   const int64_t most = 1280, groups = ((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack);
   const int rounds = (a.rows + NG - 1) / NG, parts = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, most / groups));
   a.part = (rounds + parts - 1) / parts * NG;
@@ -290,7 +290,7 @@ int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
   // Past the caches, as far as it pays: stores where each covers whole 64 bytes (16 for each lane of a head that is rotated,
   // and of those that are not), loads where each covers whole lines of 128, and of inputs that the GPU's L2 caches (32 MB)
   // cannot hold: smaller ones the projection may just have written.  Plain, stores and all past the caches:
-  //   24000 tokens of 40 heads of 128, bf16 108.4, 100.5, 94.8 us       3000 of them (31 MB) 16, 13.8, 16.7; 6000 -, 31.5, 30.3
+  //   24000 tokens of 40 heads of 128, bf16 108.4, 100.5, 94.8 us       3000 of them (31 MB) 18.6, 13.8, 16.7; 6000 -, 31.5, 30.3
   //   100000 of 16 of 64, f16 92.2, 89.3, 94.2                          60000 of 8 of 64, float32 56.3, 55.8, 59.7
   //   and with 48 dims of 64 rotated 66.4, 107.6, 118.2                 24000 of 40 with 112 of 128 rotated 108.7, 124.2, 139.0
   const int turned = a.rd, rest = HD - a.rd;  // bytes of a store: 16 for each 16 dims
