@@ -645,7 +645,8 @@ int mlcv_kv_fork(const int32_t* parents, int32_t n, const int32_t* block_table, 
   MLCV_REQUIRE(n == 0 || (parents && new_lens && (new_table || max_pages == 0)), "null row array");
   MLCV_REQUIRE(B == 0 || (kv_lens && (block_table || max_pages == 0)), "null request array");
   MLCV_REQUIRE(n_free == 0 || free_pages, "null free_pages");
-  const Ints arrays[] = {{new_table, (int64_t)n * max_pages}, {new_lens, n}, {status, 2}, {parents, n}, {block_table, (int64_t)B * max_pages}, {kv_lens, B}, {free_pages, n_free},
+  const Ints arrays[] = {{new_table, (int64_t)n * max_pages}, {new_lens, n}, {status, 2},
+                         {parents, n}, {block_table, (int64_t)B * max_pages}, {kv_lens, B}, {free_pages, n_free},
                          {free_count, free_count ? 1 : 0}};
   MLCV_REQUIRE(!overlap(arrays, 3, 8), "outputs overlap the inputs or one another");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

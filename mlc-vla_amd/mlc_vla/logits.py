@@ -54,7 +54,7 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, scale: float = 1.0, out
     if tokens is not None:
         t = _t(tokens)
         shape = t.shape
-        given = 1 if t.dim() == 1 else shape[-1]
+        given = 1 if t.dim() == 1 else shape[-1] if shape else -1
         if not (t.dtype is _I32 and t.dim() in (1, 2) and shape[0] == rows and t.is_contiguous()
                 and t.get_device() == dev):
             _refuse("token_logprobs", dev, (("tokens", t, (_I32,), (rows,) if t.dim() < 2 else (rows, None), True),))

@@ -380,3 +380,10 @@ def test_token_logprobs_arguments():
     with pytest.raises(N.MlcvError, match="workspace"):
         L.token_logprobs(big, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"), top=5)
     assert L.token_logprobs(x[:0], t[:0], top=2).top_ids.shape == (0, 2)
+
+
+def test_token_logprobs_refuses_one_token_without_a_row():
+    x = torch.zeros((1, 100), dtype=torch.float16, device="cuda")
+    for t in (_ints([3])[0], _ints([3]).reshape(1, 1, 1)):
+        with pytest.raises(ValueError, match="tokens expects"):
+            L.token_logprobs(x, t)
