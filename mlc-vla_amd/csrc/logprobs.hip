@@ -1,8 +1,10 @@
 // Log probabilities from logits (mlcv_token_logprobs): of given tokens, of the best alternatives, and the entropy, in one
 // pass over the row.  With m = max x, c = scale * log2(e) and y = c (x - m):
 //   s = sum 2^y, u = sum -y 2^y      log p(t) = scale (x_t - m) - ln s      H = ln s + ln 2 * u / s
-// m is the wave's running maximum, so that no y is positive, both sums have terms of one sign and the entropy of a
-// row that is almost certain keeps its digits; the sums are rebased where the maximum grows.  float32 throughout.
+// m is the wave's running maximum, so that y is 0 for it and negative otherwise whatever its size: s is at least 1, both sums
+// have terms of one sign and the entropy is never negative; the sums are rebased where the maximum grows.  float32 throughout.
+// As one fused operation, c x - (c m), y would be an instruction less, but for the maximum the rounding of c m, which passes 128
+// where c |m| passes 2^32: a wave that meets only logits masked with -1e10 would have an infinite sum.
 //
 // Alternatives are ranked by a 64-bit key, the logit's bits in an order of integers over the complement of its index:
 // no two are equal, and equal logits rank by their index.  A wave holds its best 64 sorted, one per lane.  A logit that passes
@@ -156,26 +158,15 @@ __device__ __forceinline__ V sort64(V v, bool falling, int lane) {
 // the best 64 of a falling and a rising list, falling
 __device__ __forceinline__ u64 merge64(u64 a, u64 b, int lane) { return settle<64>(a > b ? a : b, true, lane); }
 
-// Sums relative to a maximum.  y = x * ce - mc in one fused operation: ce is c, but 2^-20 where c |m| would leave float32's
-// range; logits of that size are equal or 2^70 apart.
+// Sums relative to a maximum
 struct Sums {
   float m, s, u;
 };
-struct Base {
-  float ce, mc;
-};
-__device__ __forceinline__ Base base_of(float m, float c) {
-#pragma clang fp contract(off)  // mc is the rounded product wherever it is used
-  Base b;
-  b.ce = fabsf(m) * c < 0x1p120f ? c : 0x1p-20f;
-  b.mc = m == -INFINITY ? 0.f : m * b.ce;
-  return b;
-}
-// From the own maximum to m, whose base is b.  The sums are relative to their rounded mc, and the two mc's difference is what
-// counts.
-__device__ __forceinline__ void rebase(Sums& v, float m, Base b, float c) {
-#pragma clang fp contract(off)
-  const float y = v.m == -INFINITY ? -INFINITY : base_of(v.m, c).mc - b.mc, f = __builtin_amdgcn_exp2f(y);
+// What is taken off a logit: m, but 0 where there is none yet, as -inf less itself is no number
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+// From the own maximum to m, which is not below it
+__device__ __forceinline__ void rebase(Sums& v, float m, float c) {
+  const float y = v.m == -INFINITY ? -INFINITY : (v.m - m) * c, f = __builtin_amdgcn_exp2f(y);
   v.u = f * (v.u - v.s * fmaxf(y, -1000.f));  // f = 0 below
   v.s *= f;
   v.m = m;
@@ -189,8 +180,8 @@ __device__ __forceinline__ float below(float x) {
 
 template <bool TOP, int WPR>
 struct Scan {
-  Sums v;       // the maximum is the wave's, the sums each lane's
-  Base base;
+  Sums v;        // the maximum is the wave's, the sums each lane's
+  float base;    // base_of it
   float c, thr;  // what a logit has to pass to matter beyond the sums
   u64 list;
   u64* buf;            // 576 keys of the wave
@@ -209,14 +200,14 @@ struct Scan {
     // ballot of that into an instruction which is true for NaN.
     asm volatile("" : "+v"(v.m), "+v"(thr));
     v.s = v.u = 0.f;
-    base = base_of(v.m, c);
+    base = base_of(v.m);
     list = 0;
   }
   __device__ __forceinline__ void raise(float big) {
     if (!__any(big > v.m)) return;
     const float wm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(all_max(big))));
-    base = base_of(wm, c);
-    rebase(v, wm, base, c);
+    base = base_of(wm);
+    rebase(v, wm, c);
   }
   // one key of the wave's into the list
   __device__ __forceinline__ void insert(u64 key) {
@@ -322,7 +313,7 @@ struct Scan {
       float s[8], u[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = __builtin_fmaf(x[n][e], base.ce, -base.mc);
+        const float y = (x[n][e] - base) * c;
         s[e] = __builtin_amdgcn_exp2f(y);
         u[e] = fmaxf(y, -1000.f);  // a masked logit's y is -inf, its weight 0
       }
@@ -351,12 +342,10 @@ template <int TYPE>
 __device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 list, int lane, float z0, bool there) {
   typedef typename LpType<TYPE>::T T;
   const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
-  // the sums are relative to the rounded mc; its distance from m c counts where the two meet
-  const Base b0 = base_of(v.m, a.c);
-  const float le = logf(v.s), ls = le - (fabsf(v.m) < INFINITY ? LN2 * __builtin_fmaf(v.m, b0.ce, -b0.mc) : 0.f);
+  const float ls = logf(v.s);
   // a row whose mask leaves nothing: s = 0
   auto lp = [&](float z) { return v.s == 0.f ? -INFINITY : (z - v.m) * a.scale - ls; };
-  if (lane == 0 && a.entropy) a.entropy[row] = v.s == 0.f ? 0.f : le + LN2 * (v.u / v.s);
+  if (lane == 0 && a.entropy) a.entropy[row] = v.s == 0.f ? 0.f : ls + LN2 * (v.u / v.s);
   for (int i = lane; i < a.given; i += 64) {
     if (i != lane) z0 = given_logit<TYPE>(a, row, i, there);
     a.lp[(int64_t)row * a.given + i] = there ? lp(z0) : 0.f;
@@ -451,12 +440,11 @@ __global__ __launch_bounds__(64 * LP_W) void logprobs_kernel(const LpArgs a) {
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < LP_W; ++i) m = fmaxf(m, part[i].m);
-    const Base b = base_of(m, a.c);
     Sums v{m, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < LP_W; ++i) {
       Sums q = part[i];
-      rebase(q, m, b, a.c);
+      rebase(q, m, a.c);
       v.s += q.s;
       v.u += q.u;
     }
@@ -518,10 +506,9 @@ __global__ __launch_bounds__(64 * LP_JW) void logprobs_join_kernel(const LpArgs 
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     if (s0 > 0) p = s0 + lane < a.S ? load_global(reinterpret_cast<const f4*>(a.stats) + o + s0 + lane) : (f4){-INFINITY, 0.f, 0.f, 0.f};
     const float m = fmaxf(v.m, all_max(p[0]));
-    const Base b = base_of(m, a.c);
     Sums q{p[0], p[1], p[2]};
-    rebase(q, m, b, a.c);
-    rebase(v, m, b, a.c);
+    rebase(q, m, a.c);
+    rebase(v, m, a.c);
     v.s += all_sum(q.s);
     v.u += all_sum(q.u);
   }

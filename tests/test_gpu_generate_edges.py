@@ -1,0 +1,109 @@
+"""The operators around a decode step's attention where their ordinary tests do not reach: masks of every finite size, scaled
+logits past 2^31, rows that are almost certain, against plain implementations in 64 bits (stepref.py)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import stepref as S
+from mlc_vla import logits as L
+from test_gpu_request_step import _check_logprobs, _host, _tokens
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+@pytest.fixture(autouse=True)
+def _named(request):
+    print(request.node.name, flush=True)
+
+
+def _ints(v):
+    return torch.from_numpy(np.ascontiguousarray(np.asarray(v, np.int32))).cuda()
+
+
+# ---- log probabilities: finite masks and large logits ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("mask", [-1e9, -1e10, -1e12, -1e20, -1e30, -1e35])
+def test_token_logprobs_finite_masks(dt, mask):
+    """Masks that cover a wave's first round, all of a wave, a split, a row; scores, no and many alternatives, four waves for
+    a row and one."""
+    rng = np.random.default_rng(int(-np.log10(-mask)) % 97)
+    for rows, vocab in ((7, 16384), (7, 40000), (1000, 4000)):
+        x = rng.standard_normal((rows, vocab)) * 2
+        x[0, 40:] = mask                      # only the first wave of the first split meets anything else
+        x[1, :vocab - 40] = mask              # only the last does, and late
+        x[2] = mask                           # nothing is left: uniform
+        x[3, 512:2048] = mask                 # other waves' first rounds
+        x[4, rng.random(vocab) < 0.999] = mask
+        x[5, vocab // 2:] = -np.inf           # beside masks of -inf
+        x[5, :vocab // 2 - 3] = mask
+        x = torch.from_numpy(x).to(TYPES[dt]).cuda()
+        for scale in ((0.5, 1.0, 4.0) if rows < 10 else (1.0,)):
+            for top in (0, 20) if rows < 10 else (20,):
+                _check_logprobs(x, scale, _tokens(rng, rows, 2, vocab), top)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("scale", [1e3, 1e6])
+def test_token_logprobs_of_large_scaled_logits(dt, scale):
+    """Logits around 1e3 and 1e4 of either sign at the smallest temperatures."""
+    rng = np.random.default_rng(int(scale) % 1009)
+    for vocab in (1500, 9001, 30000):
+        x = rng.standard_normal((6, vocab))
+        x[:2] += 3000
+        x[2:4] -= 12000
+        x[4] = -12000
+        x[5] = 20000
+        _check_logprobs(torch.from_numpy(x).to(TYPES[dt]).cuda(), scale, _tokens(rng, 6, 2, vocab), 9)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_token_logprobs_of_rising_maxima(dt, scale):
+    """A row's largest logit grows from round to round through every size up to the type's largest."""
+    vocab = 30000
+    up = np.linspace(90, 127.9, vocab)
+    x = np.stack([2.0 ** up, -2.0 ** up[::-1], 2.0 ** np.linspace(118, 122, vocab), 2.0 ** np.linspace(20, 40, vocab),
+                  np.where(np.arange(vocab) < vocab // 2, -2.0 ** 127, 2.0 ** 127)])
+    _check_logprobs(torch.from_numpy(x).to(TYPES[dt]).cuda(), scale, _tokens(np.random.default_rng(1), 5, 2, vocab), 5)
+
+
+@pytest.mark.parametrize("vocab", [1000, 5000, 40000])
+def test_token_logprobs_keep_the_entropy_of_certain_rows(vocab):
+    """One other logit of probability t: the entropy is ln(1 + t) + t / (1 + t) ln(1 / t).
+    1 + t as float32 is off by at most t and by at most half a step, 2^-24: so is its logarithm.  The other sum has one term but
+    zeros: the difference, the scale, their product, the exponential (of an argument of up to 48, each of three roundings
+    counts 48 half steps), and where it is rebased the same again; the logarithm and the sums 16 half steps."""
+    gaps = np.array([0.5, 1.0, 3.0, 8.0, 12.0, 15.0, 17.0, 18.0, 20.0, 24.0, 28.0, 33.0])
+    rel = (2 * 3 * 48 + 16) * S.E32
+    for at, other in ((17, 18), (17, 17 + 512 % (vocab - 30)), (vocab - 1, 3), (2, vocab - 1), (600, 80)):
+        for top in (1.977, 30.0, -5e3, 1e6):
+            x = np.full((len(gaps), vocab), -np.inf, np.float32)
+            x[:, at] = top
+            x[:, other] = np.float32(top) - gaps.astype(np.float32)
+            d = x[:, at].astype(np.float64) - x[:, other]  # what float32 holds
+            t = np.exp(-d)
+            want = np.log1p(t) + t / (1 + t) * d
+            got = L.token_logprobs(torch.from_numpy(x).cuda(), _ints([at] * len(gaps)), top=1)
+            h, lp = _host(got.entropy.torch), _host(got.logprobs.torch)
+            ends = 1.01 * np.minimum(t, S.E32)
+            assert (h >= 0).all() and (np.abs(h - want) <= ends + rel * want).all(), (at, other, top, h, want)
+            assert (lp <= 0).all() and (np.abs(lp + np.log1p(t)) <= ends + rel * np.log1p(t)).all()
+
+
+def test_token_logprobs_entropy_is_not_negative():
+    """Rows of one token that nothing else comes near, at many sizes of the largest logit."""
+    rng = np.random.default_rng(2)
+    x = np.full((400, 3000), -np.inf, np.float32)
+    top = np.linspace(1, 40, 400)
+    x[np.arange(400), rng.integers(0, 1500, 400)] = top
+    x[np.arange(400), rng.integers(1500, 3000, 400)] = top - rng.uniform(17, 50, 400)
+    for scale in (0.7, 1.0, 1.3):
+        h = L.token_logprobs(torch.from_numpy(x).cuda(), scale=scale).entropy.torch
+        assert (h >= 0).all() and (h < 1e-4).all()
