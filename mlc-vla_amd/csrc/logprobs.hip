@@ -240,9 +240,20 @@ struct Scan {
       thr = fmaxf(thr, below(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(low)))));
     }
   }
-  // Logits x[n] of indices i0[n] .. + 7, the largest of each big[n], of all `top`; some lane's passes thr.
+  // Logits x[n] of indices i0[n] .. + 7, the largest of each big[n], of all `top` (NaN where one is among them); some lane's
+  // passes thr or is NaN.
   template <int U>
-  __device__ __forceinline__ void look(const float (&x)[U][8], const int (&i0)[U], const float (&big)[U], float top) {
+  __device__ __forceinline__ void look(const float (&x)[U][8], const int (&i0)[U], float (&big)[U], float top) {
+    if (__any(top != top)) {  // the largest of the others
+      top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < U; ++n) {
+        big[n] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big[n] = x[n][e] > big[n] ? x[n][e] : big[n];
+        top = fmaxf(top, big[n]);
+      }
+    }
     raise(top);
     if constexpr (!TOP) {
       thr = v.m;
@@ -298,16 +309,20 @@ struct Scan {
   }
   template <int U>
   __device__ __forceinline__ void add(const float (&x)[U][8], const int (&i0)[U], bool begin) {
+    // The maximum that keeps a NaN.  fmaxf of a signalling one and a number may be NaN too, so a number next to it would be
+    // lost; it is sorted out where there is one, and no logit has to be made quiet first, an instruction each (1001 rows of
+    // 257152 97.6 -> 92.1 us).
+    auto max3 = [](float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); };
     float big[U], top = -INFINITY;
 #pragma unroll
     for (int n = 0; n < U; ++n) {
       const float* y = x[n];
-      big[n] = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-      top = n ? fmaxf(top, big[n]) : big[n];
+      big[n] = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), __builtin_elementwise_maximum(y[6], y[7]));
+      top = __builtin_elementwise_maximum(top, big[n]);
     }
     if constexpr (TOP && WPR > 1)
       if (begin) meet(top);
-    if (__any(top > thr)) look<U>(x, i0, big, top);
+    if (__any(!(top <= thr))) look<U>(x, i0, big, top);
 #pragma unroll
     for (int n = 0; n < U; ++n) {
       float s[8], u[8];

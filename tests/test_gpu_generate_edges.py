@@ -107,3 +107,22 @@ def test_token_logprobs_entropy_is_not_negative():
     for scale in (0.7, 1.0, 1.3):
         h = L.token_logprobs(torch.from_numpy(x).cuda(), scale=scale).entropy.torch
         assert (h >= 0).all() and (h < 1e-4).all()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+def test_token_logprobs_order_beside_nan(dt):
+    """Quiet and signalling NaN next to the largest logits: the alternatives are the numbers, in their order."""
+    rng = np.random.default_rng(5)
+    bits = {"f16": (np.uint16, 0x7e00, 0x7c01), "bf16": (np.uint16, 0x7fc0, 0x7f81), "f32": (np.uint32, 0x7fc00000, 0x7f800001)}
+    kind, quiet, loud = bits[dt]
+    for vocab in (1500, 9001, 40000):
+        x = torch.from_numpy(rng.standard_normal((6, vocab)) * 3).to(TYPES[dt])
+        raw = x.view(torch.int16 if dt != "f32" else torch.int32).numpy().view(kind)
+        best = _host(x).argsort(1)[:, -30:]
+        for r, nan in ((0, quiet), (1, loud)):
+            near = (best[r][:, None] // 8 * 8 + np.arange(8)).ravel()  # the eight logits that a lane takes at once
+            raw[r, [i for i in near if i < vocab and i not in best[r]]] = nan
+            raw[2 + r, rng.random(vocab) < 0.3] = nan
+            raw[4 + r, rng.integers(0, vocab)] = nan
+        for top in (1, 20, 64):
+            _check_logprobs(x.cuda(), 1.0, _tokens(rng, 6, 2, vocab), top)
