@@ -358,8 +358,8 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, Sums v, u64 lis
   typedef typename LpType<TYPE>::T T;
   const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
   const float ls = logf(v.s);
-  // a row whose mask leaves nothing: s = 0
-  auto lp = [&](float z) { return v.s == 0.f ? -INFINITY : (z - v.m) * a.scale - ls; };
+  // a row whose mask leaves nothing: s = 0.  Halves, as the difference of the largest logits of either sign is past float32.
+  auto lp = [&](float z) { return v.s == 0.f ? -INFINITY : (0.5f * z - 0.5f * v.m) * (2.f * a.scale) - ls; };
   if (lane == 0 && a.entropy) a.entropy[row] = v.s == 0.f ? 0.f : ls + LN2 * (v.u / v.s);
   for (int i = lane; i < a.given; i += 64) {
     if (i != lane) z0 = given_logit<TYPE>(a, row, i, there);

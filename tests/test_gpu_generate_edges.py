@@ -126,3 +126,14 @@ def test_token_logprobs_order_beside_nan(dt):
             raw[4 + r, rng.integers(0, vocab)] = nan
         for top in (1, 20, 64):
             _check_logprobs(x.cuda(), 1.0, _tokens(rng, 6, 2, vocab), top)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 0.25, 0.5, 1.0])
+def test_token_logprobs_of_the_largest_distances(dt, scale):
+    """Logits further apart than the largest float32, whose log probabilities are within it, or just past it."""
+    for vocab in (100, 9001):
+        x = np.full((3, vocab), -3.2e38)
+        x[0, 7], x[1, ::3], x[2, 50:] = 3e38, 2.1e38, -1e38
+        ids = torch.tensor([[0, 7], [1, 3], [3, 60]], dtype=torch.int32, device="cuda")
+        _check_logprobs(torch.from_numpy(x).to(TYPES[dt]).cuda(), scale, ids, 60)
