@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import stepref as S
+from mlc_vla import kv_cache as C
 from mlc_vla import logits as L
 from test_gpu_request_step import _check_logprobs, _host, _tokens
 
@@ -137,3 +138,30 @@ def test_token_logprobs_of_the_largest_distances(dt, scale):
         x[0, 7], x[1, ::3], x[2, 50:] = 3e38, 2.1e38, -1e38
         ids = torch.tensor([[0, 7], [1, 3], [3, 60]], dtype=torch.int32, device="cuda")
         _check_logprobs(torch.from_numpy(x).to(TYPES[dt]).cuda(), scale, ids, 60)
+
+
+# ---- pages -------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("pages", [0, 2, 500, 4097, 20000, 300000])
+def test_results_do_not_keep_a_large_workspace(pages):
+    """What kv_free and kv_compact return holds no more beside itself than 64 KB or a quarter of its size."""
+    rng = np.random.default_rng(pages)
+    table = _ints(rng.permutation(pages)[:min(pages, 40)].reshape(2, -1))
+    lens = _ints([table.shape[1] * 16] * 2)
+    cache = C.PagedKVCache(pages, 16, 1, 64)
+    for t, m in ((table, lens), (torch.cat([table] * 400, 1), lens)):
+        got = cache.free(t, m)
+        want, n = S.free(t.cpu().numpy(), m.cpu().numpy(), pages, 16)
+        np.testing.assert_array_equal(got.free_pages.numpy(), want)
+        assert got.free_count.numpy().tolist() == [n]
+        size = 4 * (pages + 1)
+        assert got.free_pages.torch.untyped_storage().nbytes() <= size + max(1 << 16, size // 4) + 16
+        dense = cache.compact(t, m)
+        assert dense.status.numpy()[0] == pages - n
+        size = 4 * (t.numel() + 2)
+        assert dense.block_table.torch.untyped_storage().nbytes() <= size + max(1 << 16, size // 4) + 16
+        # into given tensors, with and without a given workspace
+        for kw in ({}, dict(workspace=torch.zeros(C.kv_compact_workspace(pages), dtype=torch.uint8, device="cuda"))):
+            np.testing.assert_array_equal(cache.free(t, m, out=got, **kw).free_pages.numpy(), want)
+            assert cache.compact(t, m, out=dense, **kw).status.numpy()[0] == pages - n
