@@ -458,8 +458,8 @@ int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, co
  * past float32's range is normed to zeros).
  * The position of a token is positions[t] (any int32), or, with positions NULL, its place in the cache as
  * mlcv_kv_attention has it: kv_lens[b] - n + i for token i of request b's n (a refused request's, with kv_lens 0, are
- * negative); rows behind the last request are then left as they were.  An out may be its own input, with its strides; it
- * must not otherwise overlap the other input or output, and its rows lie apart (-2). */
+ * negative); rows behind the last request are then left as they were.  An out may be its own input, with its strides; otherwise
+ * no out may overlap an input or the other out, and its rows lie apart (-2). */
 int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                  int32_t dtype, int32_t tokens, const int32_t* cu_seqlens, int32_t B, const int32_t* kv_lens,
                  const int32_t* positions, int32_t H, int32_t KV, int32_t hd, int32_t rotary, double theta, int32_t norm,

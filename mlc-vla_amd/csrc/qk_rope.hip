@@ -10,6 +10,7 @@
 // 5.2), by latency for few (16 tokens of 9 heads of 256: 4 us).
 #include "kernels.h"
 #include "mlcvla.h"
+#include "rows.h"
 
 #include <algorithm>
 #include <cmath>
@@ -346,6 +347,15 @@ extern "C" int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const 
                "an out that is its input must have its strides");
   MLCV_REQUIRE(rows_apart(tokens, qo_tok, H, qo_head, hd) && rows_apart(tokens, ko_tok, KV, ko_head, hd),
                "rows of out overlap");
+  const Rows::Int size = dtype == MLCV_DTYPE_F32 ? 4 : 2, w_size = w_dtype == MLCV_DTYPE_F32 ? 4 : 2;
+  auto rows = [&](const void* p, int64_t tok, int64_t heads, int64_t head) {
+    return Rows(p, tokens, tok * size, heads, head * size, hd * size);
+  };
+  const Rows arrays[] = {rows(q_out, qo_tok, H, qo_head), rows(k_out, ko_tok, KV, ko_head),
+                         rows(q == q_out ? nullptr : q, q_tok, H, q_head), rows(k == k_out ? nullptr : k, k_tok, KV, k_head),
+                         Rows(cu_seqlens, 4 * ((int64_t)B + 1)), Rows(kv_lens, 4 * (int64_t)B),
+                         Rows(positions, 4 * (int64_t)tokens), Rows(q_weight, hd * w_size), Rows(k_weight, hd * w_size)};
+  MLCV_REQUIRE(!any_meet(arrays, 2, 9), "an out overlaps an input or the other out");
   RopeArgs a{};
   a.x[0] = q;
   a.x[1] = k;

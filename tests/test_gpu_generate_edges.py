@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import stepref as S
+from mlc_vla import _native as N
 from mlc_vla import kv_cache as C
 from mlc_vla import logits as L
 from test_gpu_request_step import _check_logprobs, _host, _tokens
@@ -165,3 +166,40 @@ def test_results_do_not_keep_a_large_workspace(pages):
         for kw in ({}, dict(workspace=torch.zeros(C.kv_compact_workspace(pages), dtype=torch.uint8, device="cuda"))):
             np.testing.assert_array_equal(cache.free(t, m, out=got, **kw).free_pages.numpy(), want)
             assert cache.compact(t, m, out=dense, **kw).status.numpy()[0] == pages - n
+
+
+# ---- norm and rotation -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_qk_rope_within_one_buffer(dt):
+    """Outs beside their inputs, between their rows and in their place are taken where no element is shared, and refused where
+    one is."""
+    rng = np.random.default_rng(8)
+    t, h, kv, hd = 21, 6, 2, 64
+    pos = _ints(rng.integers(0, 9000, t))
+    base = torch.from_numpy(rng.standard_normal((t, 2 * (h + kv) + 1, hd))).to(TYPES[dt]).cuda()
+    q, k = base[:, :h], base[:, h:h + kv]
+    want = [x.torch.clone() for x in C.qk_rope(q.contiguous(), k.contiguous(), positions=pos)]
+
+    def check(q, k, out):
+        got = C.qk_rope(q, k, positions=pos, out=out)
+        assert all(torch.equal(g.torch, w) and torch.equal(o, w) for g, o, w in zip(got, out, want))
+
+    for made in (lambda b: (b[:, h + kv:2 * h + kv], b[:, 2 * h + kv:-1]),      # each token's outs behind its inputs
+                 lambda b: (b[:, h + kv:2 * h + kv], b[:, h:h + kv]),          # k in place
+                 lambda b: (b[:, :h], b[:, -kv:]),                              # q in place
+                 lambda b: (b[:, :h], b[:, h:h + kv]),                          # both
+                 lambda b: (b.new_zeros(t, h, hd), b[:, h + kv::4][:, :kv])):     # every fourth head
+        b = base.clone()
+        check(b[:, :h], b[:, h:h + kv], made(b))
+    wide = torch.zeros((t, 3, h, hd), dtype=TYPES[dt], device="cuda")  # outs of other strides than the inputs, rows between rows
+    wide[:, 0] = q
+    check(wide[:, 0], k, (wide[:, 1], wide[:, 2, :kv]))
+    for made in (lambda b: (b[:, 1:h + 1], b[:, -kv:]), lambda b: (b[:, h:2 * h], b[:, -kv:]),
+                 lambda b: (b[:, -h:], b[:, -kv:]), lambda b: (b[:, :h], b[:, h - 1:h - 1 + kv]),
+                 lambda b: (b[:, h + kv:2 * h + kv], b[:, :kv])):
+        b = base.clone()
+        with pytest.raises(N.MlcvError, match="overlaps an input or the other out"):
+            C.qk_rope(b[:, :h], b[:, h:h + kv], positions=pos, out=made(b))
+        assert torch.equal(b, base)

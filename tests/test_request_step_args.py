@@ -140,3 +140,14 @@ def test_workspaces_of_the_pages():
             N.call(name, 5, None)
         with pytest.raises(N.MlcvError, match="num_pages"):
             N.call(name, -1, ctypes.byref(ctypes.c_size_t()))
+
+
+@pytest.mark.parametrize("bad", [
+    dict(qo=P + 128), dict(ko=P), dict(qo=2 * P, ko=2 * P + 2048), dict(k=2 * P + 2558), dict(ko=P + 2558), dict(ko=2 * P - 1278),
+    dict(qo=P, k=P + 384, k_tok=256), dict(qo=P, k=P + 500, k_tok=256, H=3),                    # in place in a fused row, k in q's
+    dict(qo=P, ko=P + 768 - 2, ko_tok=384, q_tok=384, qo_tok=384, H=6),
+    dict(lens=2 * P + 4), dict(cu=3 * P + 8), dict(cu=None, lens=None, pos=2 * P), dict(norm=1, qw=2 * P), dict(norm=1, kw=3 * P + 126),
+    dict(tokens=4, q_tok=-256, q=P + 6 * 512, ko=P + 3 * 512)])
+def test_outs_of_rope_over_other_arrays_are_refused(bad):
+    with pytest.raises(N.MlcvError, match="overlaps an input or the other out"):
+        _rope(**bad)
