@@ -475,7 +475,7 @@ int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, in
  * entropy 0 and log probabilities of -inf.  A row with a NaN or +inf has NaN for its probabilities and entropy; NaN ranks
  * last.  Logits of the type's lowest value are ordinary ones.  A log probability below float32's range is -inf.
  * workspace: mlcv_token_logprobs_workspace bytes of device memory, 16-byte aligned, for this call alone while it runs.
- * Outputs must not overlap the inputs. */
+ * Neither outputs nor workspace may overlap an input or one another (-2). */
 int mlcv_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, size_t* bytes);
 int mlcv_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, float scale,
                         const int32_t* tokens, int32_t given, float* logprobs, float* entropy, int32_t top,

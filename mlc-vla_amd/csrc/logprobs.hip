@@ -16,6 +16,7 @@
 // latency of selecting (16 rows: 9.1 us in 512 workgroups and 3.8 in the join; without alternatives 8.6 in all).
 #include "kernels.h"
 #include "mlcvla.h"
+#include "rows.h"
 
 #include <algorithm>
 #include <cmath>
@@ -610,6 +611,12 @@ int mlcv_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32
   MLCV_REQUIRE(p.bytes == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                                 workspace_bytes >= p.bytes),
                "workspace missing, not 16-byte aligned or too small");
+  const Rows::Int size = dtype == MLCV_DTYPE_F32 ? 4 : 2;
+  const int64_t ints = 4 * (int64_t)rows;
+  const Rows arrays[] = {Rows(given ? logprobs : nullptr, ints * given), Rows(entropy, ints), Rows(top ? top_ids : nullptr, ints * top),
+                         Rows(top ? top_logprobs : nullptr, ints * top), Rows(workspace, (int64_t)p.bytes),
+                         Rows(logits, rows, stride * size, 1, 0, vocab * size), Rows(given ? tokens : nullptr, ints * given)};
+  MLCV_REQUIRE(!any_meet(arrays, 5, 7), "outputs or workspace overlap the inputs or one another");
   LpArgs a{};
   a.x = logits;
   a.stride = stride;

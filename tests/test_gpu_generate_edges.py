@@ -141,6 +141,24 @@ def test_token_logprobs_of_the_largest_distances(dt, scale):
         _check_logprobs(torch.from_numpy(x).to(TYPES[dt]).cuda(), scale, ids, 60)
 
 
+def test_token_logprobs_within_one_buffer():
+    """Results in a padded vocabulary's padding are taken, results over the logits are not."""
+    rng = np.random.default_rng(6)
+    x = torch.from_numpy(rng.standard_normal((5, 600))).float().cuda()
+    pad = x.view(torch.int32)
+    tokens = _tokens(rng, 5, 1, 500)
+    want = L.token_logprobs(x[:, :500], tokens, top=4)
+    given = L.TokenLogprobs(x[4, 500:505], x[0, 520:525], pad[1, 540:560].view(5, 4), x[2, 570:590].view(5, 4))
+    L.token_logprobs(x[:, :500], tokens, top=4, out=given)
+    assert all(torch.equal(a, b.torch) for a, b in zip(given, want))
+    for bad in (dict(logprobs=x[2, 497:502]), dict(entropy=given.logprobs), dict(top_ids=pad[3, 490:510].view(5, 4)),
+                dict(top_logprobs=given.top_ids.view(torch.float32)), dict(logprobs=tokens.view(torch.float32))):
+        before = x.clone()
+        with pytest.raises(N.MlcvError, match="overlap the inputs or one another"):
+            L.token_logprobs(x[:, :500], tokens, top=4, out=given._replace(**bad))
+        assert torch.equal(x, before)
+
+
 # ---- pages -------------------------------------------------------------------------------------------------
 
 

@@ -151,3 +151,13 @@ def test_workspaces_of_the_pages():
 def test_outs_of_rope_over_other_arrays_are_refused(bad):
     with pytest.raises(N.MlcvError, match="overlaps an input or the other out"):
         _rope(**bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(lp=P + 598), dict(lp=2 * P), dict(entropy=3 * P), dict(ids=4 * P + 8), dict(tlp=5 * P - 44), dict(tlp=P),
+    dict(stride=200, lp=P + 588), dict(stride=-100, entropy=P - 200), dict(given=3, lp=4 * P - 4),
+    dict(rows=3, vocab=257152, stride=257152, ws=P + 16, ws_bytes=1 << 40)])
+def test_outputs_of_logprobs_over_other_arrays_are_refused(bad):
+    a = dict(tokens=2 * P, lp=3 * P, entropy=4 * P, ids=5 * P, tlp=6 * P)
+    with pytest.raises(N.MlcvError, match="overlap the inputs or one another"):
+        _logprobs(**{**a, **bad})
