@@ -19,7 +19,10 @@ namespace mlcv {
 
 namespace {
 
-constexpr int RP_NT = 256;  // threads per workgroup: four waves, a token each
+constexpr int RP_NT = 256;       // threads per workgroup: four waves, a token each
+constexpr int RP_GROUPS = 1280;  // workgroups at most
+constexpr int RP_PACK = 8;       // tokens of a wave at once at most: 16 heads of 64, two or more of a token
+constexpr int RP_ROUND = RP_GROUPS * (RP_NT / 64) * RP_PACK;  // tokens that all of them take at once at most
 
 struct RopeArgs {
   const void *x[2], *w[2];  // queries, keys; their norms' weights
@@ -280,11 +283,12 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
 template <int TYPE, int HD, bool NORM>
 int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
   constexpr int NG = 64 / (HD / 16);
+  static_assert(NG / 2 <= RP_PACK, "a round of tokens");
   a.pack = std::max(1, NG / a.rows);
   // What the GPU holds at once, five waves a SIMD, each taking tokens in turn: 24000 tokens of 40 heads of 128 with norms take
   // 90.9 us with 1280 workgroups, 91.9 with 1024, 30000 of 9 heads of 256 57.1 and 60.1; with twice as many it is 96 and 67.
   // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 7.2 us, with one 14.1).
-  const int64_t most = 1280, groups = ((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack);
+  const int64_t most = RP_GROUPS, groups = ((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack);
   const int rounds = (a.rows + NG - 1) / NG, parts = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, most / groups));
   a.part = (rounds + parts - 1) / parts * NG;
   const dim3 grid((unsigned)std::min(groups, most), (unsigned)((a.rows + a.part - 1) / a.part));
@@ -337,8 +341,9 @@ extern "C" int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const 
   MLCV_REQUIRE(!positions != !(cu_seqlens || kv_lens) || tokens == 0, "positions, or cu_seqlens and kv_lens");
   if (tokens == 0 || (!positions && B == 0)) return 0;
   MLCV_REQUIRE(q && k && q_out && k_out && (positions || (cu_seqlens && kv_lens)), "null pointer");
-  // the last round of a wave's tokens (at most 4096 waves' 16) still is an int
-  MLCV_REQUIRE(tokens <= INT32_MAX - 65536, "more than 2^31 - 65537 tokens");
+  // a token of the round behind the last still is an int
+  static_assert(RP_ROUND == 40960, "in the message");
+  MLCV_REQUIRE(tokens <= INT32_MAX - RP_ROUND, "more than 2^31 - 40961 tokens");
   auto in_place = [&](int64_t tok, int64_t otok, int64_t heads, int64_t head, int64_t ohead) {
     return (tokens == 1 || tok == otok) && (heads == 1 || head == ohead);
   };

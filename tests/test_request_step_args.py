@@ -161,3 +161,8 @@ def test_outputs_of_logprobs_over_other_arrays_are_refused(bad):
     a = dict(tokens=2 * P, lp=3 * P, entropy=4 * P, ids=5 * P, tlp=6 * P)
     with pytest.raises(N.MlcvError, match="overlap the inputs or one another"):
         _logprobs(**{**a, **bad})
+
+
+def test_rope_refuses_tokens_whose_next_round_passes_an_int():
+    with pytest.raises(N.MlcvError, match="2\\^31 - 40961"):
+        _rope(tokens=2 ** 31 - 1 - 40960 + 1)
