@@ -454,8 +454,8 @@ int mlcv_kv_compact(const int32_t* block_table, int32_t B, int32_t max_pages, co
  *   position * theta^(-2 i / rotary); dims from `rotary` on (a multiple of 16, 0 to hd) stay y
  * q, k and their outs: element (t, h, d) at t * tok + h * head + d elements, MLCV_DTYPE_F16, _BF16 or _F32 throughout (any
  * strides; where all rows are 16-byte aligned they are read faster); hd 64, 128 or 256; weights [hd] of that type or
- * _F32.  float32 between the load and one rounding at the end, the angles of far positions in more (so a head whose squares sum
- * past float32's range is normed to zeros).
+ * _F32.  float32 between the load and one rounding at the end, the angles of far positions in more; a head whose squares leave
+ * float32's range is normed like any other.
  * The position of a token is positions[t] (any int32), or, with positions NULL, its place in the cache as
  * mlcv_kv_attention has it: kv_lens[b] - n + i for token i of request b's n (a refused request's, with kv_lens 0, are
  * negative); rows behind the last request are then left as they were.  An out may be its own input, with its strides; otherwise

@@ -243,12 +243,24 @@ __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
         x[8 + e] = (float)v.v[e];
       }
       if constexpr (NORM) {
-        float sq = 0.f;
+        auto squares = [&] {
+          float sq = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sq = __builtin_fmaf(x[e], x[e], sq);
+          for (int e = 0; e < 16; ++e) sq = __builtin_fmaf(x[e], x[e], sq);
 #pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor(sq, o);
-        const float n = 1.0f / sqrtf(__builtin_fmaf(sq, 1.0f / HD, a.eps));
+          for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor(sq, o);
+          return sq;
+        };
+        float sq = squares(), eps = a.eps;
+        // a head whose squares leave float32's range (where eps does not hide them) is normed in other units
+        const float unit = sq == INFINITY ? 0x1p-70f : sq < 0x1p-100f && eps < 0x1p-100f ? 0x1p100f : 1.0f;
+        if (TYPE != MLCV_DTYPE_F16 && unit != 1.0f) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] *= unit;
+          sq = squares();
+          eps = eps * unit * unit;
+        }
+        const float n = 1.0f / sqrtf(__builtin_fmaf(sq, 1.0f / HD, eps));
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const f4 y = *reinterpret_cast<const f4*>(wt + z * HD + (e < 8 ? lo : hi) + (e & 4 ? gap : 0));

@@ -11,7 +11,7 @@ import stepref as S
 from mlc_vla import _native as N
 from mlc_vla import kv_cache as C
 from mlc_vla import logits as L
-from test_gpu_request_step import _check_logprobs, _host, _tokens
+from test_gpu_request_step import _check_logprobs, _check_rope, _host, _tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -187,6 +187,24 @@ def test_results_do_not_keep_a_large_workspace(pages):
 
 
 # ---- norm and rotation -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("hd,rd", [(64, 64), (128, 96), (256, 256)])
+@pytest.mark.parametrize("eps", [0.0, 1e-44, 1e-38, 1e-20, 1e-6])
+def test_qk_rope_norms_heads_of_every_size(dt, hd, rd, eps):
+    """Heads whose squares sum past the largest float32 or below the smallest, beside ordinary ones, with every size of eps."""
+    rng = np.random.default_rng(hd)
+    sizes = 10.0 ** (np.arange(-7, 4.5, 0.5) if dt == "f16" else np.arange(-37, 38, 1.5))
+    x = rng.uniform(0.5, 1, (len(sizes), 3, hd)) * rng.choice([-1, 1], (len(sizes), 3, hd))
+    x *= np.stack([sizes, sizes[::-1], np.ones(len(sizes))], 1)[..., None]
+    x[:, :2, 5] *= 1e-3
+    x = torch.from_numpy(x).to(TYPES[dt]).cuda()
+    pos = rng.integers(0, 5000, len(sizes))
+    w = torch.from_numpy(0.3 * rng.standard_normal(hd)).float().cuda()
+    got = C.qk_rope(x, x[:, :1], positions=_ints(pos), rotary_dim=rd, norm=True, q_weight=w, k_weight=w, eps=eps)
+    there = np.ones(len(sizes), bool)
+    _check_rope(x, x[:, :1], pos, there, got, rd, 10000.0, True, (w, w), 1.0, float(np.float32(eps)))
 
 
 @pytest.mark.parametrize("dt", ["f16", "f32"])
