@@ -239,3 +239,39 @@ def test_qk_rope_within_one_buffer(dt):
         with pytest.raises(N.MlcvError, match="overlaps an input or the other out"):
             C.qk_rope(b[:, :h], b[:, h:h + kv], positions=pos, out=made(b))
         assert torch.equal(b, base)
+
+
+def test_refused_requests_keep_their_pages_over_a_fork():
+    """A plan refuses a request that does not fit; the step goes on with the lengths that the requests hold: no page of the
+    refused one is free, no copy goes there, and its row goes on as it was."""
+    cache = C.PagedKVCache(12, 16, 1, 64, layers=2)
+    table = torch.full((3, 8), -1, dtype=torch.int32, device="cuda")
+    lens = _ints([0, 0, 0])
+    x = torch.from_numpy(np.random.default_rng(3).standard_normal((200, 1, 64))).half().cuda()
+
+    def step(new):
+        free = cache.free(table, lens)
+        plan = cache.plan(lens, _ints(new), table, free.free_pages, sum(new), free_count=free.free_count)
+        for y in range(2):
+            cache.write(x[:sum(new)], x[:sum(new)], plan, y)
+        return plan
+
+    plan = step([50, 33, 70])  # 4, 3 and 5 pages: none is free
+    assert plan.status.numpy().tolist() == [12, 0]
+    lens = plan.kv_lens.torch.clone()
+    lens[2] = 0                # the last one has ended
+    plan = step([1, 100, 1])   # the second would need 6 more; the third starts anew
+    assert plan.kv_lens.numpy().tolist() == [51, 0, 1] and plan.status.numpy().tolist() == [1, 1]
+    held = torch.where(plan.kv_lens.torch > 0, plan.kv_lens.torch, lens)
+    assert held.cpu().tolist() == [51, 33, 1]
+    mine = table[1, :3].long()
+    before = [t.view(torch.uint8)[:, mine].clone() for t in cache.all_layers()]
+    free = cache.free(table, held)
+    n = int(free.free_count.numpy()[0])
+    assert n == 4 and not set(free.free_pages.numpy()[:n].tolist()) & set(mine.cpu().tolist())
+    fork = cache.fork(_ints([0, 0, 1, 1, 2]), table, held, *free)
+    assert fork.kv_lens.numpy().tolist() == [51, 51, 33, 33, 1] and fork.status.numpy().tolist() == [2, 0]
+    assert torch.equal(fork.block_table.torch[2, :3], table[1, :3])
+    for t, b in zip(cache.all_layers(), before):
+        assert torch.equal(t.view(torch.uint8)[:, mine], b)
+        assert torch.equal(t.view(torch.uint8)[:, fork.block_table.torch[3, 2].long()], b[:, 2])  # the copy of its last page
