@@ -469,11 +469,11 @@ int mlcv_qk_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, in
 /* Log probabilities from logits: row r, element i at r * stride + i elements (any stride), MLCV_DTYPE_F16, _BF16 or _F32;
  *   log p(i) = z_i - log(sum_j exp(z_j)),  z = scale * x        scale between 1e-6 and 1e6 (one over the temperature)
  *   logprobs [rows][given]      of tokens [rows][given]; 0 for a token outside [0, vocab) (padding)
- *   entropy [rows]              -sum p log p (NULL: not wanted)
+ *   entropy [rows]              -sum p log p, at least 0 (NULL: not wanted)
  *   top_ids, top_logprobs [rows][top]   the `top` (up to 64) largest logits in descending order, equal ones by their index
  * all in float32, read in one pass.  Masked logits (-inf) have probability 0 and rank behind the others; a row of them alone has
  * entropy 0 and log probabilities of -inf.  A row with a NaN or +inf has NaN for its probabilities and entropy; NaN ranks
- * last.  Logits of the type's lowest value are ordinary ones.  A log probability below float32's range is -inf.
+ * last.  Logits of every finite size, the type's lowest value too, are ordinary ones.  A log probability below float32's range is -inf.
  * workspace: mlcv_token_logprobs_workspace bytes of device memory, 16-byte aligned, for this call alone while it runs.
  * Neither outputs nor workspace may overlap an input or one another (-2). */
 int mlcv_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, size_t* bytes);

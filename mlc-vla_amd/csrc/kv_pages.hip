@@ -354,9 +354,10 @@ struct CopyArgs {
 constexpr int CP_PIECE = 2048;  // bytes that a wave moves at a time: 2 loads of 16 per lane
 
 // Units of one page, layer, side and piece; a wave takes one after another.  Bound by memory: 4001 pages of 32 KB of two layers
-// take 99.6 us, 5.3 TB/s read and written.  Small units in many waves, and stores past the caches, which leaves those to pages that
-// are read several times: 8 KB per wave and plain stores take 103.4 us, 431 pages forked from 64 in 6 layers 28.1 (20.3), a
-// pool of 12000 pages of 32 KB made dense (2954 move) 51.1 (41.6); 1 KB per wave 110, 26 and 52.
+// take 105.7 us, 5.0 TB/s read and written.  Small units in many waves, and stores past the caches, which leaves those to pages that
+// are read several times.  On end in a graph over three pools in turn: these copies, 431 pages forked from 64 in 6 layers, and a pool
+// of 12000 pages of 32 KB made dense (2954 move) take 108.8, 22.8 and 43.5 us; with plain stores 110.7, 28.4 and 52.1, with 8 KB per
+// wave 109.3, 27.5 and 48.0, with both 111.6, 29.5 and 56.1; with 1 KB per wave 113.6, 24.0 and 53.0.
 // pair(i) gives pages (from, into) number i of n.
 template <class Pair>
 __device__ __forceinline__ void copy_pages(const CopyArgs& a, int n, long long unit, long long step, Pair pair) {
@@ -464,7 +465,7 @@ __global__ __launch_bounds__(MK_NT) void dense_kernel(const MarkArgs a, const Co
 }
 
 // Workgroups for `most` pages, of which there may be fewer: up to 16384.  With 2048 (about what the GPU holds at once) the
-// copies above take 101.2, 20.4 and 43.0 us.
+// copies above take 113.5, 22.7 and 46.0 us.
 unsigned copy_groups(const CopyArgs& a) {
   const int64_t units = (int64_t)a.most * a.layers * 2 * a.pieces;
   return (unsigned)std::min<int64_t>((units + CP_NT / 64 - 1) / (CP_NT / 64), 16384);

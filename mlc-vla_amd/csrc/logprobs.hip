@@ -11,9 +11,9 @@
 // the threshold is inserted; where many do, as at the row's beginning, they are sorted and merged by the bitonic network.  The
 // threshold is the wave's k-th best, or the least that the waves of the row know to be below k.
 //
-// Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 93.6 us, 5.5 TB/s; with loads that stay in
-// the caches 100.3), with 9.5 vector instructions per logit and lane beside it; for few rows by the
-// latency of selecting (16 rows: 9.1 us in 512 workgroups and 3.8 in the join; without alternatives 8.6 in all).
+// Bound by the read of the logits where there are many rows (1001 of 257152 in bf16: 95.3 us, 5.4 TB/s), with 9.5 vector
+// instructions per logit and lane beside it; for few rows by the latency of selecting (16 rows: 8.6 us in 512 workgroups and
+// 3.8 in the join; without alternatives 7.9 in all).
 #include "kernels.h"
 #include "mlcvla.h"
 #include "rows.h"
@@ -312,7 +312,7 @@ struct Scan {
   __device__ __forceinline__ void add(const float (&x)[U][8], const int (&i0)[U], bool begin) {
     // The maximum that keeps a NaN.  fmaxf of a signalling one and a number may be NaN too, so a number next to it would be
     // lost; it is sorted out where there is one, and no logit has to be made quiet first, an instruction each (1001 rows of
-    // 257152 97.6 -> 92.1 us).
+    // 257152, the same logits again, 97.6 -> 92.1 us).
     auto max3 = [](float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); };
     float big[U], top = -INFINITY;
 #pragma unroll
@@ -539,15 +539,16 @@ struct LpPlan {
 LpPlan lp_plan(int rows, int vocab, int k) {
   LpPlan p;
   // A wave for each row where there are enough of them, as it selects once and not four times: 4000 rows of 4096, 8192 and
-  // 32000 logits take 19.9, 29.6 and 70.8 us, with four waves 29.3, 31.5 and 75.4; 2000 of 8192 21.8 and 19.6, 1000 of 4096
-  // 12.5 and 12.4, 64 of 4096 11.1 and 8.3.  Up to 2048 logits are one round of one wave.
+  // 32000 logits take 19.4, 28.4 and 68.0 us, with four waves 28.1, 29.3 and 72.1; 4000 of 257152 336 and 331 (without
+  // alternatives 329 and 313); 2000 of 8192 21.1 and 18.8, 1000 of 4096 11.6 and 11.5, 64 of 4096 10.8 and 7.4.  Up to 2048 logits
+  // are one round of one wave.
   p.wpr = vocab <= 2048 || rows >= (vocab <= 4096 ? 1000 : 4000) ? 1 : LP_W;
   const int chunks = (int)(((int64_t)vocab + 7 + 7) >> 3);
   // Splits that make about 1200 workgroups, of a round of loads (8192 logits) at least, and none of less than three rounds,
-  // where the join's launch costs more.  257152 logits, 20 alternatives (5 from 300 rows on): 16 rows 14.3 us with 32
-  // splits, 16.1 with 16, 57.6 with one; 64 rows 23.4, 22.3 and 59.2; 300 rows 44.6 with 4, 46.8 with 8, 51.1 with 2, 62.8 with
-  // one; 1001 rows 103.2 with one, 111.5 with 2 (the same logits again, in a graph).  32000 logits: 64 rows 12.7 with 4, 17.5
-  // with one; 16384: 16 rows 12.9 with 2, 9.9 with one.
+  // where the join's launch costs more.  257152 logits, 20 alternatives (5 from 300 rows on): 16 rows 13.7 us with 32
+  // splits, 15.3 with 16, 58.5 with one; 64 rows 22.8, 21.7 and 60.8; 300 rows 42.4 with 4, 44.3 with 8, 48.4 with 2, 60.3 with
+  // one; 1001 rows 96.8 with one, 101.9 with 2 (20 calls on end, without the host).  32000 logits: 64 rows 12.1 with 4, 16.5
+  // with one; 16384: 16 rows 13.9 with 2, 10.7 with one.
   const int rounds = (int)(((int64_t)vocab + 8 * LP_GROUP - 1) / (8 * LP_GROUP));
   int S = p.wpr == 1 || rounds < 3 ? 1 : std::max(1, std::min((int)((1200 + (int64_t)rows / 2) / rows), rounds));
   p.per = (chunks + S - 1) / S;

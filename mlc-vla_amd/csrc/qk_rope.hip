@@ -6,8 +6,8 @@
 // float32 angle is off by 2^-8 of a radian.  They are float64 products in turns, of which whole turns are taken off before
 // they become float32.
 //
-// Bound by memory for many tokens (24000 tokens of 40 heads of 128 in bf16: 91 us, 5.4 TB/s read and written; a copy reaches
-// 5.2), by latency for few (16 tokens of 9 heads of 256: 4 us).
+// Bound by memory for many tokens (24124 tokens of 40 heads of 128 in bf16: 90 us, 5.5 TB/s read and written; a copy reaches
+// 5.1), by latency for few (16 tokens of 9 heads of 256: 4.1 us).  Figures below are of calls on end in a graph, without the host.
 #include "kernels.h"
 #include "mlcvla.h"
 #include "rows.h"
@@ -120,7 +120,7 @@ __device__ __forceinline__ int find_request(const int32_t* cu, int B, int t, int
 // so a wave 1024 / HD heads at a time, and a pair never leaves its lane: heads of one token, one round after another, or of
 // a.pack tokens at once where they have few.  Sines and cosines are computed once per token and pair, spread over the lanes,
 // and handed round through LDS; by each lane for its own pairs they are four to sixteen times as many (100000 tokens of 3
-// heads of 64, one token at a time: 76 us; now 23.1).
+// heads of 64 in bf16, one token at a time: 76 us; now 21.6, and 42.9 with the sines handed round but one token at a time).
 template <int TYPE, int HD, bool NORM, int ACCESS>
 __global__ __launch_bounds__(RP_NT, 4) void qk_rope_kernel(const RopeArgs a) {
   typedef typename RopeType<TYPE>::T T;
@@ -298,8 +298,8 @@ int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
   static_assert(NG / 2 <= RP_PACK, "a round of tokens");
   a.pack = std::max(1, NG / a.rows);
   // What the GPU holds at once, five waves a SIMD, each taking tokens in turn: 24000 tokens of 40 heads of 128 with norms take
-  // 90.9 us with 1280 workgroups, 91.9 with 1024, 30000 of 9 heads of 256 57.1 and 60.1; with twice as many it is 96 and 67.
-  // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 7.2 us, with one 14.1).
+  // 87.1 us with 1280 workgroups, 87.7 with 1024, 30000 of 9 heads of 256 56.0 and 59.2; with twice as many it is 87.2 and 57.9.
+  // Few tokens: several waves for each, as far as there are rounds of heads (16 tokens of 40 heads of 256 3.9 us, with one 8.0).
   const int64_t most = RP_GROUPS, groups = ((int64_t)a.tokens + 4 * a.pack - 1) / (4 * a.pack);
   const int rounds = (a.rows + NG - 1) / NG, parts = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, most / groups));
   a.part = (rounds + parts - 1) / parts * NG;
@@ -307,9 +307,9 @@ int rope_launch(RopeArgs a, bool vec, hipStream_t st) {
   // Past the caches, as far as it pays: stores where each covers whole 64 bytes (16 for each lane of a head that is rotated,
   // and of those that are not), loads where each covers whole lines of 128, and of inputs that the GPU's L2 caches (32 MB)
   // cannot hold: smaller ones the projection may just have written.  Plain, stores and all past the caches:
-  //   24000 tokens of 40 heads of 128, bf16 108.4, 100.5, 94.8 us       3000 of them (31 MB) 18.6, 13.8, 16.7; 6000 -, 31.5, 30.3
-  //   100000 of 16 of 64, f16 92.2, 89.3, 94.2                          60000 of 8 of 64, float32 56.3, 55.8, 59.7
-  //   and with 48 dims of 64 rotated 66.4, 107.6, 118.2                 24000 of 40 with 112 of 128 rotated 108.7, 124.2, 139.0
+  //   24000 tokens of 40 heads of 128, bf16 97.3, 93.2, 87.7 us      3000 of them (31 MB) 17.2, 13.0, 15.3; 6000 31.3, 29.9, 28.2
+  //   100000 of 16 of 64, f16 83.2, 83.8, 92.4                       60000 of 8 of 64, float32 52.0, 52.3, 54.4
+  //   and with 48 dims of 64 rotated 60.3, 117.4, 126.1              24000 of 40 with 112 of 128 rotated 102.9, 114.5, 130.0
   const int turned = a.rd, rest = HD - a.rd;  // bytes of a store: 16 for each 16 dims
   const bool far = (int64_t)a.tokens * a.rows * HD * (TYPE == MLCV_DTYPE_F32 ? 4 : 2) > (int64_t)40 << 20;
   if (!vec) qk_rope_kernel<TYPE, HD, NORM, RP_SINGLE><<<grid, RP_NT, 0, st>>>(a);
