@@ -191,8 +191,8 @@ def qk_rope(q, k, cu_seqlens=None, kv_lens=None, *, positions=None, theta: float
     The tokens' places in the cache, from a plan's ``cu_seqlens`` and ``kv_lens``, or ``positions`` [tokens] int32.
     ``rotary_dim``: the first dims of a head that are turned (default: all); ``norm``: each head is divided by its root mean
     square, and times ``weight_offset`` + its weight [hd] (of the type of q or float32) where there is one.  ``out``: two
-    tensors; they may be q and k themselves, but share no other element with an input or one another.  Rows behind the last request are left as they were, so by default they are
-    not initialized."""
+    tensors; they may be q and k themselves, but share no other element with an input or one another.  Rows behind the
+    last request are left as they were, so by default they are not initialized."""
     q, k = _t(q), _t(k)
     dev, dt = q.get_device(), q.dtype
     code = _CODE.get(dt)

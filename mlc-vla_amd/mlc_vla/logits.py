@@ -42,7 +42,8 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, scale: float = 1.0, out
 
     tokens [rows] or [rows, n] int32: the given tokens; one outside [0, vocab) counts 0.  ``top``: how many alternatives, up
     to 64, the likeliest first and equal logits by their index.  ``out``: contiguous tensors of the same sizes to write into,
-    which share nothing with the inputs or one another; ``workspace``: uint8 tensor of ``token_logprobs_workspace`` bytes (default: allocated here)."""
+    which share nothing with the inputs or one another; ``workspace``: uint8 tensor of ``token_logprobs_workspace`` bytes
+    (default: allocated here)."""
     x = _t(logits)
     dev, code = x.get_device(), _CODE.get(x.dtype)
     rows, vocab = x.shape if x.dim() == 2 else (-1, -1)
